@@ -1,0 +1,129 @@
+"""What the operators on rows of channels refuse (include/fhc_seq.h): every refusal is an error status with a message
+before any device work, so these run without a GPU; the pointers are never followed."""
+import ctypes
+
+import pytest
+
+import fhtest  # noqa: F401
+
+P = 0x10000  # an aligned address that nothing reads
+
+
+def mod():
+    import fhseq
+    return fhseq
+
+
+def glr_args(**kw):
+    m = mod()
+    a = dict(dtype=1, b=2, t=5, d=8, rate=8.0, lam=P, lengths=None)
+    seqs = dict(x=(P, 40, 8), r=(P, 40, 8), i=(P, 40, 8), y=(P, 40, 8), dy=(P, 40, 8), dx=(P, 40, 8), dr=(P, 40, 8),
+                di=(P, 40, 8))
+    a.update({k: v for k, v in kw.items() if k in a})
+    seqs.update({k: v for k, v in kw.items() if k in seqs})
+    g = ctypes.byref(m.GlrDesc(*a.values()))
+    return g, {k: None if v is None else ctypes.byref(m.FhcSeq(*v)) for k, v in seqs.items()}
+
+
+def glr_forward(**kw):
+    L = mod()._lib()
+    g, s = glr_args(**kw)
+    return L.fhc_glr_forward(kw.get("desc", g), s["x"], s["r"], s["i"], None, s["y"], None, None, kw.get("ws", P),
+                             kw.get("ws_bytes", 1 << 40), None)
+
+
+def glr_backward(**kw):
+    L = mod()._lib()
+    g, s = glr_args(**kw)
+    return L.fhc_glr_backward(g, s["x"], s["r"], s["i"], kw.get("states", P), s["dy"], None, s["dx"], s["dr"], s["di"],
+                              kw.get("dlam", P), None, kw.get("ws", P), kw.get("ws_bytes", 1 << 40), None)
+
+
+def refused(rc, text):
+    msg = mod().fhconv.last_error()
+    assert rc == -1 and text in msg, (rc, msg)
+
+
+@pytest.mark.parametrize("bad,text", [
+    (dict(dtype=3), "dtype 3"), (dict(rate=float("nan")), "rate"), (dict(rate=-1.0), "rate"),
+    (dict(b=1 << 20, d=1 << 12), "columns"), (dict(t=0xFFFFFFFF), "steps"), (dict(lam=None), "null lam"),
+    (dict(x=None), "null x"), (dict(r=(None, 40, 8)), "null pointer of r"), (dict(i=(P + 1, 40, 8)), "not aligned"),
+    (dict(y=(P, 40, 4)), "overlap"), (dict(y=(P, 3, 8)), "overlap"), (dict(desc=None), "null descriptor"),
+])
+def test_glr_forward_refuses(bad, text):
+    refused(glr_forward(**bad), text)
+
+
+@pytest.mark.parametrize("bad,text", [
+    (dict(states=None), "null states"), (dict(dlam=None), "null dlam"), (dict(dy=None), "null dy"),
+    (dict(dx=(P, 40, 4)), "overlap"), (dict(ws=None), "null workspace"), (dict(ws_bytes=8), "workspace of 8"),
+    (dict(ws=P + 16), "256-byte"), (dict(dtype=9), "dtype 9"),
+])
+def test_glr_backward_refuses(bad, text):
+    refused(glr_backward(**bad), text)
+
+
+def test_glr_workspace_is_checked_where_chunks_are_chained():
+    g, _ = glr_args(t=1000)
+    need = mod()._lib().fhc_glr_workspace_bytes(g, 0)
+    assert need > 0
+    kw = dict(t=1000, x=(P, 8000, 8), r=(P, 8000, 8), i=(P, 8000, 8), y=(P, 8000, 8))
+    refused(glr_forward(ws=None, **kw), "null workspace")
+    refused(glr_forward(ws_bytes=need - 1, **kw), "needed")
+
+
+def test_glr_nothing_to_do_is_fine():
+    assert glr_forward(b=0) == 0 and glr_forward(d=0) == 0 and glr_backward(d=0) == 0
+    L = mod()._lib()
+    assert L.fhc_glr_states_bytes(None) == 0 and L.fhc_glr_workspace_bytes(None, 1) == 0
+
+
+def norm_call(back, **kw):
+    m = mod()
+    L = m._lib()
+    a = dict(dtype=1, rows=6, c=16, rows_per_group=3, alpha=1.0, eps=1e-6, w_post=P, w_pre=P, gate=P)
+    r = {k: (P, 16) for k in ("x", "o", "y", "u", "dy", "du", "dx", "dout")}
+    a.update({k: v for k, v in kw.items() if k in a})
+    r.update({k: v for k, v in kw.items() if k in r})
+    n = None if kw.get("desc", 1) is None else ctypes.byref(m.NormDesc(*a.values()))
+    r = {k: None if v is None else ctypes.byref(m.FhcRows(*v)) for k, v in r.items()}
+    if back:
+        return L.fhc_norm_block_backward(n, r["x"], r["o"], r["dy"], r["du"], r["dx"], r["dout"], kw.get("dw_post", P),
+                                         kw.get("dgate", P), P, kw.get("ws", P), kw.get("ws_bytes", 1 << 40), None)
+    return L.fhc_norm_block(n, r["x"], r["o"], r["y"], r["u"], None)
+
+
+@pytest.mark.parametrize("bad,text", [
+    (dict(desc=None), "null descriptor"), (dict(dtype=4), "dtype 4"), (dict(c=16385), "channels"),
+    (dict(rows=1 << 31), "rows"), (dict(rows_per_group=0), "rows_per_group"), (dict(alpha=float("inf")), "alpha"),
+    (dict(eps=0.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(w_pre=P + 1), "not aligned"),
+    (dict(x=None), "null x"), (dict(o=(None, 16)), "null pointer of o"), (dict(y=(P, 15)), "apart"),
+    (dict(u=(P + 1, 16)), "not aligned"), (dict(y=None, u=None), "neither y nor u"), (dict(o=None), "without o"),
+])
+def test_norm_block_refuses(bad, text):
+    refused(norm_call(False, **bad), text)
+
+
+@pytest.mark.parametrize("bad,text", [
+    (dict(dx=None), "null dx"), (dict(dout=None), "null dout"), (dict(dy=None, du=None), "neither dy nor du"),
+    (dict(o=None), "without o"), (dict(gate=None), "dgate without a gate"), (dict(ws=None), "null workspace"),
+    (dict(ws_bytes=100), "workspace of 100"), (dict(ws=P + 8), "256-byte"), (dict(c=20000), "channels"),
+])
+def test_norm_block_backward_refuses(bad, text):
+    refused(norm_call(True, **bad), text)
+
+
+def test_norm_block_nothing_to_do_is_fine():
+    assert norm_call(False, rows=0) == 0 and norm_call(False, c=0) == 0 and norm_call(True, c=0) == 0
+
+
+def test_tensors_are_checked_before_the_call():
+    import torch
+    m = mod()
+    x = torch.zeros(2, 3, 4)
+    with pytest.raises(m.FhcError, match="current GPU"):
+        m.glr(x, x, x, torch.zeros(4))
+    with pytest.raises(m.FhcError, match="f16, bf16 or f32"):
+        m.glr(x.double(), x, x, torch.zeros(4))
+    with pytest.raises(m.FhcError, match="rows, channels"):
+        m.norm_block(x, x, None, None, None)

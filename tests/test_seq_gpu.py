@@ -1,0 +1,361 @@
+"""The operators on rows of channels (through fhseq.py and the C ABI, include/fhc_seq.h) against plain 64-bit forms,
+on the GPU. The tolerances are the forms' own error bounds (tests/seqref.py) plus half a step of each output's type."""
+import math
+
+import pytest
+
+import fhtest  # noqa: F401  (puts the package on sys.path)
+import seqref
+
+pytestmark = pytest.mark.gpu
+
+
+def say(*a):
+    print(*a, flush=True)
+
+
+def mod():
+    import fhseq
+    return fhseq
+
+
+def types():
+    import torch
+    return {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+
+
+class Rand:
+    def __init__(self, seed):
+        import torch
+        self.torch, self.g = torch, torch.Generator(device="cuda")
+        self.g.manual_seed(seed)
+
+    def normal(self, *shape, scale=1.0, dtype=None):
+        v = self.torch.randn(*shape, generator=self.g, device="cuda") * scale
+        return v.to(dtype) if dtype is not None else v
+
+    def uniform(self, *shape, lo=0.0, hi=1.0):
+        return self.torch.rand(*shape, generator=self.g, device="cuda") * (hi - lo) + lo
+
+    def ints(self, lo, hi, n):
+        return self.torch.randint(lo, hi, (n,), generator=self.g, device="cuda", dtype=self.torch.int32)
+
+
+# ---- the gated linear recurrence --------------------------------------------------------------------------------
+
+GLR = [  # b, t, d: one step; less and more than a wave's stretch, a chunk; odd widths; each way of walking the chunks
+    (1, 1, 1), (5, 1, 64), (3, 2, 7), (2, 8, 130), (2, 16, 66), (2, 17, 66), (1, 64, 33), (3, 65, 34), (2, 200, 128),
+    (1, 1000, 130), (1, 1537, 3), (2, 700, 250), (40, 70, 2048), (70, 130, 1001), (300, 20, 2048), (1030, 9, 512),
+]
+
+
+def glr_inputs(q, b, t, d, dtype, time_major=False, ragged=False):
+    def seq():
+        return q.normal(t, b, d, dtype=dtype).transpose(0, 1) if time_major else q.normal(b, t, d, dtype=dtype)
+
+    lengths = None
+    if ragged:
+        lengths = q.ints(0, t + 1, b)
+        lengths[-1] = 0
+        lengths[0] = t
+    return dict(x=seq(), r=seq(), i=seq(), lam=q.normal(d, scale=1.5) - 4, h0=q.normal(b, d), dy=seq(),
+                dht=q.normal(b, d), lengths=lengths)
+
+
+def glr_check(v, rate=8.0):
+    m = mod()
+    y, ht, states = m.glr(v["x"], v["r"], v["i"], v["lam"], rate, h0=v["h0"], lengths=v["lengths"], train=True)
+    grads = m.glr_backward(v["x"], v["r"], v["i"], v["lam"], states, v["dy"], rate, dht=v["dht"],
+                           lengths=v["lengths"])
+    ref, err = seqref.glr(v["x"], v["r"], v["i"], v["lam"], rate, v["h0"], v["lengths"], v["dy"], v["dht"])
+    for name, got, want, tol in zip(("y", "ht", "dx", "dr", "di", "dlam", "dh0"), (y, ht) + grads, ref, err):
+        seqref.close(got, want, tol, name)
+    return (y, ht) + grads
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("shape", GLR, ids=str)
+def test_glr(shape, dtype):
+    say("glr", shape, dtype)
+    q = Rand(sum(shape))
+    glr_check(glr_inputs(q, *shape, types()[dtype], time_major=shape[2] % 3 == 0, ragged=shape[1] % 2 == 1))
+
+
+@pytest.mark.parametrize("shape", [(4, 9, 10), (3, 131, 64), (40, 140, 2048)], ids=str)
+def test_glr_masked_places_are_not_read(shape):
+    """NaN and infinities past the lengths, empty sequences, lengths outside [0, t]."""
+    say("glr masked", shape)
+    import torch
+    q = Rand(7)
+    v = glr_inputs(q, *shape, torch.float16, ragged=True)
+    v["lengths"][1], v["lengths"][2] = shape[1] + 1000, -3
+    past = torch.arange(shape[1], device="cuda")[None] >= v["lengths"][:, None]
+    clean = glr_check(v)
+    for k, bad in (("x", math.nan), ("r", math.inf), ("i", math.nan), ("dy", -math.inf)):
+        v[k] = v[k].masked_fill(past[:, :, None], bad)
+    m = mod()
+    y, ht, st = m.glr(v["x"], v["r"], v["i"], v["lam"], h0=v["h0"], lengths=v["lengths"], train=True)
+    got = (y, ht) + m.glr_backward(v["x"], v["r"], v["i"], v["lam"], st, v["dy"], dht=v["dht"], lengths=v["lengths"])
+    assert all(torch.equal(a, b) for a, b in zip(got, clean))
+    assert not y[past].any() and not got[2][past].any()
+    assert torch.equal(ht[2], v["h0"][2])  # an empty sequence's state
+
+
+@pytest.mark.parametrize("t", [0, 1, 40, 300])
+def test_glr_gates_at_their_ends(t):
+    """Gates shut and open beyond f32's exponent range: the state stays, or is replaced; no gradient is NaN."""
+    say("glr ends", t)
+    import torch
+    q = Rand(3)
+    v = glr_inputs(q, 2, t, 48, torch.float32)
+    v["r"][:, :, :8], v["r"][:, :, 8:16] = -200.0, 200.0
+    v["i"][:, :, 16:24], v["i"][:, :, 24:32] = -200.0, 200.0
+    v["r"][:, :, 32:36] = -math.inf
+    v["lam"][36:40], v["lam"][40:44] = -120.0, 40.0
+    m = mod()
+    y, ht, st = m.glr(v["x"], v["r"], v["i"], v["lam"], h0=v["h0"], train=True)
+    grads = m.glr_backward(v["x"], v["r"], v["i"], v["lam"], st, v["dy"], dht=v["dht"])
+    assert all(torch.isfinite(k).all() for k in (y, ht) + grads)
+    assert torch.equal(ht[:, :8], v["h0"][:, :8]) and torch.equal(ht[:, 32:36], v["h0"][:, 32:36])
+    if t:
+        ref, _ = seqref.glr(v["x"], v["r"], v["i"], v["lam"], 8.0, v["h0"])
+        assert torch.allclose(y.double(), ref[0], rtol=1e-4, atol=1e-5)
+
+
+def test_glr_views_strides_and_states_in_place():
+    """Views into wider buffers, at odd offsets, equal the dense call; the state may be updated in place."""
+    say("glr views")
+    import torch
+    q = Rand(11)
+    b, t, d = 3, 150, 40
+    m = mod()
+    for off in (0, 1, 2):
+        wide = [q.normal(t, b, 3 * d + 5, dtype=torch.bfloat16) for _ in range(3)]
+        x, r, i = (w[:, :, off:off + d].transpose(0, 1) for w in wide)
+        lam, h0 = q.normal(d) - 4, q.normal(b, d)
+        y, ht = m.glr(x, r, i, lam, h0=h0)
+        y2, ht2 = m.glr(x.contiguous(), r.contiguous(), i.contiguous(), lam, h0=h0)
+        assert torch.equal(y, y2) and torch.equal(ht, ht2)
+    # step by step over the same tokens, the state in place
+    L = m._lib()
+    import ctypes
+    state = h0.clone()
+    for k in range(t):
+        step = [v[:, k:k + 1] for v in (x, r, i)]
+        g = m.GlrDesc(1, b, 1, d, 8.0, lam.data_ptr(), None)
+        out = torch.empty((b, 1, d), dtype=torch.bfloat16, device="cuda")
+        s = [ctypes.byref(m.FhcSeq(v.data_ptr(), v.stride(0), v.stride(1))) for v in step + [out]]
+        assert L.fhc_glr_forward(ctypes.byref(g), s[0], s[1], s[2], state.data_ptr(), s[3], state.data_ptr(), None,
+                                 None, 0, torch.cuda.current_stream().cuda_stream) == 0
+    ref, err = seqref.glr(x, r, i, lam, 8.0, h0)
+    seqref.close(state, ref[1], err[1], "state after single steps")
+
+
+def test_glr_gradient_against_differences():
+    """The kernels' gradients along random directions against central differences of the 64-bit loss."""
+    say("glr differences")
+    import torch
+    q = Rand(5)
+    v = glr_inputs(q, 2, 90, 20, torch.float32, ragged=True)
+    got = dict(zip(("x", "r", "i", "lam", "h0"), glr_check(v)[2:]))
+
+    def loss(**change):
+        w = {k: (v[k].double() + change[k] if k in change else v[k].double()) for k in ("x", "r", "i", "lam", "h0")}
+        (y, ht), _ = seqref.glr(w["x"], w["r"], w["i"], w["lam"], 8.0, w["h0"], v["lengths"])
+        return float((y * v["dy"].double()).sum() + (ht * v["dht"].double()).sum())
+
+    for k, grad in got.items():
+        u = q.normal(*v[k].shape).double()
+        s = 1e-5
+        slope = (loss(**{k: s * u}) - loss(**{k: -s * u})) / (2 * s)
+        want = float((grad.double() * u).sum())
+        # f32 gradients, and the third difference's s^2
+        assert abs(slope - want) <= 1e-4 * float((grad.double() * u).abs().sum()), (k, slope, want)
+
+
+def test_glr_long_offsets():
+    """A tensor whose last rows lie past 2^31 elements."""
+    say("glr long offsets")
+    import torch
+    b, t, d = 2, 8, 64
+    far = (1 << 30) + 64
+    buf = torch.zeros(2 * far + 4096, dtype=torch.float16, device="cuda")
+    q = Rand(2)
+    dense = q.normal(b, t, d, dtype=torch.float16)
+    x = torch.as_strided(buf, (b, t, d), (2 * far, d, 1))
+    x.copy_(dense)
+    m = mod()
+    lam = q.normal(d) - 4
+    assert torch.equal(m.glr(x, dense, dense, lam)[0], m.glr(dense, dense, dense, lam)[0])
+    xt = torch.as_strided(buf, (1, 3, d), (0, far, 1))
+    xt.copy_(dense[:1, :3])
+    assert torch.equal(m.glr(xt, dense[:1, :3], dense[:1, :3], lam)[0], m.glr(*(dense[:1, :3],) * 3, lam)[0])
+
+
+@pytest.mark.parametrize("shape", [(2, 1, 64), (2, 300, 64), (40, 70, 2048)], ids=str)
+def test_glr_in_a_graph_and_on_another_stream(shape):
+    """Captured and replayed with other work between, every replay equals the eager call; so does a side stream."""
+    say("glr graph", shape)
+    import torch
+    v = glr_inputs(Rand(9), *shape, torch.bfloat16)
+    m = mod()
+
+    def call(stream=None):
+        y, ht, st = m.glr(v["x"], v["r"], v["i"], v["lam"], h0=v["h0"], train=True, stream=stream)
+        return (y, ht) + m.glr_backward(v["x"], v["r"], v["i"], v["lam"], st, v["dy"], dht=v["dht"], stream=stream)
+
+    want = [k.clone() for k in call()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    other = call(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(other, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for k in range(4):
+        for o in out:
+            o.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+        call()
+
+
+# ---- the norms around a block -----------------------------------------------------------------------------------
+
+NORM = [  # rows, channels, rows per group (0: no gate)
+    (1, 1, 1), (3, 5, 2), (7, 32, 7), (50, 128, 11), (33, 129, 33), (64, 257, 1), (20, 512, 20), (9, 1000, 4),
+    (300, 1024, 100), (40, 1931, 40), (5, 4096, 5), (17, 8192, 3), (6, 8200, 0), (3, 16384, 2), (5000, 64, 1250),
+    (2100, 40, 1), (1, 2048, 0),
+]
+
+
+def norm_inputs(q, rows, c, rpg, dtype):
+    g = -(-rows // rpg) if rpg else 0
+    return dict(x=q.normal(rows, c, dtype=dtype), o=q.normal(rows, c, scale=3.0, dtype=dtype),
+                w_post=(1 + 0.1 * q.normal(c)).to(dtype), w_pre=(1 + 0.1 * q.normal(c)).to(dtype),
+                gate=q.normal(g, c, scale=0.5, dtype=dtype) if rpg else None,
+                dy=q.normal(rows, c, dtype=dtype), du=q.normal(rows, c, dtype=dtype))
+
+
+NORM_OUT = ("y", "u", "dx", "do", "dw_post", "dgate", "dw_pre")
+
+
+def norm_check(v, alpha, eps, rpg):
+    m = mod()
+    w = [v[k] for k in ("x", "o", "w_post", "gate", "w_pre")]
+    got = m.norm_block(*w, alpha, eps, max(rpg, 1)) + m.norm_block_backward(*w, v["dy"], v["du"], alpha, eps,
+                                                                          max(rpg, 1))
+    ref, err = seqref.norm_block(*w, alpha, eps, max(rpg, 1), v["dy"], v["du"])
+    for name, g, want, tol in zip(NORM_OUT, got, ref, err):
+        if g is not None:
+            seqref.close(g, want, tol, name)
+    return got
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("shape", NORM, ids=str)
+def test_norm_block(shape, dtype):
+    say("norm", shape, dtype)
+    norm_check(norm_inputs(Rand(sum(shape)), *shape, types()[dtype]), math.sqrt(0.5), 1e-6, shape[2])
+
+
+def test_norm_block_parts_left_out():
+    """Without the block (the first norm of a stack), without either weight, the gate, dy or du."""
+    say("norm parts")
+    import torch
+    for gone in (("o", "w_post", "gate"), ("w_post",), ("w_pre",), ("gate",), ("dy",), ("du",), ("w_post", "w_pre", "gate")):
+        v = norm_inputs(Rand(4), 37, 200, 10, torch.bfloat16)
+        v.update({k: None for k in gone})
+        got = dict(zip(NORM_OUT, norm_check(v, 1.0, 1e-5, 10)))
+        assert all((got["d" + k] is None) == (k in gone) for k in ("w_post", "gate", "w_pre"))
+
+
+def test_norm_block_zero_rows_and_empty_tensors():
+    say("norm zeros")
+    import torch
+    m = mod()
+    v = norm_inputs(Rand(6), 12, 64, 4, torch.float32)
+    v["x"][3], v["o"][3], v["o"][5] = 0, 0, 0  # rms of the eps alone
+    norm_check(v, 0.5, 1e-6, 4)
+    e = norm_inputs(Rand(6), 0, 64, 4, torch.float32)
+    w = [e[k] for k in ("x", "o", "w_post", "gate", "w_pre")]
+    y, u = m.norm_block(*w, rows_per_group=4)
+    assert y.shape == u.shape == (0, 64)
+    back = m.norm_block_backward(*w, e["dy"], e["du"], rows_per_group=4)
+    torch.cuda.synchronize()
+    assert not back[2].any() and not back[4].any() and back[3].shape == (0, 64)
+
+
+@pytest.mark.parametrize("c", [64, 65, 600])
+def test_norm_block_views_and_in_place(c):
+    """Row views of wider buffers at odd offsets; y over x, u over o; dx over dy, do over du."""
+    say("norm views", c)
+    import ctypes
+    import torch
+    m, rows = mod(), 30
+    v = norm_inputs(Rand(8), rows, c, 10, torch.float16)
+    w = [v[k] for k in ("x", "o", "w_post", "gate", "w_pre")]
+    y, u = m.norm_block(*w, rows_per_group=10)
+    grads = m.norm_block_backward(*w, v["dy"], v["du"], rows_per_group=10)
+    wide = {k: torch.full((rows, c + 19), 7.0, dtype=torch.float16, device="cuda") for k in ("x", "o", "dy", "du")}
+    views = {k: b[:, 3:3 + c] for k, b in wide.items()}
+    for k, b in views.items():
+        b.copy_(v[k])
+    n = m.NormDesc(0, rows, c, 10, 1.0, 1e-6, v["w_post"].data_ptr(), v["w_pre"].data_ptr(), v["gate"].data_ptr())
+    at = {k: ctypes.byref(m.FhcRows(b.data_ptr(), b.stride(0))) for k, b in views.items()}
+    L, s = m._lib(), torch.cuda.current_stream().cuda_stream
+    size = L.fhc_norm_block_workspace_bytes(ctypes.byref(n))
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    assert L.fhc_norm_block_backward(ctypes.byref(n), at["x"], at["o"], at["dy"], at["du"], at["dy"], at["du"], None,
+                                     None, None, ws.data_ptr(), size, s) == 0
+    assert L.fhc_norm_block(ctypes.byref(n), at["x"], at["o"], at["x"], at["o"], s) == 0
+    torch.cuda.synchronize()
+    for got, want in ((views["x"], y), (views["o"], u), (views["dy"], grads[0]), (views["du"], grads[1])):
+        assert torch.equal(got, want)
+    for b in wide.values():
+        assert (b[:, :3] == 7).all() and (b[:, 3 + c:] == 7).all()
+
+
+def test_norm_block_gradient_against_differences():
+    say("norm differences")
+    import torch
+    q = Rand(12)
+    v = norm_inputs(q, 24, 48, 7, torch.float32)
+    got = dict(zip(("x", "o", "w_post", "gate", "w_pre"), norm_check(v, 0.7, 1e-6, 7)[2:]))
+
+    def loss(**change):
+        w = [v[k].double() + change.get(k, 0) for k in ("x", "o", "w_post", "gate", "w_pre")]
+        (y, u), _ = seqref.norm_block(*w, 0.7, 1e-6, 7)
+        return float((y * v["dy"].double()).sum() + (u * v["du"].double()).sum())
+
+    for k, grad in got.items():
+        d = q.normal(*v[k].shape).double()
+        s = 1e-5
+        slope = (loss(**{k: s * d}) - loss(**{k: -s * d})) / (2 * s)
+        want = float((grad.double() * d).sum())
+        assert abs(slope - want) <= 1e-4 * float((grad.double() * d).abs().sum()), (k, slope, want)
+
+
+def test_norm_block_in_a_graph():
+    say("norm graph")
+    import torch
+    m = mod()
+    v = norm_inputs(Rand(13), 500, 300, 125, torch.bfloat16)
+    w = [v[k] for k in ("x", "o", "w_post", "gate", "w_pre")]
+
+    def call():
+        return m.norm_block(*w, rows_per_group=125) + m.norm_block_backward(*w, v["dy"], v["du"], rows_per_group=125)
+
+    want = [k.clone() for k in call()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for k in range(4):
+        for o in out:
+            o.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+        call()
