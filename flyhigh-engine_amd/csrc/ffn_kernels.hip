@@ -1,0 +1,402 @@
+// The gated feed-forward block (include/fhc_seq.h): the launches around the products of ffn_gemm.h, and the products
+// of few rows.
+//
+// Forward: one product with gate and up rows side by side whose epilogue is the activation and the product, one with
+// wd. Backward: dh = dy wd with dL/dgate, dL/dup in its epilogue; dx = [dL/dgate dL/dup] [wg; wu] as one product over
+// both halves of K; dwg and dwu (one launch), dwd, with the rows as K.
+#include "ffn_gemm.h"
+
+namespace fhc {
+namespace seq {
+namespace {
+
+// out = the sum of the splits' partial sums, in their order
+template <class T>
+__global__ __launch_bounds__(256) void ffn_join(const float* part, int splits, int m, int n, int64_t ldpart,
+                                                uint16_t* o0, uint16_t* o1, int64_t ldo) {
+    const int quads = (n + 3) / 4;
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= (int64_t)m * quads) return;
+    const int64_t row = at / quads;
+    const int c = (int)(at - row * quads) * 4;
+    const float* p = part + ((int64_t)blockIdx.y * splits * m + row) * ldpart + c;
+    f4 s = *reinterpret_cast<const f4*>(p);
+    for (int z = 1; z < splits; z++) s += *reinterpret_cast<const f4*>(p + (int64_t)z * m * ldpart);
+    uint16_t q[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) q[r] = narrow(T{}, s[r]);
+    store4((blockIdx.y ? o1 : o0) + row * ldo + c, n - c, q);
+}
+
+// ---- few rows: a wave streams 16 weight rows past the matrix unit straight from global memory (each weight is used
+// once, so LDS would only add a step), NB blocks of 16 token rows as the other operand; the NW waves of a workgroup
+// split K and add their sums in LDS in the waves' order.
+struct SkinnyArgs {
+    const uint16_t *x, *w0, *w1;
+    int64_t ldx, ldw;
+    int rows, n, k;
+    uint16_t* out;
+    int64_t ldo;
+    uint32_t act;
+};
+
+// 8 elements from k on, all of them inside
+template <bool AL>
+__device__ __forceinline__ u4_t load_k(const uint16_t* row, int k) {
+    if constexpr (AL) return *reinterpret_cast<const u4_t*>(row + k);
+    else return load_some(row + k, 8);
+}
+
+template <class T, bool GLU, int NB, int NW, bool AL>
+__global__ __launch_bounds__(64 * NW) void ffn_skinny(SkinnyArgs g) {
+    constexpr int P = GLU ? 2 : 1;
+    __shared__ f4 sums[NW][P * NB][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int f0 = blockIdx.x * 16, f = min(f0 + (lane & 15), g.n - 1);  // a row past the end: the last one again
+    const int kl = 8 * (lane >> 4);
+    const int steps = (g.k + 31) / 32, per = (steps + NW - 1) / NW;
+    const int s0 = wave * per, s1 = min(steps, s0 + per);
+    const uint16_t* w0 = g.w0 + (int64_t)f * g.ldw;
+    const uint16_t* w1 = GLU ? g.w1 + (int64_t)f * g.ldw : nullptr;
+    const uint16_t* x[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) x[b] = g.x + (int64_t)min(b * 16 + (lane & 15), g.rows - 1) * g.ldx;
+    f4 acc[P][NB];
+#pragma unroll
+    for (int p = 0; p < P; p++)
+#pragma unroll
+        for (int b = 0; b < NB; b++) acc[p][b] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int U = NB == 4 ? 4 : 8;  // steps whose loads are in flight together
+    auto multiply = [&](const u4_t (&w)[P], const u4_t (&v)[NB]) {
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int b = 0; b < NB; b++) acc[p][b] = mfma16(T{}, w[p], v[b], acc[p][b]);
+    };
+    const int full = g.k / 32;  // the last step may be cut
+    int s = s0;
+    for (; s + U <= min(s1, full); s += U) {
+        u4_t w[U][P], v[U][NB];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int k = (s + u) * 32 + kl;
+            w[u][0] = load_k<AL>(w0, k);
+            if constexpr (GLU) w[u][1] = load_k<AL>(w1, k);
+#pragma unroll
+            for (int b = 0; b < NB; b++) v[u][b] = load_k<AL>(x[b], k);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) multiply(w[u], v[u]);
+    }
+    for (; s < s1; s++) {
+        const int k = s * 32 + kl;
+        u4_t w[P], v[NB];
+        w[0] = load_some(w0 + k, g.k - k);
+        if constexpr (GLU) w[1] = load_some(w1 + k, g.k - k);
+#pragma unroll
+        for (int b = 0; b < NB; b++) v[b] = load_some(x[b] + k, g.k - k);
+        multiply(w, v);
+    }
+#pragma unroll
+    for (int p = 0; p < P; p++)
+#pragma unroll
+        for (int b = 0; b < NB; b++) sums[wave][p * NB + b][lane] = acc[p][b];
+    __syncthreads();
+    // wave b finishes token block b (f = f0 + 4 (lane >> 4) + r of row b * 16 + (lane & 15))
+    for (int b = wave; b < NB; b += NW) {
+        f4 t[P];
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+            t[p] = sums[0][p * NB + b][lane];
+            for (int w = 1; w < NW; w++) t[p] += sums[w][p * NB + b][lane];
+        }
+        const int row = b * 16 + (lane & 15), at = f0 + 4 * (lane >> 4);
+        if (row >= g.rows || at >= g.n) continue;
+        uint16_t q[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            q[r] = narrow(T{}, GLU ? act_of(g.act, t[0][r]) * t[P - 1][r] : t[0][r]);
+        store4(g.out + row * g.ldo + at, g.n - at, q);
+    }
+}
+
+// ---- host side ----------------------------------------------------------------------------------------------------
+
+constexpr uint32_t kSkinnyRows = 64;  // up to here the weights' bytes are all that counts
+
+int check_desc(const char* op, const fhc_ffn_desc* d) {
+    if (!d) return fail(-1, "%s: null descriptor", op);
+    if (d->dtype > FHC_BF16) return fail(-1, "%s: dtype %u is neither f16 nor bf16", op, d->dtype);
+    if (d->act > FHC_ACT_GELU) return fail(-1, "%s: act %u", op, d->act);
+    if (d->c > 1u << 20 || d->f > 1u << 20) return fail(-1, "%s: %u x %u channels, at most 2^20", op, d->c, d->f);
+    if (d->rows > 0x7FFFFF00u) return fail(-1, "%s: %u rows", op, d->rows);
+    return 0;
+}
+int check_rows(const char* op, const char* name, const fhc_rows* r, uint32_t c) {
+    if (!r) return fail(-1, "%s: null %s", op, name);
+    if (!r->p) return fail(-1, "%s: null pointer of %s", op, name);
+    if (r->ld < (int64_t)c) return fail(-1, "%s: rows of %s are %lld apart, below %u channels", op, name, (long long)r->ld, c);
+    if (!aligned(r->p, 2)) return fail(-1, "%s: %s is not aligned to its elements", op, name);
+    return 0;
+}
+int check_weight(const char* op, const char* name, const void* p) {
+    if (!p) return fail(-1, "%s: null %s", op, name);
+    if (!aligned(p, 2)) return fail(-1, "%s: %s is not aligned to its elements", op, name);
+    return 0;
+}
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+int64_t padded(uint32_t f) { return ((int64_t)f + 7) / 8 * 8; }
+size_t hidden_bytes(const fhc_ffn_desc* d) { return up256((size_t)d->rows * padded(d->f) * 2); }
+size_t pre_bytes(const fhc_ffn_desc* d) { return up256((size_t)d->rows * padded(d->f) * 4); }
+
+struct Shape {  // a product's tiles and splits
+    bool big;   // 256 x 256 tiles of 8 waves, else 128 x 128 of 4
+    int tiles_m, tiles_n, slabs, per_split, splits;
+    size_t part_bytes;
+};
+// Tiles of 256 where they fill the chip's 256 CUs; else tiles of 128, with K split (where the epilogue allows it)
+// until there are two workgroups a CU, at least 4 slabs each.
+Shape shape_of(int64_t m, int64_t n, int64_t k, int segments, int pairs, bool glu, bool may_split, bool dma) {
+    Shape s{};
+    auto tiles = [&](int bm, int bn) { return ceil_div(m, bm) * ceil_div(n, bn); };
+    s.big = dma && tiles(256, glu ? 128 : 256) * pairs >= 224;
+    const int bm = s.big ? 256 : 128, bn = (s.big ? 256 : 128) / (glu ? 2 : 1);
+    s.tiles_m = (int)ceil_div(m, bm), s.tiles_n = (int)ceil_div(n, bn);
+    s.slabs = (int)ceil_div(k, 128) * 2 * segments;
+    s.splits = 1;
+    const int64_t wgs = (int64_t)s.tiles_m * s.tiles_n * pairs;
+    if (may_split && wgs < 256 && s.slabs >= 8) {
+        int64_t z = ceil_div(512, wgs);
+        if (z > s.slabs / 4) z = s.slabs / 4;
+        s.splits = z < 1 ? 1 : (int)z;
+    }
+    s.per_split = (int)ceil_div(s.slabs, 2 * s.splits) * 2;
+    s.splits = s.slabs ? (int)ceil_div(s.slabs, s.per_split) : 1;
+    s.part_bytes = s.splits > 1 ? up256((size_t)pairs * s.splits * m * ((n + 3) / 4 * 4) * 4) : 0;
+    return s;
+}
+
+// LDS DMA: chunks at 4-byte steps whose offsets within a tile stay below 2^31
+bool dma_ok(const GemmArgs& g) {
+    if (g.lda % 2 || g.ldb % 2 || g.lda > 1 << 21 || g.ldb > 1 << 21) return false;
+    if (g.k % 2 || g.m % 2 || g.n % 2) return false;
+    for (const void* p : {g.a0, g.a1, g.b0, g.b1})
+        if (!aligned(p, 4)) return false;
+    return true;
+}
+
+template <class T, bool AC, bool BC, Epi E>
+void launch_tiles(const Shape& s, const GemmArgs& g, hipStream_t st) {
+    const dim3 grid(s.tiles_m * s.tiles_n, 1, s.splits * g.pairs);
+    if (s.big) {
+        hipLaunchKernelGGL((ffn_gemm<T, AC, BC, E, 8, 2, 4, true>), grid, dim3(512), 0, st, g);
+    } else {
+        if (dma_ok(g)) hipLaunchKernelGGL((ffn_gemm<T, AC, BC, E, 4, 2, 2, true>), grid, dim3(256), 0, st, g);
+        else hipLaunchKernelGGL((ffn_gemm<T, AC, BC, E, 4, 2, 2, false>), grid, dim3(256), 0, st, g);
+    }
+}
+
+// g without tiles and splits
+template <class T, bool AC, bool BC, Epi E>
+int product(const char* op, GemmArgs g, float* part, hipStream_t st) {
+    if (g.m == 0 || g.n == 0) return 0;
+    g.segments = g.segments ? g.segments : 1, g.pairs = g.pairs ? g.pairs : 1;
+    const Shape s = shape_of(g.m, g.n, g.k, g.segments, g.pairs, E == kGlu, E == kStore, dma_ok(g));
+    g.tiles_m = s.tiles_m, g.tiles_n = s.tiles_n, g.slabs = s.slabs, g.per_split = s.per_split, g.splits = s.splits;
+    if ((int64_t)s.tiles_m * s.tiles_n >= 1ll << 31) return fail(-1, "%s: too many tiles", op);
+    if constexpr (E == kStore) {
+        if (s.splits > 1) {
+            g.part = part, g.ldpart = ((int64_t)g.n + 3) / 4 * 4;
+            launch_tiles<T, AC, BC, kPart>(s, g, st);
+            FHC_TRY(launched(op));
+            const uint64_t items = (uint64_t)g.m * ((g.n + 3) / 4);
+            hipLaunchKernelGGL((ffn_join<T>), dim3((uint32_t)ceil_div(items, 256), g.pairs), dim3(256), 0, st, g.part,
+                               s.splits, g.m, g.n, g.ldpart, g.o0, g.o1, g.ldo);
+            return launched(op);
+        }
+    }
+    launch_tiles<T, AC, BC, E>(s, g, st);
+    return launched(op);
+}
+
+template <class T, bool GLU>
+int skinny(const char* op, const SkinnyArgs& a, hipStream_t st) {
+    if (a.n == 0) return 0;
+    constexpr int NW = GLU ? 4 : 16;
+    const dim3 grid((uint32_t)ceil_div(a.n, 16));
+    const bool al = a.k % 8 == 0 && a.ldx % 8 == 0 && a.ldw % 8 == 0 && aligned(a.x, 16) && aligned(a.w0, 16) &&
+                    aligned(a.w1, 16);
+#define SKINNY(NB)                                                                                              \
+    do {                                                                                                        \
+        if (al) hipLaunchKernelGGL((ffn_skinny<T, GLU, NB, NW, true>), grid, dim3(64 * NW), 0, st, a);          \
+        else hipLaunchKernelGGL((ffn_skinny<T, GLU, NB, NW, false>), grid, dim3(64 * NW), 0, st, a);            \
+    } while (0)
+    if (a.rows <= 16) SKINNY(1);
+    else if (a.rows <= 32) SKINNY(2);
+    else SKINNY(4);
+#undef SKINNY
+    return launched(op);
+}
+
+// the partial sums' bytes of a product, whichever way its operands' alignment has it go
+size_t part_of(int64_t m, int64_t n, int64_t k, int segments, int pairs) {
+    const size_t a = shape_of(m, n, k, segments, pairs, false, true, true).part_bytes;
+    const size_t b = shape_of(m, n, k, segments, pairs, false, true, false).part_bytes;
+    return a > b ? a : b;
+}
+
+size_t workspace(const fhc_ffn_desc* d, bool backward) {
+    if (!backward) {  // h, where nothing is kept, and the second product's partial sums
+        return hidden_bytes(d) + part_of(d->rows, d->c, d->f, 1, 1);
+    }
+    size_t part = 0;
+    for (const size_t n : {part_of(d->rows, d->c, d->f, 2, 1), part_of(d->f, d->c, d->rows, 1, 2),
+                           part_of(d->f, d->c, d->rows, 1, 1), part_of(d->c, d->f, d->rows, 1, 1)})
+        part = n > part ? n : part;
+    return 2 * hidden_bytes(d) + part;
+}
+
+template <class T>
+int forward(const char* op, const fhc_ffn_desc* d, const fhc_rows* x, const void* wg, const void* wu, const void* wd,
+            const fhc_rows* y, void* saved, void* ws, hipStream_t st) {
+    const int64_t fp = padded(d->f);
+    char* keep = static_cast<char*>(saved);
+    char* w = static_cast<char*>(ws);
+    uint16_t* h = reinterpret_cast<uint16_t*>(saved ? keep : w);
+    auto u16 = [](const void* p) { return static_cast<const uint16_t*>(p); };
+    if (!saved && d->rows <= kSkinnyRows) {
+        SkinnyArgs a{u16(x->p), u16(wg), u16(wu), x->ld, (int64_t)d->c, (int)d->rows, (int)d->f, (int)d->c, h, fp, d->act};
+        FHC_TRY((skinny<T, true>(op, a, st)));
+        SkinnyArgs b{h, u16(wd), nullptr, fp, (int64_t)d->f, (int)d->rows, (int)d->c, (int)d->f,
+                     static_cast<uint16_t*>(y->p), y->ld, d->act};
+        return skinny<T, false>(op, b, st);
+    }
+    GemmArgs g{};
+    g.a0 = u16(x->p), g.b0 = u16(wg), g.b1 = u16(wu), g.lda = x->ld, g.ldb = d->c;
+    g.m = d->rows, g.n = d->f, g.k = d->c, g.o0 = h, g.ldo = fp, g.ldpre = fp, g.act = d->act;
+    if (saved) {
+        g.pre_g = reinterpret_cast<float*>(keep + hidden_bytes(d));
+        g.pre_u = reinterpret_cast<float*>(keep + hidden_bytes(d) + pre_bytes(d));
+    }
+    FHC_TRY((product<T, false, false, kGlu>(op, g, nullptr, st)));
+    GemmArgs p{};
+    p.a0 = h, p.b0 = u16(wd), p.lda = fp, p.ldb = d->f, p.m = d->rows, p.n = d->c, p.k = d->f;
+    p.o0 = static_cast<uint16_t*>(y->p), p.ldo = y->ld;
+    return product<T, false, false, kStore>(op, p, reinterpret_cast<float*>(w + hidden_bytes(d)), st);
+}
+
+template <class T>
+int backward(const char* op, const fhc_ffn_desc* d, const fhc_rows* x, const void* wg, const void* wu, const void* wd,
+             const void* saved, const fhc_rows* dy, const fhc_rows* dx, void* dwg, void* dwu, void* dwd, void* ws,
+             hipStream_t st) {
+    const int64_t fp = padded(d->f);
+    char* keep = const_cast<char*>(static_cast<const char*>(saved));
+    char* w = static_cast<char*>(ws);
+    auto u16 = [](const void* p) { return static_cast<const uint16_t*>(p); };
+    auto out = [](void* p) { return static_cast<uint16_t*>(p); };
+    uint16_t *dg = out(w), *du = out(w + hidden_bytes(d));
+    float* part = reinterpret_cast<float*>(w + 2 * hidden_bytes(d));
+    if (dx || dwg || dwu) {
+        GemmArgs g{};
+        g.a0 = u16(dy->p), g.b0 = u16(wd), g.lda = dy->ld, g.ldb = d->f, g.m = d->rows, g.n = d->f, g.k = d->c;
+        g.o0 = dg, g.o1 = du, g.ldo = fp, g.ldpre = fp, g.act = d->act;
+        g.pre_g = reinterpret_cast<float*>(keep + hidden_bytes(d));
+        g.pre_u = reinterpret_cast<float*>(keep + hidden_bytes(d) + pre_bytes(d));
+        FHC_TRY((product<T, false, true, kGrad>(op, g, nullptr, st)));
+    }
+    if (dx) {
+        GemmArgs g{};
+        g.a0 = dg, g.a1 = du, g.b0 = u16(wg), g.b1 = u16(wu), g.lda = fp, g.ldb = d->c, g.segments = 2;
+        g.m = d->rows, g.n = d->c, g.k = d->f, g.o0 = out(dx->p), g.ldo = dx->ld;
+        FHC_TRY((product<T, false, true, kStore>(op, g, part, st)));
+    }
+    if (dwg || dwu) {
+        GemmArgs g{};
+        g.a0 = dwg ? dg : du, g.a1 = du, g.b0 = u16(x->p), g.lda = fp, g.ldb = x->ld, g.pairs = dwg && dwu ? 2 : 1;
+        g.m = d->f, g.n = d->c, g.k = d->rows, g.o0 = out(dwg ? dwg : dwu), g.o1 = out(dwu), g.ldo = d->c;
+        FHC_TRY((product<T, true, true, kStore>(op, g, part, st)));
+    }
+    if (dwd) {
+        GemmArgs g{};
+        g.a0 = u16(dy->p), g.b0 = reinterpret_cast<const uint16_t*>(keep), g.lda = dy->ld, g.ldb = fp;
+        g.m = d->c, g.n = d->f, g.k = d->rows, g.o0 = out(dwd), g.ldo = d->f;
+        FHC_TRY((product<T, true, true, kStore>(op, g, part, st)));
+    }
+    return 0;
+}
+
+}  // namespace
+}  // namespace seq
+}  // namespace fhc
+
+using namespace fhc;
+using namespace fhc::seq;
+
+extern "C" size_t fhc_ffn_saved_bytes(const fhc_ffn_desc* d) {
+    return guard((size_t)0, [&]() -> size_t {
+        clear_error();
+        if (check_desc("ffn_saved_bytes", d) < 0) return 0;
+        return hidden_bytes(d) + 2 * pre_bytes(d);
+    });
+}
+
+extern "C" size_t fhc_ffn_workspace_bytes(const fhc_ffn_desc* d, int back) {
+    return guard((size_t)0, [&]() -> size_t {
+        clear_error();
+        if (check_desc("ffn_workspace_bytes", d) < 0) return 0;
+        return workspace(d, back != 0);
+    });
+}
+
+extern "C" int fhc_ffn_forward(const fhc_ffn_desc* d, const fhc_rows* x, const void* wg, const void* wu,
+                               const void* wd, const fhc_rows* y, void* saved, void* ws, size_t ws_bytes,
+                               void* stream) {
+    return guard(-3, [&]() -> int {
+        clear_error();
+        const char* op = "ffn_forward";
+        FHC_TRY(check_desc(op, d));
+        if (d->rows == 0 || d->c == 0) return 0;
+        FHC_TRY(check_rows(op, "x", x, d->c));
+        FHC_TRY(check_rows(op, "y", y, d->c));
+        if (d->f) {
+            FHC_TRY(check_weight(op, "wg", wg));
+            FHC_TRY(check_weight(op, "wu", wu));
+            FHC_TRY(check_weight(op, "wd", wd));
+        }
+        if (saved && !aligned(saved, 256)) return fail(-1, "%s: saved is not 256-byte aligned", op);
+        FHC_TRY(check_workspace(op, workspace(d, false), ws, ws_bytes));
+        const hipStream_t st = (hipStream_t)stream;
+        return d->dtype == FHC_F16 ? forward<F16>(op, d, x, wg, wu, wd, y, saved, ws, st)
+                                   : forward<BF16>(op, d, x, wg, wu, wd, y, saved, ws, st);
+    });
+}
+
+extern "C" int fhc_ffn_backward(const fhc_ffn_desc* d, const fhc_rows* x, const void* wg, const void* wu,
+                                const void* wd, const void* saved, const fhc_rows* dy, const fhc_rows* dx, void* dwg,
+                                void* dwu, void* dwd, void* ws, size_t ws_bytes, void* stream) {
+    return guard(-3, [&]() -> int {
+        clear_error();
+        const char* op = "ffn_backward";
+        FHC_TRY(check_desc(op, d));
+        if (d->c == 0) return 0;
+        if (d->rows) {
+            FHC_TRY(check_rows(op, "x", x, d->c));
+            FHC_TRY(check_rows(op, "dy", dy, d->c));
+            if (dx) FHC_TRY(check_rows(op, "dx", dx, d->c));
+            if (d->f) {
+                FHC_TRY(check_weight(op, "wg", wg));
+                FHC_TRY(check_weight(op, "wu", wu));
+                FHC_TRY(check_weight(op, "wd", wd));
+                if (!saved) return fail(-1, "%s: null saved", op);
+                if (!aligned(saved, 256)) return fail(-1, "%s: saved is not 256-byte aligned", op);
+            }
+        }
+        if (!aligned(dwg, 2) || !aligned(dwu, 2) || !aligned(dwd, 2))
+            return fail(-1, "%s: a weight's gradient is not aligned to its elements", op);
+        FHC_TRY(check_workspace(op, workspace(d, true), ws, ws_bytes));
+        const hipStream_t st = (hipStream_t)stream;
+        return d->dtype == FHC_F16 ? backward<F16>(op, d, x, wg, wu, wd, saved, dy, dx, dwg, dwu, dwd, ws, st)
+                                   : backward<BF16>(op, d, x, wg, wu, wd, saved, dy, dx, dwg, dwu, dwd, ws, st);
+    });
+}

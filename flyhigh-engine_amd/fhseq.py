@@ -1,9 +1,9 @@
 """Python host driver of the operators on rows of channels (ctypes over include/fhc_seq.h in libfhconv.so): a gated
-linear recurrence (``glr``), the norms around a block with its gate and the scaled residual (``norm_block``), each
-with its backward pass.
+linear recurrence (``glr``), the norms around a block with its gate and the scaled residual (``norm_block``) and a
+gated feed-forward block (``ffn``), each with its backward pass.
 
-Inputs are torch tensors on the current GPU in f16, bf16 or f32, all of one call in the same type; states and the
-gradients of weights are f32. Each function returns new tensors. ``stream`` (a torch stream) is where the call runs,
+Inputs are torch tensors on the current GPU in f16, bf16 or (not ``ffn``) f32, all of one call in the same type; states
+and the gradients of the recurrence's and norms' weights are f32. Each function returns new tensors. ``stream`` (a torch stream) is where the call runs,
 the current stream if None; what it allocates belongs to that stream. The module only passes device pointers: when the
 library is missing, loading it raises, and nothing is computed on the host.
 """
@@ -37,6 +37,10 @@ class FhcRows(ctypes.Structure):
     _fields_ = [("p", _P), ("ld", _I64)]
 
 
+class FfnDesc(ctypes.Structure):
+    _fields_ = [("dtype", _U), ("act", _U), ("rows", _U), ("c", _U), ("f", _U)]
+
+
 _typed = None
 
 
@@ -44,7 +48,7 @@ def _lib():
     global _typed
     if _typed is None:
         L = fhconv.load()
-        G, S, N, R = (ctypes.POINTER(t) for t in (GlrDesc, FhcSeq, NormDesc, FhcRows))
+        G, S, N, R, D = (ctypes.POINTER(t) for t in (GlrDesc, FhcSeq, NormDesc, FhcRows, FfnDesc))
         sig = {
             "fhc_glr_states_bytes": ([G], _SZ),
             "fhc_glr_workspace_bytes": ([G, ctypes.c_int], _SZ),
@@ -53,6 +57,10 @@ def _lib():
             "fhc_norm_block": ([N, R, R, R, R, _P], ctypes.c_int),
             "fhc_norm_block_workspace_bytes": ([N], _SZ),
             "fhc_norm_block_backward": ([N, R, R, R, R, R, R, _P, _P, _P, _P, _SZ, _P], ctypes.c_int),
+            "fhc_ffn_saved_bytes": ([D], _SZ),
+            "fhc_ffn_workspace_bytes": ([D, ctypes.c_int], _SZ),
+            "fhc_ffn_forward": ([D, R, _P, _P, _P, R, _P, _P, _SZ, _P], ctypes.c_int),
+            "fhc_ffn_backward": ([D, R, _P, _P, _P, _P, R, R, _P, _P, _P, _P, _SZ, _P], ctypes.c_int),
         }
         for name, (args, res) in sig.items():
             f = getattr(L, name)
@@ -233,3 +241,51 @@ def norm_block_backward(x, o, w_post, gate, w_pre, dy, du, alpha=1.0, eps=1e-6, 
                                            _rows(op, "du", du), _rows(op, "dx", dx), _rows(op, "do", do),
                                            _ptr(dw_post), _ptr(dgate), _ptr(dw_pre), _ptr(ws), size, _handle(stream)))
     return dx, do, dw_post, dgate, dw_pre
+
+
+ACTS = {"silu": 0, "gelu": 1}
+
+
+def _ffn_desc(name, x, wg, wu, wd, act):
+    if x.dim() != 2 or wg.dim() != 2:
+        raise FhcError(f"{name}: x is [rows, channels] and wg [features, channels], got {tuple(x.shape)}, "
+                       f"{tuple(wg.shape)}")
+    if act not in ACTS:
+        raise FhcError(f"{name}: act {act!r} is none of {', '.join(ACTS)}")
+    rows, c = x.shape
+    f = wg.shape[0]
+    dtype = _dtype(x)
+    _same(name, x, wg=(wg, (f, c), x.dtype), wu=(wu, (f, c), x.dtype), wd=(wd, (c, f), x.dtype))
+    _dense(name, wg=wg, wu=wu, wd=wd)
+    return FfnDesc(dtype, ACTS[act], rows, c, f)
+
+
+def ffn(x, wg, wu, wd, act="silu", train=False, stream=None):
+    """(act(x wg^T) * (x wu^T)) wd^T of rows x [rows, c] with wg, wu [f, c] and wd [c, f], act "silu" or "gelu" (tanh
+    form), in f16 or bf16. With train: (y, what ``ffn_backward`` takes)."""
+    L, op = _lib(), "ffn"
+    d = _ffn_desc(op, x, wg, wu, wd, act)
+    with _on(stream):
+        y = x.new_empty(x.shape)
+        saved = _bytes(x, L.fhc_ffn_saved_bytes(d)) if train else None
+        n = L.fhc_ffn_workspace_bytes(d, 0)
+        ws = _bytes(x, n)
+        _run(op, L.fhc_ffn_forward(d, _rows(op, "x", x), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(),
+                                   _rows(op, "y", y), _ptr(saved), _ptr(ws), n, _handle(stream)))
+    return (y, saved) if train else y
+
+
+def ffn_backward(x, wg, wu, wd, saved, dy, act="silu", stream=None):
+    """(dx, dwg, dwu, dwd), in the inputs' type, for dy; ``saved`` from the training ``ffn`` call of the same inputs."""
+    L, torch, op = _lib(), _torch(), "ffn_backward"
+    d = _ffn_desc(op, x, wg, wu, wd, act)
+    size = L.fhc_ffn_saved_bytes(d)
+    _same(op, x, dy=(dy, x.shape, x.dtype), saved=(saved, (size,), torch.uint8) if size else (None, (), None))
+    with _on(stream):
+        dx, dwg, dwu, dwd = (t.new_empty(t.shape) for t in (x, wg, wu, wd))
+        n = L.fhc_ffn_workspace_bytes(d, 1)
+        ws = _bytes(x, n)
+        _run(op, L.fhc_ffn_backward(d, _rows(op, "x", x), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), _ptr(saved),
+                                    _rows(op, "dy", dy), _rows(op, "dx", dx), dwg.data_ptr(), dwu.data_ptr(),
+                                    dwd.data_ptr(), _ptr(ws), n, _handle(stream)))
+    return dx, dwg, dwu, dwd

@@ -96,6 +96,34 @@ int fhc_norm_block_backward(const fhc_norm_desc* n, const fhc_rows* x, const fhc
                             const fhc_rows* du, const fhc_rows* dx, const fhc_rows* dout, float* dw_post, float* dgate,
                             float* dw_pre, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- The gated feed-forward block on rows of c channels, f wide inside:
+ *     y = h wd^T,   h = act(x wg^T) * (x wu^T)      act: silu, v sigmoid(v), or gelu in its tanh form
+ * wg, wu are dense [f][c], wd dense [c][f], in dtype (f16 or bf16). The products accumulate in f32; h, and in the
+ * backward pass dL/d(x wg^T) and dL/d(x wu^T), are rounded to dtype once, since they are the next products' operands
+ * (the matrix units take 16 bits). A training forward keeps x wg^T and x wu^T in f32, so no gradient is taken at a
+ * rounded value. f16: the caller scales the loss so that these stay in f16's range. */
+#define FHC_ACT_SILU 0u
+#define FHC_ACT_GELU 1u
+
+typedef struct fhc_ffn_desc {
+    uint32_t dtype; /* FHC_F16 or FHC_BF16 */
+    uint32_t act;   /* FHC_ACT_SILU, FHC_ACT_GELU */
+    uint32_t rows, c, f; /* c, f <= 2^20 */
+} fhc_ffn_desc;
+
+/* Bytes of what a training forward keeps for the backward pass, and of the workspace of either call. */
+size_t fhc_ffn_saved_bytes(const fhc_ffn_desc* d);
+size_t fhc_ffn_workspace_bytes(const fhc_ffn_desc* d, int backward);
+
+/* saved: NULL, or a 256-byte aligned buffer that the backward pass of the same descriptor takes. */
+int fhc_ffn_forward(const fhc_ffn_desc* d, const fhc_rows* x, const void* wg, const void* wu, const void* wd,
+                    const fhc_rows* y, void* saved, void* ws, size_t ws_bytes, void* stream);
+
+/* dx and the weights' gradients (dense, in dtype) for dy; those that are not wanted may be NULL. */
+int fhc_ffn_backward(const fhc_ffn_desc* d, const fhc_rows* x, const void* wg, const void* wu, const void* wd,
+                     const void* saved, const fhc_rows* dy, const fhc_rows* dx, void* dwg, void* dwu, void* dwd,
+                     void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -123,3 +123,47 @@ def norm_block(x, o, w_post, gate, w_pre, alpha, eps, rpg, dy=None, du=None):
             (ga.abs() * (eq + s * q.abs())).sum(0), wp.abs() * per(eq + s * q.abs()),
             (du.abs() * (eny + s * ny.abs())).sum(0)]
     return res, err
+
+
+def _act(v, act):
+    """act(v) and its derivative."""
+    if act == "silu":
+        p = torch.sigmoid(v)
+        return v * p, p * (1 + v * (1 - p))
+    s, b = (2 / torch.pi) ** 0.5, 0.044715
+    th = torch.tanh(s * (v + b * v ** 3))
+    return 0.5 * v * (1 + th), 0.5 * (1 + th) + 0.5 * v * (1 - th * th) * s * (1 + 3 * b * v * v)
+
+
+def ffn(x, wg, wu, wd, act, dy=None):
+    """(results, bounds): y, and with dy also dx, dwg, dwu, dwd. h and the gradients at the two projections are rounded
+    to the inputs' type on the way, so half a step of each is in the bounds."""
+    hs, tiny = half_step(x.dtype), torch.finfo(x.dtype).tiny * torch.finfo(x.dtype).eps / 2
+    x, wg, wu, wd = (v.double() for v in (x, wg, wu, wd))
+    rows, c = x.shape
+    f = wg.shape[0]
+    chain = lambda k: (k / 32 + 34) * U  # noqa: E731  (32 products a matrix instruction, then one sum after the other)
+    g, u = x @ wg.t(), x @ wu.t()
+    eg, eu = (chain(c) * (x.abs() @ w.abs().t()) for w in (wg, wu))
+    a, da = _act(g, act)
+    ea = 1.2 * eg + 64 * U * a.abs()  # |act'| < 1.13; the exponent's argument is rounded, |k(v)| at most 60 where it counts
+    h = a * u
+    eh = ea * u.abs() + a.abs() * eu + 2 * U * h.abs()
+    ehr = eh + hs * (h.abs() + eh) + tiny
+    y, ey = h @ wd.t(), ehr @ wd.abs().t() + chain(f) * (h.abs() @ wd.abs().t())
+    if dy is None:
+        return [y], [ey]
+    dy = dy.double()
+    dh, edh = dy @ wd, chain(c) * (dy.abs() @ wd.abs())
+    eda = 1.2 * eg + 64 * U * (da.abs() + 1)  # |act''| < 1
+    dg, du = dh * u * da, dh * a
+    edg = edh * (u * da).abs() + dh.abs() * (eu * da.abs() + u.abs() * eda) + 4 * U * dg.abs()
+    edu = edh * a.abs() + dh.abs() * ea + 2 * U * du.abs()
+    edg, edu = edg + hs * (dg.abs() + edg) + tiny, edu + hs * (du.abs() + edu) + tiny
+    dx = dg @ wg + du @ wu
+    edx = edg @ wg.abs() + edu @ wu.abs() + chain(2 * f) * (dg.abs() @ wg.abs() + du.abs() @ wu.abs())
+    res, err = [y, dx], [ey, edx]
+    for p, ep in ((dg, edg), (du, edu)):
+        res.append(p.t() @ x), err.append(ep.t() @ x.abs() + chain(rows) * (p.abs().t() @ x.abs()))
+    res.append(dy.t() @ h), err.append(dy.abs().t() @ ehr + chain(rows) * (dy.abs().t() @ h.abs()))
+    return res, err

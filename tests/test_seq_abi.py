@@ -117,6 +117,46 @@ def test_norm_block_nothing_to_do_is_fine():
     assert norm_call(False, rows=0) == 0 and norm_call(False, c=0) == 0 and norm_call(True, c=0) == 0
 
 
+def ffn_call(back, **kw):
+    m = mod()
+    L = m._lib()
+    a = dict(dtype=1, act=0, rows=100, c=16, f=24)
+    r = {k: (P, 16) for k in ("x", "y", "dy", "dx")}
+    w = dict(wg=P, wu=P, wd=P, saved=P, dwg=P, dwu=P, dwd=P, ws=P, ws_bytes=1 << 40)
+    for d in (a, r, w):
+        d.update({k: v for k, v in kw.items() if k in d})
+    d = None if kw.get("desc", 1) is None else ctypes.byref(m.FfnDesc(*a.values()))
+    r = {k: None if v is None else ctypes.byref(m.FhcRows(*v)) for k, v in r.items()}
+    if back:
+        return L.fhc_ffn_backward(d, r["x"], w["wg"], w["wu"], w["wd"], w["saved"], r["dy"], r["dx"], w["dwg"],
+                                  w["dwu"], w["dwd"], w["ws"], w["ws_bytes"], None)
+    return L.fhc_ffn_forward(d, r["x"], w["wg"], w["wu"], w["wd"], r["y"], w["saved"], w["ws"], w["ws_bytes"], None)
+
+
+@pytest.mark.parametrize("bad,text", [
+    (dict(desc=None), "null descriptor"), (dict(dtype=2), "neither f16 nor bf16"), (dict(act=2), "act 2"),
+    (dict(c=(1 << 20) + 1), "channels"), (dict(rows=0x7FFFFF01), "rows"), (dict(x=None), "null x"),
+    (dict(y=(None, 16)), "null pointer of y"), (dict(y=(P, 15)), "apart"), (dict(x=(P + 1, 16)), "not aligned"),
+    (dict(wu=None), "null wu"), (dict(wd=P + 1), "not aligned"), (dict(saved=P + 16), "saved is not"),
+    (dict(ws=None), "null workspace"), (dict(ws_bytes=16), "workspace of 16"), (dict(ws=P + 128), "256-byte"),
+])
+def test_ffn_forward_refuses(bad, text):
+    refused(ffn_call(False, **bad), text)
+
+
+@pytest.mark.parametrize("bad,text", [
+    (dict(dy=None), "null dy"), (dict(saved=None), "null saved"), (dict(saved=P + 8), "saved is not"),
+    (dict(dx=(P, 3)), "apart"), (dict(wg=None), "null wg"), (dict(dwu=P + 1), "not aligned"),
+    (dict(ws=None), "null workspace"), (dict(ws_bytes=16), "workspace of 16"), (dict(dtype=7), "neither"),
+])
+def test_ffn_backward_refuses(bad, text):
+    refused(ffn_call(True, **bad), text)
+
+
+def test_ffn_nothing_to_do_is_fine():
+    assert ffn_call(False, rows=0) == 0 and ffn_call(False, c=0) == 0 and ffn_call(True, c=0) == 0
+
+
 def test_tensors_are_checked_before_the_call():
     import torch
     m = mod()

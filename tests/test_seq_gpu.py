@@ -359,3 +359,176 @@ def test_norm_block_in_a_graph():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), k
         call()
+
+
+# ---- the gated feed-forward block -------------------------------------------------------------------------------
+
+FFN = [  # rows, c, f: few rows (each width of the streaming product) and tiles; widths odd, even, cut in a group of 8
+    (1, 1, 1), (1, 64, 128), (3, 40, 72), (16, 128, 100), (17, 96, 130), (33, 256, 512), (64, 130, 62), (65, 64, 64),
+    (128, 128, 128), (130, 257, 129), (200, 100, 300), (257, 72, 514), (1000, 128, 512), (300, 512, 1030),
+    (700, 33, 65), (5000, 64, 96), (4100, 512, 1024), (2049, 1024, 2050),
+]
+
+
+def ffn_inputs(q, rows, c, f, dtype):
+    return dict(x=q.normal(rows, c, dtype=dtype), wg=q.normal(f, c, scale=c ** -0.5, dtype=dtype),
+                wu=q.normal(f, c, scale=c ** -0.5, dtype=dtype), wd=q.normal(c, f, scale=f ** -0.5, dtype=dtype),
+                dy=q.normal(rows, c, dtype=dtype))
+
+
+FFN_OUT = ("y", "dx", "dwg", "dwu", "dwd")
+
+
+def ffn_check(v, act):
+    m = mod()
+    w = [v[k] for k in ("x", "wg", "wu", "wd")]
+    serve = m.ffn(*w, act)
+    y, saved = m.ffn(*w, act, train=True)
+    got = (y,) + m.ffn_backward(*w, saved, v["dy"], act)
+    ref, err = seqref.ffn(*w, act, v["dy"])
+    seqref.close(serve, ref[0], err[0], "y without states kept")
+    for name, g, want, tol in zip(FFN_OUT, got, ref, err):
+        seqref.close(g, want, tol, name)
+    return got
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("shape", FFN, ids=str)
+def test_ffn(shape, dtype):
+    say("ffn", shape, dtype)
+    ffn_check(ffn_inputs(Rand(sum(shape)), *shape, types()[dtype]), "silu" if shape[0] % 2 else "gelu")
+
+
+def test_ffn_what_lies_beside_a_row_is_not_read():
+    """Row views whose neighbours are NaN, widths cut inside a group of 8, outputs in wider buffers."""
+    say("ffn views")
+    import ctypes
+    import torch
+    m = mod()
+    for rows, c, f, off in ((40, 36, 44, 8), (40, 36, 44, 1), (150, 36, 44, 2), (150, 35, 43, 3), (300, 100, 92, 4)):
+        v = ffn_inputs(Rand(rows + off), rows, c, f, torch.bfloat16)
+        want = m.ffn(v["x"], v["wg"], v["wu"], v["wd"])
+        y, saved = m.ffn(v["x"], v["wg"], v["wu"], v["wd"], train=True)
+        grads = m.ffn_backward(v["x"], v["wg"], v["wu"], v["wd"], saved, v["dy"])
+        wide = {k: torch.full((rows, c + 20), math.nan, dtype=torch.bfloat16, device="cuda") for k in ("x", "dy")}
+        views = {k: b[:, off:off + c] for k, b in wide.items()}
+        for k, b in views.items():
+            b.copy_(v[k])
+        # weights with NaN right behind them
+        pool = {k: torch.full((v[k].numel() + 64,), math.nan, dtype=torch.bfloat16, device="cuda")
+                for k in ("wg", "wu", "wd")}
+        w = []
+        for k, b in pool.items():
+            b[:v[k].numel()] = v[k].flatten()
+            w.append(b[:v[k].numel()].view(v[k].shape))
+        assert torch.equal(m.ffn(views["x"], *w), want)
+        y2, saved2 = m.ffn(views["x"], *w, train=True)
+        assert torch.equal(y2, y)
+        got = m.ffn_backward(views["x"], *w, saved2, views["dy"])
+        for name, a, b in zip(FFN_OUT[1:], got, grads):
+            assert torch.equal(a, b), (rows, c, f, off, name)
+        out = torch.full((rows, c + 20), 7.0, dtype=torch.bfloat16, device="cuda")
+        d = m.FfnDesc(1, 0, rows, c, f)
+        L = m._lib()
+        n = L.fhc_ffn_workspace_bytes(ctypes.byref(d), 0)
+        ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+        o = out[:, off:off + c]
+        assert L.fhc_ffn_forward(ctypes.byref(d), m._rows("", "", views["x"]), w[0].data_ptr(), w[1].data_ptr(),
+                                 w[2].data_ptr(), m._rows("", "", o), None, ws.data_ptr(), n,
+                                 torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(o, want) and (out[:, :off] == 7).all() and (out[:, off + c:] == 7).all()
+
+
+def test_ffn_empty_sides():
+    say("ffn empty")
+    import torch
+    m = mod()
+    for rows, c, f in ((0, 8, 16), (5, 8, 0), (200, 8, 0), (0, 8, 0)):
+        v = ffn_inputs(Rand(1), rows, max(c, 1), max(f, 1), torch.float16)
+        w = [v["wg"][:f].contiguous(), v["wu"][:f].contiguous(), v["wd"][:, :f].contiguous()]
+        y, saved = m.ffn(v["x"], *w, train=True)
+        grads = m.ffn_backward(v["x"], *w, saved, v["dy"])
+        torch.cuda.synchronize()
+        assert y.shape == (rows, c) and not y.any() and not any(g.any() for g in grads)
+
+
+def test_ffn_values_that_are_not_finite_stay_in_their_rows():
+    say("ffn not finite")
+    import torch
+    m = mod()
+    for rows in (20, 300):
+        v = ffn_inputs(Rand(3), rows, 72, 136, torch.bfloat16)
+        clean = m.ffn(v["x"], v["wg"], v["wu"], v["wd"])
+        v["x"][7, 3], v["x"][11, 70] = math.nan, math.inf
+        got = m.ffn(v["x"], v["wg"], v["wu"], v["wd"])
+        assert not torch.isfinite(got[7]).any() and not torch.isfinite(got[11]).all()
+        keep = [r for r in range(rows) if r not in (7, 11)]
+        assert torch.equal(got[keep], clean[keep])
+
+
+def test_ffn_activation_at_its_ends():
+    """Pre-activations far outside exp's range: act is 0 on one side and the identity on the other."""
+    say("ffn ends")
+    import torch
+    m = mod()
+    for act in ("silu", "gelu"):
+        x = torch.tensor([[1.0], [-1.0]], dtype=torch.bfloat16, device="cuda").repeat(70, 1)
+        wg = torch.tensor([[300.0], [2.0 ** 30]], dtype=torch.bfloat16, device="cuda")
+        one = torch.ones_like(wg)
+        y, saved = m.ffn(x, wg, one, one.t().contiguous(), act, train=True)
+        grads = m.ffn_backward(x, wg, one, one.t().contiguous(), saved, torch.ones_like(x), act)
+        assert torch.equal(y[0], (wg.float().sum()).to(torch.bfloat16)[None]) and not y[1].any()
+        assert all(torch.isfinite(g).all() for g in grads)
+
+
+def test_ffn_gradient_against_differences():
+    say("ffn differences")
+    import torch
+    q = Rand(14)
+    for act in ("silu", "gelu"):
+        v = ffn_inputs(q, 90, 40, 56, torch.float16)
+        got = dict(zip(("x", "wg", "wu", "wd"), ffn_check(v, act)[1:]))
+
+        def loss(**change):
+            w = [v[k].double() + change.get(k, 0) for k in ("x", "wg", "wu", "wd")]
+            h = seqref._act(w[0] @ w[1].t(), act)[0] * (w[0] @ w[2].t())
+            return float(((h @ w[3].t()) * v["dy"].double()).sum())
+
+        for k, grad in got.items():
+            d = q.normal(*v[k].shape).double()
+            s = 1e-5
+            slope = (loss(**{k: s * d}) - loss(**{k: -s * d})) / (2 * s)
+            want = float((grad.double() * d).sum())
+            # f16 gradients: two roundings each
+            assert abs(slope - want) <= 2 ** -10 * float((grad.double() * d).abs().sum()), (act, k, slope, want)
+
+
+@pytest.mark.parametrize("shape", [(8, 128, 256), (300, 128, 256)], ids=str)
+def test_ffn_in_a_graph_and_on_another_stream(shape):
+    say("ffn graph", shape)
+    import torch
+    m = mod()
+    v = ffn_inputs(Rand(15), *shape, torch.bfloat16)
+    w = [v[k] for k in ("x", "wg", "wu", "wd")]
+
+    def call(stream=None):
+        serve = m.ffn(*w, stream=stream)
+        y, saved = m.ffn(*w, train=True, stream=stream)
+        return (serve, y) + m.ffn_backward(*w, saved, v["dy"], stream=stream)
+
+    want = [k.clone() for k in call()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    other = call(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(other, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for k in range(4):
+        for o in out:
+            o.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+        call()
