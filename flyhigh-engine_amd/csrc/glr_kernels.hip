@@ -13,8 +13,8 @@
 //            the chip). Chunks form runs of kRun; the state that reaches a chunk is the one at the head of its run
 //            folded through the maps of the run's chunks before it, and the run's last chunk publishes the next head:
 //            a step of the serial chain is a run long, not a chunk.
-// In the chain, chunks are taken in order by a ticket, so every chunk waited for is held by a workgroup that already
-// runs and itself waits for earlier tickets only: every wait ends. What is published is one 8-byte word (A, S), or
+// In the chain, the chunks of a column block are taken in order by its ticket, so every chunk waited for is held by a
+// workgroup that already runs and itself waits for earlier tickets only: every wait ends. What is published is one 8-byte word (A, S), or
 // (0, state), written once and read by atomic accesses of the whole word, so no fence orders anything; its A is -1
 // until then (decays are >= 0). Only the first chunk reads the initial state (it publishes it as the first head), so
 // the last one may write the final state over it.
@@ -24,9 +24,36 @@ namespace fhc {
 namespace seq {
 namespace {
 
-struct Col {  // a sequence tensor in elements
+struct Col {  // a sequence tensor, strides in bytes
     char* p;
     int64_t bs, ts;
+};
+// A wave's view of it: the step t of its first lane at p + t * ts, the same for all lanes, and a lane's own 32-bit
+// offset from there (no vector arithmetic for an address).
+struct Wave {
+    char* p;
+    int64_t ts;
+    uint32_t lane;
+    __device__ __forceinline__ Wave(const Col& c, uint32_t b, uint32_t ch, uint32_t elem) : ts(c.ts) {
+        const uint32_t b0 = __builtin_amdgcn_readfirstlane(b), c0 = __builtin_amdgcn_readfirstlane(ch);
+        p = c.p + b0 * c.bs + (uint64_t)c0 * elem;
+        lane = (b - b0) * (uint32_t)c.bs + (ch - c0) * elem;
+    }
+    // the step's address is made scalar in so many words: the lane's offset is else folded into a vector product
+    __device__ __forceinline__ __attribute__((address_space(1))) char* row(uint32_t t) const {
+        const uint64_t at = reinterpret_cast<uint64_t>(p) + (uint64_t)((int64_t)t * ts);
+        const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)at);
+        const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
+        return (__attribute__((address_space(1))) char*)((uint64_t)hi << 32 | lo) + lane;
+    }
+    template <class C>
+    __device__ __forceinline__ C load(uint32_t t) const {
+        return __builtin_bit_cast(C, *(__attribute__((address_space(1))) const typename C::Mem*)row(t));
+    }
+    template <class C>
+    __device__ __forceinline__ void store(uint32_t t, C c) const {
+        *(__attribute__((address_space(1))) typename C::Mem*)row(t) = __builtin_bit_cast(typename C::Mem, c);
+    }
 };
 
 struct GlrArgs {
@@ -41,64 +68,135 @@ struct GlrArgs {
     float* part;      // dlam's partial sums, [part rows][d]
     uint64_t* agg;    // chain: published maps [chunk][b * d],
     uint64_t* heads;  // and the first states of the runs [run][b * d]
-    uint32_t* ticket;
-    uint32_t b, t, d, groups, cols;  // groups: column groups of a sequence; cols = b * groups
+    uint32_t* tickets;
+    uint32_t b, t, d, groups;  // groups: lanes that a sequence's channels take
     uint32_t nchunk, colblocks, nstates;
+    uint32_t spacing;  // log2 of the steps from one kept state to the next: the backward pass's chunk
     float rate;
 };
 
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
-// e^-v, at most 1e37: its reciprocal and the product with it stay normal, so sigmoid(v) -> 0 and 1 - sigmoid(v) -> 1
-// for the largest negative v (a NaN stays: fminf would drop it, the select keeps it)
-__device__ __forceinline__ float exp_neg(float v) {
-    const float e = __builtin_amdgcn_exp2f(v * -kLog2e);
-    return e > 1e37f ? 1e37f : e;
+// 1 - 2^(2z) for z <= 0, a2 = 2^(2z). Near 0 the difference cancels, so a polynomial there: (1 - 2^(2z)) / -z
+// interpolated at the 4 Chebyshev nodes of [-0.18, 0], off by 2.8e-7 of it, which is what the difference loses at the
+// border. A NaN z goes the second way and stays.
+__device__ __forceinline__ float one_minus_square(float z, float a) {
+    float p = __builtin_fmaf(0.1393723995578612f, z, 0.4424283742923703f);
+    p = __builtin_fmaf(p, z, 0.9608486733131862f);
+    p = __builtin_fmaf(p, z, 1.3862940389244018f);
+    return z > -0.18f ? -z * p : __builtin_fmaf(-a, a, 1.0f);
 }
 
-// 1 - e^z for z <= 0. Near 0 the difference cancels, so -expm1's series there: 8 terms at z > -1/2 leave 2^-24 of it
-__device__ __forceinline__ float one_minus_exp(float z, float ez) {
-    float p = 1.0f / 40320.0f;
-    p = __builtin_fmaf(p, z, 1.0f / 5040.0f);
-    p = __builtin_fmaf(p, z, 1.0f / 720.0f);
-    p = __builtin_fmaf(p, z, 1.0f / 120.0f);
-    p = __builtin_fmaf(p, z, 1.0f / 24.0f);
-    p = __builtin_fmaf(p, z, 1.0f / 6.0f);
-    p = __builtin_fmaf(p, z, 0.5f);
-    p = __builtin_fmaf(p, z, 1.0f);
-    return z > -0.5f ? -z * p : 1.0f - ez;
+// One step of one channel. Logits of -inf shut their gates: the exponential is inf, its reciprocal 0. A step that is not
+// there (past a length) is read as x = 0, r = i = -inf, which leaves the state as it is (a = 1, no input).
+struct Gates {
+    float er, ei, sr, si, z, a, v;  // e^-r, e^-i; the sigmoids; log2 a; a; 1 - a^2
+};
+// k2 = -rate * softplus(lam) * log2(e)
+__device__ __forceinline__ Gates gates_of(float k2, float r, float i) {
+    Gates g;
+    g.er = __builtin_amdgcn_exp2f(r * -kLog2e), g.ei = __builtin_amdgcn_exp2f(i * -kLog2e);
+    g.sr = __builtin_amdgcn_rcpf(1.0f + g.er), g.si = __builtin_amdgcn_rcpf(1.0f + g.ei);
+    g.z = k2 * g.sr;
+    g.a = __builtin_amdgcn_exp2f(g.z);
+    g.v = one_minus_square(g.z, g.a);
+    return g;
 }
+// 1 - sigmoid(u) = e^-u sigmoid(u), accurate where it is small; inf * 0 where e^-u overflows, and 1 then (a NaN u's is 1
+// too, but everything that it multiplies is NaN)
+__device__ __forceinline__ float shut(float e, float s) { return __builtin_fminf(e * s, 1.0f); }
 
-struct Step {  // one step of one channel
-    float a, sr, nr, si, ni, m, w, la, rm;  // nr, ni: 1 - sr, 1 - si; w = si * x; rm = 1 / m
+// The V channels of a lane as they lie in memory: a pair of 16-bit elements stays one register until it is used.
+template <class T, int V>
+struct Cell {
+    typedef typename T::Raw Mem __attribute__((ext_vector_type(V)));
+    typename T::Raw e[V];
+    static constexpr float kLow = -__builtin_inff();
+    __device__ __forceinline__ float at(int v) const { return widen(T{}, e[v]); }
+    static __device__ __forceinline__ Cell of(const float (&f)[V]) {
+        Cell c;
+#pragma unroll
+        for (int v = 0; v < V; v++) c.e[v] = narrow(T{}, f[v]);
+        return c;
+    }
+    __device__ __forceinline__ Cell where(bool on) const {
+        Cell c;
+#pragma unroll
+        for (int v = 0; v < V; v++) c.e[v] = on ? e[v] : typename T::Raw(0);
+        return c;
+    }
+    __device__ __forceinline__ void forget() {
+#pragma unroll
+        for (int v = 0; v < V; v++) asm volatile("" : "+v"(e[v]));
+    }
+    static __device__ __forceinline__ Cell zero() { return Cell{}; }
+    static __device__ __forceinline__ Cell lowest() {
+        float f[V];
+#pragma unroll
+        for (int v = 0; v < V; v++) f[v] = kLow;
+        return of(f);
+    }
+};
+template <class T>
+struct Pair {
+    using Mem = uint32_t;
+    uint32_t e;
+    __device__ __forceinline__ float at(int v) const { return widen(T{}, (uint16_t)(v ? e >> 16 : e)); }
+    static __device__ __forceinline__ Pair of(const float (&f)[2]) {
+        return {(uint32_t)narrow(T{}, f[0]) | (uint32_t)narrow(T{}, f[1]) << 16};
+    }
+    __device__ __forceinline__ Pair where(bool on) const { return {on ? e : 0u}; }
+    __device__ __forceinline__ void forget() { asm volatile("" : "+v"(e)); }
+    static __device__ __forceinline__ Pair zero() { return {0u}; }
+    static __device__ __forceinline__ Pair lowest() {
+        return {T::id == FHC_F16 ? 0xFC00FC00u : 0xFF80FF80u};
+    }
+};
+template <>
+struct Cell<F16, 2> : Pair<F16> {
+    __device__ Cell() = default;
+    __device__ __forceinline__ Cell(Pair<F16> p) : Pair<F16>(p) {}
+};
+template <>
+struct Cell<BF16, 2> : Pair<BF16> {
+    __device__ Cell() = default;
+    __device__ __forceinline__ Cell(Pair<BF16> p) : Pair<BF16>(p) {}
 };
 
-// k = -rate * softplus(lam)
-template <bool GRAD>
-__device__ __forceinline__ Step step_of(float k, float x, float r, float i) {
-    Step s;
-    const float er = exp_neg(r), ei = exp_neg(i);
-    s.sr = __builtin_amdgcn_rcpf(1.0f + er), s.si = __builtin_amdgcn_rcpf(1.0f + ei);
-    s.la = k * s.sr;
-    s.a = __builtin_amdgcn_exp2f(s.la * kLog2e);
-    const float v = one_minus_exp(2.0f * s.la, s.a * s.a);
-    s.w = s.si * x;
-    if constexpr (GRAD) {
-        s.nr = er * s.sr, s.ni = ei * s.si;
-        // v is 0 where nothing decays (a = 1): no input either, and the gradient through m is taken at its limit 0 (a
-        // subnormal v, which the instruction takes for 0, the same)
-        s.rm = v >= 1.17549435e-38f ? __builtin_amdgcn_rsqf(v) : 0.0f * v;
-        s.m = v * s.rm;
+// L steps from t0 on of the lane's channels, those at and past n as `absent`. Where no lane of the wave has such a
+// step, the loads stand without a branch.
+template <class C, int L>
+__device__ __forceinline__ void load_steps(const Wave& w, uint32_t t0, uint32_t n, bool full, C absent, C (&o)[L]) {
+    if (full) {
+#pragma unroll
+        for (int l = 0; l < L; l++) o[l] = w.load<C>(t0 + l);
     } else {
-        s.m = __builtin_amdgcn_sqrtf(v);
+#pragma unroll
+        for (int l = 0; l < L; l++) {
+            o[l] = absent;
+            if (t0 + l < n) o[l] = w.load<C>(t0 + l);
+        }
     }
-    return s;
 }
 
+// log2 of the decay of an open gate: -rate * softplus(lam) * log2(e), softplus = max(lam, 0) + log1p(e^-|lam|).
+// Short, since a lane may use it for few steps: e^-|lam| with its argument's rounding put back, and log1p(e) = 2 atanh(s),
+// s = e / (2 + e) <= 1/3, whose series' 7 terms leave 1.4e-8 of it.
 __device__ __forceinline__ float decay_rate(float rate, float lam) {
-    // softplus without overflow: max(lam, 0) + log1p(e^-|lam|)
-    const float sp = (lam > 0.0f ? lam : lam < 0.0f ? 0.0f : lam) + log1pf(expf(-fabsf(lam)));
-    return -rate * sp;
+    const float u = -__builtin_fabsf(lam), t = u * kLog2e;
+    const float lost = __builtin_fmaf(u, kLog2e, -t) + u * 1.92596299e-8f;  // log2(e) - kLog2e
+    float e = __builtin_amdgcn_exp2f(t);
+    e = e > 0.0f ? __builtin_fmaf(e * kLn2, lost, e) : lam == lam ? 0.0f : lam;  // of 0 and -inf: no correction
+    const float s = e * __builtin_amdgcn_rcpf(2.0f + e), q = s * s;
+    float p = __builtin_fmaf(q, 1.0f / 13.0f, 1.0f / 11.0f);
+    p = __builtin_fmaf(p, q, 1.0f / 9.0f);
+    p = __builtin_fmaf(p, q, 1.0f / 7.0f);
+    p = __builtin_fmaf(p, q, 1.0f / 5.0f);
+    p = __builtin_fmaf(p, q, 1.0f / 3.0f);
+    p = __builtin_fmaf(p, q, 1.0f);
+    const float sp = (lam > 0.0f ? lam : 0.0f) + 2.0f * s * p;
+    const float k = -rate * sp * kLog2e;
+    return k < -3.4e38f ? -3.4e38f : k;  // finite: times a shut gate's 0 it is 0
 }
 
 __device__ __forceinline__ uint64_t word_of(float a, float s) {
@@ -110,10 +208,12 @@ __device__ __forceinline__ void publish(uint64_t* p, float a, float s) {
 }
 constexpr uint32_t kRun = 16;  // chunks of a run
 
-__global__ __launch_bounds__(256) void glr_clear(uint64_t* agg, uint64_t n, uint32_t* ticket) {
+constexpr uint32_t kTicketStep = 32;  // a column block's ticket has 128 bytes of its own
+
+__global__ __launch_bounds__(256) void glr_clear(uint64_t* agg, uint64_t n, uint32_t* tickets, uint32_t colblocks) {
     const uint64_t k = (uint64_t)blockIdx.x * 256 + threadIdx.x;
     if (k < n) agg[k] = kUnpublished;
-    if (k == 0) *ticket = 0;
+    if (k < colblocks) tickets[k * kTicketStep] = 0;
 }
 
 // The chain's search: the state that reaches this lane's columns of a chunk, `k` chunks after the head of its run.
@@ -154,26 +254,33 @@ __device__ __forceinline__ void chain_find(uint32_t k, uint32_t tw, uint32_t slo
     }
 }
 
+// Which columns and chunk a workgroup has. Every column block has a ticket of its own: its chunks are taken in order.
+template <bool CHAIN>
+__device__ __forceinline__ uint32_t take_chunk(const GlrArgs& g, uint32_t& cb) {
+    if constexpr (!CHAIN) return 0;
+    __shared__ uint32_t taken;
+    cb = blockIdx.x % g.colblocks;
+    if (threadIdx.x == 0) taken = atomicAdd(g.tickets + cb * kTicketStep, 1u);
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(taken);
+}
+
 // W waves of consecutive stretches x CW waves of column groups
 template <class T, int V, int L, int W, int CW, bool CHAIN>
-__global__ __launch_bounds__(64 * W * CW) void glr_fwd(GlrArgs g) {
+__global__ __launch_bounds__(64 * W * CW, L > 8 ? (CHAIN && sizeof(typename T::Raw) == 2 ? 4 : 3) : 1) void glr_fwd(GlrArgs g) {
     using R = typename T::Raw;
+    using C = Cell<T, V>;
     constexpr int CL = W * L;
     __shared__ float2 maps[W > 1 ? W : 1][W > 1 ? CW * 64 * V : 1];
     __shared__ float2 far[CHAIN ? kRun : 1][CHAIN ? 64 * V : 1];
     static_assert(!CHAIN || CW == 1, "a chained chunk's columns are one wave wide");
-    __shared__ uint32_t taken;
-    uint32_t cb = blockIdx.x, chunk = 0;
-    if constexpr (CHAIN) {
-        if (threadIdx.x == 0) taken = atomicAdd(g.ticket, 1u);
-        __syncthreads();
-        chunk = taken / g.colblocks, cb = taken - chunk * g.colblocks;
-    }
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t cb = blockIdx.x, chunk = take_chunk<CHAIN>(g, cb);
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t tw = W > 1 ? wave % W : 0, slot = (W > 1 ? wave / W : wave) * 64 + lane;
     const uint32_t col = cb * (CW * 64) + slot;
-    const bool live = col < g.cols;
-    const uint32_t b = live ? col / g.groups : 0, ch = live ? (col - b * g.groups) * V : 0;
+    uint32_t b = col / g.groups, ch = (col - b * g.groups) * V;
+    const bool live = b < g.b && ch < g.d;
+    if (!live) b = ch = 0;
     const uint64_t flat = (uint64_t)b * g.d + ch;
     const uint32_t n = live ? (g.lengths ? (uint32_t)min(max(g.lengths[b], 0), (int32_t)g.t) : g.t) : 0;
 
@@ -183,33 +290,25 @@ __global__ __launch_bounds__(64 * W * CW) void glr_fwd(GlrArgs g) {
         k[v] = live ? decay_rate(g.rate, g.lam[ch + v]) : 0.0f;
         h[v] = live && g.h0 && (!CHAIN || chunk == 0) ? g.h0[flat + v] : 0.0f;
     }
-    const R* xp = reinterpret_cast<const R*>(g.x.p) + b * g.x.bs + ch;
-    const R* rp = reinterpret_cast<const R*>(g.r.p) + b * g.r.bs + ch;
-    const R* ip = reinterpret_cast<const R*>(g.i.p) + b * g.i.bs + ch;
-    R* yp = reinterpret_cast<R*>(g.y.p) + b * g.y.bs + ch;
+    const Wave wx(g.x, b, ch, sizeof(R)), wr(g.r, b, ch, sizeof(R)), wi(g.i, b, ch, sizeof(R)), wy(g.y, b, ch, sizeof(R));
 
     const uint32_t last = CHAIN ? chunk + 1 : g.nchunk;
     for (; chunk < last; chunk++) {
         const uint32_t t0 = chunk * CL + tw * L;
-        R xr[L][V] = {}, rr[L][V] = {}, ir[L][V] = {};
-#pragma unroll
-        for (int l = 0; l < L; l++) {
-            if (t0 + l < n) {
-                load_raw<R, V, true>(xp + (int64_t)(t0 + l) * g.x.ts, xr[l]);
-                load_raw<R, V, true>(rp + (int64_t)(t0 + l) * g.r.ts, rr[l]);
-                load_raw<R, V, true>(ip + (int64_t)(t0 + l) * g.i.ts, ir[l]);
-            }
-        }
+        C xr[L], rr[L], ir[L];
+        const bool full = __all(t0 + L <= n);
+        load_steps(wr, t0, n, full, C(C::lowest()), rr);
+        load_steps(wi, t0, n, full, C(C::lowest()), ir);
+        load_steps(wx, t0, n, full, C(C::zero()), xr);
         float a[L][V], in[L][V], A[V], S[V];
 #pragma unroll
         for (int v = 0; v < V; v++) A[v] = 1.0f, S[v] = 0.0f;
 #pragma unroll
         for (int l = 0; l < L; l++) {
-            const bool on = t0 + l < n;
 #pragma unroll
             for (int v = 0; v < V; v++) {
-                const Step s = step_of<false>(k[v], widen(T{}, xr[l][v]), widen(T{}, rr[l][v]), widen(T{}, ir[l][v]));
-                a[l][v] = on ? s.a : 1.0f, in[l][v] = on ? s.m * s.w : 0.0f;
+                const Gates q = gates_of(k[v], rr[l].at(v), ir[l].at(v));
+                a[l][v] = q.a, in[l][v] = __builtin_amdgcn_sqrtf(q.v) * (q.si * xr[l].at(v));
                 if constexpr (W > 1) {
                     S[v] = __builtin_fmaf(a[l][v], S[v], in[l][v]);
                     A[v] *= a[l][v];
@@ -223,11 +322,15 @@ __global__ __launch_bounds__(64 * W * CW) void glr_fwd(GlrArgs g) {
             __syncthreads();
             float pa[V], ps[V], ta[V], ts[V];  // the maps of the stretches before this one, and of the whole chunk
 #pragma unroll
-            for (int v = 0; v < V; v++) {
-                ta[v] = 1.0f, ts[v] = 0.0f;
+            for (int v = 0; v < V; v++) pa[v] = ta[v] = 1.0f, ps[v] = ts[v] = 0.0f;
 #pragma unroll
-                for (int w = 0; w < W; w++) {
-                    if (w == (int)tw) pa[v] = ta[v], ps[v] = ts[v];
+            for (int w = 0; w < W; w++) {
+                if (w == (int)tw) {
+#pragma unroll
+                    for (int v = 0; v < V; v++) pa[v] = ta[v], ps[v] = ts[v];
+                }
+#pragma unroll
+                for (int v = 0; v < V; v++) {
                     const float2 q = maps[w][slot * V + v];
                     ts[v] = __builtin_fmaf(q.x, ts[v], q.y);
                     ta[v] *= q.x;
@@ -260,19 +363,18 @@ __global__ __launch_bounds__(64 * W * CW) void glr_fwd(GlrArgs g) {
 #pragma unroll
             for (int v = 0; v < V; v++) h[v] = __builtin_fmaf(pa[v], h[v], ps[v]);
         }
-        if (live && g.states && tw == 0 && t0 < g.t) {
+        // the states that the backward pass starts its chunks from
+        if (g.states && live && (t0 & ((1u << g.spacing) - 1)) == 0 && t0 < g.t) {
 #pragma unroll
-            for (int v = 0; v < V; v++) g.states[((uint64_t)b * g.nstates + chunk) * g.d + ch + v] = h[v];
+            for (int v = 0; v < V; v++) g.states[((uint64_t)b * g.nstates + (t0 >> g.spacing)) * g.d + ch + v] = h[v];
         }
 #pragma unroll
         for (int l = 0; l < L; l++) {
-            R out[V];
 #pragma unroll
-            for (int v = 0; v < V; v++) {
-                h[v] = __builtin_fmaf(a[l][v], h[v], in[l][v]);
-                out[v] = narrow(T{}, t0 + l < n ? h[v] : 0.0f);
-            }
-            if (live && t0 + l < g.t) store_raw<R, V, true>(yp + (int64_t)(t0 + l) * g.y.ts, out);
+            for (int v = 0; v < V; v++) h[v] = __builtin_fmaf(a[l][v], h[v], in[l][v]);
+            const C out = C::of(h);
+            if (full || (live && t0 + l < g.t))
+                wy.store(t0 + l, C(out.where(full || t0 + l < n)));
         }
         if constexpr (W > 1) {
 #pragma unroll
@@ -285,26 +387,27 @@ __global__ __launch_bounds__(64 * W * CW) void glr_fwd(GlrArgs g) {
     }
 }
 
+// Backward. With g_t = dy_t + c_t, c_(t-1) = a_t g_t the gradient that reaches the state before a step:
+//     dx = g m si,   di = g m si x (1 - si),   d/d(log a) = a g (h_(t-1) - a w / m),   w = si x, m = sqrt(1 - a^2)
+//     dr = d/d(log a) log a (1 - sr),   dlam = sum of d/d(log a) sr * -rate sigmoid(lam)
+// A lane keeps six values a step while the chunk's maps are exchanged (and x and dy as they were read): more registers
+// would cost the waves that hide the loads.
 template <class T, int V, int L, int W, int CW, bool CHAIN>
-__global__ __launch_bounds__(64 * W * CW) void glr_bwd(GlrArgs g) {
+__global__ __launch_bounds__(64 * W * CW, L > 1 ? 3 : 1) void glr_bwd(GlrArgs g) {
     using R = typename T::Raw;
+    using C = Cell<T, V>;
     constexpr int CL = W * L;
     __shared__ float2 maps[W > 1 ? W : 1][W > 1 ? CW * 64 * V : 1];  // (A, S) forward
     __shared__ float back[W > 1 ? W : 1][W > 1 ? CW * 64 * V : 1];   // the R of c -> A c + R
     __shared__ float2 far[CHAIN ? kRun : 1][CHAIN ? 64 * V : 1];
     static_assert(!CHAIN || CW == 1, "a chained chunk's columns are one wave wide");
-    __shared__ uint32_t taken;
-    uint32_t cb = blockIdx.x, done = 0;  // chunks go from the last to the first; done: those already passed
-    if constexpr (CHAIN) {
-        if (threadIdx.x == 0) taken = atomicAdd(g.ticket, 1u);
-        __syncthreads();
-        done = taken / g.colblocks, cb = taken - done * g.colblocks;
-    }
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t cb = blockIdx.x, done = take_chunk<CHAIN>(g, cb);  // chunks go from the last to the first
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t tw = W > 1 ? wave % W : 0, slot = (W > 1 ? wave / W : wave) * 64 + lane;
     const uint32_t col = cb * (CW * 64) + slot;
-    const bool live = col < g.cols;
-    const uint32_t b = live ? col / g.groups : 0, ch = live ? (col - b * g.groups) * V : 0;
+    uint32_t b = col / g.groups, ch = (col - b * g.groups) * V;
+    const bool live = b < g.b && ch < g.d;
+    if (!live) b = ch = 0;
     const uint64_t flat = (uint64_t)b * g.d + ch;
     const uint32_t n = live ? (g.lengths ? (uint32_t)min(max(g.lengths[b], 0), (int32_t)g.t) : g.t) : 0;
 
@@ -315,48 +418,49 @@ __global__ __launch_bounds__(64 * W * CW) void glr_bwd(GlrArgs g) {
         c[v] = live && g.dht && (!CHAIN || done == 0) ? g.dht[flat + v] : 0.0f;
         lam_sum[v] = 0.0f;
     }
-    const R* xp = reinterpret_cast<const R*>(g.x.p) + b * g.x.bs + ch;
-    const R* rp = reinterpret_cast<const R*>(g.r.p) + b * g.r.bs + ch;
-    const R* ip = reinterpret_cast<const R*>(g.i.p) + b * g.i.bs + ch;
-    const R* dyp = reinterpret_cast<const R*>(g.dy.p) + b * g.dy.bs + ch;
-    R* dxp = reinterpret_cast<R*>(g.dx.p) + b * g.dx.bs + ch;
-    R* drp = reinterpret_cast<R*>(g.dr.p) + b * g.dr.bs + ch;
-    R* dip = reinterpret_cast<R*>(g.di.p) + b * g.di.bs + ch;
+    const Wave wx(g.x, b, ch, sizeof(R)), wr(g.r, b, ch, sizeof(R)), wi(g.i, b, ch, sizeof(R)),
+        wdy(g.dy, b, ch, sizeof(R)), wdx(g.dx, b, ch, sizeof(R)), wdr(g.dr, b, ch, sizeof(R)), wdi(g.di, b, ch, sizeof(R));
 
     const uint32_t last = CHAIN ? done + 1 : g.nchunk;
     for (; done < last; done++) {
         const uint32_t chunk = g.nchunk - 1 - done, t0 = chunk * CL + tw * L;
-        R xr[L][V] = {}, rr[L][V] = {}, ir[L][V] = {}, gr[L][V] = {};
+        C xr[L], rr[L], ir[L], gr[L];
+        const bool full = __all(t0 + L <= n);
         float h[V];
 #pragma unroll
         for (int v = 0; v < V; v++)
             h[v] = live && chunk < g.nstates ? g.states[((uint64_t)b * g.nstates + chunk) * g.d + ch + v] : 0.0f;
-#pragma unroll
-        for (int l = 0; l < L; l++) {
-            if (t0 + l < n) {
-                load_raw<R, V, true>(xp + (int64_t)(t0 + l) * g.x.ts, xr[l]);
-                load_raw<R, V, true>(rp + (int64_t)(t0 + l) * g.r.ts, rr[l]);
-                load_raw<R, V, true>(ip + (int64_t)(t0 + l) * g.i.ts, ir[l]);
-                load_raw<R, V, true>(dyp + (int64_t)(t0 + l) * g.dy.ts, gr[l]);
-            }
-        }
-        Step s[L][V];
-        float dy[L][V], A[V], S[V], B[V];
+        load_steps(wr, t0, n, full, C(C::lowest()), rr);
+        load_steps(wi, t0, n, full, C(C::lowest()), ir);
+        load_steps(wx, t0, n, full, C(C::zero()), xr);
+        load_steps(wdy, t0, n, full, C(C::zero()), gr);
+        // p = m si; q = a w / m, later h_(t-1) - q
+        float a[L][V], p[L][V], q[L][V], sr[L][V], lr[L][V], ni[L][V], A[V], S[V], B[V];
 #pragma unroll
         for (int v = 0; v < V; v++) A[v] = 1.0f, S[v] = 0.0f, B[v] = 0.0f;
 #pragma unroll
         for (int l = 0; l < L; l++) {
-            const bool on = t0 + l < n;
+            // one step after the other: with every step's exponentials taken first, as the compiler would, the gates of
+            // all steps are alive together
+            rr[l].forget(), ir[l].forget();
 #pragma unroll
             for (int v = 0; v < V; v++) {
-                s[l][v] = step_of<true>(k[v], widen(T{}, xr[l][v]), widen(T{}, rr[l][v]), widen(T{}, ir[l][v]));
-                dy[l][v] = on ? widen(T{}, gr[l][v]) : 0.0f;
-                if (!on) s[l][v].a = 1.0f, s[l][v].m = 0.0f, s[l][v].w = 0.0f;
+                const Gates s = gates_of(k[v], rr[l].at(v), ir[l].at(v));
+                const float x = xr[l].at(v), dy = gr[l].at(v);
+                // 1 - a^2 is 0 where nothing decays, and no larger than log a: the gradient that passes through m's
+                // root, log a / m, is 0 at this limit (times a finite value)
+                const float rm = __builtin_amdgcn_rsqf(__builtin_fmaxf(s.v, 1.17549435e-38f));
+                a[l][v] = s.a, sr[l][v] = s.sr;
+                lr[l][v] = s.z * kLn2 * shut(s.er, s.sr);
+                ni[l][v] = shut(s.ei, s.si);
+                p[l][v] = s.v * rm * s.si;
+                q[l][v] = s.a * rm * (s.si * x);
                 if constexpr (W > 1) {
-                    S[v] = __builtin_fmaf(s[l][v].a, S[v], s[l][v].m * s[l][v].w);
-                    A[v] *= s[l][v].a;
-                    B[v] = __builtin_fmaf(A[v], dy[l][v], B[v]);  // dy_l reaches the front through a_1 .. a_l
+                    S[v] = __builtin_fmaf(s.a, S[v], p[l][v] * x);
+                    A[v] *= s.a;
+                    B[v] = __builtin_fmaf(A[v], dy, B[v]);  // dy_l reaches the front through a_1 .. a_l
                 }
+                asm volatile("" : "+v"(p[l][v]), "+v"(q[l][v]), "+v"(lr[l][v]), "+v"(ni[l][v]));
             }
         }
         float end[V];  // what the chunk hands to the chunk before it
@@ -369,19 +473,25 @@ __global__ __launch_bounds__(64 * W * CW) void glr_bwd(GlrArgs g) {
             __syncthreads();
             float pa[V], ps[V], ta[V], ts[V];  // c of this stretch, and of the whole chunk, from the chunk's c
 #pragma unroll
-            for (int v = 0; v < V; v++) {
+            for (int v = 0; v < V; v++) pa[v] = ta[v] = 1.0f, ps[v] = ts[v] = 0.0f;
+            for (int w = 0; w < (int)tw; w++) {  // the state that reaches the stretch
 #pragma unroll
-                for (int w = 0; w < W; w++) {  // the state that reaches the stretch
-                    const float2 q = maps[w][slot * V + v];
-                    if (w < (int)tw) h[v] = __builtin_fmaf(q.x, h[v], q.y);
+                for (int v = 0; v < V; v++) {
+                    const float2 m = maps[w][slot * V + v];
+                    h[v] = __builtin_fmaf(m.x, h[v], m.y);
                 }
-                ta[v] = 1.0f, ts[v] = 0.0f;
+            }
 #pragma unroll
-                for (int w = W - 1; w >= 0; w--) {
-                    if (w == (int)tw) pa[v] = ta[v], ps[v] = ts[v];
-                    const float qa = maps[w][slot * V + v].x;
-                    ts[v] = __builtin_fmaf(qa, ts[v], back[w][slot * V + v]);
-                    ta[v] *= qa;
+            for (int w = W - 1; w >= 0; w--) {
+                if (w == (int)tw) {
+#pragma unroll
+                    for (int v = 0; v < V; v++) pa[v] = ta[v], ps[v] = ts[v];
+                }
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    const float m = maps[w][slot * V + v].x;
+                    ts[v] = __builtin_fmaf(m, ts[v], back[w][slot * V + v]);
+                    ta[v] *= m;
                 }
             }
             if constexpr (CHAIN) {
@@ -411,36 +521,35 @@ __global__ __launch_bounds__(64 * W * CW) void glr_bwd(GlrArgs g) {
 #pragma unroll
             for (int v = 0; v < V; v++) c[v] = __builtin_fmaf(pa[v], c[v], ps[v]);
         }
-        float hp[L][V];  // the state before each step
+        // what was derived from x and dy is derived again: the compiler would keep it in registers across the exchange
+#pragma unroll
+        for (int l = 0; l < L; l++) xr[l].forget(), gr[l].forget();
 #pragma unroll
         for (int l = 0; l < L; l++) {
 #pragma unroll
             for (int v = 0; v < V; v++) {
-                hp[l][v] = h[v];
-                h[v] = __builtin_fmaf(s[l][v].a, h[v], s[l][v].m * s[l][v].w);
+                q[l][v] = h[v] - q[l][v];
+                h[v] = __builtin_fmaf(a[l][v], h[v], p[l][v] * xr[l].at(v));
             }
         }
 #pragma unroll
         for (int l = L - 1; l >= 0; l--) {
-            const bool on = t0 + l < n;
-            R ox[V], orr[V], oi[V];
+            const bool on = full || t0 + l < n;
+            float ox[V], orr[V], oi[V];
 #pragma unroll
             for (int v = 0; v < V; v++) {
-                const Step& q = s[l][v];
-                const float gt = dy[l][v] + c[v];
-                c[v] = q.a * gt;
-                // d/d(log a): a h_(t-1) from the decay, -(a^2 / m) w from the input's normalisation
-                const float dla = c[v] * (hp[l][v] - q.a * q.rm * q.w);
-                const float gm = gt * q.m;
-                ox[v] = narrow(T{}, on ? gm * q.si : 0.0f);
-                orr[v] = narrow(T{}, on ? dla * q.la * q.nr : 0.0f);
-                oi[v] = narrow(T{}, on ? gm * q.w * q.ni : 0.0f);
-                lam_sum[v] += on ? dla * q.sr : 0.0f;
+                const float gt = gr[l].at(v) + c[v];
+                c[v] = a[l][v] * gt;
+                const float dla = on ? c[v] * q[l][v] : 0.0f;
+                ox[v] = gt * p[l][v];
+                orr[v] = dla * lr[l][v];
+                oi[v] = ox[v] * xr[l].at(v) * ni[l][v];
+                lam_sum[v] = __builtin_fmaf(dla, sr[l][v], lam_sum[v]);
             }
-            if (live && t0 + l < g.t) {
-                store_raw<R, V, true>(dxp + (int64_t)(t0 + l) * g.dx.ts, ox);
-                store_raw<R, V, true>(drp + (int64_t)(t0 + l) * g.dr.ts, orr);
-                store_raw<R, V, true>(dip + (int64_t)(t0 + l) * g.di.ts, oi);
+            if (full || (live && t0 + l < g.t)) {
+                wdx.store(t0 + l, C(C(C::of(ox)).where(on)));
+                wdr.store(t0 + l, C(C::of(orr)));
+                wdi.store(t0 + l, C(C(C::of(oi)).where(on)));
             }
         }
         if constexpr (W > 1) {
@@ -472,65 +581,73 @@ __global__ __launch_bounds__(64 * W * CW) void glr_bwd(GlrArgs g) {
     }
 }
 
-// Column sums of the partial rows: 64 columns x 16 row lanes a workgroup, rows y, y + gridDim.y * 16, ...; a second
+// Column sums of the partial rows: 16 columns x 64 row lanes a workgroup, rows y, y + gridDim.y * 64, ...; a second
 // launch with one row block finishes. In f64: millions of terms of either sign meet here.
 template <class In, bool LAST>
 __global__ __launch_bounds__(1024) void glr_sum(const In* part, uint64_t rows, uint32_t d, double* out, float* dlam,
                                                 const float* lam, float rate) {
-    __shared__ double s[16][64];
-    const uint32_t ch = blockIdx.x * 64 + (threadIdx.x & 63), y = threadIdx.x >> 6;
+    __shared__ double s[64][17];
+    const uint32_t x = threadIdx.x & 15, ch = blockIdx.x * 16 + x, y = threadIdx.x >> 4;
     double acc = 0.0;
     if (ch < d) {
-#pragma unroll 4
-        for (uint64_t r = (uint64_t)blockIdx.y * 16 + y; r < rows; r += (uint64_t)gridDim.y * 16)
+#pragma unroll 8
+        for (uint64_t r = (uint64_t)blockIdx.y * 64 + y; r < rows; r += (uint64_t)gridDim.y * 64)
             acc += (double)part[r * d + ch];
     }
-    s[y][threadIdx.x & 63] = acc;
+    s[y][x] = acc;
     __syncthreads();
-    if (y == 0 && ch < d) {
+    if (threadIdx.x < 64) {  // 4 lanes a column, 16 rows each
+        const uint32_t col = threadIdx.x >> 2, q = threadIdx.x & 3, c = blockIdx.x * 16 + col;
+        acc = 0.0;
 #pragma unroll
-        for (int k = 1; k < 16; k++) acc += s[k][threadIdx.x];
-        if constexpr (LAST) {
-            const float e = expf(-fabsf(lam[ch]));  // d softplus / d lam = sigmoid(lam)
-            const float sg = (lam[ch] >= 0.0f ? 1.0f : e) / (1.0f + e);
-            dlam[ch] = (float)(acc * -(double)rate * (double)sg);
-        } else {
-            out[(uint64_t)blockIdx.y * d + ch] = acc;
+        for (int k = 0; k < 16; k++) acc += s[q * 16 + k][col];
+        acc += __shfl_xor(acc, 1);
+        acc += __shfl_xor(acc, 2);
+        if (q == 0 && c < d) {
+            if constexpr (LAST) {
+                const float e = expf(-fabsf(lam[c]));  // d softplus / d lam = sigmoid(lam)
+                const float sg = (lam[c] >= 0.0f ? 1.0f : e) / (1.0f + e);
+                dlam[c] = (float)(acc * -(double)rate * (double)sg);
+            } else {
+                out[(uint64_t)blockIdx.y * d + c] = acc;
+            }
         }
     }
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------
 
-constexpr int kL = 8;         // steps a lane holds
-constexpr int kW = 8;         // waves of a chunk, where a chunk has more than one
-constexpr int kChunk = kL * kW;
+constexpr int kL = 8;              // steps a lane holds
 constexpr uint32_t kSumRows = 64;  // row blocks of the first sum
 
 struct Plan {
-    bool split, chain;  // split: chunks of kW waves
-    uint32_t v, groups, cols, chunk, nchunk, colblocks, nstates;
+    int l, w;    // steps of a stretch; stretches (waves) of a chunk
+    bool chain;
+    uint32_t v, groups, nchunk, colblocks, nstates, spacing;
     uint64_t words;  // of the chain: maps, then heads
     size_t agg_bytes, part_bytes, sum_bytes;
 };
 
-// One wave per column group walks kL steps at a time where that alone fills the chip or there is little to split;
-// else kW waves share a chunk, and chunks are chained where the columns give fewer than two workgroups a CU. v: the
-// channels a lane takes.
-Plan plan_of(const fhc_glr_desc* g, uint32_t v) {
+// One wave per column group walks kL steps at a time (one, for a single token) where that alone fills the chip or
+// there is little to split; else up to 8 waves share a chunk, and chunks are chained where the columns give fewer than
+// two workgroups a CU. v: the channels a lane takes; near: a wave's columns may run over sequences, since the offsets
+// between them fit a lane's 32 bits; else each sequence starts a wave of its own.
+Plan plan_of(const fhc_glr_desc* g, bool backward, uint32_t v, bool near) {
     Plan p{};
     p.v = v;
-    p.groups = g->d / v;
-    p.cols = g->b * p.groups;
+    p.groups = near ? g->d / v : (uint32_t)ceil_div(g->d / v, 64) * 64;
+    const uint64_t cols = (uint64_t)g->b * p.groups;
     const uint64_t flat = (uint64_t)g->b * g->d;
-    p.split = g->t > 2 * kL && flat < (1u << 19);
-    p.chunk = p.split ? kChunk : kL;
-    p.nchunk = (uint32_t)(g->t ? ceil_div(g->t, p.chunk) : 1);
-    p.nstates = (uint32_t)ceil_div(g->t, p.chunk);
-    p.colblocks = (uint32_t)ceil_div(p.cols, p.split ? 64 : 256);
-    p.chain = p.split && p.nchunk > 1 && flat < (1u << 16);
+    p.l = g->t == 1 ? 1 : kL;
+    p.w = flat >= (1u << 19) || g->t <= kL ? 1 : g->t <= 2 * kL ? 2 : g->t <= 4 * kL ? 4 : 8;
+    if (!backward && g->t >= 16 * kL && p.w == 8) p.l = 2 * kL;
+    p.nchunk = (uint32_t)(g->t ? ceil_div(g->t, p.l * p.w) : 1);
+    p.spacing = p.w == 1 ? 3 : p.w == 2 ? 4 : p.w == 4 ? 5 : 6;
+    p.nstates = (uint32_t)ceil_div(g->t, 1u << p.spacing);
+    p.colblocks = (uint32_t)ceil_div(cols, p.w >= 4 ? 64 : p.w == 2 ? 128 : 256);
+    p.chain = p.nchunk > 1 && p.w == 8 && flat < (1u << 16);
     p.words = p.chain ? (p.nchunk + ceil_div(p.nchunk, kRun)) * flat : 0;
-    p.agg_bytes = p.chain ? p.words * 8 + 256 : 0;
+    p.agg_bytes = p.chain ? p.words * 8 + (size_t)g->b * ceil_div(g->d, 64) * kTicketStep * 4 : 0;
     p.part_bytes = (size_t)ceil_div((p.chain ? p.nchunk : 1) * flat * 4, 256) * 256;
     p.sum_bytes = (size_t)kSumRows * g->d * 8;
     return p;
@@ -559,15 +676,20 @@ int check_out(const char* op, const char* name, const fhc_seq* s, const fhc_glr_
     return 0;
 }
 
-Col col(const fhc_seq* s) { return Col{static_cast<char*>(s->p), s->bs, s->ts}; }
+Col col(const fhc_seq* s, uint32_t dtype) {
+    const int64_t e = elem_bytes(dtype);
+    return Col{static_cast<char*>(s->p), s->bs * e, s->ts * e};
+}
 
-// pairs of channels as one load where every tensor allows it
-bool pairs(const fhc_glr_desc* g, std::initializer_list<const fhc_seq*> all) {
-    if (g->d % 2) return false;
-    for (const fhc_seq* s : all)
-        if ((g->b > 1 && s->bs % 2) || (g->t > 1 && s->ts % 2) || !aligned(s->p, 2 * elem_bytes(g->dtype)))
-            return false;
-    return true;
+// the plan for these tensors: pairs of channels as one load, waves over several sequences, where every one allows it
+Plan plan_for(const fhc_glr_desc* g, bool backward, std::initializer_list<const fhc_seq*> all) {
+    bool pairs = g->d % 2 == 0, near = true;
+    const int64_t e = elem_bytes(g->dtype);
+    for (const fhc_seq* s : all) {
+        if ((g->b > 1 && s->bs % 2) || (g->t > 1 && s->ts % 2) || !aligned(s->p, 2 * (uint32_t)e)) pairs = false;
+        if (g->b > 1 && (s->bs < 0 || s->bs >= (1 << 30) / 64 / e)) near = false;
+    }
+    return plan_of(g, backward, pairs ? 2 : 1, near);
 }
 
 template <class F>
@@ -586,22 +708,34 @@ void launch(const Plan& p, const GlrArgs& a, hipStream_t s) {
         else                                                                                                \
             hipLaunchKernelGGL((glr_fwd<T, V, L, W, CW, CHAIN>), dim3(GRID), dim3(64 * W * CW), 0, s, a);   \
     } while (0)
-    if (p.chain) GLR(kL, kW, 1, true, p.colblocks * p.nchunk);
-    else if (p.split) GLR(kL, kW, 1, false, p.colblocks);
+    if constexpr (!BWD) {
+        if (p.l > kL) {
+            if (p.chain) GLR(2 * kL, 8, 1, true, p.colblocks * p.nchunk);
+            else GLR(2 * kL, 8, 1, false, p.colblocks);
+            return;
+        }
+    }
+    if (p.chain) GLR(kL, 8, 1, true, p.colblocks * p.nchunk);
+    else if (p.w == 8) GLR(kL, 8, 1, false, p.colblocks);
+    else if (p.w == 4) GLR(kL, 4, 1, false, p.colblocks);
+    else if (p.w == 2) GLR(kL, 2, 2, false, p.colblocks);
+    else if (p.l == 1) GLR(1, 1, 4, false, p.colblocks);
     else GLR(kL, 1, 4, false, p.colblocks);
 #undef GLR
 }
 
 template <bool BWD>
 int run(const char* op, const Plan& p, GlrArgs& a, uint32_t dtype, void* ws, hipStream_t s) {
-    if ((uint64_t)p.colblocks * p.nchunk >= 1ull << 31) return fail(-1, "%s: too many chunks", op);
-    a.groups = p.groups, a.cols = p.cols, a.nchunk = p.nchunk, a.colblocks = p.colblocks, a.nstates = p.nstates;
+    if ((uint64_t)p.colblocks * p.nchunk >= 1ull << 31 || (uint64_t)a.b * p.groups >= 1ull << 31) return fail(-1, "%s: too many chunks", op);
+    a.groups = p.groups, a.nchunk = p.nchunk, a.colblocks = p.colblocks, a.nstates = p.nstates;
+    a.spacing = p.spacing;
     char* w = static_cast<char*>(ws);
     if (p.chain) {
-        a.ticket = reinterpret_cast<uint32_t*>(w);
-        a.agg = reinterpret_cast<uint64_t*>(w + 256);
+        a.agg = reinterpret_cast<uint64_t*>(w);
         a.heads = a.agg + (uint64_t)p.nchunk * a.b * a.d;
-        hipLaunchKernelGGL(glr_clear, dim3((uint32_t)ceil_div(p.words, 256)), dim3(256), 0, s, a.agg, p.words, a.ticket);
+        a.tickets = reinterpret_cast<uint32_t*>(a.agg + p.words);
+        hipLaunchKernelGGL(glr_clear, dim3((uint32_t)ceil_div(p.words, 256)), dim3(256), 0, s, a.agg, p.words,
+                           a.tickets, p.colblocks);
         FHC_TRY(launched(op));
     }
     with_type(dtype, [&](auto t) {
@@ -628,7 +762,7 @@ extern "C" size_t fhc_glr_states_bytes(const fhc_glr_desc* g) {
     return guard((size_t)0, [&]() -> size_t {
         clear_error();
         if (check_desc("glr_states_bytes", g) < 0) return 0;
-        return (size_t)g->b * plan_of(g, 1).nstates * g->d * 4;
+        return (size_t)g->b * plan_of(g, true, 1, true).nstates * g->d * 4;
     });
 }
 
@@ -636,7 +770,7 @@ extern "C" size_t fhc_glr_workspace_bytes(const fhc_glr_desc* g, int backward) {
     return guard((size_t)0, [&]() -> size_t {
         clear_error();
         if (check_desc("glr_workspace_bytes", g) < 0 || (uint64_t)g->b * g->d == 0) return 0;
-        return workspace_of(plan_of(g, 1), backward != 0);
+        return workspace_of(plan_of(g, backward != 0, 1, true), backward != 0);
     });
 }
 
@@ -652,10 +786,10 @@ extern "C" int fhc_glr_forward(const fhc_glr_desc* g, const fhc_seq* x, const fh
         FHC_TRY(check_seq(op, "r", r, g));
         FHC_TRY(check_seq(op, "i", i, g));
         FHC_TRY(check_out(op, "y", y, g));
-        const Plan p = plan_of(g, pairs(g, {x, r, i, y}) ? 2 : 1);
+        const Plan p = plan_for(g, false, {x, r, i, y});
         FHC_TRY(check_workspace(op, workspace_of(p, false), ws, ws_bytes));
         GlrArgs a{};
-        a.x = col(x), a.r = col(r), a.i = col(i), a.y = col(y);
+        a.x = col(x, g->dtype), a.r = col(r, g->dtype), a.i = col(i, g->dtype), a.y = col(y, g->dtype);
         a.lam = g->lam, a.lengths = g->lengths, a.h0 = h0, a.ht = ht, a.states = states;
         a.b = g->b, a.t = g->t, a.d = g->d, a.rate = g->rate;
         return run<false>(op, p, a, g->dtype, ws, (hipStream_t)stream);
@@ -673,8 +807,7 @@ extern "C" int fhc_glr_backward(const fhc_glr_desc* g, const fhc_seq* x, const f
         if (g->d == 0) return 0;
         if (!dlam) return fail(-1, "%s: null dlam", op);
         const hipStream_t s = (hipStream_t)stream;
-        Plan p = plan_of(g, 1);
-        const uint32_t dblocks = (uint32_t)ceil_div(g->d, 64);
+                const uint32_t dblocks = (uint32_t)ceil_div(g->d, 16);
         if (g->b == 0) {  // an empty sum
             if (!g->lam) return fail(-1, "%s: null lam", op);
             hipLaunchKernelGGL((glr_sum<float, true>), dim3(dblocks), dim3(1024), 0, s, (const float*)nullptr,
@@ -689,10 +822,10 @@ extern "C" int fhc_glr_backward(const fhc_glr_desc* g, const fhc_seq* x, const f
         FHC_TRY(check_out(op, "dr", dr, g));
         FHC_TRY(check_out(op, "di", di, g));
         if (g->t && !states) return fail(-1, "%s: null states", op);
-        if (pairs(g, {x, r, i, dy, dx, dr, di})) p = plan_of(g, 2);
+        const Plan p = plan_for(g, true, {x, r, i, dy, dx, dr, di});
         FHC_TRY(check_workspace(op, workspace_of(p, true), ws, ws_bytes));
         GlrArgs a{};
-        a.x = col(x), a.r = col(r), a.i = col(i), a.dy = col(dy), a.dx = col(dx), a.dr = col(dr), a.di = col(di);
+        a.x = col(x, g->dtype), a.r = col(r, g->dtype), a.i = col(i, g->dtype), a.dy = col(dy, g->dtype), a.dx = col(dx, g->dtype), a.dr = col(dr, g->dtype), a.di = col(di, g->dtype);
         a.lam = g->lam, a.lengths = g->lengths, a.states = const_cast<float*>(states), a.dht = dht, a.dh0 = dh0;
         a.b = g->b, a.t = g->t, a.d = g->d, a.rate = g->rate;
         char* w = static_cast<char*>(ws) + (p.agg_bytes + 255) / 256 * 256;
