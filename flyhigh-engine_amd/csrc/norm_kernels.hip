@@ -2,9 +2,9 @@
 //
 // Both directions are bound by HBM: x and o in, y and u out; x, o, dy, du in, dx and do out. So a row is read once into
 // registers, every statistic comes from there, and y (which u and its statistics need unrounded) is never read back:
-// the backward pass computes it again from x and o in place of reading it. A row is held by `tpr` threads, 8 channels
-// each (K such groups for the widest rows): a part of a wave for narrow rows, so that a wave takes several pixels, up
-// to a workgroup for wide ones.
+// the backward pass computes it again from x and o in place of reading it. A row is held by threads of 8 channels each
+// (K such groups for the widest rows): a part of a wave for narrow rows, so that a wave takes several pixels, as many
+// waves as it needs (up to 16) for wide ones.
 #include "seq_common.h"
 
 namespace fhc {
@@ -19,144 +19,203 @@ struct Rows {
 struct NormArgs {
     Rows x, o, y, u, dy, du, dx, dout;
     const void *w_post, *w_pre, *gate;
-    float *dgate, *part_post, *part_pre, *part_gate;  // see norm_bwd
+    float *dgate, *part_post, *part_pre;  // see norm_bwd
     uint32_t rows, c, rpg, groups;
     uint32_t per_group, part_rows;  // parts of a group, rows of a part; per_group 0: a workgroup takes whole groups
     uint32_t wg_groups;             // groups of a workgroup, where per_group is 0
     float alpha, eps;
 };
 
-template <class T, bool AL>
-__device__ __forceinline__ void load8(const void* base, int64_t at, uint32_t ch, uint32_t c, float (&f)[8]) {
-    using R = typename T::Raw;
-    const R* p = reinterpret_cast<const R*>(base) + at + ch;
-    if (AL || ch + 8 <= c) {
-        R q[8];
-        load_raw<R, 8, AL>(p, q);
-#pragma unroll
-        for (int i = 0; i < 8; i++) f[i] = widen(T{}, q[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const R q = p[(ch + i < c ? i : 0)];
-            f[i] = ch + i < c ? widen(T{}, q) : 0.0f;
-        }
+// 8 adjacent channels of a row as they lie in memory, held in registers until they are used: all of a row's loads are
+// then under way together.
+template <class T>
+struct Chunk {
+    typedef uint32_t Vec __attribute__((ext_vector_type(4)));
+    Vec w;
+    __device__ __forceinline__ float at(int i) const { return widen(T{}, (uint16_t)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1])); }
+    __device__ __forceinline__ void set(int i, uint16_t v) {
+        w[i >> 1] = i & 1 ? (w[i >> 1] & 0xFFFFu) | (uint32_t)v << 16 : (w[i >> 1] & 0xFFFF0000u) | v;
     }
+};
+template <>
+struct Chunk<F32> {
+    typedef float Vec __attribute__((ext_vector_type(8)));
+    Vec w;
+    __device__ __forceinline__ float at(int i) const { return w[i]; }
+    __device__ __forceinline__ void set(int i, float v) { w[i] = v; }
+};
+
+// Where a thread's 8 channels are. AL: c is a multiple of 8 and every address one of 16 bytes. Otherwise the last
+// thread of a row takes the row's last 8 channels, of which the first `skip` belong to the thread before it: they are
+// read again, count for nothing and are not stored (c < 8: one thread, element by element).
+struct Place {
+    uint32_t ch, skip;
+    bool in;
+};
+template <bool AL>
+__device__ __forceinline__ Place place_of(uint32_t thread, uint32_t c) {
+    const uint32_t ch = thread * 8;
+    if (AL || c < 8) return {ch, 0, ch < c};
+    const uint32_t at = ch + 8 <= c ? ch : c - 8;
+    return {at, ch < c ? ch - at : 8, ch < c};
 }
 template <class T, bool AL>
-__device__ __forceinline__ void store8(void* base, int64_t at, uint32_t ch, uint32_t c, const float (&f)[8]) {
+__device__ __forceinline__ Chunk<T> load8(const void* base, int64_t at, Place p, uint32_t c) {
     using R = typename T::Raw;
-    R* p = reinterpret_cast<R*>(base) + at + ch;
-    R q[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) q[i] = narrow(T{}, f[i]);
-    if (AL || ch + 8 <= c) {
-        store_raw<R, 8, AL>(p, q);
-    } else {
+    typedef typename Chunk<T>::Vec Mem __attribute__((aligned(AL ? 16 : sizeof(R))));
+    const R* q = reinterpret_cast<const R*>(base) + at + p.ch;
+    Chunk<T> v{};
+    if (AL || c >= 8) {
+        if (p.in) v.w = *reinterpret_cast<const Mem*>(q);
+    } else if (p.in) {
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            if (ch + i < c) p[i] = q[i];
+            if (i < (int)c) v.set(i, q[i]);
+    }
+    return v;
+}
+// the values, 0 where they are another thread's
+template <class T, bool AL>
+__device__ __forceinline__ void widen8(const Chunk<T>& v, Place p, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) f[i] = AL || i >= (int)p.skip ? v.at(i) : 0.0f;
+}
+template <class T, bool AL>
+__device__ __forceinline__ void store8(void* base, int64_t at, Place p, uint32_t c, const float (&f)[8]) {
+    using R = typename T::Raw;
+    typedef typename Chunk<T>::Vec Mem __attribute__((aligned(AL ? 16 : sizeof(R))));
+    R* q = reinterpret_cast<R*>(base) + at + p.ch;
+    Chunk<T> v{};
+#pragma unroll
+    for (int i = 0; i < 8; i++) v.set(i, narrow(T{}, f[i]));
+    if (AL || (p.skip == 0 && c >= 8)) {
+        if (p.in) *reinterpret_cast<Mem*>(q) = v.w;
+    } else if (p.in) {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i >= (int)p.skip && i < (int)c) q[i] = narrow(T{}, f[i]);
     }
 }
 // 8 weights, 1 where there are none
 template <class T, bool AL>
-__device__ __forceinline__ void weight8(const void* base, int64_t at, uint32_t ch, uint32_t c, float (&f)[8]) {
-    if (base) {
-        load8<T, AL>(base, at, ch, c, f);
-    } else {
+__device__ __forceinline__ Chunk<T> weight8(const void* base, int64_t at, Place p, uint32_t c) {
+    if (base) return load8<T, AL>(base, at, p, c);
+    Chunk<T> v{};
 #pragma unroll
-        for (int i = 0; i < 8; i++) f[i] = 1.0f;
-    }
+    for (int i = 0; i < 8; i++) v.set(i, narrow(T{}, 1.0f));
+    return v;
 }
 
-// Sums of N values over the TPR threads of a row. Within a wave by lane exchange; a row of several waves goes through
-// LDS, two buffers in turn so that one barrier a sum is enough.
-template <int TPR, int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], float (*lds)[N][TPR > 64 ? TPR / 64 : 1]) {
-#pragma unroll
-    for (int m = 1; m < (TPR < 64 ? TPR : 64); m *= 2) {
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] += __shfl_xor(v[i], m);
+template <int CTRL>
+__device__ __forceinline__ float dpp_plus(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+// the sum over TPR <= 64 lanes, in each of them: within 16 lanes by the adder's own lane selection (neighbours, pairs,
+// mirrored halves), then by exchanging rows of 16 and of 32
+template <int TPR>
+__device__ __forceinline__ float lane_sum(float v) {
+    v = dpp_plus<0xB1>(v);
+    v = dpp_plus<0x4E>(v);
+    v = dpp_plus<0x141>(v);
+    v = dpp_plus<0x140>(v);
+    if constexpr (TPR >= 32) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, v);
+        const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        const uint32_t a = s[0], b = s[1];  // (a bit cast of an element itself reads the first one)
+        v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
     }
-    if constexpr (TPR > 64) {
-        constexpr int NW = TPR / 64;
-        if ((threadIdx.x & 63) == 0) {
+    if constexpr (TPR >= 64) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, v);
+        const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        const uint32_t a = s[0], b = s[1];
+        v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+    }
+    return v;
+}
+constexpr int kWide = 1024;  // TPR of rows that a whole workgroup of up to 16 waves holds
+// Sums of N values over the threads of a row. Rows of several waves go through LDS, the buffers of successive sums in
+// turn so that one barrier a sum is enough; each wave adds all waves' sums.
+template <int TPR, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float (*lds)[N][16], uint32_t waves) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = lane_sum<TPR>(v[i]);
+    if constexpr (TPR == kWide) {
+        const uint32_t lane = threadIdx.x & 63;
+        if (lane == 0) {
 #pragma unroll
             for (int i = 0; i < N; i++) (*lds)[i][threadIdx.x >> 6] = v[i];
         }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            v[i] = 0.0f;
-#pragma unroll
-            for (int w = 0; w < NW; w++) v[i] += (*lds)[i][w];
+            const float q = (*lds)[i][lane & 15];
+            v[i] = lane_sum<16>((lane & 15) < waves ? q : 0.0f);
         }
     }
 }
 
+// threads of a workgroup: several narrow rows, or one wide one
 template <int TPR>
-constexpr int kBlock = TPR <= 64 ? 256 : TPR;  // rows of several waves have a workgroup each: its barriers are theirs
+constexpr int kBlock = TPR <= 64 ? 256 : TPR;
 
 template <class T, int TPR, int K, bool AL>
 __global__ __launch_bounds__(kBlock<TPR>) void norm_fwd(NormArgs g) {
-    constexpr int RPB = kBlock<TPR> / TPR, NW = TPR > 64 ? TPR / 64 : 1;
-    __shared__ float lds[2][1][NW];
-    const uint32_t lane = threadIdx.x % TPR, row = blockIdx.x * RPB + threadIdx.x / TPR;
-    const bool live = row < g.rows;  // a row past the end keeps pace with the barriers
+    __shared__ float lds[2][1][16];
+    const uint32_t tpr = TPR == kWide ? blockDim.x : TPR, waves = blockDim.x / 64;
+    const uint32_t lane = TPR == kWide ? threadIdx.x : threadIdx.x % TPR;
+    const uint32_t row = TPR == kWide ? blockIdx.x : blockIdx.x * (kBlock<TPR> / TPR) + threadIdx.x / TPR;
+    const bool live = row < g.rows;  // a row past the end keeps pace
     const int64_t group = g.gate && live ? row / g.rpg : 0;
     const float inv_c = 1.0f / (float)g.c;
-    float x[K][8], o[K][8], s[1] = {0.0f};
+    Place at[K];
+    Chunk<T> xr[K], orr[K], wp[K], ga[K], wn[K];
 #pragma unroll
     for (int k = 0; k < K; k++) {
-        const uint32_t ch = (k * TPR + lane) * 8;
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[k][i] = o[k][i] = 0.0f;
-        if (live && ch < g.c) {
-            load8<T, AL>(g.x.p, row * g.x.ld, ch, g.c, x[k]);
-            if (g.o.p) load8<T, AL>(g.o.p, row * g.o.ld, ch, g.c, o[k]);
+        at[k] = place_of<AL>(k * tpr + lane, g.c);
+        at[k].in &= live;
+        xr[k] = load8<T, AL>(g.x.p, row * g.x.ld, at[k], g.c);
+        orr[k] = Chunk<T>{};
+        if (g.o.p) {
+            orr[k] = load8<T, AL>(g.o.p, row * g.o.ld, at[k], g.c);
+            wp[k] = weight8<T, AL>(g.w_post, 0, at[k], g.c);
+            ga[k] = weight8<T, AL>(g.gate, group * g.c, at[k], g.c);
         }
+        wn[k] = weight8<T, AL>(g.w_pre, 0, at[k], g.c);
     }
+    float x[K][8], o[K][8], s[1] = {0.0f};
+#pragma unroll
+    for (int k = 0; k < K; k++) widen8<T, AL>(orr[k], at[k], o[k]);
     if (g.o.p) {
 #pragma unroll
         for (int k = 0; k < K; k++)
 #pragma unroll
             for (int i = 0; i < 8; i++) s[0] = __builtin_fmaf(o[k][i], o[k][i], s[0]);
-        row_sum<TPR, 1>(s, &lds[0]);
+        row_sum<TPR, 1>(s, &lds[0], waves);
         const float ro = __builtin_amdgcn_rsqf(__builtin_fmaf(s[0], inv_c, g.eps));
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            const uint32_t ch = (k * TPR + lane) * 8;
-            if (!live || ch >= g.c) continue;
-            float w[8], ga[8];
-            weight8<T, AL>(g.w_post, 0, ch, g.c, w);
-            weight8<T, AL>(g.gate, group * g.c, ch, g.c, ga);
+        for (int k = 0; k < K; k++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) o[k][i] *= ro * w[i] * ga[i];
-        }
+            for (int i = 0; i < 8; i++) o[k][i] *= ro * wp[k].at(i) * ga[k].at(i);
     }
     s[0] = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; k++) {
-        const uint32_t ch = (k * TPR + lane) * 8;
+        widen8<T, AL>(xr[k], at[k], x[k]);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             x[k][i] = __builtin_fmaf(g.alpha, x[k][i], o[k][i]);
             s[0] = __builtin_fmaf(x[k][i], x[k][i], s[0]);
         }
-        if (g.y.p && live && ch < g.c) store8<T, AL>(g.y.p, row * g.y.ld, ch, g.c, x[k]);
+        if (g.y.p) store8<T, AL>(g.y.p, row * g.y.ld, at[k], g.c, x[k]);
     }
     if (!g.u.p) return;
-    row_sum<TPR, 1>(s, &lds[1]);
+    row_sum<TPR, 1>(s, &lds[1], waves);
     const float ry = __builtin_amdgcn_rsqf(__builtin_fmaf(s[0], inv_c, g.eps));
 #pragma unroll
     for (int k = 0; k < K; k++) {
-        const uint32_t ch = (k * TPR + lane) * 8;
-        if (!live || ch >= g.c) continue;
-        float w[8];
-        weight8<T, AL>(g.w_pre, 0, ch, g.c, w);
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[k][i] *= ry * w[i];
-        store8<T, AL>(g.u.p, row * g.u.ld, ch, g.c, x[k]);
+        for (int i = 0; i < 8; i++) x[k][i] *= ry * wn[k].at(i);
+        store8<T, AL>(g.u.p, row * g.u.ld, at[k], g.c, x[k]);
     }
 }
 
@@ -165,144 +224,173 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_fwd(NormArgs g) {
 //     dx = alpha dY,   do = (z - n_o mean(z n_o)) / rms(o)
 //     dgate = w_post * sum dY n_o,   dw_post = sum gate dY n_o,   dw_pre = sum du n_y
 // mean(z n_o) is linear in dY, so its sum splits into three that need only o and y; they are taken together with
-// those of y, and a row costs two exchanges in place of four.
+// those of y, and a row costs two exchanges in place of four. The next row's loads are under way while a row is worked
+// on (without that the loads' latency was half of the time).
 //
-// A workgroup (tpr threads a row, RPB rows at a time) owns the sums of its rows in registers. Where groups are long, a
-// workgroup takes a part of one group (group = part / per_group), and its dY n_o sum is a partial sum of dgate; where
-// they are short, every RPB-th group of a run of wg_groups is one slot's, which then writes dgate itself. dw_post and
-// dw_pre leave one partial row a workgroup. norm_sum adds the partial rows in their order.
-template <class T, int TPR, int K, bool AL>
-__global__ __launch_bounds__(kBlock<TPR>) void norm_bwd(NormArgs g) {
-    constexpr int RPB = kBlock<TPR> / TPR, NW = TPR > 64 ? TPR / 64 : 1;
-    __shared__ float lds1[2][1][NW];
-    __shared__ float lds5[2][5][NW];
+// A workgroup (one wide row or RPB narrow ones at a time) owns the sums of its rows in registers. PARTS: groups are
+// long, a workgroup takes a part of one group (group = part / per_group), and its dY n_o sum is a partial sum of dgate
+// and, times the gate, of dw_post. Otherwise every RPB-th group of a run of wg_groups is one slot's, which writes dgate
+// itself and leaves a partial sum of dw_post. norm_sum adds the partial rows in their order.
+// waves a SIMD that the registers are held to; the narrow rows' larger variants spill at 4
+template <int TPR, int ELEM, bool PARTS>
+constexpr int kWaves = TPR == kWide || (PARTS && ELEM == 2) ? 4 : 3;
+
+template <class T, int TPR, int K, bool AL, bool PARTS>
+__global__ __launch_bounds__(kBlock<TPR>, (kWaves<TPR, sizeof(typename T::Raw), PARTS>)) void norm_bwd(NormArgs g) {
+    constexpr int RPB = kBlock<TPR> / TPR;
+    __shared__ float lds1[2][1][16];
+    __shared__ float lds5[2][5][16];
     __shared__ float fold[RPB > 1 ? RPB * TPR * 8 : 1];
-    const uint32_t lane = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+    const uint32_t tpr = TPR == kWide ? blockDim.x : TPR, waves = blockDim.x / 64;
+    const uint32_t lane = TPR == kWide ? threadIdx.x : threadIdx.x % TPR;
+    const uint32_t slot = TPR == kWide ? 0 : threadIdx.x / TPR;
     const float inv_c = 1.0f / (float)g.c;
     const bool has_o = g.o.p != nullptr;
-    float wp[K][8], wn[K][8], q[K][8], post[K][8], pre[K][8];
+    // the groups and rows of this slot: group gr, gr + gstep, ... below g1; rows r, r + rstep, ... below hi of each
+    uint32_t gr, g1, r, lo = 0, hi;
+    constexpr uint32_t gstep = RPB, rstep = PARTS ? RPB : 1;
+    auto rows_of = [&](uint32_t group) {
+        const uint64_t base = (uint64_t)group * g.rpg;
+        return (uint32_t)min((uint64_t)g.rpg, g.rows - base);
+    };
+    if constexpr (PARTS) {
+        gr = blockIdx.x / g.per_group, g1 = gr + 1;
+        const uint32_t part = blockIdx.x - gr * g.per_group;
+        lo = part * g.part_rows, hi = min(lo + g.part_rows, rows_of(gr));
+        lo += slot;
+    } else {
+        gr = blockIdx.x * g.wg_groups + slot, g1 = min((blockIdx.x + 1) * g.wg_groups, g.groups);
+        hi = gr < g1 ? rows_of(gr) : 0;
+    }
+    r = lo;
+    bool more = gr < g1 && r < hi;
+
+    Place at[K];
+    float wn[K][8], gw[K][8], q[K][8], pre[K][8], post[PARTS ? 1 : K][8];
+    Chunk<T> wp[PARTS ? 1 : K], xr[K], orr[K], dyr[K], dur[K], gar[PARTS ? 1 : K];
+    auto fetch = [&](bool ok) {
+        const int64_t row = (int64_t)((uint64_t)gr * g.rpg + r);
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            Place p = at[k];
+            p.in &= ok;
+            xr[k] = load8<T, AL>(g.x.p, row * g.x.ld, p, g.c);
+            if (has_o) orr[k] = load8<T, AL>(g.o.p, row * g.o.ld, p, g.c);
+            if (g.dy.p) dyr[k] = load8<T, AL>(g.dy.p, row * g.dy.ld, p, g.c);
+            if (g.du.p) dur[k] = load8<T, AL>(g.du.p, row * g.du.ld, p, g.c);
+            if constexpr (!PARTS) gar[k] = weight8<T, AL>(g.gate, (int64_t)gr * g.c, p, g.c);
+        }
+    };
 #pragma unroll
     for (int k = 0; k < K; k++) {
-        const uint32_t ch = (k * TPR + lane) * 8;
+        at[k] = place_of<AL>(k * tpr + lane, g.c);
+        orr[k] = dyr[k] = dur[k] = Chunk<T>{};
+    }
+    fetch(more);
 #pragma unroll
-        for (int i = 0; i < 8; i++) wp[k][i] = wn[k][i] = q[k][i] = post[k][i] = pre[k][i] = 0.0f;
-        if (ch < g.c) {
-            weight8<T, AL>(g.w_post, 0, ch, g.c, wp[k]);
-            weight8<T, AL>(g.w_pre, 0, ch, g.c, wn[k]);
+    for (int k = 0; k < K; k++) {
+        const Chunk<T> pw = weight8<T, AL>(g.w_post, 0, at[k], g.c), nw = weight8<T, AL>(g.w_pre, 0, at[k], g.c);
+        widen8<T, AL>(nw, at[k], wn[k]);
+        if constexpr (PARTS) {
+            const Chunk<T> ga = weight8<T, AL>(g.gate, (int64_t)gr * g.c, at[k], g.c);
+#pragma unroll
+            for (int i = 0; i < 8; i++) gw[k][i] = pw.at(i) * ga.at(i);
+        } else {
+            wp[k] = pw;
         }
+#pragma unroll
+        for (int i = 0; i < 8; i++) q[k][i] = pre[k][i] = post[PARTS ? 0 : k][i] = 0.0f;
     }
-    // the groups and rows of this slot: group g0, g0 + gstep, ... below g1; rows r0 + slot offset, + rstep, ... of each
-    uint32_t g0, g1, gstep, first, rstep;
-    uint32_t part = 0;
-    if (g.per_group) {
-        g0 = blockIdx.x / g.per_group, g1 = g0 + 1, gstep = 1;
-        part = blockIdx.x - g0 * g.per_group;
-        first = slot, rstep = RPB;
-    } else {
-        g0 = blockIdx.x * g.wg_groups + slot, g1 = min((blockIdx.x + 1) * g.wg_groups, g.groups), gstep = RPB;
-        first = 0, rstep = 1;
-    }
-    // all slots of a workgroup make the same number of passes, so that barriers meet (rows of several waves have one
-    // slot; the passes of slots within a wave may differ, and their lane exchanges stay inside the slot)
+
     uint32_t turn = 0;
-    for (uint32_t gr = g0; gr < g1; gr += gstep) {
-        float ga[K][8];
+    while (more) {
+        const int64_t row = (int64_t)((uint64_t)gr * g.rpg + r);
+        const uint32_t group = gr;
+        float x[K][8], o[K][8], dy[K][8], du[K][8];
+        Chunk<T> ga[PARTS ? 1 : K];
+        float s1[1] = {0.0f}, s5[5] = {};
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const uint32_t ch = (k * TPR + lane) * 8;
+            widen8<T, AL>(xr[k], at[k], x[k]);
+            widen8<T, AL>(orr[k], at[k], o[k]);
+            widen8<T, AL>(dyr[k], at[k], dy[k]);
+            widen8<T, AL>(dur[k], at[k], du[k]);
+            if constexpr (!PARTS) {
+                ga[k] = gar[k];
 #pragma unroll
-            for (int i = 0; i < 8; i++) ga[k][i] = 0.0f;
-            if (ch < g.c) weight8<T, AL>(g.gate, (int64_t)gr * g.c, ch, g.c, ga[k]);
-        }
-        const uint64_t base = (uint64_t)gr * g.rpg;
-        const uint32_t in_group = (uint32_t)min((uint64_t)g.rpg, g.rows - base);
-        const uint32_t lo = g.per_group ? part * g.part_rows : 0;
-        const uint32_t hi = g.per_group ? min(lo + g.part_rows, in_group) : in_group;
-        for (uint32_t r = lo + first; r < hi; r += rstep, turn ^= 1) {
-            const int64_t row = (int64_t)(base + r);
-            float x[K][8], o[K][8], dy[K][8], dn[K][8];
-            float s1[1] = {0.0f}, s5[5] = {};
-#pragma unroll
-            for (int k = 0; k < K; k++) {
-                const uint32_t ch = (k * TPR + lane) * 8;
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[k][i] = o[k][i] = dy[k][i] = dn[k][i] = 0.0f;
-                if (ch < g.c) {
-                    load8<T, AL>(g.x.p, row * g.x.ld, ch, g.c, x[k]);
-                    if (has_o) load8<T, AL>(g.o.p, row * g.o.ld, ch, g.c, o[k]);
-                    if (g.dy.p) load8<T, AL>(g.dy.p, row * g.dy.ld, ch, g.c, dy[k]);
-                    if (g.du.p) load8<T, AL>(g.du.p, row * g.du.ld, ch, g.c, dn[k]);
-                }
-            }
-            float ro = 0.0f;
-            if (has_o) {
-#pragma unroll
-                for (int k = 0; k < K; k++)
-#pragma unroll
-                    for (int i = 0; i < 8; i++) s1[0] = __builtin_fmaf(o[k][i], o[k][i], s1[0]);
-                row_sum<TPR, 1>(s1, &lds1[turn]);
-                ro = __builtin_amdgcn_rsqf(__builtin_fmaf(s1[0], inv_c, g.eps));
-            }
-#pragma unroll
-            for (int k = 0; k < K; k++) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    o[k][i] *= ro;  // n_o
-                    const float zo = ga[k][i] * wp[k][i] * o[k][i], w = wn[k][i] * dn[k][i];
-                    x[k][i] = __builtin_fmaf(g.alpha, x[k][i], zo);  // y
-                    s5[0] = __builtin_fmaf(x[k][i], x[k][i], s5[0]);
-                    s5[1] = __builtin_fmaf(w, x[k][i], s5[1]);
-                    s5[2] = __builtin_fmaf(zo, dy[k][i], s5[2]);
-                    s5[3] = __builtin_fmaf(zo, w, s5[3]);
-                    s5[4] = __builtin_fmaf(zo, x[k][i], s5[4]);
-                }
-            }
-            row_sum<TPR, 5>(s5, &lds5[turn]);
-            const float ry = __builtin_amdgcn_rsqf(__builtin_fmaf(s5[0], inv_c, g.eps));
-            const float my = s5[1] * inv_c * ry * ry;                                      // mean(w du n_y) / rms(y)
-            const float mo = (s5[2] + ry * s5[3] - ry * my * s5[4]) * inv_c;                // mean(z n_o)
-#pragma unroll
-            for (int k = 0; k < K; k++) {
-                const uint32_t ch = (k * TPR + lane) * 8;
-                float dx[8], dv[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float ny = x[k][i] * ry;
-                    const float d = __builtin_fmaf(ry, wn[k][i] * dn[k][i], dy[k][i]) - ny * my;  // dY
-                    dx[i] = g.alpha * d;
-                    dv[i] = ro * (ga[k][i] * wp[k][i] * d - o[k][i] * mo);
-                    q[k][i] = __builtin_fmaf(d, o[k][i], q[k][i]);
-                    pre[k][i] = __builtin_fmaf(dn[k][i], ny, pre[k][i]);
-                }
-                if (ch < g.c) {
-                    store8<T, AL>(g.dx.p, row * g.dx.ld, ch, g.c, dx);
-                    if (has_o) store8<T, AL>(g.dout.p, row * g.dout.ld, ch, g.c, dv);
-                }
+                for (int i = 0; i < 8; i++) gw[k][i] = ga[k].at(i) * wp[k].at(i);
             }
         }
-        // a group (or this part of it) is done
+        r += rstep;
+        if (r >= hi) {
+            gr += gstep, r = lo;
+            more = !PARTS && gr < g1;
+            if (more) hi = rows_of(gr);
+        }
+        if (more) fetch(true);
+        float ro = 0.0f;
+        if (has_o) {
+#pragma unroll
+            for (int k = 0; k < K; k++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) s1[0] = __builtin_fmaf(o[k][i], o[k][i], s1[0]);
+            row_sum<TPR, 1>(s1, &lds1[turn], waves);
+            ro = __builtin_amdgcn_rsqf(__builtin_fmaf(s1[0], inv_c, g.eps));
+        }
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const uint32_t ch = (k * TPR + lane) * 8;
 #pragma unroll
-            for (int i = 0; i < 8; i++) post[k][i] = __builtin_fmaf(ga[k][i], q[k][i], post[k][i]);
-            if (!g.per_group) {
-                if (g.dgate && ch < g.c) {
+            for (int i = 0; i < 8; i++) {
+                o[k][i] *= ro;  // n_o
+                const float zo = gw[k][i] * o[k][i], w = wn[k][i] * du[k][i];
+                x[k][i] = __builtin_fmaf(g.alpha, x[k][i], zo);  // y
+                s5[0] = __builtin_fmaf(x[k][i], x[k][i], s5[0]);
+                s5[1] = __builtin_fmaf(w, x[k][i], s5[1]);
+                s5[2] = __builtin_fmaf(zo, dy[k][i], s5[2]);
+                s5[3] = __builtin_fmaf(zo, w, s5[3]);
+                s5[4] = __builtin_fmaf(zo, x[k][i], s5[4]);
+            }
+        }
+        row_sum<TPR, 5>(s5, &lds5[turn], waves);
+        turn ^= 1;
+        const float ry = __builtin_amdgcn_rsqf(__builtin_fmaf(s5[0], inv_c, g.eps));
+        const float my = s5[1] * inv_c * ry * ry;                          // mean(w_pre du n_y) / rms(y)
+        const float mo = (s5[2] + ry * s5[3] - ry * my * s5[4]) * inv_c;    // mean(z n_o)
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (ch + i < g.c) g.dgate[(uint64_t)gr * g.c + ch + i] = wp[k][i] * q[k][i];
+        for (int k = 0; k < K; k++) {
+            float dx[8], dv[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float ny = x[k][i] * ry;
+                const float d = __builtin_fmaf(-my, ny, __builtin_fmaf(ry, wn[k][i] * du[k][i], dy[k][i]));  // dY
+                dx[i] = g.alpha * d;
+                dv[i] = ro * __builtin_fmaf(-mo, o[k][i], gw[k][i] * d);
+                q[k][i] = __builtin_fmaf(d, o[k][i], q[k][i]);
+                pre[k][i] = __builtin_fmaf(du[k][i], ny, pre[k][i]);
+            }
+            store8<T, AL>(g.dx.p, row * g.dx.ld, at[k], g.c, dx);
+            if (has_o) store8<T, AL>(g.dout.p, row * g.dout.ld, at[k], g.c, dv);
+        }
+        if constexpr (!PARTS) {
+            if (gr != group) {  // the group is done
+#pragma unroll
+                for (int k = 0; k < K; k++) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        post[k][i] = __builtin_fmaf(ga[k].at(i), q[k][i], post[k][i]);
+                        if (g.dgate && at[k].in && i >= (int)at[k].skip && at[k].ch + i < g.c)
+                            g.dgate[(uint64_t)group * g.c + at[k].ch + i] = wp[k].at(i) * q[k][i];
+                        q[k][i] = 0.0f;
+                    }
                 }
-#pragma unroll
-                for (int i = 0; i < 8; i++) q[k][i] = 0.0f;
             }
         }
     }
     // the slots' sums of one workgroup, added in the slots' order by slot 0
-    auto leave = [&](float (&v)[K][8], float* out) {
+    auto leave = [&](float (*v)[8], float* out) {
         if (!out) return;
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const uint32_t ch = (k * TPR + lane) * 8;
             if constexpr (RPB > 1) {
                 __syncthreads();
 #pragma unroll
@@ -316,39 +404,69 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd(NormArgs g) {
                     }
                 }
             }
-            if (slot == 0 && ch < g.c) {
+            if (slot == 0 && at[k].in) {
 #pragma unroll
                 for (int i = 0; i < 8; i++)
-                    if (ch + i < g.c) out[(uint64_t)blockIdx.x * g.c + ch + i] = v[k][i];
+                    if (i >= (int)at[k].skip && at[k].ch + i < g.c)
+                        out[(uint64_t)blockIdx.x * g.c + at[k].ch + i] = v[k][i];
             }
         }
     };
     leave(pre, g.part_pre);
-    leave(post, g.part_post);
-    leave(q, g.part_gate);
+    leave(PARTS ? q : post, g.part_post);
 }
 
-// out[group][ch] = scale[ch] * the sum of `parts` partial rows of the group; 64 columns x 16 row lanes a workgroup
+// The partial rows' sums, 16 columns x 64 row lanes a workgroup, in f64. z 0: dw_pre, the sum of all `wgs` rows of
+// `pre`. z 1: the sum Q of `parts` rows of `post` for each group; dgate = w_post * Q, dw_post = the sum of gate * Q over
+// the groups. The 64 lanes are as many groups as there are (up to 64) times the lanes that are left for a group's parts.
 template <class T>
-__global__ __launch_bounds__(1024) void norm_sum(const float* a, float* out_a, const float* b, float* out_b,
-                                                 uint32_t parts, uint32_t c, const void* scale) {
-    __shared__ double s[16][64];
-    const uint32_t ch = blockIdx.x * 64 + (threadIdx.x & 63), y = threadIdx.x >> 6;
-    const float* part = blockIdx.z ? b : a;
-    float* out = blockIdx.z ? out_b : out_a;
-    if (!out) return;
-    double acc = 0.0;
-    if (ch < c) {
+__global__ __launch_bounds__(1024) void norm_sum(const float* pre, float* dw_pre, uint32_t wgs, const float* post,
+                                                 float* dw_post, float* dgate, const void* gate, const void* w_post,
+                                                 uint32_t groups, uint32_t parts, uint32_t part_lanes, uint32_t c) {
+    __shared__ double s[64][17];
+    using R = typename T::Raw;
+    const uint32_t x = threadIdx.x & 15, y = threadIdx.x >> 4, ch = blockIdx.x * 16 + x;
+    const bool first = blockIdx.z == 0;
+    if (first ? !dw_pre : !post) return;
+    const float* in = first ? pre : post;
+    const uint32_t rows = first ? wgs : parts, pl = first ? 64 : part_lanes, p = y % pl, gl = 64 / pl;
+    const uint32_t n = first ? 1 : groups;
+    double total = 0.0;
+    for (uint32_t g0 = 0; g0 < n; g0 += gl) {
+        const uint32_t g = g0 + y / pl;
+        double acc = 0.0;
+        if (ch < c && g < n) {
 #pragma unroll 8
-        for (uint32_t r = y; r < parts; r += 16) acc += (double)part[((uint64_t)blockIdx.y * parts + r) * c + ch];
+            for (uint32_t r = p; r < rows; r += pl) acc += (double)in[((uint64_t)g * rows + r) * c + ch];
+        }
+        if (pl > 1) {
+            __syncthreads();
+            s[y][x] = acc;
+            __syncthreads();
+            if (p == 0) {
+                for (uint32_t k = 1; k < pl; k++) acc += s[y + k][x];
+            }
+        }
+        if (p == 0 && ch < c && g < n) {
+            if (first) {
+                total = acc;
+            } else {
+                if (dgate) {
+                    const double w = w_post ? (double)widen(T{}, reinterpret_cast<const R*>(w_post)[ch]) : 1.0;
+                    dgate[(uint64_t)g * c + ch] = (float)(acc * w);
+                }
+                total += gate ? acc * (double)widen(T{}, reinterpret_cast<const R*>(gate)[(uint64_t)g * c + ch]) : acc;
+            }
+        }
     }
-    s[y][threadIdx.x & 63] = acc;
+    float* out = first ? dw_pre : dw_post;
+    if (!out) return;
+    __syncthreads();
+    s[y][x] = total;  // 0 in lanes that are not a group's first
     __syncthreads();
     if (y == 0 && ch < c) {
-#pragma unroll
-        for (int k = 1; k < 16; k++) acc += s[k][threadIdx.x];
-        if (scale) acc *= (double)widen(T{}, reinterpret_cast<const typename T::Raw*>(scale)[ch]);
-        out[(uint64_t)blockIdx.y * c + ch] = (float)acc;
+        for (uint32_t k = pl; k < 64; k += pl) total += s[k][x];
+        out[ch] = (float)total;
     }
 }
 
@@ -385,10 +503,11 @@ bool whole(const fhc_norm_desc* n, std::initializer_list<const fhc_rows*> all) {
     return true;
 }
 
-uint32_t threads_of_row(uint32_t c) {  // 8 channels a thread, 16 a thread above 8192
-    uint32_t t = 16;
-    while (t < 1024 && t * 8 < c) t *= 2;
-    return t;
+// threads of a row, 8 channels each, 16 each above 8192: a part of a wave, or whole waves
+uint32_t threads_of_row(uint32_t c) {
+    if (c <= 128) return 16;
+    if (c <= 256) return 32;
+    return (uint32_t)ceil_div(c, c > 8192 ? 1024 : 512) * 64;
 }
 
 // f(T, TPR, K, AL)
@@ -400,11 +519,8 @@ void with_shape(uint32_t dtype, uint32_t tpr, uint32_t c, bool al, F&& f) {
     };
     auto by_rows = [&](auto t) {
         using std::integral_constant;
-        if (c > 8192) by_al(t, integral_constant<int, 1024>{}, integral_constant<int, 2>{});
-        else if (tpr == 1024) by_al(t, integral_constant<int, 1024>{}, integral_constant<int, 1>{});
-        else if (tpr == 512) by_al(t, integral_constant<int, 512>{}, integral_constant<int, 1>{});
-        else if (tpr == 256) by_al(t, integral_constant<int, 256>{}, integral_constant<int, 1>{});
-        else if (tpr == 128) by_al(t, integral_constant<int, 128>{}, integral_constant<int, 1>{});
+        if (c > 8192) by_al(t, integral_constant<int, kWide>{}, integral_constant<int, 2>{});
+        else if (tpr > 64) by_al(t, integral_constant<int, kWide>{}, integral_constant<int, 1>{});
         else if (tpr == 64) by_al(t, integral_constant<int, 64>{}, integral_constant<int, 1>{});
         else if (tpr == 32) by_al(t, integral_constant<int, 32>{}, integral_constant<int, 1>{});
         else by_al(t, integral_constant<int, 16>{}, integral_constant<int, 1>{});
@@ -415,23 +531,25 @@ void with_shape(uint32_t dtype, uint32_t tpr, uint32_t c, bool al, F&& f) {
 }
 
 struct Split {
-    uint32_t tpr, rpb, groups, rpg, per_group, part_rows, wg_groups, wgs;
-    size_t pre_at, post_at, gate_at, bytes;
+    uint32_t tpr, rpb, block, groups, rpg, per_group, part_rows, wg_groups, wgs;
+    size_t post_at, bytes;
 };
-// The backward pass's workgroups: about 4 rounds of 1024 threads a CU, at least 4 rows a slot where there are so many.
-// Groups of at least 4 passes are cut into parts; shorter ones are taken whole.
+// The backward pass's workgroups: as many as its registers let the CUs hold at once, at least 4 rows a slot where there
+// are so many. Groups of at least 4 passes are cut into parts; shorter ones are taken whole.
 Split split_of(const fhc_norm_desc* n) {
     Split s{};
     s.tpr = threads_of_row(n->c);
-    const uint32_t block = s.tpr <= 64 ? 256 : s.tpr;
-    s.rpb = block / s.tpr;
+    s.block = s.tpr <= 64 ? 256 : s.tpr;
+    s.rpb = s.block / s.tpr;
     s.rpg = n->gate ? n->rows_per_group : n->rows;
     if (s.rpg > n->rows) s.rpg = n->rows;
     if (s.rpg == 0) s.rpg = 1;
     s.groups = (uint32_t)ceil_div(n->rows, s.rpg);
-    const uint32_t most = 256 * 1024 / block;
-    if (s.groups && s.rpg >= 4 * s.rpb) {
-        uint64_t per = ceil_div(most, s.groups);
+    const bool parts = s.groups && s.rpg >= 4 * s.rpb;
+    const uint32_t waves = s.tpr > 64 || (parts && n->dtype != FHC_F32) ? 16 : 12;  // a CU's, see kWaves
+    const uint32_t most = 256 * (waves * 64 / s.block);
+    if (parts) {
+        uint64_t per = s.groups >= most ? 1 : most / s.groups;
         const uint64_t cap = ceil_div(s.rpg, 4 * s.rpb);
         if (per > cap) per = cap;
         s.part_rows = (uint32_t)ceil_div(s.rpg, per);
@@ -441,9 +559,8 @@ Split split_of(const fhc_norm_desc* n) {
         s.wg_groups = (uint32_t)ceil_div(ceil_div(s.groups, most), s.rpb) * s.rpb;
         s.wgs = s.groups ? (uint32_t)ceil_div(s.groups, s.wg_groups) : 0;
     }
-    const size_t one = (size_t)ceil_div((uint64_t)s.wgs * n->c * 4, 256) * 256;
-    s.pre_at = 0, s.post_at = one, s.gate_at = 2 * one;
-    s.bytes = (s.per_group ? 3 : 2) * one;
+    s.post_at = (size_t)ceil_div((uint64_t)s.wgs * n->c * 4, 256) * 256;
+    s.bytes = 2 * s.post_at;
     return s;
 }
 
@@ -473,9 +590,10 @@ extern "C" int fhc_norm_block(const fhc_norm_desc* n, const fhc_rows* x, const f
         a.rows = n->rows, a.c = n->c, a.rpg = n->rows_per_group, a.alpha = n->alpha, a.eps = n->eps;
         const uint32_t tpr = threads_of_row(n->c);
         with_shape(n->dtype, tpr, n->c, whole(n, {x, o, y, u}), [&](auto t, auto w, auto k, auto al) {
-            constexpr int TPR = decltype(w)::value, block = kBlock<TPR>;
+            constexpr int TPR = decltype(w)::value;
+            const uint32_t block = TPR == kWide ? tpr : kBlock<TPR>;
             hipLaunchKernelGGL((norm_fwd<decltype(t), TPR, decltype(k)::value, decltype(al)::value>),
-                               dim3((uint32_t)ceil_div(n->rows, block / TPR)), dim3(block), 0, (hipStream_t)stream, a);
+                               dim3((uint32_t)ceil_div(n->rows, block / tpr)), dim3(block), 0, (hipStream_t)stream, a);
         });
         return launched(op);
     });
@@ -520,33 +638,33 @@ extern "C" int fhc_norm_block_backward(const fhc_norm_desc* n, const fhc_rows* x
         a.rows = n->rows, a.c = n->c, a.rpg = s.rpg, a.groups = s.groups, a.alpha = n->alpha, a.eps = n->eps;
         a.per_group = s.per_group, a.part_rows = s.part_rows, a.wg_groups = s.wg_groups;
         a.dgate = dgate;
-        a.part_pre = dw_pre ? reinterpret_cast<float*>(w + s.pre_at) : nullptr;
-        a.part_post = dw_post ? reinterpret_cast<float*>(w + s.post_at) : nullptr;
-        a.part_gate = dgate && s.per_group ? reinterpret_cast<float*>(w + s.gate_at) : nullptr;
+        const bool parts = s.per_group != 0;
+        a.part_pre = dw_pre ? reinterpret_cast<float*>(w) : nullptr;
+        a.part_post = dw_post || (dgate && parts) ? reinterpret_cast<float*>(w + s.post_at) : nullptr;
         const hipStream_t st = (hipStream_t)stream;
         if (s.wgs) {
             with_shape(n->dtype, s.tpr, n->c, whole(n, {x, o, dy, du, dx, dout}), [&](auto t, auto tpr, auto k, auto al) {
-                constexpr int TPR = decltype(tpr)::value, block = kBlock<TPR>;
-                hipLaunchKernelGGL((norm_bwd<decltype(t), TPR, decltype(k)::value, decltype(al)::value>), dim3(s.wgs),
-                                   dim3(block), 0, st, a);
+                constexpr int TPR = decltype(tpr)::value, K = decltype(k)::value;
+                using T = decltype(t);
+                if (parts)
+                    hipLaunchKernelGGL((norm_bwd<T, TPR, K, decltype(al)::value, true>), dim3(s.wgs), dim3(s.block), 0, st, a);
+                else
+                    hipLaunchKernelGGL((norm_bwd<T, TPR, K, decltype(al)::value, false>), dim3(s.wgs), dim3(s.block), 0, st, a);
             });
             FHC_TRY(launched(op));
         }
-        const uint32_t blocks = (uint32_t)ceil_div(n->c, 64);
-        if (dw_pre || dw_post) {
-            hipLaunchKernelGGL((norm_sum<F32>), dim3(blocks, 1, 2), dim3(1024), 0, st, a.part_pre, dw_pre, a.part_post,
-                               dw_post, s.wgs, n->c, (const void*)nullptr);
-            FHC_TRY(launched(op));
-        }
-        if (a.part_gate && s.groups) {
+        if (dw_pre || dw_post || (dgate && parts)) {
+            // of whole groups, dgate is written, and what is left for dw_post is one sum of all rows
+            const uint32_t groups = parts ? s.groups : 1, rows = parts ? s.per_group : s.wgs;
+            uint32_t lanes = 64;
+            while (lanes > 1 && (uint64_t)lanes * groups > 64) lanes /= 2;
             auto sum = n->dtype == FHC_F16 ? norm_sum<F16> : n->dtype == FHC_BF16 ? norm_sum<BF16> : norm_sum<F32>;
-            for (uint32_t g = 0; g < s.groups; g += 65535) {  // the grid's limit
-                const uint32_t m = s.groups - g < 65535 ? s.groups - g : 65535;
-                hipLaunchKernelGGL(sum, dim3(blocks, m, 1), dim3(1024), 0, st,
-                                   a.part_gate + (uint64_t)g * s.per_group * n->c, dgate + (uint64_t)g * n->c,
-                                   (const float*)nullptr, (float*)nullptr, s.per_group, n->c, n->w_post);
-                FHC_TRY(launched(op));
-            }
+            // without rows there are no partial sums, but dw_post is still written: any pointer will do
+            const float* post = a.part_post || !dw_post ? a.part_post : dw_post;
+            hipLaunchKernelGGL(sum, dim3((uint32_t)ceil_div(n->c, 16), 1, 2), dim3(1024), 0, st, a.part_pre, dw_pre,
+                               s.wgs, post, dw_post, parts ? dgate : nullptr, parts ? n->gate : nullptr, n->w_post,
+                               groups, rows, lanes, n->c);
+            FHC_TRY(launched(op));
         }
         return 0;
     });
