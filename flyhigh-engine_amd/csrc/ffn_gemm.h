@@ -4,19 +4,21 @@
 // out[m][n] = sum over k of A(m, k) B(n, k). An operand is stored either with k adjacent ("rows": A's row m at
 // a + m * ld) or with m (n) adjacent ("columns": A's column k at a + k * ld), so no product needs a transposed copy.
 //
-// - A workgroup computes a BM x BN tile, wave (wm, wn) a 16 MB x 64 part of it, K in slabs of 64. Both operands' slabs
-//   go from global memory straight into LDS (LDS DMA, 16 bytes a lane), two buffers in turn: slab s + 1 loads while
-//   slab s computes, one barrier a slab.
-// - Rows: an LDS row holds 64 k (128 bytes), its 16-byte chunk c at position c ^ (row & 7), so that the 16 rows of a
-//   fragment read (16 bytes a lane) spread over all banks. Columns: an LDS row holds the tile's m (n) of one k, its
+// - A workgroup of 2 x 2 waves computes a BM x BN tile, a wave 16 MB x 16 NB of it, K in slabs of 32. Both operands'
+//   slabs go from global memory straight into LDS (LDS DMA, 16 bytes a lane), three buffers in turn: slabs s + 1 and
+//   s + 2 are on their way while slab s computes, one barrier a slab. Two workgroups share a CU (the larger tile's
+//   accumulators take half of a SIMD's registers), so one's epilogue and waits lie under the other's products.
+// - Rows: an LDS row holds 32 k (64 bytes), its 16-byte chunk c at position c ^ (row >> 2 & 2): a fragment read (16
+//   bytes a lane) goes by lanes 0-3, 12-15, 20-23, 24-27 and the like, 16 at once, which so fall on all 64 banks (other
+//   permutations of the chunks, by row >> 2 or by 8 neighbours, measured a conflict for every read). Columns: an LDS row holds the tile's m (n) of one k, its
 //   32-byte blocks permuted by f(k) = k & 3 | (k >> 3 & 1) << 2; fragments come from the transposing LDS read (16 lanes
 //   read 4 k x 16 m and receive 4 k of one m each), whose 32 lanes at once then spread over all banks too.
 // - The MFMA takes B's fragment as its first operand: a lane's 4 results are 4 adjacent n of one m.
 // - Workgroups go round-robin to the 8 XCDs, each with its own L2: the tile index is permuted so that an XCD works on
 //   neighbouring tiles, in groups of 8 tile rows.
-// - DMA needs 4-byte aligned chunks: even widths and strides. Odd ones go through registers (element-aligned loads).
-// - Past an operand's end the buffer's range check gives zeros; a k group of 8 that the end of K cuts is zeroed in LDS
-//   (both operands: what lies past a row's end may be anything, NaN included).
+// - DMA needs 4-byte aligned chunks, and a rows operand's K a multiple of 8 or padded to one with zeros. What the caller
+//   gives otherwise is copied into such a form first (ffn_pack). Past an operand's end the buffer's range check gives
+//   zeros.
 #pragma once
 #include "seq_common.h"
 #include "wave_impl.h"
@@ -46,9 +48,10 @@ struct GemmArgs {
     const uint16_t *a0, *a1, *b0, *b1;
     int64_t lda, ldb;
     int m, n, k;        // kGlu: n is the features, each a gate row of b0 and an up row of b1
+    int wide_m, wide_n;  // what a column operand's rows hold: m (n), or its padding too
     int segments;       // 2: a0 b0 and then a1 b1 along K (kStore, kPart)
     int pairs;          // 2: a0 -> o0 and a1 -> o1, both with b0 (kStore, kPart)
-    int slabs, per_split, splits;  // slabs of 64 over all segments, an even number of each; per_split even
+    int slabs, per_split, splits;  // slabs of 32 over all segments
     int tiles_m, tiles_n;
     uint16_t *o0, *o1;
     int64_t ldo;
@@ -72,24 +75,10 @@ __device__ __forceinline__ void act_grad(uint32_t act, float v, float& value, fl
     const bool silu = act == FHC_ACT_SILU;
     const float k = silu ? v : v * __builtin_fmaf(kGelu3 * v, v, kGelu1);
     const float dk = silu ? 1.0f : __builtin_fmaf(3.0f * kGelu3 * v, v, kGelu1);
-    const float p = sigmoid_of(k), q = sigmoid_of(-k);
+    const float e = __builtin_amdgcn_exp2f(k * -1.44269504088896340736f), p = __builtin_amdgcn_rcpf(1.0f + e);
+    const float q = __builtin_fminf(e * p, 1.0f);  // 1 - p; inf * 0 where e overflows
     value = v * p;
     slope = p * __builtin_fmaf(v * dk, q, 1.0f);
-}
-
-// up to 8 elements at p, `valid` of them inside
-__device__ __forceinline__ u4_t load_some(const uint16_t* p, int valid) {
-    if (valid >= 8) {
-        uint16_t q[8];
-        load_raw<uint16_t, 8, false>(p, q);
-        u4_t r;
-#pragma unroll
-        for (int i = 0; i < 4; i++) r[i] = q[2 * i] | (uint32_t)q[2 * i + 1] << 16;
-        return r;
-    }
-    u4_t r = {0, 0, 0, 0};
-    for (int i = 0; i < valid; i++) r[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
-    return r;
 }
 
 __device__ __forceinline__ void store4(uint16_t* p, int valid, const uint16_t (&q)[4]) {
@@ -100,12 +89,14 @@ __device__ __forceinline__ void store4(uint16_t* p, int valid, const uint16_t (&
     }
 }
 
-// One operand's part of a tile: R rows (or columns) of it, a slab of 64 k in LDS, 1 KB (one DMA instruction) per 8 rows
-// of 128 bytes, or per 512 / R columns.
+// One operand's part of a tile: R rows (or columns) of it, a slab of 32 k in LDS, 1 KB (one DMA instruction) per 16 rows
+// of 64 bytes, or per 512 / R columns.
 template <bool COLS, int R, int NW>
 struct Operand {
-    static constexpr int NI = R * 128 / 1024 / NW;  // DMA instructions a wave
-    static constexpr int CPI = 512 / R;             // COLS: k of an instruction
+    static constexpr int NI = R * 64 / 1024 / NW;  // DMA instructions a wave
+    static constexpr int CPI = 512 / R;            // COLS: k of an instruction
+    static constexpr int U4 = R * 4;               // 16-byte units of a slab
+    static __device__ __forceinline__ int turn(int row) { return row >> 2 & 2; }
     // the k and the first m (n) of lane `lane`'s 16 bytes of instruction q, relative to the tile and slab
     static __device__ __forceinline__ void place(int inst, int lane, int& r, int& k) {
         if constexpr (COLS) {
@@ -114,22 +105,25 @@ struct Operand {
             const int f = (k & 3) | (k >> 3 & 1) << 2;
             r = (((pos >> 1) ^ f) << 4) + ((pos & 1) << 3);
         } else {
-            r = inst * 8 + (lane >> 3);
-            k = ((lane & 7) ^ (lane >> 3)) * 8;
+            r = inst * 16 + (lane >> 2);
+            k = ((lane & 3) ^ turn(r)) * 8;
         }
     }
-    // the fragment of rows base .. base + 15, k step ks of 32: lane l has row l & 15, k 8 (l >> 4) .. + 7
-    static __device__ __forceinline__ u4_t frag(const uint4* lds, int base, int ks, int lane) {
+    // the fragment of rows base .. base + 15: lane l has row l & 15, k 8 (l >> 4) .. + 7
+    static __device__ __forceinline__ u4_t frag(const uint4* lds, int base, int lane) {
         const char* p = reinterpret_cast<const char*>(lds);
         if constexpr (COLS) {
             const int j = (lane & 15) >> 2, g = lane >> 4;
             const int f = j | (g & 1) << 2;
-            [[maybe_unused]] const char* at =
-                p + (ks * 32 + g * 8 + j) * (R * 2) + (((base >> 4) ^ f) << 5) + (lane & 3) * 8;
+            // Each address one opaque offset from the buffer: of a sum with a constant the compiler makes a chain, behind
+            // which it no longer knows the buffer that is read, and it then waits for the DMA of all.
+            [[maybe_unused]] int lo_at = (g * 8 + j) * (R * 2) + (((base >> 4) ^ f) << 5) + (lane & 3) * 8;
+            [[maybe_unused]] int hi_at = lo_at + 4 * (R * 2);
+            asm("" : "+v"(hi_at));
 #if defined(__HIP_DEVICE_COMPILE__)
             typedef __attribute__((address_space(3))) s4_t* lds_s4;
-            const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)at);
-            const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at + 4 * (R * 2)));
+            const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + lo_at));
+            const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + hi_at));
             typedef short s8_t __attribute__((ext_vector_type(8)));
             return __builtin_bit_cast(u4_t, (s8_t)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 #else
@@ -137,22 +131,38 @@ struct Operand {
 #endif
         } else {
             const int row = base + (lane & 15);
-            return *reinterpret_cast<const u4_t*>(p + row * 128 + (((ks * 4 + (lane >> 4)) ^ (lane & 7)) << 4));
+            return *reinterpret_cast<const u4_t*>(p + row * 64 + (((lane >> 4) ^ turn(row)) << 4));
         }
     }
 };
 
 constexpr uint32_t kFar = 0x80000000u;  // an offset out of every buffer's range
 
-// WM x WN waves of 16 MB x 64; GLU interleaves B's tile by waves: 32 gate rows, then the same features' 32 up rows
-template <class T, bool AC, bool BC, Epi E, int MB, int WM, int WN, bool DMA>
-__global__ __launch_bounds__(64 * WM * WN) void ffn_gemm(GemmArgs g) {
-    constexpr int NW = WM * WN, BM = 16 * MB * WM, BN = 64 * WN;
-    constexpr int FN = E == kGlu ? BN / 2 : BN;  // features of a tile
+__host__ __device__ constexpr int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
+template <class P>
+__device__ __forceinline__ P* uniform(P* p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return reinterpret_cast<P*>((uint64_t)hi << 32 | lo);
+}
+// waits until at most N of the wave's vector memory operations are under way, and its LDS reads have arrived
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);
+}
+
+// WM x WN waves of 16 MB x 16 NB; GLU interleaves B's tile by waves: 8 NB gate rows, then the same features' up rows
+template <class T, bool AC, bool BC, Epi E, int MB, int NB, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void ffn_gemm(GemmArgs g) {
+    constexpr int NW = WM * WN, BM = 16 * MB * WM, BN = 16 * NB * WN;
+    constexpr int FW = E == kGlu ? 8 * NB : 16 * NB, FN = FW * WN;  // features of a wave, of a tile
     using OA = Operand<AC, BM, NW>;
     using OB = Operand<BC, BN, NW>;
+    constexpr int NI = OA::NI + OB::NI;
+    constexpr bool TURNS = NW == 8;
     // one object per buffer: the compiler's wait for a DMA then covers only reads of the buffer it fills
-    __shared__ __align__(1024) uint4 as0[BM * 8], as1[BM * 8], bs0[BN * 8], bs1[BN * 8];
+    __shared__ __align__(1024) uint4 as0[OA::U4], bs0[OB::U4], as1[OA::U4], bs1[OB::U4], as2[OA::U4], bs2[OB::U4];
+    __shared__ __align__(1024) uint4 as3[TURNS ? OA::U4 : 1], bs3[TURNS ? OB::U4 : 1];
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -172,174 +182,212 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm(GemmArgs g) {
 
     // per-lane offsets of the DMA (bytes from the tile's first element), and k within the slab of a row's chunk
     uint32_t offa[OA::NI], offb[OB::NI];
-    int ka[OA::NI], kb[OB::NI], ra[OA::NI], rb[OB::NI];
+    int ka[OA::NI], kb[OB::NI];
 #pragma unroll
     for (int q = 0; q < OA::NI; q++) {
-        OA::place(wave * OA::NI + q, lane, ra[q], ka[q]);
-        offa[q] = (uint32_t)(AC ? ka[q] * (int)g.lda + ra[q] : ra[q] * (int)g.lda + ka[q]) * 2u;
+        int r;
+        OA::place(wave * OA::NI + q, lane, r, ka[q]);
+        offa[q] = (uint32_t)(AC ? ka[q] * (int)g.lda + r : r * (int)g.lda + ka[q]) * 2u;
     }
 #pragma unroll
     for (int q = 0; q < OB::NI; q++) {
-        OB::place(wave * OB::NI + q, lane, rb[q], kb[q]);
-        if constexpr (E == kGlu) rb[q] = (rb[q] >> 6) * 32 + (rb[q] & 31);  // the feature; gate or up is the wave's
-        offb[q] = (uint32_t)(BC ? kb[q] * (int)g.ldb + rb[q] : rb[q] * (int)g.ldb + kb[q]) * 2u;
+        int r;
+        OB::place(wave * OB::NI + q, lane, r, kb[q]);
+        if constexpr (E == kGlu) r = r / (2 * FW) * FW + r % FW;  // the feature; gate or up is the instruction's
+        offb[q] = (uint32_t)(BC ? kb[q] * (int)g.ldb + r : r * (int)g.ldb + kb[q]) * 2u;
     }
 
-    auto range = [](int64_t bytes) { return (int)(bytes < 0 ? 0 : bytes > 0x7FFFFFFF ? 0x7FFFFFFF : bytes); };
-    u4_t rega[DMA ? 1 : OA::NI], regb[DMA ? 1 : OB::NI];
-    // starts slab s's way into the buffers (into registers on the odd path)
-    auto fetch = [&](int s, uint4* la, uint4* lb) {
-        const int seg = s >= seg_slabs ? 1 : 0;
-        const int k0 = (s - seg * seg_slabs) * 64;
-        const uint16_t* a = seg + pair ? g.a1 : g.a0;
-        const uint16_t* b = seg ? g.b1 : g.b0;
-        if constexpr (DMA) {
-            const int64_t ea = AC ? (int64_t)k0 * g.lda + m0 : (int64_t)m0 * g.lda;
-            const int64_t eb = BC ? (int64_t)k0 * g.ldb + n0 : (int64_t)n0 * g.ldb;
-            const int64_t enda = AC ? (int64_t)(g.k - 1) * g.lda + g.m : (int64_t)(g.m - 1) * g.lda + g.k;
-            const int64_t endb = BC ? (int64_t)(g.k - 1) * g.ldb + g.n : (int64_t)(g.n - 1) * g.ldb + g.k;
-            const auto rsa = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a + ea), (short)0,
-                                                               range((enda - ea) * 2), 0x00020000);
-            const auto rsb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(b + eb), (short)0,
-                                                               range((endb - eb) * 2), 0x00020000);
-            const auto rsu = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<uint16_t*>((E == kGlu ? g.b1 : b) + eb), (short)0, range((endb - eb) * 2), 0x00020000);
-#pragma unroll
-            for (int q = 0; q < OA::NI; q++) {
-                uint32_t off = offa[q];
-                if constexpr (!AC) off = k0 + ka[q] < g.k ? off + 2u * k0 : kFar;
-                lds_dma16(rsa, la + (wave * OA::NI + q) * 64, off);
-            }
-#pragma unroll
-            for (int q = 0; q < OB::NI; q++) {
-                const int inst = wave * OB::NI + q;
-                uint32_t off = offb[q];
-                if constexpr (!BC) off = k0 + kb[q] < g.k ? off + 2u * k0 : kFar;
-                lds_dma16(E == kGlu && (inst & 4) ? rsu : rsb, lb + inst * 64, off);
-            }
-        } else {
-#pragma unroll
-            for (int q = 0; q < OA::NI; q++) {
-                const int r = m0 + ra[q], k = k0 + ka[q];
-                const int valid = AC ? (k < g.k ? g.m - r : 0) : (r < g.m ? g.k - k : 0);
-                rega[q] = load_some(a + (AC ? (int64_t)k * g.lda + r : (int64_t)r * g.lda + k), valid);
-            }
-#pragma unroll
-            for (int q = 0; q < OB::NI; q++) {
-                const int r = n0 + rb[q], k = k0 + kb[q];
-                const int valid = BC ? (k < g.k ? g.n - r : 0) : (r < g.n ? g.k - k : 0);
-                const uint16_t* p = E == kGlu && (wave * OB::NI + q & 4) ? g.b1 : b;
-                regb[q] = load_some(p + (BC ? (int64_t)k * g.ldb + r : (int64_t)r * g.ldb + k), valid);
-            }
-        }
+    // The fetches run through the slabs in order. Of each operand: the address of the tile's part of the next slab, and
+    // the bytes from there to its end, behind which the range check gives zeros.
+    const int64_t step_a = (AC ? 32 * g.lda : 32) * 2, step_b = (BC ? 32 * g.ldb : 32) * 2;
+    const char *pa, *pb, *pu;
+    int64_t ra, rb;
+    int kleft, switch_at = g.segments > 1 && s0 < seg_slabs ? seg_slabs - s0 : -1;  // fetches until the second segment
+    auto start = [&](int seg, int slab) {
+        const int64_t k0 = slab * 32;
+        const int64_t ea = AC ? k0 * g.lda + m0 : m0 * g.lda + k0, eb = BC ? k0 * g.ldb + n0 : n0 * g.ldb + k0;
+        const int64_t enda = AC ? (g.k - 1) * g.lda + g.wide_m : (g.m - 1) * g.lda + up8(g.k);
+        const int64_t endb = BC ? (g.k - 1) * g.ldb + g.wide_n : (g.n - 1) * g.ldb + up8(g.k);
+        pa = uniform(reinterpret_cast<const char*>((seg + pair ? g.a1 : g.a0) + ea));
+        pb = uniform(reinterpret_cast<const char*>((seg ? g.b1 : g.b0) + eb));
+        if constexpr (E == kGlu) pu = uniform(reinterpret_cast<const char*>(g.b1 + eb));
+        ra = (enda - ea) * 2, rb = (endb - eb) * 2, kleft = g.k - (int)k0;
     };
-    auto land = [&](uint4* la, uint4* lb) {
-        if constexpr (!DMA) {
-#pragma unroll
-            for (int q = 0; q < OA::NI; q++)
-                *reinterpret_cast<u4_t*>(la + (wave * OA::NI + q) * 64 + lane) = rega[q];
-#pragma unroll
-            for (int q = 0; q < OB::NI; q++)
-                *reinterpret_cast<u4_t*>(lb + (wave * OB::NI + q) * 64 + lane) = regb[q];
-        }
+    start(g.segments > 1 && s0 >= seg_slabs, g.segments > 1 && s0 >= seg_slabs ? s0 - seg_slabs : s0);
+    auto resource = [](const char* p, int64_t bytes) {
+        const int hi = (int)(bytes >> 32), n = hi < 0 ? 0 : hi > 0 || (int)bytes < 0 ? 0x7FFFFFFF : (int)bytes;
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), (short)0, n, 0x00020000);
     };
-    // zeroes the end of the 8-group that the end of K cuts in slab s
-    auto trim = [&](int s, uint4* la, uint4* lb) {
-        if constexpr (DMA) {
-            const int left = g.k - (s >= seg_slabs ? s - seg_slabs : s) * 64;
-            if (left >= 64 || left <= 0 || !(left & 7)) return;
-            auto cut = [&](uint4* p, int rows) {
-                for (int r = tid; r < rows; r += 64 * NW) {
-                    uint16_t* e = reinterpret_cast<uint16_t*>(p + r * 8 + ((left >> 3) ^ (r & 7)));
-                    for (int i = left & 7; i < 8; i++) e[i] = 0;
-                }
-            };
-            if constexpr (!AC) cut(la, BM);
-            if constexpr (!BC) cut(lb, BN);
-            __syncthreads();
+    // starts the next slab's way into the buffers
+    auto fetch = [&](uint4* la, uint4* lb) {
+        if (switch_at-- == 0) start(1, 0);
+        const auto rsa = resource(pa, ra), rsb = resource(pb, rb), rsu = resource(E == kGlu ? pu : pb, rb);
+        const bool whole = kleft >= 32;  // else a row's chunk past the end of K lies in the next row
+#pragma unroll
+        for (int q = 0; q < OA::NI; q++)
+            lds_dma16(rsa, la + (wave * OA::NI + q) * 64, AC || whole || ka[q] < kleft ? offa[q] : kFar);
+#pragma unroll
+        for (int q = 0; q < OB::NI; q++) {
+            const int inst = wave * OB::NI + q;
+            const bool up = E == kGlu && (inst * 16 & FW);
+            lds_dma16(up ? rsu : rsb, lb + inst * 64, BC || whole || kb[q] < kleft ? offb[q] : kFar);
         }
+        pa += step_a, pb += step_b, ra -= step_a, rb -= step_b, kleft -= 32;
+        if constexpr (E == kGlu) pu += step_b;
     };
 
-    f4 acc[MB][4];
+    f4 acc[MB][NB];
 #pragma unroll
     for (int i = 0; i < MB; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    auto compute = [&](const uint4* la, const uint4* lb) {
+        for (int j = 0; j < NB; j++) acc[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    u4_t fb[NB], fa[MB];
+    auto read = [&](const uint4* la, const uint4* lb) {
+        int at = lane;
 #pragma unroll
-        for (int ks = 0; ks < 2; ks++) {
-            u4_t fb[4], fa[MB];
+        for (int j = 0; j < NB; j++) fb[j] = OB::frag(lb, (wn * NB + j) * 16, at);
 #pragma unroll
-            for (int j = 0; j < 4; j++) fb[j] = OB::frag(lb, wn * 64 + j * 16, ks, lane);
-#pragma unroll
-            for (int i = 0; i < MB; i++) fa[i] = OA::frag(la, wm * 16 * MB + i * 16, ks, lane);
-#pragma unroll
-            for (int i = 0; i < MB; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = mfma16(T{}, fb[j], fa[i], acc[i][j]);
-            __builtin_amdgcn_sched_barrier(0);  // no fragment of the next step is read early: registers
-        }
+        for (int i = 0; i < MB; i++) fa[i] = OA::frag(la, (wm * MB + i) * 16, at);
     };
-
-    // slabs come in pairs (the host rounds up; one past the end of K is all zeros): a loop left in its middle would
-    // need a second copy of the accumulators
-    fetch(s0, as0, bs0);
-    land(as0, bs0);
-    __syncthreads();
-    for (int s = s0; s < s1; s += 2) {
-        trim(s, as0, bs0);
-        fetch(s + 1, as1, bs1);
-        compute(as0, bs0);
-        land(as1, bs1);
-        __syncthreads();
-        trim(s + 1, as1, bs1);
-        if (s + 2 < s1) fetch(s + 2, as0, bs0);
-        compute(as1, bs1);
-        if (s + 2 < s1) land(as0, bs0);
-        __syncthreads();
+    auto multiply = [&] {
+#pragma unroll
+        for (int i = 0; i < MB; i++)
+#pragma unroll
+            for (int j = 0; j < NB; j++) acc[i][j] = mfma16(T{}, fb[j], fa[i], acc[i][j]);
+    };
+    // What would follow the last slab is fetched too, so that the number under way is known at every wait; no kernel may
+    // end before it has landed. The fetches stay in this order: the waits count them.
+    auto fence = [] { asm volatile("" ::: "memory"); };
+    fetch(as0, bs0);
+    fence();
+    fetch(as1, bs1);
+    fence();
+    int s = s0;
+    // (what is left over is not an exit from the loop's middle: the compiler would join it with the loop's head, and its
+    // own waits would then be for both)
+    if constexpr (TURNS) {
+        // The two halves of the workgroup, one wave of each on every SIMD, take turns: while one reads a slab's
+        // fragments and starts the fetch of slab s + 3, the other multiplies. A barrier ends every phase; the second
+        // half enters one phase late and leaves one late.
+        //   A half's phase of reading s: slab s has landed in all waves (each waits for its share of slab s + 1 at the
+        //   end of its reading of s, two phases before anyone reads that), and slab s - 1, whose buffers s + 3 takes, was
+        //   last read one phase ago, with its reads waited for before the barrier.
+        auto phase_end = [&] {
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            fence();
+        };
+        auto step = [&](const uint4* la, const uint4* lb, uint4* na, uint4* nb) {
+            fetch(na, nb);
+            read(la, lb);
+            wait_vm<2 * NI>();
+            phase_end();
+            __builtin_amdgcn_s_setprio(1);
+            multiply();
+            __builtin_amdgcn_s_setprio(0);
+            phase_end();
+        };
+        fetch(as2, bs2);
+        wait_vm<2 * NI>();
+        phase_end();
+        if (wave >= NW / 2) phase_end();
+        for (; s + 4 <= s1; s += 4) {
+            step(as0, bs0, as3, bs3);
+            step(as1, bs1, as0, bs0);
+            step(as2, bs2, as1, bs1);
+            step(as3, bs3, as2, bs2);
+        }
+        if (s < s1) step(as0, bs0, as3, bs3);
+        if (s + 1 < s1) step(as1, bs1, as0, bs0);
+        if (s + 2 < s1) step(as2, bs2, as1, bs1);
+        if (wave < NW / 2) phase_end();
+    } else {
+        // Slab s has landed, and every wave is done with slab s - 1, whose buffers slab s + 2 takes while s computes.
+        auto step = [&](const uint4* la, const uint4* lb, uint4* na, uint4* nb) {
+            wait_vm<NI>();
+            __builtin_amdgcn_s_barrier();
+            fence();
+            fetch(na, nb);
+            read(la, lb);
+            multiply();
+            fence();
+        };
+        for (; s + 3 <= s1; s += 3) {
+            step(as0, bs0, as2, bs2);
+            step(as1, bs1, as0, bs0);
+            step(as2, bs2, as1, bs1);
+        }
+        if (s < s1) step(as0, bs0, as2, bs2);
+        if (s + 1 < s1) step(as1, bs1, as0, bs0);
     }
+    wait_vm<0>();
 
     const int mw = m0 + wm * 16 * MB + (lane & 15), quad = 4 * (lane >> 4);
+    if constexpr (E == kGrad) {  // o0 and o1 have rows of up8(n), whose ends are zeros
+        // both products of the next 16 rows are on their way while 16 rows are worked on; past the edge, the last ones
+        f4 ga[2][NB], up[2][NB];
+        auto load = [&](int i) {
+            const int64_t row = min(mw + i * 16, g.m - 1) * g.ldpre;
+#pragma unroll
+            for (int j = 0; j < NB; j++) {
+                const int64_t at = row + min(n0 + wn * FW + j * 16 + quad, (int)g.ldpre - 4);
+                ga[i & 1][j] = *reinterpret_cast<const f4*>(g.pre_g + at);
+                up[i & 1][j] = *reinterpret_cast<const f4*>(g.pre_u + at);
+            }
+        };
+        load(0);
+#pragma unroll
+        for (int i = 0; i < MB; i++) {
+            if (i + 1 < MB) load(i + 1);
+            const int m = mw + i * 16;
+#pragma unroll
+            for (int j = 0; j < NB; j++) {
+                const int n = n0 + wn * FW + j * 16 + quad;
+                const f4 v = acc[i][j];
+                uint16_t qg[4], qu[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    float value, slope;
+                    act_grad(g.act, ga[i & 1][j][r], value, slope);
+                    qg[r] = n + r < g.n ? narrow(T{}, v[r] * up[i & 1][j][r] * slope) : (uint16_t)0;
+                    qu[r] = n + r < g.n ? narrow(T{}, v[r] * value) : (uint16_t)0;
+                }
+                if (m < g.m && n < g.ldo) {
+                    store_raw<uint16_t, 4, true>(g.o0 + m * g.ldo + n, qg);
+                    store_raw<uint16_t, 4, true>(g.o1 + m * g.ldo + n, qu);
+                }
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < MB; i++) {
         const int m = mw + i * 16;
         if (m >= g.m) continue;
-        if constexpr (E == kGlu) {
+        if constexpr (E == kGlu) {  // o0, pre_g and pre_u have rows of up8(n) as well
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int f = n0 + wn * 32 + j * 16 + quad;
-                if (f >= g.n) continue;
-                const f4 ga = acc[i][j], up = acc[i][j + 2];
+            for (int j = 0; j < NB / 2; j++) {
+                const int f = n0 + wn * FW + j * 16 + quad;
+                if (f >= g.ldo) continue;
+                const f4 ga = acc[i][j], up = acc[i][j + NB / 2];
                 uint16_t q[4];
 #pragma unroll
-                for (int r = 0; r < 4; r++) q[r] = narrow(T{}, act_of(g.act, ga[r]) * up[r]);
-                store4(g.o0 + m * g.ldo + f, g.n - f, q);
-                if (g.pre_g) {  // rows padded to 8: a whole vector always fits
+                for (int r = 0; r < 4; r++) q[r] = f + r < g.n ? narrow(T{}, act_of(g.act, ga[r]) * up[r]) : (uint16_t)0;
+                store_raw<uint16_t, 4, true>(g.o0 + m * g.ldo + f, q);
+                if (g.pre_g) {
                     *reinterpret_cast<f4*>(g.pre_g + m * g.ldpre + f) = ga;
                     *reinterpret_cast<f4*>(g.pre_u + m * g.ldpre + f) = up;
                 }
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int n = n0 + wn * 64 + j * 16 + quad;
+            for (int j = 0; j < NB; j++) {
+                const int n = n0 + wn * FW + j * 16 + quad;
                 if (n >= g.n) continue;
                 const f4 v = acc[i][j];
                 if constexpr (E == kPart) {
                     *reinterpret_cast<f4*>(g.part + ((int64_t)(pair * g.splits + split) * g.m + m) * g.ldpart + n) = v;
-                } else if constexpr (E == kGrad) {
-                    const f4 ga = *reinterpret_cast<const f4*>(g.pre_g + m * g.ldpre + n);
-                    const f4 up = *reinterpret_cast<const f4*>(g.pre_u + m * g.ldpre + n);
-                    uint16_t qg[4], qu[4];
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        float value, slope;
-                        act_grad(g.act, ga[r], value, slope);
-                        qg[r] = narrow(T{}, v[r] * up[r] * slope);
-                        qu[r] = narrow(T{}, v[r] * value);
-                    }
-                    store4(g.o0 + m * g.ldo + n, g.n - n, qg);
-                    store4(g.o1 + m * g.ldo + n, g.n - n, qu);
                 } else {
                     uint16_t q[4];
 #pragma unroll

@@ -10,22 +10,70 @@ namespace fhc {
 namespace seq {
 namespace {
 
-// out = the sum of the splits' partial sums, in their order
-template <class T>
+// out = the sum of the splits' partial sums; LANES threads take every LANES-th split of a quad of columns each, and their
+// sums are added in order
+template <class T, int LANES>
 __global__ __launch_bounds__(256) void ffn_join(const float* part, int splits, int m, int n, int64_t ldpart,
                                                 uint16_t* o0, uint16_t* o1, int64_t ldo) {
-    const int quads = (n + 3) / 4;
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= (int64_t)m * quads) return;
-    const int64_t row = at / quads;
-    const int c = (int)(at - row * quads) * 4;
+    constexpr int Q = 256 / LANES;
+    __shared__ f4 s[LANES > 1 ? LANES : 1][LANES > 1 ? Q : 1];
+    const int quads = (n + 3) / 4, x = threadIdx.x % Q, y = threadIdx.x / Q;
+    const int64_t at = (int64_t)blockIdx.x * Q + x;
+    const bool live = at < (int64_t)m * quads;
+    const int64_t row = live ? at / quads : 0;
+    const int c = live ? (int)(at - row * quads) * 4 : 0;
     const float* p = part + ((int64_t)blockIdx.y * splits * m + row) * ldpart + c;
-    f4 s = *reinterpret_cast<const f4*>(p);
-    for (int z = 1; z < splits; z++) s += *reinterpret_cast<const f4*>(p + (int64_t)z * m * ldpart);
+    f4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (live) {
+#pragma unroll 4
+        for (int z = y; z < splits; z += LANES) sum += *reinterpret_cast<const f4*>(p + (int64_t)z * m * ldpart);
+    }
+    if constexpr (LANES > 1) {
+        s[y][x] = sum;
+        __syncthreads();
+        if (y > 0) return;
+#pragma unroll
+        for (int k = 1; k < LANES; k++) sum += s[k][x];
+    }
+    if (!live) return;
     uint16_t q[4];
 #pragma unroll
-    for (int r = 0; r < 4; r++) q[r] = narrow(T{}, s[r]);
+    for (int r = 0; r < 4; r++) q[r] = narrow(T{}, sum[r]);
     store4((blockIdx.y ? o1 : o0) + row * ldo + c, n - c, q);
+}
+
+// up to 8 elements at p, `valid` of them inside
+__device__ __forceinline__ u4_t load_some(const uint16_t* p, int valid) {
+    if (valid >= 8) {
+        uint16_t q[8];
+        load_raw<uint16_t, 8, false>(p, q);
+        u4_t r;
+#pragma unroll
+        for (int i = 0; i < 4; i++) r[i] = q[2 * i] | (uint32_t)q[2 * i + 1] << 16;
+        return r;
+    }
+    u4_t r = {0, 0, 0, 0};
+    for (int i = 0; i < valid; i++) r[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+    return r;
+}
+
+// Copies of up to five matrices with rows of up8(width) elements, the last ones zeros: 8 elements a thread.
+struct PackArgs {
+    const uint16_t* in[5];
+    uint16_t* out[5];
+    int64_t ld[5];
+    int rows[5], width[5];
+};
+__global__ __launch_bounds__(256) void ffn_pack(PackArgs g) {
+    const uint16_t* in = g.in[blockIdx.y];
+    uint16_t* out = g.out[blockIdx.y];
+    const int width = g.width[blockIdx.y], groups = (width + 7) / 8;
+    const int64_t items = (int64_t)g.rows[blockIdx.y] * groups, ld = g.ld[blockIdx.y];
+    for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < items; k += (int64_t)gridDim.x * 256) {
+        const int64_t row = k / groups;
+        const int c = (int)(k - row * groups) * 8;
+        *reinterpret_cast<u4_t*>(out + k * 8) = load_some(in + row * ld + c, width - c);
+    }
 }
 
 // ---- few rows: a wave streams 16 weight rows past the matrix unit straight from global memory (each weight is used
@@ -37,6 +85,8 @@ struct SkinnyArgs {
     int rows, n, k;
     uint16_t* out;
     int64_t ldo;
+    int width;  // columns of out that are written, zeros from n on
+    float *pre_g, *pre_u;  // GLU: both products, rows of ldo, or null
     uint32_t act;
 };
 
@@ -111,12 +161,18 @@ __global__ __launch_bounds__(64 * NW) void ffn_skinny(SkinnyArgs g) {
             for (int w = 1; w < NW; w++) t[p] += sums[w][p * NB + b][lane];
         }
         const int row = b * 16 + (lane & 15), at = f0 + 4 * (lane >> 4);
-        if (row >= g.rows || at >= g.n) continue;
+        if (row >= g.rows || at >= g.width) continue;
         uint16_t q[4];
 #pragma unroll
-        for (int r = 0; r < 4; r++)
+        for (int r = 0; r < 4; r++) {
+            if (GLU && at + r >= g.n) t[0][r] = t[P - 1][r] = 0.0f;
             q[r] = narrow(T{}, GLU ? act_of(g.act, t[0][r]) * t[P - 1][r] : t[0][r]);
-        store4(g.out + row * g.ldo + at, g.n - at, q);
+        }
+        store4(g.out + row * g.ldo + at, g.width - at, q);
+        if (GLU && g.pre_g) {
+            *reinterpret_cast<f4*>(g.pre_g + row * g.ldo + at) = t[0];
+            *reinterpret_cast<f4*>(g.pre_u + row * g.ldo + at) = t[P - 1];
+        }
     }
 }
 
@@ -146,55 +202,80 @@ int check_weight(const char* op, const char* name, const void* p) {
 }
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
-int64_t padded(uint32_t f) { return ((int64_t)f + 7) / 8 * 8; }
-size_t hidden_bytes(const fhc_ffn_desc* d) { return up256((size_t)d->rows * padded(d->f) * 2); }
-size_t pre_bytes(const fhc_ffn_desc* d) { return up256((size_t)d->rows * padded(d->f) * 4); }
+size_t hidden_bytes(const fhc_ffn_desc* d) { return up256((size_t)d->rows * up8(d->f) * 2); }
+size_t pre_bytes(const fhc_ffn_desc* d) { return up256((size_t)d->rows * up8(d->f) * 4); }
 
 struct Shape {  // a product's tiles and splits
-    bool big;   // 256 x 256 tiles of 8 waves, else 128 x 128 of 4
+    bool big;   // 128 x 256 tiles, else 128 x 128
     int tiles_m, tiles_n, slabs, per_split, splits;
     size_t part_bytes;
 };
-// Tiles of 256 where they fill the chip's 256 CUs; else tiles of 128, with K split (where the epilogue allows it)
-// until there are two workgroups a CU, at least 4 slabs each.
-Shape shape_of(int64_t m, int64_t n, int64_t k, int segments, int pairs, bool glu, bool may_split, bool dma) {
+// The larger tiles where they fill the chip's 256 CUs twice; else the smaller ones, with K split (where the epilogue
+// allows it) until there are two workgroups a CU, at least 8 slabs each.
+Shape shape_of(int64_t m, int64_t n, int64_t k, int segments, int pairs, bool glu, bool may_split) {
     Shape s{};
     auto tiles = [&](int bm, int bn) { return ceil_div(m, bm) * ceil_div(n, bn); };
-    s.big = dma && tiles(256, glu ? 128 : 256) * pairs >= 224;
-    const int bm = s.big ? 256 : 128, bn = (s.big ? 256 : 128) / (glu ? 2 : 1);
-    s.tiles_m = (int)ceil_div(m, bm), s.tiles_n = (int)ceil_div(n, bn);
-    s.slabs = (int)ceil_div(k, 128) * 2 * segments;
+    s.big = tiles(256, glu ? 128 : 256) * pairs >= 224;
+    const int bn = (s.big ? 256 : 128) / (glu ? 2 : 1);
+    s.tiles_m = (int)ceil_div(m, s.big ? 256 : 128), s.tiles_n = (int)ceil_div(n, bn);
+    s.slabs = (int)ceil_div(k, 32) * segments;
     s.splits = 1;
     const int64_t wgs = (int64_t)s.tiles_m * s.tiles_n * pairs;
-    if (may_split && wgs < 256 && s.slabs >= 8) {
+    if (may_split && wgs < (s.big ? 0 : 384) && s.slabs >= 16) {
         int64_t z = ceil_div(512, wgs);
-        if (z > s.slabs / 4) z = s.slabs / 4;
+        if (z > s.slabs / 8) z = s.slabs / 8;
         s.splits = z < 1 ? 1 : (int)z;
     }
-    s.per_split = (int)ceil_div(s.slabs, 2 * s.splits) * 2;
+    s.per_split = (int)ceil_div(s.slabs, s.splits);
     s.splits = s.slabs ? (int)ceil_div(s.slabs, s.per_split) : 1;
     s.part_bytes = s.splits > 1 ? up256((size_t)pairs * s.splits * m * ((n + 3) / 4 * 4) * 4) : 0;
     return s;
 }
 
-// LDS DMA: chunks at 4-byte steps whose offsets within a tile stay below 2^31
-bool dma_ok(const GemmArgs& g) {
-    if (g.lda % 2 || g.ldb % 2 || g.lda > 1 << 21 || g.ldb > 1 << 21) return false;
-    if (g.k % 2 || g.m % 2 || g.n % 2) return false;
-    for (const void* p : {g.a0, g.a1, g.b0, g.b1})
-        if (!aligned(p, 4)) return false;
-    return true;
-}
+// A matrix of a product as it can be fetched: itself, or a copy with padded rows.
+struct Operands {
+    PackArgs args;
+    int count;
+    char* at;  // the workspace's next byte
+    // rows x width elements ld apart; k: the width is a product's K
+    bool direct(const void* p, int64_t ld, int64_t width, bool k) const {
+        return ld % 2 == 0 && width % (k ? 8 : 2) == 0 && ld <= 1 << 20 && aligned(p, 4);
+    }
+    const uint16_t* take(const void* p, int64_t& ld, uint32_t rows, uint32_t width, bool k, bool copied = false) {
+        const uint16_t* q = static_cast<const uint16_t*>(p);
+        if (!copied && direct(p, ld, width, k)) return q;
+        args.in[count] = q, args.ld[count] = ld, args.rows[count] = (int)rows, args.width[count] = (int)width;
+        args.out[count] = reinterpret_cast<uint16_t*>(at);
+        at += pack_bytes(rows, width);
+        ld = up8(width);
+        return args.out[count++];
+    }
+    // two matrices of one shape, which a product reads with one stride: both as they are or both copied
+    void take_two(const void* p, const void* q, int64_t& ld, uint32_t rows, uint32_t width, bool k, const uint16_t*& a,
+                  const uint16_t*& b) {
+        const bool copied = !direct(p, ld, width, k) || !direct(q, ld, width, k);
+        int64_t other = ld;
+        a = take(p, other, rows, width, k, copied), b = take(q, ld, rows, width, k, copied);
+    }
+    static size_t pack_bytes(uint32_t rows, uint32_t width) { return up256((size_t)rows * up8(width) * 2); }
+    int copy(const char* op, hipStream_t st) const {
+        if (!count) return 0;
+        uint64_t items = 1;
+        for (int i = 0; i < count; i++) {
+            const uint64_t n = (uint64_t)args.rows[i] * ((args.width[i] + 7) / 8);
+            items = n > items ? n : items;
+        }
+        const uint64_t blocks = ceil_div(items, 256);
+        hipLaunchKernelGGL(ffn_pack, dim3((uint32_t)(blocks < 4096 ? blocks : 4096), count), dim3(256), 0, st, args);
+        return launched(op);
+    }
+};
 
 template <class T, bool AC, bool BC, Epi E>
 void launch_tiles(const Shape& s, const GemmArgs& g, hipStream_t st) {
     const dim3 grid(s.tiles_m * s.tiles_n, 1, s.splits * g.pairs);
-    if (s.big) {
-        hipLaunchKernelGGL((ffn_gemm<T, AC, BC, E, 8, 2, 4, true>), grid, dim3(512), 0, st, g);
-    } else {
-        if (dma_ok(g)) hipLaunchKernelGGL((ffn_gemm<T, AC, BC, E, 4, 2, 2, true>), grid, dim3(256), 0, st, g);
-        else hipLaunchKernelGGL((ffn_gemm<T, AC, BC, E, 4, 2, 2, false>), grid, dim3(256), 0, st, g);
-    }
+    if (s.big) hipLaunchKernelGGL((ffn_gemm<T, AC, BC, E, 8, 4, 2, 4>), grid, dim3(512), 0, st, g);
+    else hipLaunchKernelGGL((ffn_gemm<T, AC, BC, E, 4, 4, 2, 2>), grid, dim3(256), 0, st, g);
 }
 
 // g without tiles and splits
@@ -202,8 +283,10 @@ template <class T, bool AC, bool BC, Epi E>
 int product(const char* op, GemmArgs g, float* part, hipStream_t st) {
     if (g.m == 0 || g.n == 0) return 0;
     g.segments = g.segments ? g.segments : 1, g.pairs = g.pairs ? g.pairs : 1;
-    const Shape s = shape_of(g.m, g.n, g.k, g.segments, g.pairs, E == kGlu, E == kStore, dma_ok(g));
+    const Shape s = shape_of(g.m, g.n, g.k, g.segments, g.pairs, E == kGlu, E == kStore);
     g.tiles_m = s.tiles_m, g.tiles_n = s.tiles_n, g.slabs = s.slabs, g.per_split = s.per_split, g.splits = s.splits;
+    // a padded operand's rows hold more than its columns
+    g.wide_m = (int)(up8(g.m) <= g.lda ? up8(g.m) : g.m), g.wide_n = (int)(up8(g.n) <= g.ldb ? up8(g.n) : g.n);
     if ((int64_t)s.tiles_m * s.tiles_n >= 1ll << 31) return fail(-1, "%s: too many tiles", op);
     if constexpr (E == kStore) {
         if (s.splits > 1) {
@@ -211,8 +294,12 @@ int product(const char* op, GemmArgs g, float* part, hipStream_t st) {
             launch_tiles<T, AC, BC, kPart>(s, g, st);
             FHC_TRY(launched(op));
             const uint64_t items = (uint64_t)g.m * ((g.n + 3) / 4);
-            hipLaunchKernelGGL((ffn_join<T>), dim3((uint32_t)ceil_div(items, 256), g.pairs), dim3(256), 0, st, g.part,
-                               s.splits, g.m, g.n, g.ldpart, g.o0, g.o1, g.ldo);
+            if (s.splits >= 16)
+                hipLaunchKernelGGL((ffn_join<T, 8>), dim3((uint32_t)ceil_div(items, 32), g.pairs), dim3(256), 0, st,
+                                   g.part, s.splits, g.m, g.n, g.ldpart, g.o0, g.o1, g.ldo);
+            else
+                hipLaunchKernelGGL((ffn_join<T, 1>), dim3((uint32_t)ceil_div(items, 256), g.pairs), dim3(256), 0, st,
+                                   g.part, s.splits, g.m, g.n, g.ldpart, g.o0, g.o1, g.ldo);
             return launched(op);
         }
     }
@@ -239,67 +326,83 @@ int skinny(const char* op, const SkinnyArgs& a, hipStream_t st) {
     return launched(op);
 }
 
-// the partial sums' bytes of a product, whichever way its operands' alignment has it go
 size_t part_of(int64_t m, int64_t n, int64_t k, int segments, int pairs) {
-    const size_t a = shape_of(m, n, k, segments, pairs, false, true, true).part_bytes;
-    const size_t b = shape_of(m, n, k, segments, pairs, false, true, false).part_bytes;
-    return a > b ? a : b;
+    return shape_of(m, n, k, segments, pairs, false, true).part_bytes;
 }
 
+// Copies of the operands are counted whether a call makes them or not: that depends on its pointers and strides.
 size_t workspace(const fhc_ffn_desc* d, bool backward) {
+    const size_t rows = Operands::pack_bytes(d->rows, d->c), up = Operands::pack_bytes(d->f, d->c),
+                 down = Operands::pack_bytes(d->c, d->f);
     if (!backward) {  // h, where nothing is kept, and the second product's partial sums
-        return hidden_bytes(d) + part_of(d->rows, d->c, d->f, 1, 1);
+        const size_t copies = d->rows > kSkinnyRows ? rows + 2 * up + down : 0;
+        return hidden_bytes(d) + part_of(d->rows, d->c, d->f, 1, 1) + copies;
     }
     size_t part = 0;
     for (const size_t n : {part_of(d->rows, d->c, d->f, 2, 1), part_of(d->f, d->c, d->rows, 1, 2),
                            part_of(d->f, d->c, d->rows, 1, 1), part_of(d->c, d->f, d->rows, 1, 1)})
         part = n > part ? n : part;
-    return 2 * hidden_bytes(d) + part;
+    return 2 * hidden_bytes(d) + part + 2 * rows + 2 * up + down;
 }
 
 template <class T>
 int forward(const char* op, const fhc_ffn_desc* d, const fhc_rows* x, const void* wg, const void* wu, const void* wd,
             const fhc_rows* y, void* saved, void* ws, hipStream_t st) {
-    const int64_t fp = padded(d->f);
+    const int64_t fp = up8(d->f);
     char* keep = static_cast<char*>(saved);
     char* w = static_cast<char*>(ws);
     uint16_t* h = reinterpret_cast<uint16_t*>(saved ? keep : w);
     auto u16 = [](const void* p) { return static_cast<const uint16_t*>(p); };
-    if (!saved && d->rows <= kSkinnyRows) {
-        SkinnyArgs a{u16(x->p), u16(wg), u16(wu), x->ld, (int64_t)d->c, (int)d->rows, (int)d->f, (int)d->c, h, fp, d->act};
+    float* pre_g = saved ? reinterpret_cast<float*>(keep + hidden_bytes(d)) : nullptr;
+    float* pre_u = saved ? reinterpret_cast<float*>(keep + hidden_bytes(d) + pre_bytes(d)) : nullptr;
+    if (d->rows <= kSkinnyRows) {
+        SkinnyArgs a{u16(x->p), u16(wg), u16(wu), x->ld, (int64_t)d->c, (int)d->rows, (int)d->f, (int)d->c, h, fp, (int)fp,
+                     pre_g, pre_u, d->act};
         FHC_TRY((skinny<T, true>(op, a, st)));
         SkinnyArgs b{h, u16(wd), nullptr, fp, (int64_t)d->f, (int)d->rows, (int)d->c, (int)d->f,
-                     static_cast<uint16_t*>(y->p), y->ld, d->act};
+                     static_cast<uint16_t*>(y->p), y->ld, (int)d->c, nullptr, nullptr, d->act};
         return skinny<T, false>(op, b, st);
     }
-    GemmArgs g{};
-    g.a0 = u16(x->p), g.b0 = u16(wg), g.b1 = u16(wu), g.lda = x->ld, g.ldb = d->c;
+    char* part = w + hidden_bytes(d);
+    Operands o{{}, 0, part + part_of(d->rows, d->c, d->f, 1, 1)};
+    GemmArgs g{}, p{};
+    g.lda = x->ld, g.ldb = d->c, p.ldb = d->f;
+    g.a0 = o.take(x->p, g.lda, d->rows, d->c, true);
+    o.take_two(wg, wu, g.ldb, d->f, d->c, true, g.b0, g.b1);
+    p.b0 = o.take(wd, p.ldb, d->c, d->f, true);
+    FHC_TRY(o.copy(op, st));
     g.m = d->rows, g.n = d->f, g.k = d->c, g.o0 = h, g.ldo = fp, g.ldpre = fp, g.act = d->act;
-    if (saved) {
-        g.pre_g = reinterpret_cast<float*>(keep + hidden_bytes(d));
-        g.pre_u = reinterpret_cast<float*>(keep + hidden_bytes(d) + pre_bytes(d));
-    }
+    g.pre_g = pre_g, g.pre_u = pre_u;
     FHC_TRY((product<T, false, false, kGlu>(op, g, nullptr, st)));
-    GemmArgs p{};
-    p.a0 = h, p.b0 = u16(wd), p.lda = fp, p.ldb = d->f, p.m = d->rows, p.n = d->c, p.k = d->f;
+    p.a0 = h, p.lda = fp, p.m = d->rows, p.n = d->c, p.k = d->f;
     p.o0 = static_cast<uint16_t*>(y->p), p.ldo = y->ld;
-    return product<T, false, false, kStore>(op, p, reinterpret_cast<float*>(w + hidden_bytes(d)), st);
+    return product<T, false, false, kStore>(op, p, reinterpret_cast<float*>(part), st);
 }
 
 template <class T>
 int backward(const char* op, const fhc_ffn_desc* d, const fhc_rows* x, const void* wg, const void* wu, const void* wd,
              const void* saved, const fhc_rows* dy, const fhc_rows* dx, void* dwg, void* dwu, void* dwd, void* ws,
              hipStream_t st) {
-    const int64_t fp = padded(d->f);
+    const int64_t fp = up8(d->f);
     char* keep = const_cast<char*>(static_cast<const char*>(saved));
     char* w = static_cast<char*>(ws);
-    auto u16 = [](const void* p) { return static_cast<const uint16_t*>(p); };
     auto out = [](void* p) { return static_cast<uint16_t*>(p); };
     uint16_t *dg = out(w), *du = out(w + hidden_bytes(d));
     float* part = reinterpret_cast<float*>(w + 2 * hidden_bytes(d));
-    if (dx || dwg || dwu) {
+    Operands o{{}, 0, w + workspace(d, true) - 2 * Operands::pack_bytes(d->rows, d->c) -
+                          2 * Operands::pack_bytes(d->f, d->c) - Operands::pack_bytes(d->c, d->f)};
+    int64_t ldx = x->ld, ldy = dy->ld, ldd = d->f, ldg = d->c;
+    const bool hidden = dx || dwg || dwu;
+    // dy is a product's rows for dL/dh (K its channels) and columns for dwd
+    const uint16_t* vdy = hidden || dwd ? o.take(dy->p, ldy, d->rows, d->c, hidden) : nullptr;
+    const uint16_t* vx = dwg || dwu ? o.take(x->p, ldx, d->rows, d->c, false) : nullptr;
+    const uint16_t* vwd = hidden ? o.take(wd, ldd, d->c, d->f, false) : nullptr;
+    const uint16_t *vwg = nullptr, *vwu = nullptr;
+    if (dx) o.take_two(wg, wu, ldg, d->f, d->c, false, vwg, vwu);
+    FHC_TRY(o.copy(op, st));
+    if (hidden) {
         GemmArgs g{};
-        g.a0 = u16(dy->p), g.b0 = u16(wd), g.lda = dy->ld, g.ldb = d->f, g.m = d->rows, g.n = d->f, g.k = d->c;
+        g.a0 = vdy, g.b0 = vwd, g.lda = ldy, g.ldb = ldd, g.m = d->rows, g.n = d->f, g.k = d->c;
         g.o0 = dg, g.o1 = du, g.ldo = fp, g.ldpre = fp, g.act = d->act;
         g.pre_g = reinterpret_cast<float*>(keep + hidden_bytes(d));
         g.pre_u = reinterpret_cast<float*>(keep + hidden_bytes(d) + pre_bytes(d));
@@ -307,19 +410,19 @@ int backward(const char* op, const fhc_ffn_desc* d, const fhc_rows* x, const voi
     }
     if (dx) {
         GemmArgs g{};
-        g.a0 = dg, g.a1 = du, g.b0 = u16(wg), g.b1 = u16(wu), g.lda = fp, g.ldb = d->c, g.segments = 2;
+        g.a0 = dg, g.a1 = du, g.b0 = vwg, g.b1 = vwu, g.lda = fp, g.ldb = ldg, g.segments = 2;
         g.m = d->rows, g.n = d->c, g.k = d->f, g.o0 = out(dx->p), g.ldo = dx->ld;
         FHC_TRY((product<T, false, true, kStore>(op, g, part, st)));
     }
     if (dwg || dwu) {
         GemmArgs g{};
-        g.a0 = dwg ? dg : du, g.a1 = du, g.b0 = u16(x->p), g.lda = fp, g.ldb = x->ld, g.pairs = dwg && dwu ? 2 : 1;
+        g.a0 = dwg ? dg : du, g.a1 = du, g.b0 = vx, g.lda = fp, g.ldb = ldx, g.pairs = dwg && dwu ? 2 : 1;
         g.m = d->f, g.n = d->c, g.k = d->rows, g.o0 = out(dwg ? dwg : dwu), g.o1 = out(dwu), g.ldo = d->c;
         FHC_TRY((product<T, true, true, kStore>(op, g, part, st)));
     }
     if (dwd) {
         GemmArgs g{};
-        g.a0 = u16(dy->p), g.b0 = reinterpret_cast<const uint16_t*>(keep), g.lda = dy->ld, g.ldb = fp;
+        g.a0 = vdy, g.b0 = reinterpret_cast<const uint16_t*>(keep), g.lda = ldy, g.ldb = fp;
         g.m = d->c, g.n = d->f, g.k = d->rows, g.o0 = out(dwd), g.ldo = d->f;
         FHC_TRY((product<T, true, true, kStore>(op, g, part, st)));
     }
