@@ -81,6 +81,21 @@ __device__ __forceinline__ void act_grad(uint32_t act, float v, float& value, fl
     slope = p * __builtin_fmaf(v * dk, q, 1.0f);
 }
 
+// up to 8 elements at p, `valid` of them inside
+__device__ __forceinline__ u4_t load_some(const uint16_t* p, int valid) {
+    if (valid >= 8) {
+        uint16_t q[8];
+        load_raw<uint16_t, 8, false>(p, q);
+        u4_t r;
+#pragma unroll
+        for (int i = 0; i < 4; i++) r[i] = q[2 * i] | (uint32_t)q[2 * i + 1] << 16;
+        return r;
+    }
+    u4_t r = {0, 0, 0, 0};
+    for (int i = 0; i < valid; i++) r[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+    return r;
+}
+
 __device__ __forceinline__ void store4(uint16_t* p, int valid, const uint16_t (&q)[4]) {
     if (valid >= 4) {
         store_raw<uint16_t, 4, false>(p, q);

@@ -4,7 +4,7 @@
 // Forward: one product with gate and up rows side by side whose epilogue is the activation and the product, one with
 // wd. Backward: dh = dy wd with dL/dgate, dL/dup in its epilogue; dx = [dL/dgate dL/dup] [wg; wu] as one product over
 // both halves of K; dwg and dwu (one launch), dwd, with the rows as K.
-#include "ffn_gemm.h"
+#include "ffn_fused.h"
 
 namespace fhc {
 namespace seq {
@@ -40,21 +40,6 @@ __global__ __launch_bounds__(256) void ffn_join(const float* part, int splits, i
 #pragma unroll
     for (int r = 0; r < 4; r++) q[r] = narrow(T{}, sum[r]);
     store4((blockIdx.y ? o1 : o0) + row * ldo + c, n - c, q);
-}
-
-// up to 8 elements at p, `valid` of them inside
-__device__ __forceinline__ u4_t load_some(const uint16_t* p, int valid) {
-    if (valid >= 8) {
-        uint16_t q[8];
-        load_raw<uint16_t, 8, false>(p, q);
-        u4_t r;
-#pragma unroll
-        for (int i = 0; i < 4; i++) r[i] = q[2 * i] | (uint32_t)q[2 * i + 1] << 16;
-        return r;
-    }
-    u4_t r = {0, 0, 0, 0};
-    for (int i = 0; i < valid; i++) r[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
-    return r;
 }
 
 // Copies of up to five matrices with rows of up8(width) elements, the last ones zeros: 8 elements a thread.
@@ -179,6 +164,10 @@ __global__ __launch_bounds__(64 * NW) void ffn_skinny(SkinnyArgs g) {
 // ---- host side ----------------------------------------------------------------------------------------------------
 
 constexpr uint32_t kSkinnyRows = 64;  // up to here the weights' bytes are all that counts
+
+// One kernel a direction (ffn_fused.h) where the channels fit its registers and the rows give it work for the chip; a
+// workgroup of it walks all features, so few rows go through the products of ffn_gemm.h, which spread over features too.
+bool fused(const fhc_ffn_desc* d) { return d->c <= 256 && d->c > 0 && d->f > 0 && d->rows >= 8192; }
 
 int check_desc(const char* op, const fhc_ffn_desc* d) {
     if (!d) return fail(-1, "%s: null descriptor", op);
@@ -326,6 +315,18 @@ int skinny(const char* op, const SkinnyArgs& a, hipStream_t st) {
     return launched(op);
 }
 
+template <class T, bool BWD>
+int run_fused(const char* op, const FusedArgs& a, hipStream_t st) {
+#define FUSED(CP, MB, NW)                                                                                    \
+    hipLaunchKernelGGL((ffn_fused<T, CP, MB, NW, BWD>), dim3((uint32_t)ceil_div(a.rows, 16 * MB * NW)), dim3(64 * NW), \
+                       0, st, a)
+    if (a.c <= 64) FUSED(64, 2, 4);
+    else if (a.c <= 128) FUSED(128, 2, 4);
+    else FUSED(256, 1, 8);
+#undef FUSED
+    return launched(op);
+}
+
 size_t part_of(int64_t m, int64_t n, int64_t k, int segments, int pairs) {
     return shape_of(m, n, k, segments, pairs, false, true).part_bytes;
 }
@@ -342,7 +343,7 @@ size_t workspace(const fhc_ffn_desc* d, bool backward) {
     for (const size_t n : {part_of(d->rows, d->c, d->f, 2, 1), part_of(d->f, d->c, d->rows, 1, 2),
                            part_of(d->f, d->c, d->rows, 1, 1), part_of(d->c, d->f, d->rows, 1, 1)})
         part = n > part ? n : part;
-    return 2 * hidden_bytes(d) + part + 2 * rows + 2 * up + down;
+    return (fused(d) ? 3 : 2) * hidden_bytes(d) + part + 2 * rows + 2 * up + down;
 }
 
 template <class T>
@@ -365,6 +366,16 @@ int forward(const char* op, const fhc_ffn_desc* d, const fhc_rows* x, const void
     }
     char* part = w + hidden_bytes(d);
     Operands o{{}, 0, part + part_of(d->rows, d->c, d->f, 1, 1)};
+    if (fused(d)) {
+        FusedArgs a{};
+        a.ldx = x->ld, a.ldg = d->c, a.ldd = d->f, a.rows = (int)d->rows, a.c = (int)d->c, a.f = (int)d->f, a.act = d->act;
+        a.x = o.take(x->p, a.ldx, d->rows, d->c, true);
+        o.take_two(wg, wu, a.ldg, d->f, d->c, true, a.wg, a.wu);
+        a.wd = o.take(wd, a.ldd, d->c, d->f, true);
+        FHC_TRY(o.copy(op, st));
+        a.out = static_cast<uint16_t*>(y->p), a.ldo = y->ld;
+        return run_fused<T, false>(op, a, st);
+    }
     GemmArgs g{}, p{};
     g.lda = x->ld, g.ldb = d->c, p.ldb = d->f;
     g.a0 = o.take(x->p, g.lda, d->rows, d->c, true);
@@ -387,20 +398,28 @@ int backward(const char* op, const fhc_ffn_desc* d, const fhc_rows* x, const voi
     char* keep = const_cast<char*>(static_cast<const char*>(saved));
     char* w = static_cast<char*>(ws);
     auto out = [](void* p) { return static_cast<uint16_t*>(p); };
+    const bool one = fused(d);
     uint16_t *dg = out(w), *du = out(w + hidden_bytes(d));
-    float* part = reinterpret_cast<float*>(w + 2 * hidden_bytes(d));
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(one ? w + 2 * hidden_bytes(d) : keep);
+    float* part = reinterpret_cast<float*>(w + (one ? 3 : 2) * hidden_bytes(d));
     Operands o{{}, 0, w + workspace(d, true) - 2 * Operands::pack_bytes(d->rows, d->c) -
                           2 * Operands::pack_bytes(d->f, d->c) - Operands::pack_bytes(d->c, d->f)};
     int64_t ldx = x->ld, ldy = dy->ld, ldd = d->f, ldg = d->c;
-    const bool hidden = dx || dwg || dwu;
+    const bool hidden = one || dx || dwg || dwu;
     // dy is a product's rows for dL/dh (K its channels) and columns for dwd
     const uint16_t* vdy = hidden || dwd ? o.take(dy->p, ldy, d->rows, d->c, hidden) : nullptr;
-    const uint16_t* vx = dwg || dwu ? o.take(x->p, ldx, d->rows, d->c, false) : nullptr;
-    const uint16_t* vwd = hidden ? o.take(wd, ldd, d->c, d->f, false) : nullptr;
+    const uint16_t* vx = one || dwg || dwu ? o.take(x->p, ldx, d->rows, d->c, one) : nullptr;
+    const uint16_t* vwd = hidden ? o.take(wd, ldd, d->c, d->f, one) : nullptr;
     const uint16_t *vwg = nullptr, *vwu = nullptr;
-    if (dx) o.take_two(wg, wu, ldg, d->f, d->c, false, vwg, vwu);
+    if (one || dx) o.take_two(wg, wu, ldg, d->f, d->c, one, vwg, vwu);
     FHC_TRY(o.copy(op, st));
-    if (hidden) {
+    if (one) {
+        FusedArgs a{};
+        a.x = vx, a.wg = vwg, a.wu = vwu, a.wd = vwd, a.dy = vdy, a.ldx = ldx, a.ldg = ldg, a.ldd = ldd, a.ldy = ldy;
+        a.rows = (int)d->rows, a.c = (int)d->c, a.f = (int)d->f, a.act = d->act;
+        a.out = dx ? out(dx->p) : nullptr, a.ldo = dx ? dx->ld : 0, a.dg = dg, a.du = du, a.h = out(w + 2 * hidden_bytes(d));
+        FHC_TRY((run_fused<T, true>(op, a, st)));
+    } else if (hidden) {
         GemmArgs g{};
         g.a0 = vdy, g.b0 = vwd, g.lda = ldy, g.ldb = ldd, g.m = d->rows, g.n = d->f, g.k = d->c;
         g.o0 = dg, g.o1 = du, g.ldo = fp, g.ldpre = fp, g.act = d->act;
@@ -408,7 +427,7 @@ int backward(const char* op, const fhc_ffn_desc* d, const fhc_rows* x, const voi
         g.pre_u = reinterpret_cast<float*>(keep + hidden_bytes(d) + pre_bytes(d));
         FHC_TRY((product<T, false, true, kGrad>(op, g, nullptr, st)));
     }
-    if (dx) {
+    if (dx && !one) {
         GemmArgs g{};
         g.a0 = dg, g.a1 = du, g.b0 = vwg, g.b1 = vwu, g.lda = fp, g.ldb = ldg, g.segments = 2;
         g.m = d->rows, g.n = d->c, g.k = d->f, g.o0 = out(dx->p), g.ldo = dx->ld;
@@ -422,7 +441,7 @@ int backward(const char* op, const fhc_ffn_desc* d, const fhc_rows* x, const voi
     }
     if (dwd) {
         GemmArgs g{};
-        g.a0 = vdy, g.b0 = reinterpret_cast<const uint16_t*>(keep), g.lda = ldy, g.ldb = fp;
+        g.a0 = vdy, g.b0 = h, g.lda = ldy, g.ldb = fp;
         g.m = d->c, g.n = d->f, g.k = d->rows, g.o0 = out(dwd), g.ldo = d->f;
         FHC_TRY((product<T, true, true, kStore>(op, g, part, st)));
     }
@@ -440,7 +459,7 @@ extern "C" size_t fhc_ffn_saved_bytes(const fhc_ffn_desc* d) {
     return guard((size_t)0, [&]() -> size_t {
         clear_error();
         if (check_desc("ffn_saved_bytes", d) < 0) return 0;
-        return hidden_bytes(d) + 2 * pre_bytes(d);
+        return fused(d) ? 256 : hidden_bytes(d) + 2 * pre_bytes(d);
     });
 }
 

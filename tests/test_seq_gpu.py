@@ -532,3 +532,76 @@ def test_ffn_in_a_graph_and_on_another_stream(shape):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), k
         call()
+
+
+# few channels and many rows: the one-kernel form; widths short of and past each of its sizes, tails of rows and features
+FFN_FUSED = [(8192, 64, 128), (8200, 128, 512), (8193, 256, 100), (9000, 100, 90), (8192, 65, 129), (8500, 200, 264),
+             (8192, 7, 33), (20001, 129, 31)]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("shape", FFN_FUSED, ids=str)
+def test_ffn_many_rows_of_few_channels(shape, dtype):
+    say("ffn fused", shape, dtype)
+    ffn_check(ffn_inputs(Rand(sum(shape)), *shape, types()[dtype]), "silu" if shape[0] % 2 else "gelu")
+
+
+def test_ffn_many_rows_some_gradients_only_views_and_rows_not_finite():
+    """dx or the weights' gradients alone are those of the whole call; row views with NaN beside them; a row of NaN."""
+    say("ffn fused parts")
+    import ctypes
+    import torch
+    m, (rows, c, f) = mod(), (8195, 72, 136)
+    v = ffn_inputs(Rand(21), rows, c, f, torch.bfloat16)
+    w = [v[k] for k in ("wg", "wu", "wd")]
+    y, saved = m.ffn(v["x"], *w, train=True)
+    grads = m.ffn_backward(v["x"], *w, saved, v["dy"])
+    wide = {k: torch.full((rows, c + 20), math.nan, dtype=torch.bfloat16, device="cuda") for k in ("x", "dy")}
+    for off in (1, 2, 8):
+        views = {k: b[:, off:off + c] for k, b in wide.items()}
+        for k, b in views.items():
+            b.copy_(v[k])
+        assert torch.equal(m.ffn(views["x"], *w), y)
+        assert all(torch.equal(a, b) for a, b in zip(m.ffn_backward(views["x"], *w, saved, views["dy"]), grads))
+        for b in wide.values():
+            b.fill_(math.nan)
+    L, d = m._lib(), m.FfnDesc(1, 0, rows, c, f)
+    n = L.fhc_ffn_workspace_bytes(ctypes.byref(d), 1)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    for only in range(4):
+        out = [torch.full_like(g, 7) for g in grads]
+        at = [o.data_ptr() if k == only else None for k, o in enumerate(out)]
+        assert L.fhc_ffn_backward(ctypes.byref(d), m._rows("", "", v["x"]), w[0].data_ptr(), w[1].data_ptr(),
+                                  w[2].data_ptr(), saved.data_ptr(), m._rows("", "", v["dy"]),
+                                  m._rows("", "", out[0]) if only == 0 else None, at[1], at[2], at[3], ws.data_ptr(), n,
+                                  torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(out[only], grads[only]), only
+        assert all((o == 7).all() for k, o in enumerate(out) if k != only)
+    v["x"][100, 3] = math.nan
+    got = m.ffn(v["x"], *w)
+    keep = torch.arange(rows, device="cuda") != 100
+    assert torch.equal(got[keep], y[keep]) and not torch.isfinite(got[100]).any()
+
+
+def test_ffn_many_rows_in_a_graph():
+    say("ffn fused graph")
+    import torch
+    m = mod()
+    v = ffn_inputs(Rand(22), 8192, 128, 96, torch.float16)
+    w = [v[k] for k in ("x", "wg", "wu", "wd")]
+
+    def call():
+        y, saved = m.ffn(*w, train=True)
+        return (y,) + m.ffn_backward(*w, saved, v["dy"])
+
+    want = [k.clone() for k in call()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for k in range(4):
+        for o in out:
+            o.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+        call()
