@@ -112,12 +112,6 @@ __global__ __launch_bounds__(64 * NW, 2) void ffn_fused(FusedArgs g) {
     const auto og = resource(uniform(reinterpret_cast<const char*>(g.dg) + first), 0x7FFFFFFF);
     const auto ou = resource(uniform(reinterpret_cast<const char*>(g.du) + first), 0x7FFFFFFF);
     const auto oh = resource(uniform(reinterpret_cast<const char*>(g.h) + first), 0x7FFFFFFF);
-    auto put = [](auto rsrc, uint32_t a, uint32_t b, uint32_t at) {
-#if defined(__HIP_DEVICE_COMPILE__)
-        typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
-        __builtin_amdgcn_raw_buffer_store_b64(u2_t{a, b}, rsrc, at, 0, 0);
-#endif
-    };
     auto multiply = [&](int f0, const uint4* bg, const uint4* bu, const uint4* bd) __attribute__((always_inline)) {
         f4 ga[MB][2], up[MB][2], dh[BWD ? MB : 1][2];
 #pragma unroll
@@ -174,9 +168,9 @@ __global__ __launch_bounds__(64 * NW, 2) void ffn_fused(FusedArgs g) {
                     // always a store each, out of range where there is no such row or feature: the waits count them
                     const int f = f0 + j * 16 + hi * 4;
                     const uint32_t at = m < g.rows && f < (int)fp ? (uint32_t)((i * 16 + lo) * (int)fp + f) * 2u : kFar;
-                    put(og, v0[i][2 * j], v0[i][2 * j + 1], at);
-                    put(ou, v1[i][2 * j], v1[i][2 * j + 1], at);
-                    put(oh, q2[0] | (uint32_t)q2[1] << 16, q2[2] | (uint32_t)q2[3] << 16, at);
+                    put8(og, uint2{v0[i][2 * j], v0[i][2 * j + 1]}, at);
+                    put8(ou, uint2{v1[i][2 * j], v1[i][2 * j + 1]}, at);
+                    put8(oh, uint2{q2[0] | (uint32_t)q2[1] << 16, q2[2] | (uint32_t)q2[3] << 16}, at);
                 }
             }
         }

@@ -55,6 +55,7 @@ struct GemmArgs {
     int tiles_m, tiles_n;
     uint16_t *o0, *o1;
     int64_t ldo;
+    bool quads;  // kStore: outputs of whole, 8-byte aligned quads, whose offsets in a tile fit 32 bits
     float *pre_g, *pre_u;  // [m][ldpre]
     int64_t ldpre;
     float* part;           // [pair][split][m][ldpart]
@@ -159,6 +160,19 @@ __device__ __forceinline__ P* uniform(P* p) {
     const uint64_t v = reinterpret_cast<uint64_t>(p);
     const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
     return reinterpret_cast<P*>((uint64_t)hi << 32 | lo);
+}
+template <class R>
+__device__ __forceinline__ void put8(R rsrc, uint2 v, uint32_t at) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+    __builtin_amdgcn_raw_buffer_store_b64(u2_t{v.x, v.y}, rsrc, at, 0, 0);
+#endif
+}
+template <class R>
+__device__ __forceinline__ void put16(R rsrc, f4 v, uint32_t at) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, v), rsrc, at, 0, 0);
+#endif
 }
 // waits until at most N of the wave's vector memory operations are under way, and its LDS reads have arrived
 template <int N>
@@ -338,15 +352,28 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ffn_gemm(GemmArgs g) {
     }
     wait_vm<0>();
 
-    const int mw = m0 + wm * 16 * MB + (lane & 15), quad = 4 * (lane >> 4);
+    // ---- The epilogue: rows m0 + .., columns n0 + .. of the outputs, by buffer stores whose offsets are out of range
+    // where there is no such row or column (no branches: they would be most of the code, which a short launch fetches
+    // for the first time).
+    const int mr = wm * 16 * MB + (lane & 15), nr = wn * FW + 4 * (lane >> 4);  // in the tile, with 16 i and 16 j
+    auto place = [&](int i, int j, int64_t ld, int cols, uint32_t elem) -> uint32_t {
+        const int m = mr + i * 16, n = nr + j * 16;
+        return m0 + m < g.m && n0 + n < cols ? (uint32_t)(m * (int)ld + n) * elem : kFar;
+    };
+    auto at_tile = [&](auto* p, int64_t ld) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(uniform(reinterpret_cast<const char*>(p + m0 * ld + n0))),
+                                                 (short)0, 0x7FFFFFFF, 0x00020000);
+    };
+    auto pack = [](const uint16_t (&q)[4]) { return uint2{q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16}; };
     if constexpr (E == kGrad) {  // o0 and o1 have rows of up8(n), whose ends are zeros
+        const auto t0 = at_tile(g.o0, g.ldo), t1 = at_tile(g.o1, g.ldo);
         // both products of the next 16 rows are on their way while 16 rows are worked on; past the edge, the last ones
         f4 ga[2][NB], up[2][NB];
         auto load = [&](int i) {
-            const int64_t row = min(mw + i * 16, g.m - 1) * g.ldpre;
+            const int64_t row = min(m0 + mr + i * 16, g.m - 1) * g.ldpre;
 #pragma unroll
             for (int j = 0; j < NB; j++) {
-                const int64_t at = row + min(n0 + wn * FW + j * 16 + quad, (int)g.ldpre - 4);
+                const int64_t at = row + min(n0 + nr + j * 16, (int)g.ldpre - 4);
                 ga[i & 1][j] = *reinterpret_cast<const f4*>(g.pre_g + at);
                 up[i & 1][j] = *reinterpret_cast<const f4*>(g.pre_u + at);
             }
@@ -355,10 +382,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ffn_gemm(GemmArgs g) {
 #pragma unroll
         for (int i = 0; i < MB; i++) {
             if (i + 1 < MB) load(i + 1);
-            const int m = mw + i * 16;
 #pragma unroll
             for (int j = 0; j < NB; j++) {
-                const int n = n0 + wn * FW + j * 16 + quad;
+                const int n = n0 + nr + j * 16;
                 const f4 v = acc[i][j];
                 uint16_t qg[4], qu[4];
 #pragma unroll
@@ -368,47 +394,60 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ffn_gemm(GemmArgs g) {
                     qg[r] = n + r < g.n ? narrow(T{}, v[r] * up[i & 1][j][r] * slope) : (uint16_t)0;
                     qu[r] = n + r < g.n ? narrow(T{}, v[r] * value) : (uint16_t)0;
                 }
-                if (m < g.m && n < g.ldo) {
-                    store_raw<uint16_t, 4, true>(g.o0 + m * g.ldo + n, qg);
-                    store_raw<uint16_t, 4, true>(g.o1 + m * g.ldo + n, qu);
-                }
+                const uint32_t at = place(i, j, g.ldo, (int)g.ldo, 2);
+                put8(t0, pack(qg), at);
+                put8(t1, pack(qu), at);
             }
         }
-        return;
-    }
+    } else if constexpr (E == kGlu) {  // as have o0, pre_g and pre_u
+        const auto th = at_tile(g.o0, g.ldo), tg = at_tile(g.pre_g, g.ldpre), tu = at_tile(g.pre_u, g.ldpre);
 #pragma unroll
-    for (int i = 0; i < MB; i++) {
-        const int m = mw + i * 16;
-        if (m >= g.m) continue;
-        if constexpr (E == kGlu) {  // o0, pre_g and pre_u have rows of up8(n) as well
+        for (int i = 0; i < MB; i++) {
 #pragma unroll
             for (int j = 0; j < NB / 2; j++) {
-                const int f = n0 + wn * FW + j * 16 + quad;
-                if (f >= g.ldo) continue;
                 const f4 ga = acc[i][j], up = acc[i][j + NB / 2];
                 uint16_t q[4];
 #pragma unroll
-                for (int r = 0; r < 4; r++) q[r] = f + r < g.n ? narrow(T{}, act_of(g.act, ga[r]) * up[r]) : (uint16_t)0;
-                store_raw<uint16_t, 4, true>(g.o0 + m * g.ldo + f, q);
+                for (int r = 0; r < 4; r++) q[r] = narrow(T{}, act_of(g.act, ga[r]) * up[r]);  // 0 past n: both are 0
+                put8(th, pack(q), place(i, j, g.ldo, (int)g.ldo, 2));
                 if (g.pre_g) {
-                    *reinterpret_cast<f4*>(g.pre_g + m * g.ldpre + f) = ga;
-                    *reinterpret_cast<f4*>(g.pre_u + m * g.ldpre + f) = up;
+                    const uint32_t at = place(i, j, g.ldpre, (int)g.ldpre, 4);
+                    put16(tg, ga, at);
+                    put16(tu, up, at);
                 }
             }
-        } else {
+        }
+    } else if constexpr (E == kPart) {
+        const auto t = at_tile(g.part + (int64_t)(pair * g.splits + split) * g.m * g.ldpart, g.ldpart);
+#pragma unroll
+        for (int i = 0; i < MB; i++)
+#pragma unroll
+            for (int j = 0; j < NB; j++) put16(t, acc[i][j], place(i, j, g.ldpart, g.n, 4));
+    } else if (g.quads) {
+        const auto t = at_tile(pair ? g.o1 : g.o0, g.ldo);
+#pragma unroll
+        for (int i = 0; i < MB; i++) {
 #pragma unroll
             for (int j = 0; j < NB; j++) {
-                const int n = n0 + wn * FW + j * 16 + quad;
-                if (n >= g.n) continue;
-                const f4 v = acc[i][j];
-                if constexpr (E == kPart) {
-                    *reinterpret_cast<f4*>(g.part + ((int64_t)(pair * g.splits + split) * g.m + m) * g.ldpart + n) = v;
-                } else {
-                    uint16_t q[4];
+                uint16_t q[4];
 #pragma unroll
-                    for (int r = 0; r < 4; r++) q[r] = narrow(T{}, v[r]);
-                    store4((pair ? g.o1 : g.o0) + m * g.ldo + n, g.n - n, q);
-                }
+                for (int r = 0; r < 4; r++) q[r] = narrow(T{}, acc[i][j][r]);
+                put8(t, pack(q), place(i, j, g.ldo, g.n, 2));
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < MB; i++) {
+            const int m = m0 + mr + i * 16;
+            if (m >= g.m) continue;
+#pragma unroll
+            for (int j = 0; j < NB; j++) {
+                const int n = n0 + nr + j * 16;
+                if (n >= g.n) continue;
+                uint16_t q[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) q[r] = narrow(T{}, acc[i][j][r]);
+                store4((pair ? g.o1 : g.o0) + m * g.ldo + n, g.n - n, q);
             }
         }
     }

@@ -200,7 +200,7 @@ struct Shape {  // a product's tiles and splits
     size_t part_bytes;
 };
 // The larger tiles where they fill the chip's 256 CUs twice; else the smaller ones, with K split (where the epilogue
-// allows it) until there are two workgroups a CU, at least 8 slabs each.
+// allows it) to one workgroup a CU, at least 8 slabs each.
 Shape shape_of(int64_t m, int64_t n, int64_t k, int segments, int pairs, bool glu, bool may_split) {
     Shape s{};
     auto tiles = [&](int bm, int bn) { return ceil_div(m, bm) * ceil_div(n, bn); };
@@ -210,8 +210,8 @@ Shape shape_of(int64_t m, int64_t n, int64_t k, int segments, int pairs, bool gl
     s.slabs = (int)ceil_div(k, 32) * segments;
     s.splits = 1;
     const int64_t wgs = (int64_t)s.tiles_m * s.tiles_n * pairs;
-    if (may_split && wgs < (s.big ? 0 : 384) && s.slabs >= 16) {
-        int64_t z = ceil_div(512, wgs);
+    if (may_split && !s.big && wgs <= 128 && s.slabs >= 16) {
+        int64_t z = 256 / wgs;
         if (z > s.slabs / 8) z = s.slabs / 8;
         s.splits = z < 1 ? 1 : (int)z;
     }
@@ -277,6 +277,7 @@ int product(const char* op, GemmArgs g, float* part, hipStream_t st) {
     // a padded operand's rows hold more than its columns
     g.wide_m = (int)(up8(g.m) <= g.lda ? up8(g.m) : g.m), g.wide_n = (int)(up8(g.n) <= g.ldb ? up8(g.n) : g.n);
     if ((int64_t)s.tiles_m * s.tiles_n >= 1ll << 31) return fail(-1, "%s: too many tiles", op);
+    g.quads = g.n % 4 == 0 && g.ldo % 4 == 0 && g.ldo <= 1 << 21 && aligned(g.o0, 8) && aligned(g.o1, 8);
     if constexpr (E == kStore) {
         if (s.splits > 1) {
             g.part = part, g.ldpart = ((int64_t)g.n + 3) / 4 * 4;
