@@ -11,7 +11,7 @@
 // - Rows: an LDS row holds 32 k (64 bytes), its 16-byte chunk c at position c ^ (row >> 2 & 2): a fragment read (16
 //   bytes a lane) goes by lanes 0-3, 12-15, 20-23, 24-27 and the like, 16 at once, which so fall on all 64 banks (other
 //   permutations of the chunks, by row >> 2 or by 8 neighbours, measured a conflict for every read). Columns: an LDS row holds the tile's m (n) of one k, its
-//   32-byte blocks permuted by f(k) = k & 3 | (k >> 3 & 1) << 2; fragments come from the transposing LDS read (16 lanes
+//   32-byte blocks permuted by f(k) = k & 3 | (k >> 3 & 1) << 2 (64 wide: k >> 1 & 1 | (k >> 3 & 1) << 1); fragments come from the transposing LDS read (16 lanes
 //   read 4 k x 16 m and receive 4 k of one m each), whose 32 lanes at once then spread over all banks too.
 // - The MFMA takes B's fragment as its first operand: a lane's 4 results are 4 adjacent n of one m.
 // - Workgroups go round-robin to the 8 XCDs, each with its own L2: the tile index is permuted so that an XCD works on
@@ -112,13 +112,17 @@ struct Operand {
     static constexpr int NI = R * 64 / 1024 / NW;  // DMA instructions a wave
     static constexpr int CPI = 512 / R;            // COLS: k of an instruction
     static constexpr int U4 = R * 4;               // 16-byte units of a slab
+    // COLS: the permutation of a row's 32-byte blocks (4 of them in 64 columns); k and k + 4 have the same
+    static __device__ __forceinline__ int blocks_turn(int k) {
+        return R == 64 ? (k >> 1 & 1) | (k >> 3 & 1) << 1 : (k & 3) | (k >> 3 & 1) << 2;
+    }
     static __device__ __forceinline__ int turn(int row) { return row >> 2 & 2; }
     // the k and the first m (n) of lane `lane`'s 16 bytes of instruction q, relative to the tile and slab
     static __device__ __forceinline__ void place(int inst, int lane, int& r, int& k) {
         if constexpr (COLS) {
             k = inst * CPI + lane / (64 / CPI);
             const int pos = lane % (64 / CPI);
-            const int f = (k & 3) | (k >> 3 & 1) << 2;
+            const int f = blocks_turn(k);
             r = (((pos >> 1) ^ f) << 4) + ((pos & 1) << 3);
         } else {
             r = inst * 16 + (lane >> 2);
@@ -130,7 +134,7 @@ struct Operand {
         const char* p = reinterpret_cast<const char*>(lds);
         if constexpr (COLS) {
             const int j = (lane & 15) >> 2, g = lane >> 4;
-            const int f = j | (g & 1) << 2;
+            const int f = blocks_turn(g * 8 + j);
             // Each address one opaque offset from the buffer: of a sum with a constant the compiler makes a chain, behind
             // which it no longer knows the buffer that is read, and it then waits for the DMA of all.
             [[maybe_unused]] int lo_at = (g * 8 + j) * (R * 2) + (((base >> 4) ^ f) << 5) + (lane & 3) * 8;

@@ -61,9 +61,11 @@ __global__ __launch_bounds__(256) void ffn_pack(PackArgs g) {
     }
 }
 
-// ---- few rows: a wave streams 16 weight rows past the matrix unit straight from global memory (each weight is used
-// once, so LDS would only add a step), NB blocks of 16 token rows as the other operand; the NW waves of a workgroup
-// split K and add their sums in LDS in the waves' order.
+// ---- few rows: a wave streams weight rows past the matrix unit straight from global memory (each weight is used once,
+// so LDS would only add a step), NB blocks of 16 token rows as the other operand; the NW waves of a workgroup split K and
+// add their sums in LDS in the waves' order. GLU: 16 rows of wg and of wu. Else the 16 rows that the unit takes are 8
+// weight rows twice, at the two halves of K, each half with its own token fragment (the other half's result is left):
+// twice the workgroups and half the steps, where the second product has few columns to spread over the chip.
 struct SkinnyArgs {
     const uint16_t *x, *w0, *w1;
     int64_t ldx, ldw;
@@ -84,86 +86,96 @@ __device__ __forceinline__ u4_t load_k(const uint16_t* row, int k) {
 
 template <class T, bool GLU, int NB, int NW, bool AL>
 __global__ __launch_bounds__(64 * NW) void ffn_skinny(SkinnyArgs g) {
-    constexpr int P = GLU ? 2 : 1;
-    __shared__ f4 sums[NW][P * NB][64];
+    constexpr int ROWS = GLU ? 16 : 8;
+    __shared__ f4 sums[NW][2 * NB][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int f0 = blockIdx.x * 16, f = min(f0 + (lane & 15), g.n - 1);  // a row past the end: the last one again
+    const int f0 = blockIdx.x * ROWS, f = min(f0 + (lane & (ROWS - 1)), g.n - 1);  // a row past the end: the last one again
     const int kl = 8 * (lane >> 4);
-    const int steps = (g.k + 31) / 32, per = (steps + NW - 1) / NW;
+    const int all = (g.k + 31) / 32, steps = GLU ? all : (all + 1) / 2, per = (steps + NW - 1) / NW;
     const int s0 = wave * per, s1 = min(steps, s0 + per);
+    const int half = steps * 32, wk = kl + (GLU ? 0 : (lane >> 3 & 1) * half);  // the lane's k of step 0, weights
     const uint16_t* w0 = g.w0 + (int64_t)f * g.ldw;
     const uint16_t* w1 = GLU ? g.w1 + (int64_t)f * g.ldw : nullptr;
     const uint16_t* x[NB];
 #pragma unroll
     for (int b = 0; b < NB; b++) x[b] = g.x + (int64_t)min(b * 16 + (lane & 15), g.rows - 1) * g.ldx;
-    f4 acc[P][NB];
+    f4 acc[2][NB];  // gate and up; or the halves of K
 #pragma unroll
-    for (int p = 0; p < P; p++)
+    for (int p = 0; p < 2; p++)
 #pragma unroll
         for (int b = 0; b < NB; b++) acc[p][b] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int U = NB == 4 ? 4 : 8;  // steps whose loads are in flight together
-    auto multiply = [&](const u4_t (&w)[P], const u4_t (&v)[NB]) {
+    constexpr int U = 8;  // steps whose loads are in flight together
+    auto multiply = [&](u4_t wa, u4_t wb, const u4_t (&v)[NB], const u4_t (&v2)[NB]) {
 #pragma unroll
-        for (int p = 0; p < P; p++)
-#pragma unroll
-            for (int b = 0; b < NB; b++) acc[p][b] = mfma16(T{}, w[p], v[b], acc[p][b]);
+        for (int b = 0; b < NB; b++) {
+            acc[0][b] = mfma16(T{}, wa, v[b], acc[0][b]);
+            acc[1][b] = mfma16(T{}, wb, v2[b], acc[1][b]);
+        }
     };
-    const int full = g.k / 32;  // the last step may be cut
+    const int full = (g.k - (GLU ? 0 : half)) / 32;  // the last steps may be cut, and of the second half missing
     int s = s0;
     for (; s + U <= min(s1, full); s += U) {
-        u4_t w[U][P], v[U][NB];
+        u4_t w[U][2], v[U][NB], v2[U][GLU ? 1 : NB];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int k = (s + u) * 32 + kl;
-            w[u][0] = load_k<AL>(w0, k);
-            if constexpr (GLU) w[u][1] = load_k<AL>(w1, k);
+            const int k = (s + u) * 32;
+            w[u][0] = load_k<AL>(w0, k + wk);
+            if constexpr (GLU) w[u][1] = load_k<AL>(w1, k + wk);
 #pragma unroll
-            for (int b = 0; b < NB; b++) v[u][b] = load_k<AL>(x[b], k);
+            for (int b = 0; b < NB; b++) {
+                v[u][b] = load_k<AL>(x[b], k + kl);
+                if constexpr (!GLU) v2[u][b] = load_k<AL>(x[b], k + half + kl);
+            }
         }
 #pragma unroll
-        for (int u = 0; u < U; u++) multiply(w[u], v[u]);
+        for (int u = 0; u < U; u++) {
+            if constexpr (GLU) multiply(w[u][0], w[u][1], v[u], v[u]);
+            else multiply(w[u][0], w[u][0], v[u], v2[u]);
+        }
     }
     for (; s < s1; s++) {
-        const int k = s * 32 + kl;
-        u4_t w[P], v[NB];
-        w[0] = load_some(w0 + k, g.k - k);
-        if constexpr (GLU) w[1] = load_some(w1 + k, g.k - k);
+        const int k = s * 32;
+        u4_t wa = load_some(w0 + k + wk, g.k - k - wk), wb, v[NB], v2[NB];
+        if constexpr (GLU) wb = load_some(w1 + k + wk, g.k - k - wk);
 #pragma unroll
-        for (int b = 0; b < NB; b++) v[b] = load_some(x[b] + k, g.k - k);
-        multiply(w, v);
+        for (int b = 0; b < NB; b++) {
+            v[b] = load_some(x[b] + k + kl, g.k - k - kl);
+            if constexpr (!GLU) v2[b] = load_some(x[b] + k + half + kl, g.k - k - half - kl);
+        }
+        if constexpr (GLU) multiply(wa, wb, v, v);
+        else multiply(wa, wa, v, v2);
     }
 #pragma unroll
-    for (int p = 0; p < P; p++)
+    for (int p = 0; p < 2; p++)
 #pragma unroll
         for (int b = 0; b < NB; b++) sums[wave][p * NB + b][lane] = acc[p][b];
     __syncthreads();
-    // wave b finishes token block b (f = f0 + 4 (lane >> 4) + r of row b * 16 + (lane & 15))
+    // wave b finishes token block b (f0 + 4 (lane >> 4) + r of row b * 16 + (lane & 15))
     for (int b = wave; b < NB; b += NW) {
-        f4 t[P];
-#pragma unroll
-        for (int p = 0; p < P; p++) {
-            t[p] = sums[0][p * NB + b][lane];
-            for (int w = 1; w < NW; w++) t[p] += sums[w][p * NB + b][lane];
+        f4 t[2] = {f4{0.0f, 0.0f, 0.0f, 0.0f}, f4{0.0f, 0.0f, 0.0f, 0.0f}};
+        for (int w = 0; w < NW; w++) {
+            t[0] += sums[w][b][lane];
+            t[1] += sums[w][NB + b][GLU ? lane : (lane + 32) & 63];  // the second half's rows are the unit's 8 to 15
         }
         const int row = b * 16 + (lane & 15), at = f0 + 4 * (lane >> 4);
-        if (row >= g.rows || at >= g.width) continue;
+        if (row >= g.rows || at >= g.width || (!GLU && lane >= 32)) continue;
         uint16_t q[4];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            if (GLU && at + r >= g.n) t[0][r] = t[P - 1][r] = 0.0f;
-            q[r] = narrow(T{}, GLU ? act_of(g.act, t[0][r]) * t[P - 1][r] : t[0][r]);
+            if (GLU && at + r >= g.n) t[0][r] = t[1][r] = 0.0f;
+            q[r] = narrow(T{}, GLU ? act_of(g.act, t[0][r]) * t[1][r] : t[0][r] + t[1][r]);
         }
         store4(g.out + row * g.ldo + at, g.width - at, q);
         if (GLU && g.pre_g) {
             *reinterpret_cast<f4*>(g.pre_g + row * g.ldo + at) = t[0];
-            *reinterpret_cast<f4*>(g.pre_u + row * g.ldo + at) = t[P - 1];
+            *reinterpret_cast<f4*>(g.pre_u + row * g.ldo + at) = t[1];
         }
     }
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------
 
-constexpr uint32_t kSkinnyRows = 64;  // up to here the weights' bytes are all that counts
+constexpr uint32_t kSkinnyRows = 32;  // up to here the weights' bytes are all that counts
 
 // One kernel a direction (ffn_fused.h) where the channels fit its registers and the rows give it work for the chip; a
 // workgroup of it walks all features, so few rows go through the products of ffn_gemm.h, which spread over features too.
@@ -194,23 +206,34 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 size_t hidden_bytes(const fhc_ffn_desc* d) { return up256((size_t)d->rows * up8(d->f) * 2); }
 size_t pre_bytes(const fhc_ffn_desc* d) { return up256((size_t)d->rows * up8(d->f) * 4); }
 
+enum Tile { kNarrow, kMedium, kLarge };  // 128 x 64, 128 x 128, 256 x 256
 struct Shape {  // a product's tiles and splits
-    bool big;   // 128 x 256 tiles, else 128 x 128
+    Tile tile;
     int tiles_m, tiles_n, slabs, per_split, splits;
     size_t part_bytes;
 };
-// The larger tiles where they fill the chip's 256 CUs twice; else the smaller ones, with K split (where the epilogue
-// allows it) to one workgroup a CU, at least 8 slabs each.
+// The tile whose workgroups, a round of 256 at a time, take the least: a medium tile's slab counts 100, a narrow one's 75
+// and a large one's 270 (of 50 and 400 by area: the wider the tile, the less LDS traffic a product). Where K may be split
+// and there are at most 128 medium tiles, it is split to one workgroup a CU, at least 8 slabs each.
 Shape shape_of(int64_t m, int64_t n, int64_t k, int segments, int pairs, bool glu, bool may_split) {
     Shape s{};
-    auto tiles = [&](int bm, int bn) { return ceil_div(m, bm) * ceil_div(n, bn); };
-    s.big = tiles(256, glu ? 128 : 256) * pairs >= 224;
-    const int bn = (s.big ? 256 : 128) / (glu ? 2 : 1);
-    s.tiles_m = (int)ceil_div(m, s.big ? 256 : 128), s.tiles_n = (int)ceil_div(n, bn);
+    const int unit = glu ? 2 : 1;
+    const int64_t bm[3] = {128, 128, 256}, bn[3] = {64, 128, 256}, cost[3] = {75, 100, 270};
+    auto count = [&](int t) { return (int64_t)(ceil_div(m, bm[t]) * ceil_div(n, bn[t] / unit)) * pairs; };
+    s.tile = kMedium;
+    const bool split = may_split && count(kMedium) <= 128 && ceil_div(k, 32) * segments >= 16;
+    if (!split) {
+        int64_t best = 0;
+        for (int t = 0; t < 3; t++) {
+            const int64_t time = (int64_t)ceil_div(count(t), 256) * cost[t];
+            if (t == 0 || time < best) best = time, s.tile = (Tile)t;
+        }
+    }
+    s.tiles_m = (int)ceil_div(m, bm[s.tile]), s.tiles_n = (int)ceil_div(n, bn[s.tile] / unit);
     s.slabs = (int)ceil_div(k, 32) * segments;
     s.splits = 1;
     const int64_t wgs = (int64_t)s.tiles_m * s.tiles_n * pairs;
-    if (may_split && !s.big && wgs <= 128 && s.slabs >= 16) {
+    if (split) {
         int64_t z = 256 / wgs;
         if (z > s.slabs / 8) z = s.slabs / 8;
         s.splits = z < 1 ? 1 : (int)z;
@@ -263,8 +286,17 @@ struct Operands {
 template <class T, bool AC, bool BC, Epi E>
 void launch_tiles(const Shape& s, const GemmArgs& g, hipStream_t st) {
     const dim3 grid(s.tiles_m * s.tiles_n, 1, s.splits * g.pairs);
-    if (s.big) hipLaunchKernelGGL((ffn_gemm<T, AC, BC, E, 8, 4, 2, 4>), grid, dim3(512), 0, st, g);
-    else hipLaunchKernelGGL((ffn_gemm<T, AC, BC, E, 4, 4, 2, 2>), grid, dim3(256), 0, st, g);
+    if constexpr (E != kPart) {  // a split K has medium tiles
+        if (s.tile == kLarge) {
+            hipLaunchKernelGGL((ffn_gemm<T, AC, BC, E, 8, 4, 2, 4>), grid, dim3(512), 0, st, g);
+            return;
+        }
+        if (s.tile == kNarrow) {
+            hipLaunchKernelGGL((ffn_gemm<T, AC, BC, E, 4, 2, 2, 2>), grid, dim3(256), 0, st, g);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((ffn_gemm<T, AC, BC, E, 4, 4, 2, 2>), grid, dim3(256), 0, st, g);
 }
 
 // g without tiles and splits
@@ -301,7 +333,8 @@ template <class T, bool GLU>
 int skinny(const char* op, const SkinnyArgs& a, hipStream_t st) {
     if (a.n == 0) return 0;
     constexpr int NW = GLU ? 4 : 16;
-    const dim3 grid((uint32_t)ceil_div(a.n, 16));
+    const dim3 grid((uint32_t)ceil_div(a.n, GLU ? 16 : 8));
+    // a whole step's loads are 16-byte aligned (the second half of K starts at a multiple of 32)
     const bool al = a.k % 8 == 0 && a.ldx % 8 == 0 && a.ldw % 8 == 0 && aligned(a.x, 16) && aligned(a.w0, 16) &&
                     aligned(a.w1, 16);
 #define SKINNY(NB)                                                                                              \
@@ -310,8 +343,7 @@ int skinny(const char* op, const SkinnyArgs& a, hipStream_t st) {
         else hipLaunchKernelGGL((ffn_skinny<T, GLU, NB, NW, false>), grid, dim3(64 * NW), 0, st, a);            \
     } while (0)
     if (a.rows <= 16) SKINNY(1);
-    else if (a.rows <= 32) SKINNY(2);
-    else SKINNY(4);
+    else SKINNY(2);
 #undef SKINNY
     return launched(op);
 }
