@@ -44,7 +44,9 @@ struct Wave {
         const uint64_t at = reinterpret_cast<uint64_t>(p) + (uint64_t)((int64_t)t * ts);
         const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)at);
         const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
-        return (__attribute__((address_space(1))) char*)((uint64_t)hi << 32 | lo) + lane;
+        uint32_t own = lane;  // opaque: its extension to 64 bits stays here, where a load takes it for nothing
+        asm("" : "+v"(own));
+        return (__attribute__((address_space(1))) char*)((uint64_t)hi << 32 | lo) + own;
     }
     template <class C>
     __device__ __forceinline__ C load(uint32_t t) const {
@@ -271,6 +273,7 @@ __global__ __launch_bounds__(64 * W * CW, L > 8 ? (CHAIN && sizeof(typename T::R
     using R = typename T::Raw;
     using C = Cell<T, V>;
     constexpr int CL = W * L;
+    constexpr bool ONE = W > 1 && W < 8;  // these chunks hold whole sequences
     __shared__ float2 maps[W > 1 ? W : 1][W > 1 ? CW * 64 * V : 1];
     __shared__ float2 far[CHAIN ? kRun : 1][CHAIN ? 64 * V : 1];
     static_assert(!CHAIN || CW == 1, "a chained chunk's columns are one wave wide");
@@ -292,26 +295,28 @@ __global__ __launch_bounds__(64 * W * CW, L > 8 ? (CHAIN && sizeof(typename T::R
     }
     const Wave wx(g.x, b, ch, sizeof(R)), wr(g.r, b, ch, sizeof(R)), wi(g.i, b, ch, sizeof(R)), wy(g.y, b, ch, sizeof(R));
 
-    const uint32_t last = CHAIN ? chunk + 1 : g.nchunk;
+    const uint32_t last = CHAIN ? chunk + 1 : ONE ? 1 : g.nchunk;
     for (; chunk < last; chunk++) {
         const uint32_t t0 = chunk * CL + tw * L;
-        C xr[L], rr[L], ir[L];
-        const bool full = __all(t0 + L <= n);
-        load_steps(wr, t0, n, full, C(C::lowest()), rr);
-        load_steps(wi, t0, n, full, C(C::lowest()), ir);
-        load_steps(wx, t0, n, full, C(C::zero()), xr);
+        const bool full = __all(t0 + L <= n), some = __any(t0 < n);
         float a[L][V], in[L][V], A[V], S[V];
 #pragma unroll
         for (int v = 0; v < V; v++) A[v] = 1.0f, S[v] = 0.0f;
+        if (some) {
+            C xr[L], rr[L], ir[L];
+            load_steps(wr, t0, n, full, C(C::lowest()), rr);
+            load_steps(wi, t0, n, full, C(C::lowest()), ir);
+            load_steps(wx, t0, n, full, C(C::zero()), xr);
 #pragma unroll
-        for (int l = 0; l < L; l++) {
+            for (int l = 0; l < L; l++) {
 #pragma unroll
-            for (int v = 0; v < V; v++) {
-                const Gates q = gates_of(k[v], rr[l].at(v), ir[l].at(v));
-                a[l][v] = q.a, in[l][v] = __builtin_amdgcn_sqrtf(q.v) * (q.si * xr[l].at(v));
-                if constexpr (W > 1) {
-                    S[v] = __builtin_fmaf(a[l][v], S[v], in[l][v]);
-                    A[v] *= a[l][v];
+                for (int v = 0; v < V; v++) {
+                    const Gates q = gates_of(k[v], rr[l].at(v), ir[l].at(v));
+                    a[l][v] = q.a, in[l][v] = __builtin_amdgcn_sqrtf(q.v) * (q.si * xr[l].at(v));
+                    if constexpr (W > 1) {
+                        S[v] = __builtin_fmaf(a[l][v], S[v], in[l][v]);
+                        A[v] *= a[l][v];
+                    }
                 }
             }
         }
@@ -368,13 +373,17 @@ __global__ __launch_bounds__(64 * W * CW, L > 8 ? (CHAIN && sizeof(typename T::R
 #pragma unroll
             for (int v = 0; v < V; v++) g.states[((uint64_t)b * g.nstates + (t0 >> g.spacing)) * g.d + ch + v] = h[v];
         }
+        if (some) {
 #pragma unroll
-        for (int l = 0; l < L; l++) {
+            for (int l = 0; l < L; l++) {
 #pragma unroll
-            for (int v = 0; v < V; v++) h[v] = __builtin_fmaf(a[l][v], h[v], in[l][v]);
-            const C out = C::of(h);
-            if (full || (live && t0 + l < g.t))
-                wy.store(t0 + l, C(out.where(full || t0 + l < n)));
+                for (int v = 0; v < V; v++) h[v] = __builtin_fmaf(a[l][v], h[v], in[l][v]);
+                const C out = C::of(h);
+                if (full || (live && t0 + l < g.t)) wy.store(t0 + l, C(out.where(full || t0 + l < n)));
+            }
+        } else {
+            for (int l = 0; l < L; l++)
+                if (live && t0 + l < g.t) wy.store(t0 + l, C(C::zero()));
         }
         if constexpr (W > 1) {
 #pragma unroll
@@ -393,10 +402,11 @@ __global__ __launch_bounds__(64 * W * CW, L > 8 ? (CHAIN && sizeof(typename T::R
 // A lane keeps six values a step while the chunk's maps are exchanged (and x and dy as they were read): more registers
 // would cost the waves that hide the loads.
 template <class T, int V, int L, int W, int CW, bool CHAIN>
-__global__ __launch_bounds__(64 * W * CW, L > 1 ? 3 : 1) void glr_bwd(GlrArgs g) {
+__global__ __launch_bounds__(64 * W * CW, L == 1 ? 1 : W == 8 && !CHAIN ? 2 : 3) void glr_bwd(GlrArgs g) {
     using R = typename T::Raw;
     using C = Cell<T, V>;
     constexpr int CL = W * L;
+    constexpr bool ONE = W > 1 && W < 8;  // these chunks hold whole sequences
     __shared__ float2 maps[W > 1 ? W : 1][W > 1 ? CW * 64 * V : 1];  // (A, S) forward
     __shared__ float back[W > 1 ? W : 1][W > 1 ? CW * 64 * V : 1];   // the R of c -> A c + R
     __shared__ float2 far[CHAIN ? kRun : 1][CHAIN ? 64 * V : 1];
@@ -421,46 +431,49 @@ __global__ __launch_bounds__(64 * W * CW, L > 1 ? 3 : 1) void glr_bwd(GlrArgs g)
     const Wave wx(g.x, b, ch, sizeof(R)), wr(g.r, b, ch, sizeof(R)), wi(g.i, b, ch, sizeof(R)),
         wdy(g.dy, b, ch, sizeof(R)), wdx(g.dx, b, ch, sizeof(R)), wdr(g.dr, b, ch, sizeof(R)), wdi(g.di, b, ch, sizeof(R));
 
-    const uint32_t last = CHAIN ? done + 1 : g.nchunk;
+    const uint32_t last = CHAIN ? done + 1 : ONE ? 1 : g.nchunk;
     for (; done < last; done++) {
         const uint32_t chunk = g.nchunk - 1 - done, t0 = chunk * CL + tw * L;
-        C xr[L], rr[L], ir[L], gr[L];
-        const bool full = __all(t0 + L <= n);
+        C xr[L], gr[L];
+        const bool full = __all(t0 + L <= n), some = __any(t0 < n);
         float h[V];
 #pragma unroll
         for (int v = 0; v < V; v++)
             h[v] = live && chunk < g.nstates ? g.states[((uint64_t)b * g.nstates + chunk) * g.d + ch + v] : 0.0f;
-        load_steps(wr, t0, n, full, C(C::lowest()), rr);
-        load_steps(wi, t0, n, full, C(C::lowest()), ir);
-        load_steps(wx, t0, n, full, C(C::zero()), xr);
-        load_steps(wdy, t0, n, full, C(C::zero()), gr);
         // p = m si; q = a w / m, later h_(t-1) - q
         float a[L][V], p[L][V], q[L][V], sr[L][V], lr[L][V], ni[L][V], A[V], S[V], B[V];
 #pragma unroll
         for (int v = 0; v < V; v++) A[v] = 1.0f, S[v] = 0.0f, B[v] = 0.0f;
+        if (some) {
+            C rr[L], ir[L];
+            load_steps(wr, t0, n, full, C(C::lowest()), rr);
+            load_steps(wi, t0, n, full, C(C::lowest()), ir);
+            load_steps(wx, t0, n, full, C(C::zero()), xr);
+            load_steps(wdy, t0, n, full, C(C::zero()), gr);
 #pragma unroll
-        for (int l = 0; l < L; l++) {
-            // one step after the other: with every step's exponentials taken first, as the compiler would, the gates of
-            // all steps are alive together
-            rr[l].forget(), ir[l].forget();
+            for (int l = 0; l < L; l++) {
+                // one step after the other: with every step's exponentials taken first, as the compiler would, the gates of
+                // all steps are alive together
+                rr[l].forget(), ir[l].forget();
 #pragma unroll
-            for (int v = 0; v < V; v++) {
-                const Gates s = gates_of(k[v], rr[l].at(v), ir[l].at(v));
-                const float x = xr[l].at(v), dy = gr[l].at(v);
-                // 1 - a^2 is 0 where nothing decays, and no larger than log a: the gradient that passes through m's
-                // root, log a / m, is 0 at this limit (times a finite value)
-                const float rm = __builtin_amdgcn_rsqf(__builtin_fmaxf(s.v, 1.17549435e-38f));
-                a[l][v] = s.a, sr[l][v] = s.sr;
-                lr[l][v] = s.z * kLn2 * shut(s.er, s.sr);
-                ni[l][v] = shut(s.ei, s.si);
-                p[l][v] = s.v * rm * s.si;
-                q[l][v] = s.a * rm * (s.si * x);
-                if constexpr (W > 1) {
-                    S[v] = __builtin_fmaf(s.a, S[v], p[l][v] * x);
-                    A[v] *= s.a;
-                    B[v] = __builtin_fmaf(A[v], dy, B[v]);  // dy_l reaches the front through a_1 .. a_l
+                for (int v = 0; v < V; v++) {
+                    const Gates s = gates_of(k[v], rr[l].at(v), ir[l].at(v));
+                    const float x = xr[l].at(v), dy = gr[l].at(v);
+                    // 1 - a^2 is 0 where nothing decays, and no larger than log a: the gradient that passes through m's
+                    // root, log a / m, is 0 at this limit (times a finite value)
+                    const float rm = __builtin_amdgcn_rsqf(__builtin_fmaxf(s.v, 1.17549435e-38f));
+                    a[l][v] = s.a, sr[l][v] = s.sr;
+                    lr[l][v] = s.z * kLn2 * shut(s.er, s.sr);
+                    ni[l][v] = shut(s.ei, s.si);
+                    p[l][v] = s.v * rm * s.si;
+                    q[l][v] = s.a * rm * (s.si * x);
+                    if constexpr (W > 1) {
+                        S[v] = __builtin_fmaf(s.a, S[v], p[l][v] * x);
+                        A[v] *= s.a;
+                        B[v] = __builtin_fmaf(A[v], dy, B[v]);  // dy_l reaches the front through a_1 .. a_l
+                    }
+                    asm volatile("" : "+v"(p[l][v]), "+v"(q[l][v]), "+v"(lr[l][v]), "+v"(ni[l][v]));
                 }
-                asm volatile("" : "+v"(p[l][v]), "+v"(q[l][v]), "+v"(lr[l][v]), "+v"(ni[l][v]));
             }
         }
         float end[V];  // what the chunk hands to the chunk before it
@@ -521,35 +534,44 @@ __global__ __launch_bounds__(64 * W * CW, L > 1 ? 3 : 1) void glr_bwd(GlrArgs g)
 #pragma unroll
             for (int v = 0; v < V; v++) c[v] = __builtin_fmaf(pa[v], c[v], ps[v]);
         }
-        // what was derived from x and dy is derived again: the compiler would keep it in registers across the exchange
+        if (some) {
+            // what was derived from x and dy is derived again: the compiler would keep it in registers across the exchange
 #pragma unroll
-        for (int l = 0; l < L; l++) xr[l].forget(), gr[l].forget();
+            for (int l = 0; l < L; l++) xr[l].forget(), gr[l].forget();
 #pragma unroll
-        for (int l = 0; l < L; l++) {
+            for (int l = 0; l < L; l++) {
 #pragma unroll
-            for (int v = 0; v < V; v++) {
-                q[l][v] = h[v] - q[l][v];
-                h[v] = __builtin_fmaf(a[l][v], h[v], p[l][v] * xr[l].at(v));
+                for (int v = 0; v < V; v++) {
+                    q[l][v] = h[v] - q[l][v];
+                    h[v] = __builtin_fmaf(a[l][v], h[v], p[l][v] * xr[l].at(v));
+                }
             }
-        }
 #pragma unroll
-        for (int l = L - 1; l >= 0; l--) {
-            const bool on = full || t0 + l < n;
-            float ox[V], orr[V], oi[V];
+            for (int l = L - 1; l >= 0; l--) {
+                const bool on = full || t0 + l < n;
+                float ox[V], orr[V], oi[V];
 #pragma unroll
-            for (int v = 0; v < V; v++) {
-                const float gt = gr[l].at(v) + c[v];
-                c[v] = a[l][v] * gt;
-                const float dla = on ? c[v] * q[l][v] : 0.0f;
-                ox[v] = gt * p[l][v];
-                orr[v] = dla * lr[l][v];
-                oi[v] = ox[v] * xr[l].at(v) * ni[l][v];
-                lam_sum[v] = __builtin_fmaf(dla, sr[l][v], lam_sum[v]);
+                for (int v = 0; v < V; v++) {
+                    const float gt = gr[l].at(v) + c[v];
+                    c[v] = a[l][v] * gt;
+                    const float dla = on ? c[v] * q[l][v] : 0.0f;
+                    ox[v] = gt * p[l][v];
+                    orr[v] = dla * lr[l][v];
+                    oi[v] = ox[v] * xr[l].at(v) * ni[l][v];
+                    lam_sum[v] = __builtin_fmaf(dla, sr[l][v], lam_sum[v]);
+                }
+                if (full || (live && t0 + l < g.t)) {
+                    wdx.store(t0 + l, C(C(C::of(ox)).where(on)));
+                    wdr.store(t0 + l, C(C::of(orr)));
+                    wdi.store(t0 + l, C(C(C::of(oi)).where(on)));
+                }
             }
-            if (full || (live && t0 + l < g.t)) {
-                wdx.store(t0 + l, C(C(C::of(ox)).where(on)));
-                wdr.store(t0 + l, C(C::of(orr)));
-                wdi.store(t0 + l, C(C(C::of(oi)).where(on)));
+        } else {
+            for (int l = 0; l < L; l++) {
+                if (!live || t0 + l >= g.t) continue;
+                wdx.store(t0 + l, C(C::zero()));
+                wdr.store(t0 + l, C(C::zero()));
+                wdi.store(t0 + l, C(C::zero()));
             }
         }
         if constexpr (W > 1) {
