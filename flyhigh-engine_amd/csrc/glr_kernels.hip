@@ -208,7 +208,7 @@ constexpr uint64_t kUnpublished = 0xBF800000ull;  // (-1, 0)
 __device__ __forceinline__ void publish(uint64_t* p, float a, float s) {
     __hip_atomic_store(p, word_of(a, s), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-constexpr uint32_t kRun = 16;  // chunks of a run
+constexpr uint32_t kRun = 32;  // chunks of a run
 
 constexpr uint32_t kTicketStep = 32;  // a column block's ticket has 128 bytes of its own
 
@@ -220,26 +220,38 @@ __global__ __launch_bounds__(256) void glr_clear(uint64_t* agg, uint64_t n, uint
 
 // The chain's search: the state that reaches this lane's columns of a chunk, `k` chunks after the head of its run.
 // word(j) is the published map of the run's j-th chunk, head the run's first state. The W waves fetch the words
-// together; the fold is in the chunks' order whatever the order of their arrival, so results repeat bit for bit.
+// together, a wave all of its own at once, and again until they are all there; the fold is in the chunks' order whatever
+// the order of their arrival, so results repeat bit for bit.
 template <int V, int W, class Word>
 __device__ __forceinline__ void chain_find(uint32_t k, uint32_t tw, uint32_t slot, bool live, float2 (*lds)[64 * V],
                                            const uint64_t* head, Word word, float (&h)[V]) {
-    auto wait_for = [](const uint64_t* p) {
-        uint64_t w;
-        do {
-            w = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        } while ((uint32_t)w == (uint32_t)kUnpublished);
-        return float2{__builtin_bit_cast(float, (uint32_t)w), __builtin_bit_cast(float, (uint32_t)(w >> 32))};
-    };
+    constexpr uint32_t N = kRun / W;  // entries of a wave: chunks tw, tw + W, ..; the last wave's last is the head
     if (live) {
-        for (uint32_t j = tw; j < k; j += W) {
+        uint64_t w[N][V];
+        bool missing;
+        do {
 #pragma unroll
-            for (int v = 0; v < V; v++) lds[j][slot * V + v] = wait_for(word(j) + v);
-        }
-        if (tw == W - 1 && head) {  // the wave with the fewest words of chunks
+            for (uint32_t n = 0; n < N; n++) {
+                const uint32_t j = n * W + tw;
+                const uint64_t* p = j == kRun - 1 ? head : j < k ? word(j) : nullptr;
 #pragma unroll
-            for (int v = 0; v < V; v++) lds[kRun - 1][slot * V + v] = wait_for(head + v);
-        }
+                for (int v = 0; v < V; v++) {
+                    w[n][v] = 0;
+                    if (p) w[n][v] = __hip_atomic_load(p + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+            }
+            missing = false;
+#pragma unroll
+            for (uint32_t n = 0; n < N; n++)
+#pragma unroll
+                for (int v = 0; v < V; v++) missing |= (uint32_t)w[n][v] == (uint32_t)kUnpublished;
+        } while (missing);
+#pragma unroll
+        for (uint32_t n = 0; n < N; n++)
+#pragma unroll
+            for (int v = 0; v < V; v++)
+                lds[n * W + tw][slot * V + v] = float2{__builtin_bit_cast(float, (uint32_t)w[n][v]),
+                                                      __builtin_bit_cast(float, (uint32_t)(w[n][v] >> 32))};
     }
     __syncthreads();
     if (!live) return;
@@ -247,6 +259,7 @@ __device__ __forceinline__ void chain_find(uint32_t k, uint32_t tw, uint32_t slo
 #pragma unroll
         for (int v = 0; v < V; v++) h[v] = lds[kRun - 1][slot * V + v].y;
     }
+#pragma unroll 4
     for (uint32_t j = 0; j < k; j++) {
 #pragma unroll
         for (int v = 0; v < V; v++) {
