@@ -415,7 +415,7 @@ __global__ __launch_bounds__(64 * W * CW, L > 8 ? (CHAIN && sizeof(typename T::R
 // A lane keeps six values a step while the chunk's maps are exchanged (and x and dy as they were read): more registers
 // would cost the waves that hide the loads.
 template <class T, int V, int L, int W, int CW, bool CHAIN>
-__global__ __launch_bounds__(64 * W * CW, L == 1 ? 1 : W == 8 && !CHAIN ? 2 : 3) void glr_bwd(GlrArgs g) {
+__global__ __launch_bounds__(64 * W * CW, L == 1 ? 1 : L == 4 ? 4 : 3) void glr_bwd(GlrArgs g) {
     using R = typename T::Raw;
     using C = Cell<T, V>;
     constexpr int CL = W * L;
@@ -675,12 +675,17 @@ Plan plan_of(const fhc_glr_desc* g, bool backward, uint32_t v, bool near) {
     const uint64_t flat = (uint64_t)g->b * g->d;
     p.l = g->t == 1 ? 1 : kL;
     p.w = flat >= (1u << 19) || g->t <= kL ? 1 : g->t <= 2 * kL ? 2 : g->t <= 4 * kL ? 4 : 8;
-    if (!backward && g->t >= 16 * kL && p.w == 8) p.l = 2 * kL;
+    p.chain = g->t > 8 * kL && p.w == 8 && flat < (1u << 16);
+    // backward, whose steps take twice the registers: half as many a lane where chunks follow one another in a workgroup
+    // (two workgroups a CU instead of one: 1000 x 64 x 512 bf16 222 -> 191 us a training step), and one channel a lane
+    // where they are chained, whose number should not grow
+    const bool half = p.w == 8 && !p.chain;
+    p.spacing = p.w == 1 ? 3 : p.w == 2 ? 4 : p.w == 4 || half ? 5 : 6;
+    if (backward) p.l = half ? kL / 2 : p.l;
+    else if (g->t >= 16 * kL && p.w == 8) p.l = 2 * kL;
     p.nchunk = (uint32_t)(g->t ? ceil_div(g->t, p.l * p.w) : 1);
-    p.spacing = p.w == 1 ? 3 : p.w == 2 ? 4 : p.w == 4 ? 5 : 6;
     p.nstates = (uint32_t)ceil_div(g->t, 1u << p.spacing);
     p.colblocks = (uint32_t)ceil_div(cols, p.w >= 4 ? 64 : p.w == 2 ? 128 : 256);
-    p.chain = p.nchunk > 1 && p.w == 8 && flat < (1u << 16);
     p.words = p.chain ? (p.nchunk + ceil_div(p.nchunk, kRun)) * flat : 0;
     p.agg_bytes = p.chain ? p.words * 8 + (size_t)g->b * ceil_div(g->d, 64) * kTicketStep * 4 : 0;
     p.part_bytes = (size_t)ceil_div((p.chain ? p.nchunk : 1) * flat * 4, 256) * 256;
@@ -724,6 +729,7 @@ Plan plan_for(const fhc_glr_desc* g, bool backward, std::initializer_list<const 
         if ((g->b > 1 && s->bs % 2) || (g->t > 1 && s->ts % 2) || !aligned(s->p, 2 * (uint32_t)e)) pairs = false;
         if (g->b > 1 && (s->bs < 0 || s->bs >= (1 << 30) / 64 / e)) near = false;
     }
+    if (backward && plan_of(g, true, 1, near).chain) pairs = false;
     return plan_of(g, backward, pairs ? 2 : 1, near);
 }
 
@@ -750,9 +756,25 @@ void launch(const Plan& p, const GlrArgs& a, hipStream_t s) {
             return;
         }
     }
-    if (p.chain) GLR(kL, 8, 1, true, p.colblocks * p.nchunk);
-    else if (p.w == 8) GLR(kL, 8, 1, false, p.colblocks);
-    else if (p.w == 4) GLR(kL, 4, 1, false, p.colblocks);
+    if constexpr (BWD) {
+        if (p.l == kL / 2) {
+            GLR(kL / 2, 8, 1, false, p.colblocks);
+            return;
+        }
+    }
+    if constexpr (!BWD || V == 1) {
+        if (p.chain) {
+            GLR(kL, 8, 1, true, p.colblocks * p.nchunk);
+            return;
+        }
+    }
+    if constexpr (!BWD) {
+        if (p.w == 8) {
+            GLR(kL, 8, 1, false, p.colblocks);
+            return;
+        }
+    }
+    if (p.w == 4) GLR(kL, 4, 1, false, p.colblocks);
     else if (p.w == 2) GLR(kL, 2, 2, false, p.colblocks);
     else if (p.l == 1) GLR(1, 1, 4, false, p.colblocks);
     else GLR(kL, 1, 4, false, p.colblocks);
