@@ -177,9 +177,15 @@ __global__ __launch_bounds__(64 * NW) void ffn_skinny(SkinnyArgs g) {
 
 constexpr uint32_t kSkinnyRows = 32;  // up to here the weights' bytes are all that counts
 
-// One kernel a direction (ffn_fused.h) where the channels fit its registers and the rows give it work for the chip; a
-// workgroup of it walks all features, so few rows go through the products of ffn_gemm.h, which spread over features too.
-bool fused(const fhc_ffn_desc* d) { return d->c <= 256 && d->c > 0 && d->f > 0 && d->rows >= 8192; }
+// One kernel a direction (ffn_fused.h) where the channels fit its registers and the rows give it work for the chip: a
+// workgroup has 128 rows and walks all features, so the time hardly changes until the rows fill the CUs, where the
+// products of ffn_gemm.h spread few rows over features too. Measured, one kernel against products, f16, at 4096 and
+// 20000 rows: forward of c 128, f 512, 23 and 23 us against 17 and 41, its training step 93 and 103 against 64 and 159; of
+// c 128, f 8192, a training step 924 at 4096 rows against 400 and 91 ns more a row: about where those lines cross. One
+// rule for both passes and with or without states kept, so that serving gives a training forward's bits.
+bool fused(const fhc_ffn_desc* d) {
+    return d->c > 0 && d->f > 0 && d->c <= 256 && d->rows >= (d->c <= 64 ? 6000u : d->c <= 128 ? 11500u : 19500u);
+}
 
 int check_desc(const char* op, const fhc_ffn_desc* d) {
     if (!d) return fail(-1, "%s: null descriptor", op);

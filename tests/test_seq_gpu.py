@@ -605,3 +605,61 @@ def test_ffn_many_rows_in_a_graph():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), k
         call()
+
+
+# on either side of where the one-kernel form is taken, with and without states kept
+@pytest.mark.parametrize("shape", [(5999, 64, 96), (6000, 64, 96), (11499, 128, 70), (11500, 128, 72), (12003, 100, 520),
+                                   (19501, 200, 136), (23003, 72, 40), (22001, 256, 65)], ids=str)
+def test_ffn_where_the_form_changes(shape):
+    say("ffn forms", shape)
+    for k, dtype in enumerate(("f16", "bf16")):
+        ffn_check(ffn_inputs(Rand(sum(shape)), *shape, types()[dtype]), "gelu" if k else "silu")
+
+
+def test_ffn_in_one_kernel_some_gradients_only_views_and_graph():
+    """As for fewer rows: dx or the weights' gradients alone, row views with NaN beside them, replays of a graph."""
+    say("ffn one kernel parts")
+    import ctypes
+    import torch
+    m, (rows, c, f) = mod(), (11523, 72, 136)
+    v = ffn_inputs(Rand(31), rows, c, f, torch.bfloat16)
+    w = [v[k] for k in ("wg", "wu", "wd")]
+
+    def call():
+        y, saved = m.ffn(v["x"], *w, train=True)
+        return (y,) + m.ffn_backward(v["x"], *w, saved, v["dy"])
+
+    y, saved = m.ffn(v["x"], *w, train=True)
+    want = [k.clone() for k in call()]
+    wide = {k: torch.full((rows, c + 20), math.nan, dtype=torch.bfloat16, device="cuda") for k in ("x", "dy")}
+    for off in (1, 2, 8):
+        views = {k: b[:, off:off + c] for k, b in wide.items()}
+        for k, b in views.items():
+            b.copy_(v[k])
+        y2, saved2 = m.ffn(views["x"], *w, train=True)
+        got = (y2,) + m.ffn_backward(views["x"], *w, saved2, views["dy"])
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        for b in wide.values():
+            b.fill_(math.nan)
+    L, d = m._lib(), m.FfnDesc(1, 0, rows, c, f)
+    n = L.fhc_ffn_workspace_bytes(ctypes.byref(d), 1)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    for only in range(4):
+        out = [torch.full_like(g, 7) for g in want[1:]]
+        at = [o.data_ptr() if k == only else None for k, o in enumerate(out)]
+        assert L.fhc_ffn_backward(ctypes.byref(d), m._rows("", "", v["x"]), w[0].data_ptr(), w[1].data_ptr(),
+                                  w[2].data_ptr(), saved.data_ptr(), m._rows("", "", v["dy"]),
+                                  m._rows("", "", out[0]) if only == 0 else None, at[1], at[2], at[3], ws.data_ptr(), n,
+                                  torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(out[only], want[1 + only]), only
+        assert all((o == 7).all() for k, o in enumerate(out) if k != only)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for k in range(4):
+        for o in out:
+            o.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+        call()
