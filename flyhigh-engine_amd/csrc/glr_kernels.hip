@@ -10,14 +10,22 @@
 // well as wide rows of one. Chunks follow one another in one of two ways:
 //   stream   a workgroup walks all chunks of its columns, the state in registers (many columns, or few steps);
 //   chain    a workgroup takes one chunk and publishes its map (few columns, many steps: the time axis is what fills
-//            the chip). Chunks form runs of kRun; the state that reaches a chunk is the one at the head of its run
-//            folded through the maps of the run's chunks before it, and the run's last chunk publishes the next head:
-//            a step of the serial chain is a run long, not a chunk.
+//            the chip). 8 chunks form a group, 8 groups a run; the state that reaches a chunk is the one at the head of
+//            its run folded through the maps of groups and chunks before it (chain_find), and the run's last chunk
+//            publishes the next head: a step of the serial chain is a run long, not a chunk.
 // In the chain, the chunks of a column block are taken in order by its ticket, so every chunk waited for is held by a
-// workgroup that already runs and itself waits for earlier tickets only: every wait ends. What is published is one 8-byte word (A, S), or
-// (0, state), written once and read by atomic accesses of the whole word, so no fence orders anything; its A is -1
-// until then (decays are >= 0). Only the first chunk reads the initial state (it publishes it as the first head), so
-// the last one may write the final state over it.
+// workgroup that already runs and itself waits for earlier tickets only: every wait ends. What is published is one
+// 8-byte word (A, S), or (0, state), written once and read by atomic accesses of the whole word, so no fence orders
+// anything; its A is -1 until then (decays are >= 0). Only the first chunk reads the initial state (it publishes it as
+// the first head), so the last one may write the final state over it.
+//
+// What bounds it (MI355X): forward moves 4 elements an element and takes 38 vector instructions, 6 of them
+// transcendental, at a quarter of the rate: 65536 x 2048 bf16 need 213 us of HBM and about 200 us of the vector units,
+// and take 282. Hence the short polynomial and sigmoids without clamps (138 issue slots an element before), scalar row
+// addresses, and 16 steps a lane (half the exchanges of 8). Backward holds six values a step, so registers (occupancy)
+// bound it: 1000 x 64 x 512 bf16 about 135 us for 92 us of HBM. Many short sequences are near HBM's rate: 1000 x 64 x 512
+// forward 52 us (5.0 TB/s); 1620 x 24 x 128 f16 12.2 us. One long narrow sequence is bound by the chain's tickets and
+// words: 65536 x 32 30 us.
 #include "seq_common.h"
 
 namespace fhc {
@@ -69,7 +77,8 @@ struct GlrArgs {
     float* dh0;
     float* part;      // dlam's partial sums, [part rows][d]
     uint64_t* agg;    // chain: published maps [chunk][b * d],
-    uint64_t* heads;  // and the first states of the runs [run][b * d]
+    uint64_t* group_maps;  // those of whole groups [group][b * d],
+    uint64_t* heads;       // and the first states of the runs [run][b * d]
     uint32_t* tickets;
     uint32_t b, t, d, groups;  // groups: lanes that a sequence's channels take
     uint32_t nchunk, colblocks, nstates;
@@ -208,7 +217,7 @@ constexpr uint64_t kUnpublished = 0xBF800000ull;  // (-1, 0)
 __device__ __forceinline__ void publish(uint64_t* p, float a, float s) {
     __hip_atomic_store(p, word_of(a, s), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-constexpr uint32_t kRun = 32;  // chunks of a run
+constexpr uint32_t kGroup = 8, kRun = kGroup * kGroup;  // chunks of a group; of a run
 
 constexpr uint32_t kTicketStep = 32;  // a column block's ticket has 128 bytes of its own
 
@@ -218,52 +227,94 @@ __global__ __launch_bounds__(256) void glr_clear(uint64_t* agg, uint64_t n, uint
     if (k < colblocks) tickets[k * kTicketStep] = 0;
 }
 
-// The chain's search: the state that reaches this lane's columns of a chunk, `k` chunks after the head of its run.
-// word(j) is the published map of the run's j-th chunk, head the run's first state. The W waves fetch the words
-// together, a wave all of its own at once, and again until they are all there; the fold is in the chunks' order whatever
-// the order of their arrival, so results repeat bit for bit.
-template <int V, int W, class Word>
-__device__ __forceinline__ void chain_find(uint32_t k, uint32_t tw, uint32_t slot, bool live, float2 (*lds)[64 * V],
-                                           const uint64_t* head, Word word, float (&h)[V]) {
-    constexpr uint32_t N = kRun / W;  // entries of a wave: chunks tw, tw + W, ..; the last wave's last is the head
-    if (live) {
-        uint64_t w[N][V];
-        bool missing;
-        do {
+// The chain's search: the state that reaches this lane's columns of a chunk, the k-th of its run (k = 8 group + j): the
+// run's first state through the maps of the groups before the chunk's and of the j chunks before it in its group. A
+// chunk so reads 15 words a column at most, not one of every chunk before it (they go to memory, past the L2s of
+// other XCDs, and took longer than the data: 65536 x 2048 bf16 280 us). The W waves fetch the words together, a wave all
+// of its own at once, and again until they are all there; the folds are in the chunks' order whatever the order of their
+// arrival, so results repeat bit for bit.
+//   agg, groups, heads: the run's first words of this column block's lane, `flats` words from one to the next
+//   a, s: the chunk's own map. The last chunk of a group publishes the group's before it looks for anything else.
+template <int V, int W>
+__device__ __forceinline__ void chain_find(uint32_t k, bool first_run, bool more, uint32_t tw, uint32_t slot, bool live,
+                                           float2 (*lds)[64 * V], const uint64_t* agg, uint64_t* groups,
+                                           const uint64_t* head, uint64_t flats, const float (&a)[V], const float (&s)[V],
+                                           float (&h)[V]) {
+    constexpr uint32_t N = 16 / W;  // entries of a wave: 0-6 chunks, 7-13 groups, 15 the head
+    const uint32_t group = k / kGroup, j = k % kGroup;
+    const bool has_head = !first_run || k > 0;
+    auto fetch = [&](uint32_t from, uint32_t to) {
+        if (live) {
+            uint64_t w[N][V];
+            bool missing;
+            do {
+#pragma unroll
+                for (uint32_t n = 0; n < N; n++) {
+                    const uint32_t e = n * W + tw;
+                    const uint64_t* p = nullptr;
+                    if (e >= from && e < to) {
+                        if (e < 7) p = e < j ? agg + (group * kGroup + e) * flats : nullptr;
+                        else if (e < 14) p = e - 7 < group ? groups + (e - 7) * flats : nullptr;
+                        else p = e == 15 && has_head ? head : nullptr;
+                    }
+#pragma unroll
+                    for (int v = 0; v < V; v++) {
+                        w[n][v] = 0;
+                        if (p) w[n][v] = __hip_atomic_load(p + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    }
+                }
+                missing = false;
+#pragma unroll
+                for (uint32_t n = 0; n < N; n++)
+#pragma unroll
+                    for (int v = 0; v < V; v++) missing |= (uint32_t)w[n][v] == (uint32_t)kUnpublished;
+            } while (missing);
 #pragma unroll
             for (uint32_t n = 0; n < N; n++) {
-                const uint32_t j = n * W + tw;
-                const uint64_t* p = j == kRun - 1 ? head : j < k ? word(j) : nullptr;
+                const uint32_t e = n * W + tw;
+                if (e < from || e >= to) continue;
 #pragma unroll
-                for (int v = 0; v < V; v++) {
-                    w[n][v] = 0;
-                    if (p) w[n][v] = __hip_atomic_load(p + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                }
+                for (int v = 0; v < V; v++)
+                    lds[e][slot * V + v] = float2{__builtin_bit_cast(float, (uint32_t)w[n][v]),
+                                                 __builtin_bit_cast(float, (uint32_t)(w[n][v] >> 32))};
             }
-            missing = false;
+        }
+        __syncthreads();
+    };
+    const bool closes = j == kGroup - 1 && group < kGroup - 1 && more;  // the same for the whole workgroup
+    if (closes) {
+        fetch(0, 7);
+        if (live && tw == 0) {
 #pragma unroll
-            for (uint32_t n = 0; n < N; n++)
+            for (int v = 0; v < V; v++) {
+                float ga = 1.0f, gs = 0.0f;
 #pragma unroll
-                for (int v = 0; v < V; v++) missing |= (uint32_t)w[n][v] == (uint32_t)kUnpublished;
-        } while (missing);
-#pragma unroll
-        for (uint32_t n = 0; n < N; n++)
-#pragma unroll
-            for (int v = 0; v < V; v++)
-                lds[n * W + tw][slot * V + v] = float2{__builtin_bit_cast(float, (uint32_t)w[n][v]),
-                                                      __builtin_bit_cast(float, (uint32_t)(w[n][v] >> 32))};
+                for (uint32_t e = 0; e < 7; e++) {
+                    const float2 q = lds[e][slot * V + v];
+                    gs = __builtin_fmaf(q.x, gs, q.y);
+                    ga *= q.x;
+                }
+                publish(groups + group * flats + v, a[v] * ga, __builtin_fmaf(a[v], gs, s[v]));
+            }
+        }
     }
-    __syncthreads();
+    fetch(closes ? 7 : 0, 16);
     if (!live) return;
-    if (head) {
+    if (has_head) {
 #pragma unroll
-        for (int v = 0; v < V; v++) h[v] = lds[kRun - 1][slot * V + v].y;
+        for (int v = 0; v < V; v++) h[v] = lds[15][slot * V + v].y;
     }
-#pragma unroll 4
-    for (uint32_t j = 0; j < k; j++) {
+    for (uint32_t e = 0; e < group; e++) {
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            const float2 q = lds[j][slot * V + v];
+            const float2 q = lds[7 + e][slot * V + v];
+            h[v] = __builtin_fmaf(q.x, h[v], q.y);
+        }
+    }
+    for (uint32_t e = 0; e < j; e++) {
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const float2 q = lds[e][slot * V + v];
             h[v] = __builtin_fmaf(q.x, h[v], q.y);
         }
     }
@@ -288,7 +339,7 @@ __global__ __launch_bounds__(64 * W * CW, L > 8 ? (CHAIN && sizeof(typename T::R
     constexpr int CL = W * L;
     constexpr bool ONE = W > 1 && W < 8;  // these chunks hold whole sequences
     __shared__ float2 maps[W > 1 ? W : 1][W > 1 ? CW * 64 * V : 1];
-    __shared__ float2 far[CHAIN ? kRun : 1][CHAIN ? 64 * V : 1];
+    __shared__ float2 far[CHAIN ? 16 : 1][CHAIN ? 64 * V : 1];
     static_assert(!CHAIN || CW == 1, "a chained chunk's columns are one wave wide");
     uint32_t cb = blockIdx.x, chunk = take_chunk<CHAIN>(g, cb);
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -357,16 +408,17 @@ __global__ __launch_bounds__(64 * W * CW, L > 8 ? (CHAIN && sizeof(typename T::R
             if constexpr (CHAIN) {
                 const uint64_t flats = (uint64_t)g.b * g.d;
                 const uint32_t run = chunk / kRun, k = chunk - run * kRun;
-                if (tw == 0 && live && k + 1 < kRun && chunk + 1 < g.nchunk) {
+                const bool more = chunk + 1 < g.nchunk;
+                if (tw == 0 && live && k % kGroup < kGroup - 1 && more) {
 #pragma unroll
-                    for (int v = 0; v < V; v++) {
-                        publish(g.agg + chunk * flats + flat + v, ta[v], ts[v]);
-                        if (chunk == 0) publish(g.heads + flat + v, 0.0f, h[v]);
-                    }
+                    for (int v = 0; v < V; v++) publish(g.agg + chunk * flats + flat + v, ta[v], ts[v]);
                 }
-                chain_find<V, W>(
-                    k, tw, slot, live, far, chunk ? g.heads + run * flats + flat : nullptr,
-                    [&](uint32_t j) { return g.agg + (uint64_t)(run * kRun + j) * flats + flat; }, h);
+                if (tw == 0 && live && chunk == 0 && more) {
+#pragma unroll
+                    for (int v = 0; v < V; v++) publish(g.heads + flat + v, 0.0f, h[v]);
+                }
+                chain_find<V, W>(k, run == 0, more, tw, slot, live, far, g.agg + run * kRun * flats + flat,
+                                 g.group_maps + run * kGroup * flats + flat, g.heads + run * flats + flat, flats, ta, ts, h);
 #pragma unroll
                 for (int v = 0; v < V; v++) end[v] = __builtin_fmaf(ta[v], h[v], ts[v]);
                 if (tw == 0 && live && k + 1 == kRun && chunk + 1 < g.nchunk) {
@@ -422,7 +474,7 @@ __global__ __launch_bounds__(64 * W * CW, L == 1 ? 1 : L == 4 ? 4 : 3) void glr_
     constexpr bool ONE = W > 1 && W < 8;  // these chunks hold whole sequences
     __shared__ float2 maps[W > 1 ? W : 1][W > 1 ? CW * 64 * V : 1];  // (A, S) forward
     __shared__ float back[W > 1 ? W : 1][W > 1 ? CW * 64 * V : 1];   // the R of c -> A c + R
-    __shared__ float2 far[CHAIN ? kRun : 1][CHAIN ? 64 * V : 1];
+    __shared__ float2 far[CHAIN ? 16 : 1][CHAIN ? 64 * V : 1];
     static_assert(!CHAIN || CW == 1, "a chained chunk's columns are one wave wide");
     uint32_t cb = blockIdx.x, done = take_chunk<CHAIN>(g, cb);  // chunks go from the last to the first
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -523,16 +575,17 @@ __global__ __launch_bounds__(64 * W * CW, L == 1 ? 1 : L == 4 ? 4 : 3) void glr_
             if constexpr (CHAIN) {
                 const uint64_t flats = (uint64_t)g.b * g.d;
                 const uint32_t run = done / kRun, k = done - run * kRun;
-                if (tw == 0 && live && k + 1 < kRun && chunk > 0) {
+                const bool more = chunk > 0;
+                if (tw == 0 && live && k % kGroup < kGroup - 1 && more) {
 #pragma unroll
-                    for (int v = 0; v < V; v++) {
-                        publish(g.agg + done * flats + flat + v, ta[v], ts[v]);
-                        if (done == 0) publish(g.heads + flat + v, 0.0f, c[v]);
-                    }
+                    for (int v = 0; v < V; v++) publish(g.agg + done * flats + flat + v, ta[v], ts[v]);
                 }
-                chain_find<V, W>(
-                    k, tw, slot, live, far, done ? g.heads + run * flats + flat : nullptr,
-                    [&](uint32_t j) { return g.agg + (uint64_t)(run * kRun + j) * flats + flat; }, c);
+                if (tw == 0 && live && done == 0 && more) {
+#pragma unroll
+                    for (int v = 0; v < V; v++) publish(g.heads + flat + v, 0.0f, c[v]);
+                }
+                chain_find<V, W>(k, run == 0, more, tw, slot, live, far, g.agg + run * kRun * flats + flat,
+                                 g.group_maps + run * kGroup * flats + flat, g.heads + run * flats + flat, flats, ta, ts, c);
 #pragma unroll
                 for (int v = 0; v < V; v++) end[v] = __builtin_fmaf(ta[v], c[v], ts[v]);
                 if (tw == 0 && live && k + 1 == kRun && chunk > 0) {
@@ -686,7 +739,7 @@ Plan plan_of(const fhc_glr_desc* g, bool backward, uint32_t v, bool near) {
     p.nchunk = (uint32_t)(g->t ? ceil_div(g->t, p.l * p.w) : 1);
     p.nstates = (uint32_t)ceil_div(g->t, 1u << p.spacing);
     p.colblocks = (uint32_t)ceil_div(cols, p.w >= 4 ? 64 : p.w == 2 ? 128 : 256);
-    p.words = p.chain ? (p.nchunk + ceil_div(p.nchunk, kRun)) * flat : 0;
+    p.words = p.chain ? (p.nchunk + ceil_div(p.nchunk, kGroup) + ceil_div(p.nchunk, kRun)) * flat : 0;
     p.agg_bytes = p.chain ? p.words * 8 + (size_t)g->b * ceil_div(g->d, 64) * kTicketStep * 4 : 0;
     p.part_bytes = (size_t)ceil_div((p.chain ? p.nchunk : 1) * flat * 4, 256) * 256;
     p.sum_bytes = (size_t)kSumRows * g->d * 8;
@@ -789,7 +842,8 @@ int run(const char* op, const Plan& p, GlrArgs& a, uint32_t dtype, void* ws, hip
     char* w = static_cast<char*>(ws);
     if (p.chain) {
         a.agg = reinterpret_cast<uint64_t*>(w);
-        a.heads = a.agg + (uint64_t)p.nchunk * a.b * a.d;
+        a.group_maps = a.agg + (uint64_t)p.nchunk * a.b * a.d;
+        a.heads = a.group_maps + ceil_div(p.nchunk, kGroup) * a.b * a.d;
         a.tickets = reinterpret_cast<uint32_t*>(a.agg + p.words);
         hipLaunchKernelGGL(glr_clear, dim3((uint32_t)ceil_div(p.words, 256)), dim3(256), 0, s, a.agg, p.words,
                            a.tickets, p.colblocks);
