@@ -4,10 +4,16 @@
 // out[m][n] = sum over k of A(m, k) B(n, k). An operand is stored either with k adjacent ("rows": A's row m at
 // a + m * ld) or with m (n) adjacent ("columns": A's column k at a + k * ld), so no product needs a transposed copy.
 //
-// - A workgroup of 2 x 2 waves computes a BM x BN tile, a wave 16 MB x 16 NB of it, K in slabs of 32. Both operands'
-//   slabs go from global memory straight into LDS (LDS DMA, 16 bytes a lane), three buffers in turn: slabs s + 1 and
-//   s + 2 are on their way while slab s computes, one barrier a slab. Two workgroups share a CU (the larger tile's
-//   accumulators take half of a SIMD's registers), so one's epilogue and waits lie under the other's products.
+// - A workgroup of WM x WN waves computes a BM x BN tile, a wave 16 MB x 16 NB of it, K in slabs of 32. Both operands'
+//   slabs go from global memory straight into LDS (LDS DMA, 16 bytes a lane), the next slabs on their way while one
+//   computes. Tiles of 128 x 64 and 128 x 128 have four waves and three buffers in turn, one barrier a slab, and several
+//   workgroups a CU, whose epilogues and waits lie under each other's products. Tiles of 256 x 256 have eight waves and
+//   four buffers; a CU holds one such workgroup, so its halves take turns: while one reads fragments the other
+//   multiplies. Measured on the way, TFLOP/s: three buffers and one barrier a slab for all eight waves 990; turns 984
+//   with 64-bit lane addresses, 1230 once a row's address is scalar; 128 x 256 tiles, two workgroups a CU, 924 (their LDS
+//   traffic). At that rate the matrix units are busy 64% of the cycles and the card's power holds the clock at 1.8 GHz.
+//   8192 rows, 2048 channels, 8192 features, bf16: weights' gradients 1270-1350 over two runs, dx 1250-1320, y 1140-1150,
+//   GLU 890 and dL/dh 620-630, whose f32 states pass through the epilogue; a large library product reaches 1307.
 // - Rows: an LDS row holds 32 k (64 bytes), its 16-byte chunk c at position c ^ (row >> 2 & 2): a fragment read (16
 //   bytes a lane) goes by lanes 0-3, 12-15, 20-23, 24-27 and the like, 16 at once, which so fall on all 64 banks (other
 //   permutations of the chunks, by row >> 2 or by 8 neighbours, measured a conflict for every read). Columns: an LDS row holds the tile's m (n) of one k, its

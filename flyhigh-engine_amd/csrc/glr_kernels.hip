@@ -229,8 +229,8 @@ __global__ __launch_bounds__(256) void glr_clear(uint64_t* agg, uint64_t n, uint
 
 // The chain's search: the state that reaches this lane's columns of a chunk, the k-th of its run (k = 8 group + j): the
 // run's first state through the maps of the groups before the chunk's and of the j chunks before it in its group. A
-// chunk so reads 15 words a column at most, not one of every chunk before it (they go to memory, past the L2s of
-// other XCDs, and took longer than the data: 65536 x 2048 bf16 280 us). The W waves fetch the words together, a wave all
+// chunk so reads 15 words a column at most, and a run is 64 chunks (runs of 32 without groups: one sequence of 65536 x 32
+// bf16 took 43 us, with groups 30). The W waves fetch the words together, a wave all
 // of its own at once, and again until they are all there; the folds are in the chunks' order whatever the order of their
 // arrival, so results repeat bit for bit.
 //   agg, groups, heads: the run's first words of this column block's lane, `flats` words from one to the next

@@ -5,6 +5,10 @@
 // the backward pass computes it again from x and o in place of reading it. A row is held by threads of 8 channels each
 // (K such groups for the widest rows): a part of a wave for narrow rows, so that a wave takes several pixels, as many
 // waves as it needs (up to 16) for wide ones.
+//
+// MI355X, where a large copy moves 5.0 TB/s: forward of 16384 x 4096 bf16 95 us (537 MB, 5.7 TB/s), of
+// 15009 x 1931 f16, whose rows lie at any 2-byte address, 51 (4.6). Backward of the former 174 us (805 MB, 4.6 TB/s; the first form, which did not have the next row's loads under way, 289), its closing
+// sums 10 us more.
 #include "seq_common.h"
 
 namespace fhc {

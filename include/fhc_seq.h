@@ -100,8 +100,9 @@ int fhc_norm_block_backward(const fhc_norm_desc* n, const fhc_rows* x, const fhc
  *     y = h wd^T,   h = act(x wg^T) * (x wu^T)      act: silu, v sigmoid(v), or gelu in its tanh form
  * wg, wu are dense [f][c], wd dense [c][f], in dtype (f16 or bf16). The products accumulate in f32; h, and in the
  * backward pass dL/d(x wg^T) and dL/d(x wu^T), are rounded to dtype once, since they are the next products' operands
- * (the matrix units take 16 bits). A training forward keeps x wg^T and x wu^T in f32, so no gradient is taken at a
- * rounded value. f16: the caller scales the loss so that these stay in f16's range. */
+ * (the matrix units take 16 bits). A training forward keeps x wg^T and x wu^T in f32, or, for few channels and many
+ * rows, the backward pass computes them again: no gradient is taken at a rounded value. f16: the caller scales the loss
+ * so that these stay in f16's range. */
 #define FHC_ACT_SILU 0u
 #define FHC_ACT_GELU 1u
 
