@@ -54,7 +54,7 @@ struct GemmArgs {
     const uint16_t *a0, *a1, *b0, *b1;
     int64_t lda, ldb;
     int m, n, k;        // kGlu: n is the features, each a gate row of b0 and an up row of b1
-    int wide_m, wide_n;  // what a column operand's rows hold: m (n), or its padding too
+    int wide_m, wide_n;  // the columns that a column operand's last row is read to: m (n), to whole 4 bytes
     int segments;       // 2: a0 b0 and then a1 b1 along K (kStore, kPart)
     int pairs;          // 2: a0 -> o0 and a1 -> o1, both with b0 (kStore, kPart)
     int slabs, per_split, splits;  // slabs of 32 over all segments

@@ -312,8 +312,10 @@ int product(const char* op, GemmArgs g, float* part, hipStream_t st) {
     g.segments = g.segments ? g.segments : 1, g.pairs = g.pairs ? g.pairs : 1;
     const Shape s = shape_of(g.m, g.n, g.k, g.segments, g.pairs, E == kGlu, E == kStore);
     g.tiles_m = s.tiles_m, g.tiles_n = s.tiles_n, g.slabs = s.slabs, g.per_split = s.per_split, g.splits = s.splits;
-    // a padded operand's rows hold more than its columns
-    g.wide_m = (int)(up8(g.m) <= g.lda ? up8(g.m) : g.m), g.wide_n = (int)(up8(g.n) <= g.ldb ? up8(g.n) : g.n);
+    // The columns that the last row of a column operand is read to. The range check goes by 4 bytes, so an odd width needs
+    // one more: an operand of odd width has padded rows (Operands::direct). An even one may be a caller's view that ends
+    // with its buffer, whatever its stride: not an element more.
+    g.wide_m = g.m + (g.m & 1), g.wide_n = g.n + (g.n & 1);
     if ((int64_t)s.tiles_m * s.tiles_n >= 1ll << 31) return fail(-1, "%s: too many tiles", op);
     g.quads = g.n % 4 == 0 && g.ldo % 4 == 0 && g.ldo <= 1 << 21 && aligned(g.o0, 8) && aligned(g.o1, 8);
     if constexpr (E == kStore) {

@@ -663,3 +663,28 @@ def test_ffn_in_one_kernel_some_gradients_only_views_and_graph():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), k
         call()
+
+
+@pytest.mark.parametrize("shape", [(40, 20, 52), (300, 132, 78), (33, 1020, 34), (129, 6, 10), (70, 35, 51)])
+def test_ffn_views_that_end_with_their_buffer(shape):
+    """x and dy are the last columns of rows of up8(c) elements, so the last row's last element is their buffer's last:
+    every gradient equals the dense call's."""
+    rows, c, f = shape
+    say("ffn views to the end", shape)
+    import torch
+    m = mod()
+    v = ffn_inputs(Rand(11), rows, c, f, torch.bfloat16)
+    w = [v[k] for k in ("wg", "wu", "wd")]
+
+    def call(x, dy):
+        y, saved = m.ffn(x, *w, train=True)
+        return (y,) + m.ffn_backward(x, *w, saved, dy)
+
+    want = call(v["x"], v["dy"])
+    ld = (c + 7) // 8 * 8
+    views = []
+    for k in ("x", "dy"):
+        b = torch.full((rows, ld), math.nan, dtype=torch.bfloat16, device="cuda")
+        b[:, ld - c:].copy_(v[k])
+        views.append(b[:, ld - c:])
+    assert all(torch.equal(a, b) for a, b in zip(call(*views), want))
