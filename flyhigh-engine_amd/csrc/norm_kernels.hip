@@ -78,11 +78,15 @@ __device__ __forceinline__ Chunk<T> load8(const void* base, int64_t at, Place p,
     }
     return v;
 }
-// the values, 0 where they are another thread's
+// the values, 0 where they are another thread's (weights and gates too: 0 times an infinite one is not 0)
+template <class T, bool AL>
+__device__ __forceinline__ float own(const Chunk<T>& v, Place p, int i) {
+    return AL || i >= (int)p.skip ? v.at(i) : 0.0f;
+}
 template <class T, bool AL>
 __device__ __forceinline__ void widen8(const Chunk<T>& v, Place p, float (&f)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) f[i] = AL || i >= (int)p.skip ? v.at(i) : 0.0f;
+    for (int i = 0; i < 8; i++) f[i] = own<T, AL>(v, p, i);
 }
 template <class T, bool AL>
 __device__ __forceinline__ void store8(void* base, int64_t at, Place p, uint32_t c, const float (&f)[8]) {
@@ -199,7 +203,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_fwd(NormArgs g) {
 #pragma unroll
         for (int k = 0; k < K; k++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) o[k][i] *= ro * wp[k].at(i) * ga[k].at(i);
+            for (int i = 0; i < 8; i++) o[k][i] *= ro * own<T, AL>(wp[k], at[k], i) * own<T, AL>(ga[k], at[k], i);
     }
     s[0] = 0.0f;
 #pragma unroll
@@ -218,7 +222,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_fwd(NormArgs g) {
 #pragma unroll
     for (int k = 0; k < K; k++) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[k][i] *= ry * wn[k].at(i);
+        for (int i = 0; i < 8; i++) x[k][i] *= ry * own<T, AL>(wn[k], at[k], i);
         store8<T, AL>(g.u.p, row * g.u.ld, at[k], g.c, x[k]);
     }
 }
@@ -298,7 +302,7 @@ __global__ __launch_bounds__(kBlock<TPR>, (kWaves<TPR, sizeof(typename T::Raw), 
         if constexpr (PARTS) {
             const Chunk<T> ga = weight8<T, AL>(g.gate, (int64_t)gr * g.c, at[k], g.c);
 #pragma unroll
-            for (int i = 0; i < 8; i++) gw[k][i] = pw.at(i) * ga.at(i);
+            for (int i = 0; i < 8; i++) gw[k][i] = own<T, AL>(pw, at[k], i) * own<T, AL>(ga, at[k], i);
         } else {
             wp[k] = pw;
         }
@@ -322,7 +326,7 @@ __global__ __launch_bounds__(kBlock<TPR>, (kWaves<TPR, sizeof(typename T::Raw), 
             if constexpr (!PARTS) {
                 ga[k] = gar[k];
 #pragma unroll
-                for (int i = 0; i < 8; i++) gw[k][i] = ga[k].at(i) * wp[k].at(i);
+                for (int i = 0; i < 8; i++) gw[k][i] = own<T, AL>(ga[k], at[k], i) * own<T, AL>(wp[k], at[k], i);
             }
         }
         r += rstep;

@@ -688,3 +688,21 @@ def test_ffn_views_that_end_with_their_buffer(shape):
         b[:, ld - c:].copy_(v[k])
         views.append(b[:, ld - c:])
     assert all(torch.equal(a, b) for a, b in zip(call(*views), want))
+
+
+@pytest.mark.parametrize("c", [13, 131, 261, 523, 1931])
+def test_norm_block_infinite_gate_stays_in_its_channel(c):
+    """An infinite gate on one of the last 8 channels, which at odd widths are read twice: y is infinite there alone, u
+    there not a number and 0 elsewhere (a finite y over an infinite mean)."""
+    say("norm infinite gate", c)
+    import torch
+    m, q = mod(), Rand(c)
+    x, o = q.normal(5, c, dtype=torch.float16), q.normal(5, c, dtype=torch.float16)
+    one = torch.ones(c, dtype=torch.float16, device="cuda")
+    for at in range(c - 8, c):
+        gate = torch.ones(1, c, dtype=torch.float16, device="cuda")
+        gate[0, at] = math.inf
+        y, u = m.norm_block(x, o.abs() + 1, one, gate, one, rows_per_group=5)
+        others = torch.arange(c, device="cuda") != at
+        assert torch.isinf(y[:, at]).all() and torch.isfinite(y[:, others]).all(), at
+        assert torch.isnan(u[:, at]).all() and (u[:, others] == 0).all(), at
