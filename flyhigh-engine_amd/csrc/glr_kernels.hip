@@ -837,6 +837,8 @@ void launch(const Plan& p, const GlrArgs& a, hipStream_t s) {
 template <bool BWD>
 int run(const char* op, const Plan& p, GlrArgs& a, uint32_t dtype, void* ws, hipStream_t s) {
     if ((uint64_t)p.colblocks * p.nchunk >= 1ull << 31 || (uint64_t)a.b * p.groups >= 1ull << 31) return fail(-1, "%s: too many chunks", op);
+    FHC_TRY(check_grid(op, (uint64_t)p.colblocks * (p.chain ? p.nchunk : 1), p.w == 8 ? 512 : 256));
+    FHC_TRY(check_grid(op, ceil_div(p.words, 256), 256));
     a.groups = p.groups, a.nchunk = p.nchunk, a.colblocks = p.colblocks, a.nstates = p.nstates;
     a.spacing = p.spacing;
     char* w = static_cast<char*>(ws);

@@ -25,6 +25,7 @@ struct NormArgs {
     const void *w_post, *w_pre, *gate;
     float *dgate, *part_post, *part_pre;  // see norm_bwd
     uint32_t rows, c, rpg, groups;
+    uint32_t first;  // the launch's first row (forward)
     uint32_t per_group, part_rows;  // parts of a group, rows of a part; per_group 0: a workgroup takes whole groups
     uint32_t wg_groups;             // groups of a workgroup, where per_group is 0
     float alpha, eps;
@@ -171,7 +172,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_fwd(NormArgs g) {
     __shared__ float lds[2][1][16];
     const uint32_t tpr = TPR == kWide ? blockDim.x : TPR, waves = blockDim.x / 64;
     const uint32_t lane = TPR == kWide ? threadIdx.x : threadIdx.x % TPR;
-    const uint32_t row = TPR == kWide ? blockIdx.x : blockIdx.x * (kBlock<TPR> / TPR) + threadIdx.x / TPR;
+    const uint32_t row = g.first + (TPR == kWide ? blockIdx.x : blockIdx.x * (kBlock<TPR> / TPR) + threadIdx.x / TPR);
     const bool live = row < g.rows;  // a row past the end keeps pace
     const int64_t group = g.gate && live ? row / g.rpg : 0;
     const float inv_c = 1.0f / (float)g.c;
@@ -600,8 +601,13 @@ extern "C" int fhc_norm_block(const fhc_norm_desc* n, const fhc_rows* x, const f
         with_shape(n->dtype, tpr, n->c, whole(n, {x, o, y, u}), [&](auto t, auto w, auto k, auto al) {
             constexpr int TPR = decltype(w)::value;
             const uint32_t block = TPR == kWide ? tpr : kBlock<TPR>;
-            hipLaunchKernelGGL((norm_fwd<decltype(t), TPR, decltype(k)::value, decltype(al)::value>),
-                               dim3((uint32_t)ceil_div(n->rows, block / tpr)), dim3(block), 0, (hipStream_t)stream, a);
+            const uint32_t most = (1u << 31) / block * (block / tpr);  // rows of a launch
+            for (uint64_t first = 0; first < n->rows; first += most) {
+                a.first = (uint32_t)first;
+                const uint32_t count = n->rows - a.first < most ? n->rows - a.first : most;
+                hipLaunchKernelGGL((norm_fwd<decltype(t), TPR, decltype(k)::value, decltype(al)::value>),
+                                   dim3((uint32_t)ceil_div(count, block / tpr)), dim3(block), 0, (hipStream_t)stream, a);
+            }
         });
         return launched(op);
     });
@@ -628,6 +634,7 @@ extern "C" int fhc_norm_block_backward(const fhc_norm_desc* n, const fhc_rows* x
             return fail(-1, "%s: a weight, gate or gradient of the block without o", op);
         if (dgate && !n->gate) return fail(-1, "%s: dgate without a gate", op);
         const Split s = split_of(n);
+        FHC_TRY(check_grid(op, s.wgs, s.block));
         NormArgs a{};
         if (n->rows) {
             FHC_TRY(check_rows(op, "x", x, n, true));

@@ -82,6 +82,12 @@ inline int launched(const char* op) {
     return 0;
 }
 
+// a launch has fewer than 2^32 threads
+inline int check_grid(const char* op, uint64_t blocks, uint32_t threads) {
+    if (blocks >= (1ull << 32) / threads) return fail(-1, "%s: too many workgroups (%llu)", op, (unsigned long long)blocks);
+    return 0;
+}
+
 inline int check_workspace(const char* op, size_t need, const void* ws, size_t have) {
     if (!need) return 0;
     if (!ws) return fail(-1, "%s: null workspace (%zu bytes needed)", op, need);

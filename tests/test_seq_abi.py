@@ -167,3 +167,15 @@ def test_tensors_are_checked_before_the_call():
         m.glr(x.double(), x, x, torch.zeros(4))
     with pytest.raises(m.FhcError, match="rows, channels"):
         m.norm_block(x, x, None, None, None)
+
+
+def test_launches_of_too_many_threads_are_refused():
+    """One column of 2^31 steps and 2^25 groups of 64 rows each ask for more threads than a launch has."""
+    refused(glr_forward(b=1, d=1, t=0x7FFFFF00), "too many workgroups")
+    refused(glr_backward(b=1, d=1, t=0x7FFFFF00), "too many workgroups")
+    m = mod()
+    L = m._lib()
+    n = m.NormDesc(1, 0x7FFFFFFF, 1, 64, 1.0, 1e-6, None, None, P)
+    rows = ctypes.byref(m.FhcRows(P, 1))
+    refused(L.fhc_norm_block_backward(ctypes.byref(n), rows, rows, rows, rows, rows, rows, P, P, P, P, 1 << 40, None),
+            "too many workgroups")

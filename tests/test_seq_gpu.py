@@ -706,3 +706,19 @@ def test_norm_block_infinite_gate_stays_in_its_channel(c):
         others = torch.arange(c, device="cuda") != at
         assert torch.isinf(y[:, at]).all() and torch.isfinite(y[:, others]).all(), at
         assert torch.isnan(u[:, at]).all() and (u[:, others] == 0).all(), at
+
+
+def test_norm_block_more_rows_than_a_launch_has():
+    """2^28 rows of one channel are three launches: each row still finds its group's gate. o / rms(o) is 1 for o = 1."""
+    say("norm many rows")
+    import torch
+    m, rows, rpg = mod(), (1 << 28) + 37, (1 << 26) + 5
+    o = torch.ones(rows, 1, dtype=torch.float16, device="cuda")
+    x = torch.zeros_like(o)
+    gate = torch.tensor([[2.0], [-3.0], [4.0], [-5.0], [6.0]], dtype=torch.float16, device="cuda")
+    y, u = m.norm_block(x, o, None, gate, None, rows_per_group=rpg)
+    for k in range(5):
+        part = slice(k * rpg, min((k + 1) * rpg, rows))
+        # f32 statistics: off by a few 1e-7, and 1e-6 / 2 for eps, then rounded to f16 (the values are whole: no change)
+        assert (y[part] == gate[k]).all(), k
+        assert (u[part] == gate[k].sign()).all(), k
