@@ -26,6 +26,7 @@
 // bound it: 1000 x 64 x 512 bf16 about 135 us for 92 us of HBM. Many short sequences are near HBM's rate: 1000 x 64 x 512
 // forward 52 us (5.0 TB/s); 1620 x 24 x 128 f16 12.2 us. One long narrow sequence is bound by the chain's tickets and
 // words: 65536 x 32 30 us.
+#include "glr_place.h"
 #include "seq_common.h"
 
 namespace fhc {
@@ -42,10 +43,11 @@ struct Wave {
     char* p;
     int64_t ts;
     uint32_t lane;
-    __device__ __forceinline__ Wave(const Col& c, uint32_t b, uint32_t ch, uint32_t elem) : ts(c.ts) {
-        const uint32_t b0 = __builtin_amdgcn_readfirstlane(b), c0 = __builtin_amdgcn_readfirstlane(ch);
+    __device__ __forceinline__ Wave(const Col& c, uint32_t b, uint32_t ch, uint32_t elem, bool straddles) : ts(c.ts) {
+        const uint32_t b0 = __builtin_amdgcn_readfirstlane(b);
+        const uint32_t c0 = base_channel(straddles, __builtin_amdgcn_readfirstlane(ch));
         p = c.p + b0 * c.bs + (uint64_t)c0 * elem;
-        lane = (b - b0) * (uint32_t)c.bs + (ch - c0) * elem;
+        lane = lane_offset(b, ch, b0, c0, c.bs, elem);
     }
     // the step's address is made scalar in so many words: the lane's offset is else folded into a vector product
     __device__ __forceinline__ __attribute__((address_space(1))) char* row(uint32_t t) const {
@@ -83,6 +85,7 @@ struct GlrArgs {
     uint32_t b, t, d, groups;  // groups: lanes that a sequence's channels take
     uint32_t nchunk, colblocks, nstates;
     uint32_t spacing;  // log2 of the steps from one kept state to the next: the backward pass's chunk
+    bool straddles;    // a wave's columns may run over sequences
     float rate;
 };
 
@@ -357,7 +360,8 @@ __global__ __launch_bounds__(64 * W * CW, L > 8 ? (CHAIN && sizeof(typename T::R
         k[v] = live ? decay_rate(g.rate, g.lam[ch + v]) : 0.0f;
         h[v] = live && g.h0 && (!CHAIN || chunk == 0) ? g.h0[flat + v] : 0.0f;
     }
-    const Wave wx(g.x, b, ch, sizeof(R)), wr(g.r, b, ch, sizeof(R)), wi(g.i, b, ch, sizeof(R)), wy(g.y, b, ch, sizeof(R));
+    auto wave_of = [&](const Col& c) { return Wave(c, b, ch, sizeof(R), g.straddles); };
+    const Wave wx = wave_of(g.x), wr = wave_of(g.r), wi = wave_of(g.i), wy = wave_of(g.y);
 
     const uint32_t last = CHAIN ? chunk + 1 : ONE ? 1 : g.nchunk;
     for (; chunk < last; chunk++) {
@@ -493,8 +497,9 @@ __global__ __launch_bounds__(64 * W * CW, L == 1 ? 1 : L == 4 ? 4 : 3) void glr_
         c[v] = live && g.dht && (!CHAIN || done == 0) ? g.dht[flat + v] : 0.0f;
         lam_sum[v] = 0.0f;
     }
-    const Wave wx(g.x, b, ch, sizeof(R)), wr(g.r, b, ch, sizeof(R)), wi(g.i, b, ch, sizeof(R)),
-        wdy(g.dy, b, ch, sizeof(R)), wdx(g.dx, b, ch, sizeof(R)), wdr(g.dr, b, ch, sizeof(R)), wdi(g.di, b, ch, sizeof(R));
+    auto wave_of = [&](const Col& c) { return Wave(c, b, ch, sizeof(R), g.straddles); };
+    const Wave wx = wave_of(g.x), wr = wave_of(g.r), wi = wave_of(g.i), wdy = wave_of(g.dy), wdx = wave_of(g.dx),
+               wdr = wave_of(g.dr), wdi = wave_of(g.di);
 
     const uint32_t last = CHAIN ? done + 1 : ONE ? 1 : g.nchunk;
     for (; done < last; done++) {
@@ -710,7 +715,7 @@ constexpr uint32_t kSumRows = 64;  // row blocks of the first sum
 
 struct Plan {
     int l, w;    // steps of a stretch; stretches (waves) of a chunk
-    bool chain;
+    bool chain, straddles;
     uint32_t v, groups, nchunk, colblocks, nstates, spacing;
     uint64_t words;  // of the chain: maps, then heads
     size_t agg_bytes, part_bytes, sum_bytes;
@@ -722,7 +727,7 @@ struct Plan {
 // between them fit a lane's 32 bits; else each sequence starts a wave of its own.
 Plan plan_of(const fhc_glr_desc* g, bool backward, uint32_t v, bool near) {
     Plan p{};
-    p.v = v;
+    p.v = v, p.straddles = near && g->b > 1;
     p.groups = near ? g->d / v : (uint32_t)ceil_div(g->d / v, 64) * 64;
     const uint64_t cols = (uint64_t)g->b * p.groups;
     const uint64_t flat = (uint64_t)g->b * g->d;
@@ -780,7 +785,7 @@ Plan plan_for(const fhc_glr_desc* g, bool backward, std::initializer_list<const 
     const int64_t e = elem_bytes(g->dtype);
     for (const fhc_seq* s : all) {
         if ((g->b > 1 && s->bs % 2) || (g->t > 1 && s->ts % 2) || !aligned(s->p, 2 * (uint32_t)e)) pairs = false;
-        if (g->b > 1 && (s->bs < 0 || s->bs >= (1 << 30) / 64 / e)) near = false;
+        if (!near_sequences(g->b, g->d, s->bs, (uint32_t)e)) near = false;
     }
     if (backward && plan_of(g, true, 1, near).chain) pairs = false;
     return plan_of(g, backward, pairs ? 2 : 1, near);
@@ -840,7 +845,7 @@ int run(const char* op, const Plan& p, GlrArgs& a, uint32_t dtype, void* ws, hip
     FHC_TRY(check_grid(op, (uint64_t)p.colblocks * (p.chain ? p.nchunk : 1), p.w == 8 ? 512 : 256));
     FHC_TRY(check_grid(op, ceil_div(p.words, 256), 256));
     a.groups = p.groups, a.nchunk = p.nchunk, a.colblocks = p.colblocks, a.nstates = p.nstates;
-    a.spacing = p.spacing;
+    a.spacing = p.spacing, a.straddles = p.straddles;
     char* w = static_cast<char*>(ws);
     if (p.chain) {
         a.agg = reinterpret_cast<uint64_t*>(w);

@@ -722,3 +722,32 @@ def test_norm_block_more_rows_than_a_launch_has():
         # f32 statistics: off by a few 1e-7, and 1e-6 / 2 for eps, then rounded to f16 (the values are whole: no change)
         assert (y[part] == gate[k]).all(), k
         assert (u[part] == gate[k].sign()).all(), k
+
+
+@pytest.mark.parametrize("shape", [(4, 1, 48), (3, 9, 1532), (5, 40, 100), (3, 300, 48), (70, 130, 100), (7, 20, 33)],
+                         ids=str)
+def test_glr_sequences_that_share_their_elements(shape):
+    """Inputs that are one and the same for every sequence, or overlap from one to the next, give what their copies
+    give: forward, one step and backward, in each argument by itself and in all of them."""
+    say("glr shared", shape)
+    import torch
+    b, t, d = shape
+    q, m = Rand(sum(shape)), mod()
+    for dtype in (torch.bfloat16, torch.float32):
+        lam, h0, dht = q.normal(d) - 4, q.normal(b, d), q.normal(b, d)
+        dense = [q.normal(b, t, d, dtype=dtype) for _ in range(4)]
+        half = d // 2
+        width = (b - 1) * half + d
+        for form in ("one", "overlapping"):
+            if form == "one":
+                shared = [q.normal(1, t, d, dtype=dtype).expand(b, t, d) for _ in range(4)]
+            else:
+                shared = [torch.as_strided(q.normal(t, width, dtype=dtype), (b, t, d), (half, width, 1)) for _ in range(4)]
+            for which in ((0,), (1,), (2,), (3,), (0, 1, 2, 3)):
+                say(dtype, form, which)
+                v = [shared[k] if k in which else dense[k] for k in range(4)]
+                got, want = [], []
+                for out, (x, r, i, dy) in ((got, v), (want, [k.contiguous() for k in v])):
+                    y, ht, states = m.glr(x, r, i, lam, h0=h0, train=True)
+                    out += [y, ht, *m.glr_backward(x, r, i, lam, states, dy, dht=dht)]
+                assert all(torch.equal(a, w) for a, w in zip(got, want)), (form, which)
