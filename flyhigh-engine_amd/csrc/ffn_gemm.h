@@ -78,14 +78,18 @@ __device__ __forceinline__ float act_of(uint32_t act, float v) {
     const float k = act == FHC_ACT_SILU ? v : v * __builtin_fmaf(kGelu3 * v, v, kGelu1);
     return v * sigmoid_of(k);
 }
+// Far from 0 p is 0 or 1 and the slope is p. w, v held to where gelu's cube is finite, keeps what p multiplies finite: an
+// infinity times 0 is not 0. (A NaN comes through p.) This form costs 0 to 1.4% of a training step; those that hold the
+// product v k'(v) instead cost up to 4%, by the registers of the one-kernel form.
 __device__ __forceinline__ void act_grad(uint32_t act, float v, float& value, float& slope) {
     const bool silu = act == FHC_ACT_SILU;
+    const float w = __builtin_amdgcn_fmed3f(v, -1e12f, 1e12f);
     const float k = silu ? v : v * __builtin_fmaf(kGelu3 * v, v, kGelu1);
-    const float dk = silu ? 1.0f : __builtin_fmaf(3.0f * kGelu3 * v, v, kGelu1);
+    const float dk = silu ? 1.0f : __builtin_fmaf(3.0f * kGelu3 * w, w, kGelu1);
     const float e = __builtin_amdgcn_exp2f(k * -1.44269504088896340736f), p = __builtin_amdgcn_rcpf(1.0f + e);
     const float q = __builtin_fminf(e * p, 1.0f);  // 1 - p; inf * 0 where e overflows
     value = v * p;
-    slope = p * __builtin_fmaf(v * dk, q, 1.0f);
+    slope = p * __builtin_fmaf(w * dk, q, 1.0f);
 }
 
 // up to 8 elements at p, `valid` of them inside

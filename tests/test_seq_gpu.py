@@ -751,3 +751,23 @@ def test_glr_sequences_that_share_their_elements(shape):
                     y, ht, states = m.glr(x, r, i, lam, h0=h0, train=True)
                     out += [y, ht, *m.glr_backward(x, r, i, lam, states, dy, dht=dht)]
                 assert all(torch.equal(a, w) for a, w in zip(got, want)), (form, which)
+
+
+@pytest.mark.parametrize("rows", [20, 140, 8192])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_ffn_slope_far_from_zero(act, rows):
+    """Pre-activations whose cube leaves f32's range: act's slope is 1 on one side and 0 on the other. Every value is a
+    power of two, or a number of rows times one, so the results are the formula's exactly."""
+    say("ffn slope", act, rows)
+    import torch
+    m, n = mod(), rows // 2
+    x = torch.tensor([[1.0], [-1.0]], dtype=torch.bfloat16, device="cuda").repeat(n, 1)
+    wg = torch.tensor([[2.0 ** 44], [2.0 ** 70]], dtype=torch.bfloat16, device="cuda")
+    one = torch.ones_like(wg)
+    y, saved = m.ffn(x, wg, one, one.t().contiguous(), act, train=True)
+    dx, dwg, dwu, dwd = m.ffn_backward(x, wg, one, one.t().contiguous(), saved, torch.ones_like(x), act)
+    total = wg.double().sum()
+    for got, want in ((y, total), (dx, 2 * total)):  # dL/dgate = slope, dL/dup = act = wg; of x = -1 both are 0
+        assert (got[::2] == want.to(torch.bfloat16)).all() and not got[1::2].any()
+    assert (dwg == n).all()
+    assert torch.equal(dwu, (wg.double() * n).to(torch.bfloat16)) and torch.equal(dwd, dwu.t())
