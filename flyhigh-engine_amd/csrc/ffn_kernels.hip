@@ -227,7 +227,8 @@ Shape shape_of(int64_t m, int64_t n, int64_t k, int segments, int pairs, bool gl
     const int64_t bm[3] = {128, 128, 256}, bn[3] = {64, 128, 256}, cost[3] = {75, 100, 270};
     auto count = [&](int t) { return (int64_t)(ceil_div(m, bm[t]) * ceil_div(n, bn[t] / unit)) * pairs; };
     s.tile = kMedium;
-    const bool split = may_split && count(kMedium) <= 128 && ceil_div(k, 32) * segments >= 16;
+    const int64_t medium = count(kMedium);  // none where there are no rows or no columns
+    const bool split = may_split && medium > 0 && medium <= 128 && ceil_div(k, 32) * segments >= 16;
     if (!split) {
         int64_t best = 0;
         for (int t = 0; t < 3; t++) {

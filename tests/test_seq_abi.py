@@ -179,3 +179,16 @@ def test_launches_of_too_many_threads_are_refused():
     rows = ctypes.byref(m.FhcRows(P, 1))
     refused(L.fhc_norm_block_backward(ctypes.byref(n), rows, rows, rows, rows, rows, rows, P, P, P, P, 1 << 40, None),
             "too many workgroups")
+
+
+@pytest.mark.parametrize("c,f", [(0, 4096), (4096, 0), (300, 520), (2048, 8192)])
+def test_ffn_sizes_without_rows(c, f):
+    """A batch may be empty, and so may the channels or the features: the sizes are those of the copies of the weights."""
+    import ctypes
+    m = mod()
+    L = m._lib()
+    for rows in (0, 1, 100):
+        d = ctypes.byref(m.FfnDesc(1, 0, rows, c, f))
+        for back in (0, 1):
+            assert L.fhc_ffn_workspace_bytes(d, back) < 1 << 30
+        assert L.fhc_ffn_saved_bytes(d) < 1 << 30

@@ -771,3 +771,16 @@ def test_ffn_slope_far_from_zero(act, rows):
         assert (got[::2] == want.to(torch.bfloat16)).all() and not got[1::2].any()
     assert (dwg == n).all()
     assert torch.equal(dwu, (wg.double() * n).to(torch.bfloat16)) and torch.equal(dwd, dwu.t())
+
+
+@pytest.mark.parametrize("c,f", [(300, 520), (1024, 2048)])
+def test_ffn_of_an_empty_batch_and_a_wide_hidden_layer(c, f):
+    say("ffn empty batch", c, f)
+    import torch
+    m = mod()
+    v = ffn_inputs(Rand(1), 0, c, f, torch.bfloat16)
+    w = [v[k] for k in ("x", "wg", "wu", "wd")]
+    y, saved = m.ffn(*w, train=True)
+    dx, *grads = m.ffn_backward(*w, saved, v["dy"])
+    torch.cuda.synchronize()
+    assert m.ffn(*w).shape == y.shape == dx.shape == (0, c) and not any(g.any() for g in grads)
