@@ -556,6 +556,9 @@ extern "C" int fhc_ffn_backward(const fhc_ffn_desc* d, const fhc_rows* x, const 
                 if (!aligned(saved, 256)) return fail(-1, "%s: saved is not 256-byte aligned", op);
             }
         }
+        // without rows there is nothing behind x, dy and dx, and they may be null; dense, the products' ranges are empty
+        const fhc_rows none{nullptr, (int64_t)d->c};
+        if (!d->rows) x = dy = &none, dx = nullptr;
         if (!aligned(dwg, 2) || !aligned(dwu, 2) || !aligned(dwd, 2))
             return fail(-1, "%s: a weight's gradient is not aligned to its elements", op);
         FHC_TRY(check_workspace(op, workspace(d, true), ws, ws_bytes));

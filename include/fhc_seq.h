@@ -120,7 +120,8 @@ size_t fhc_ffn_workspace_bytes(const fhc_ffn_desc* d, int backward);
 int fhc_ffn_forward(const fhc_ffn_desc* d, const fhc_rows* x, const void* wg, const void* wu, const void* wd,
                     const fhc_rows* y, void* saved, void* ws, size_t ws_bytes, void* stream);
 
-/* dx and the weights' gradients (dense, in dtype) for dy; those that are not wanted may be NULL. */
+/* dx and the weights' gradients (dense, in dtype) for dy; those that are not wanted may be NULL. Without rows x, dy and
+ * dx are not read, and the weights' gradients are 0. */
 int fhc_ffn_backward(const fhc_ffn_desc* d, const fhc_rows* x, const void* wg, const void* wu, const void* wd,
                      const void* saved, const fhc_rows* dy, const fhc_rows* dx, void* dwg, void* dwu, void* dwd,
                      void* ws, size_t ws_bytes, void* stream);

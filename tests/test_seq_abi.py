@@ -192,3 +192,9 @@ def test_ffn_sizes_without_rows(c, f):
         for back in (0, 1):
             assert L.fhc_ffn_workspace_bytes(d, back) < 1 << 30
         assert L.fhc_ffn_saved_bytes(d) < 1 << 30
+
+
+def test_ffn_backward_without_rows_reads_no_descriptor():
+    assert ffn_call(True, rows=0, x=None, dy=None, dx=None, dwg=None, dwu=None, dwd=None) == 0
+    assert ffn_call(True, rows=0, x=(None, 0), dy=(None, 0), dx=(None, 0), dwg=None, dwu=None, dwd=None) == 0
+    assert ffn_call(False, rows=0, x=None, y=None) == 0

@@ -784,3 +784,23 @@ def test_ffn_of_an_empty_batch_and_a_wide_hidden_layer(c, f):
     dx, *grads = m.ffn_backward(*w, saved, v["dy"])
     torch.cuda.synchronize()
     assert m.ffn(*w).shape == y.shape == dx.shape == (0, c) and not any(g.any() for g in grads)
+
+
+@pytest.mark.parametrize("c,f", [(16, 24), (33, 17), (300, 520)])
+def test_ffn_backward_without_rows(c, f):
+    """The weights' gradients of no rows are 0, whatever the descriptors of x and dy hold."""
+    say("ffn no rows", c, f)
+    import ctypes
+    import torch
+    m = mod()
+    L, d = m._lib(), m.FfnDesc(1, 0, 0, c, f)
+    n = L.fhc_ffn_workspace_bytes(ctypes.byref(d), 1)
+    ws = torch.empty(max(n, 1), dtype=torch.uint8, device="cuda")
+    v = ffn_inputs(Rand(1), 1, c, f, torch.bfloat16)
+    w = [v[k].data_ptr() for k in ("wg", "wu", "wd")]
+    for rows in (None, m.FhcRows(None, 0), m.FhcRows(None, c)):
+        out = [torch.full_like(v[k], 7) for k in ("wg", "wu", "wd")]
+        assert L.fhc_ffn_backward(ctypes.byref(d), rows, *w, None, rows, rows, *(o.data_ptr() for o in out),
+                                  ws.data_ptr(), n, torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        assert not any(o.any() for o in out), rows
