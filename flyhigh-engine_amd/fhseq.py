@@ -187,6 +187,13 @@ def _seq(name, what, t):
     return _SEQ(t.data_ptr(), bs, ts)
 
 
+def _new_seq(k, x):
+    """An output of x's shape, in x's order in memory (time-major inputs give time-major outputs) where it has one with
+    the channels adjacent: sequences or steps that overlap by all but one element have none."""
+    y = k.empty_like(x)
+    return y if y.stride(2) == 1 or y.shape[2] <= 1 else k.new(x)
+
+
 def _like_seq(name, what, t, x, at):
     if t.dtype is not x.dtype or t.shape != x.shape or t.get_device() != at:
         _match(name, what, t, x.shape, x.dtype, at)
@@ -224,7 +231,7 @@ def glr(x, r, i, lam, rate=8.0, h0=None, lengths=None, train=False, stream=None)
     g, sizes, at, sx, sr, si = _glr_desc(k, op, x, r, i, lam, rate, lengths)
     b, _, d = x.shape
     start = _dense(op, "h0", h0, (b, d), k.f32, at)
-    y = k.empty_like(x)  # in x's order in memory: time-major inputs give time-major outputs
+    y = _new_seq(k, x)
     ht = k.empty((b, d), dtype=k.f32, device=at) if h0 is None else k.empty_like(h0)
     states = k.empty((sizes[0],), dtype=k.u8, device=at) if train else None
     n = sizes[1]
@@ -247,7 +254,7 @@ def glr_backward(x, r, i, lam, states, dy, rate=8.0, dht=None, lengths=None, str
     end = _dense(op, "dht", dht, (b, d), k.f32, at)
     kept = _dense(op, "states", states, (sizes[0],), k.u8, at)
     sdy = _like_seq(op, "dy", dy, x, at)
-    dx, dr, di = k.empty_like(x), k.empty_like(r), k.empty_like(i)
+    dx, dr, di = _new_seq(k, x), _new_seq(k, r), _new_seq(k, i)
     dlam = k.empty((d,), dtype=k.f32, device=at)
     dh0 = k.empty((b, d), dtype=k.f32, device=at)
     n = sizes[2]

@@ -804,3 +804,23 @@ def test_ffn_backward_without_rows(c, f):
                                   ws.data_ptr(), n, torch.cuda.current_stream().cuda_stream) == 0
         torch.cuda.synchronize()
         assert not any(o.any() for o in out), rows
+
+
+def test_glr_outputs_of_overlapping_windows():
+    """Inputs that overlap have no order in memory of their own to give to the outputs: windows that move by one element
+    from step to step or from sequence to sequence give what their copies give."""
+    say("glr windows")
+    import torch
+    q, m = Rand(17), mod()
+    b, t, d = 3, 5, 12
+    lam, dy = q.normal(d) - 4, q.normal(b, t, d)
+    r, i = q.normal(b, t, d), q.normal(b, t, d)
+    for strides in ((t + d - 1, 1, 1), (1, d + b - 1, 1), (1, 1, 1)):
+        say(strides)
+        win = torch.as_strided(q.normal(200), (b, t, d), strides)
+        for x, rr, ii in ((win, r, i), (r, win, win)):
+            got, want = [], []
+            for out, (a, e, f) in ((got, (x, rr, ii)), (want, [v.contiguous() for v in (x, rr, ii)])):
+                y, ht, states = m.glr(a, e, f, lam, train=True)
+                out += [y, ht, *m.glr_backward(a, e, f, lam, states, dy)]
+            assert all(torch.equal(a, w) for a, w in zip(got, want)), strides
