@@ -48,6 +48,8 @@ class RecurrentBlock:
         s = out[0].reshape(-1, c)
         o1 = s @ p["wo"].t()
         rows = max(t, 1)
+        if t == 0:  # no rows, no groups of them
+            gate1, gate2 = (None if g is None else g[:0] for g in (gate1, gate2))
         y1, u1 = fhseq.norm_block(xr, o1, p["post1"], gate1, p["pre1"], self.alpha, self.eps, rows)
         o2 = fhseq.ffn(u1, p["wg"], p["wu"], p["wd"], self.act, train=train)
         kept = None
@@ -84,6 +86,9 @@ class RecurrentBlock:
             g[k] = d.t() @ ur
             du0 = d @ p[k] if du0 is None else du0.addmm_(d, p[k])
         g["x"], g["u"] = dx.view(b, t, c), du0.view(b, t, c)
+        if t == 0:
+            for k in ("gate1", "gate2"):
+                g[k] = None if g[k] is None else g[k].new_zeros(b, c)
         return g
 
 

@@ -116,3 +116,23 @@ def test_block_learns():
             d = grads[k].float()
             q -= (0.02 * d / (d.square().mean().sqrt() + 1e-12) * q.float().square().mean().sqrt()).to(q.dtype)
     assert losses[-1] < 0.8 * losses[0], losses
+
+
+def test_block_of_no_steps():
+    """A call of no steps leaves the state, and its gradients are 0 bar the state's, with and without gates."""
+    import fhblock
+    import torch
+    print("block of no steps", flush=True)
+    b, c = 3, 64
+    block = fhblock.RecurrentBlock(c, 96, torch.bfloat16, seed=11)
+    x, u, state, g1, g2, n = inputs(b, 0, c, 12, torch.bfloat16)
+    ds = n(b, c)
+    for a1, a2 in ((None, None), (g1, g2), (g1, None)):
+        y, un, end, kept = block.forward(x, u, state, a1, a2, train=True)
+        assert y.shape == un.shape == (b, 0, c) and torch.equal(end, state)
+        g = block.backward(kept, torch.zeros_like(x), torch.zeros_like(x), ds)
+        assert torch.equal(g.pop("state"), ds)
+        for k, gate in (("gate1", a1), ("gate2", a2)):
+            assert (g[k] is None) == (gate is None) and (gate is None or g[k].shape == gate.shape), k
+        assert g["x"].shape == g["u"].shape == (b, 0, c)
+        assert not any(v.any() for v in g.values() if v is not None)
