@@ -141,6 +141,13 @@ __device__ __forceinline__ float lane_sum(float v) {
     }
     return v;
 }
+// 1 / sqrt(mean + eps). The instruction takes f32's subnormal numbers for 0, which only an eps that small leads to (a row
+// of zeros is still a row of zeros then). A NaN stays.
+__device__ __forceinline__ float inv_rms(float sum, float inv_c, float eps) {
+    const float v = __builtin_fmaf(sum, inv_c, eps);
+    if (eps < 0x1p-126f && v < 0x1p-126f) return __builtin_amdgcn_rsqf(v * 0x1p64f) * 0x1p32f;
+    return __builtin_amdgcn_rsqf(v);
+}
 constexpr int kWide = 1024;  // TPR of rows that a whole workgroup of up to 16 waves holds
 // Sums of N values over the threads of a row. Rows of several waves go through LDS, the buffers of successive sums in
 // turn so that one barrier a sum is enough; each wave adds all waves' sums.
@@ -200,7 +207,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_fwd(NormArgs g) {
 #pragma unroll
             for (int i = 0; i < 8; i++) s[0] = __builtin_fmaf(o[k][i], o[k][i], s[0]);
         row_sum<TPR, 1>(s, &lds[0], waves);
-        const float ro = __builtin_amdgcn_rsqf(__builtin_fmaf(s[0], inv_c, g.eps));
+        const float ro = inv_rms(s[0], inv_c, g.eps);
 #pragma unroll
         for (int k = 0; k < K; k++)
 #pragma unroll
@@ -219,7 +226,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_fwd(NormArgs g) {
     }
     if (!g.u.p) return;
     row_sum<TPR, 1>(s, &lds[1], waves);
-    const float ry = __builtin_amdgcn_rsqf(__builtin_fmaf(s[0], inv_c, g.eps));
+    const float ry = inv_rms(s[0], inv_c, g.eps);
 #pragma unroll
     for (int k = 0; k < K; k++) {
 #pragma unroll
@@ -344,7 +351,7 @@ __global__ __launch_bounds__(kBlock<TPR>, (kWaves<TPR, sizeof(typename T::Raw), 
 #pragma unroll
                 for (int i = 0; i < 8; i++) s1[0] = __builtin_fmaf(o[k][i], o[k][i], s1[0]);
             row_sum<TPR, 1>(s1, &lds1[turn], waves);
-            ro = __builtin_amdgcn_rsqf(__builtin_fmaf(s1[0], inv_c, g.eps));
+            ro = inv_rms(s1[0], inv_c, g.eps);
         }
 #pragma unroll
         for (int k = 0; k < K; k++) {
@@ -362,7 +369,7 @@ __global__ __launch_bounds__(kBlock<TPR>, (kWaves<TPR, sizeof(typename T::Raw), 
         }
         row_sum<TPR, 5>(s5, &lds5[turn], waves);
         turn ^= 1;
-        const float ry = __builtin_amdgcn_rsqf(__builtin_fmaf(s5[0], inv_c, g.eps));
+        const float ry = inv_rms(s5[0], inv_c, g.eps);
         const float my = s5[1] * inv_c * ry * ry;                          // mean(w_pre du n_y) / rms(y)
         const float mo = (s5[2] + ry * s5[3] - ry * my * s5[4]) * inv_c;    // mean(z n_o)
 #pragma unroll

@@ -824,3 +824,17 @@ def test_glr_outputs_of_overlapping_windows():
                 y, ht, states = m.glr(a, e, f, lam, train=True)
                 out += [y, ht, *m.glr_backward(a, e, f, lam, states, dy)]
             assert all(torch.equal(a, w) for a, w in zip(got, want)), strides
+
+
+@pytest.mark.parametrize("eps", [2.0 ** -126, 2.0 ** -127, 2.0 ** -130, 2.0 ** -140])
+@pytest.mark.parametrize("c", [40, 300])
+def test_norm_block_of_zeros_under_a_subnormal_eps(c, eps):
+    """Rows of zeros: of the block's output, or of the residual stream without one. 1 / rms is 2^63 to 2^70 there."""
+    say("norm subnormal eps", c, eps)
+    import torch
+    v = norm_inputs(Rand(c), 12, c, 4, torch.float32)
+    v["o"][3], v["o"][8] = 0, 0
+    norm_check(v, 0.5, eps, 4)
+    v.update(o=None, w_post=None, gate=None)
+    v["x"][5], v["x"][11] = 0, 0
+    norm_check(v, 0.5, eps, 4)
