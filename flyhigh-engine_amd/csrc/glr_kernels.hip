@@ -675,12 +675,13 @@ __global__ __launch_bounds__(64 * W * CW, L == 1 ? 1 : L == 4 ? 4 : 3) void glr_
 }
 
 // Column sums of the partial rows: 16 columns x 64 row lanes a workgroup, rows y, y + gridDim.y * 64, ...; a second
-// launch with one row block finishes. In f64: millions of terms of either sign meet here.
+// launch with one row block finishes. In f64: millions of terms of either sign meet here. `first`: the launch's first 16
+// columns.
 template <class In, bool LAST>
 __global__ __launch_bounds__(1024) void glr_sum(const In* part, uint64_t rows, uint32_t d, double* out, float* dlam,
-                                                const float* lam, float rate) {
+                                                const float* lam, float rate, uint32_t first) {
     __shared__ double s[64][17];
-    const uint32_t x = threadIdx.x & 15, ch = blockIdx.x * 16 + x, y = threadIdx.x >> 4;
+    const uint32_t c0 = (first + blockIdx.x) * 16, x = threadIdx.x & 15, ch = c0 + x, y = threadIdx.x >> 4;
     double acc = 0.0;
     if (ch < d) {
 #pragma unroll 8
@@ -690,7 +691,7 @@ __global__ __launch_bounds__(1024) void glr_sum(const In* part, uint64_t rows, u
     s[y][x] = acc;
     __syncthreads();
     if (threadIdx.x < 64) {  // 4 lanes a column, 16 rows each
-        const uint32_t col = threadIdx.x >> 2, q = threadIdx.x & 3, c = blockIdx.x * 16 + col;
+        const uint32_t col = threadIdx.x >> 2, q = threadIdx.x & 3, c = c0 + col;
         acc = 0.0;
 #pragma unroll
         for (int k = 0; k < 16; k++) acc += s[q * 16 + k][col];
@@ -711,13 +712,15 @@ __global__ __launch_bounds__(1024) void glr_sum(const In* part, uint64_t rows, u
 // ---- host side ----------------------------------------------------------------------------------------------------
 
 constexpr int kL = 8;              // steps a lane holds
-constexpr uint32_t kSumRows = 64;  // row blocks of the first sum
+constexpr uint32_t kOneSum = 512;  // partial rows up to which one launch adds them
+constexpr uint32_t kSumRows = 64;  // row blocks of the first sum otherwise
 
 struct Plan {
     int l, w;    // steps of a stretch; stretches (waves) of a chunk
     bool chain, straddles;
     uint32_t v, groups, nchunk, colblocks, nstates, spacing;
-    uint64_t words;  // of the chain: maps, then heads
+    uint64_t words;      // of the chain: maps, then heads
+    uint64_t part_rows;  // of dlam's partial sums
     size_t agg_bytes, part_bytes, sum_bytes;
 };
 
@@ -747,7 +750,8 @@ Plan plan_of(const fhc_glr_desc* g, bool backward, uint32_t v, bool near) {
     p.words = p.chain ? (p.nchunk + ceil_div(p.nchunk, kGroup) + ceil_div(p.nchunk, kRun)) * flat : 0;
     p.agg_bytes = p.chain ? p.words * 8 + (size_t)g->b * ceil_div(g->d, 64) * kTicketStep * 4 : 0;
     p.part_bytes = (size_t)ceil_div((p.chain ? p.nchunk : 1) * flat * 4, 256) * 256;
-    p.sum_bytes = (size_t)kSumRows * g->d * 8;
+    p.part_rows = (uint64_t)(p.chain ? p.nchunk : 1) * g->b;
+    p.sum_bytes = p.part_rows > kOneSum ? (size_t)kSumRows * g->d * 8 : 0;
     return p;
 }
 
@@ -839,6 +843,19 @@ void launch(const Plan& p, const GlrArgs& a, hipStream_t s) {
 #undef GLR
 }
 
+// a launch has fewer than 2^32 threads: wide rows take several
+template <class In, bool LAST>
+int sum(const char* op, const In* part, uint64_t rows, uint32_t d, uint32_t row_blocks, double* out, float* dlam,
+        const float* lam, float rate, hipStream_t s) {
+    const uint32_t blocks = (uint32_t)ceil_div(d, 16), most = (1u << 21) / row_blocks;
+    for (uint32_t first = 0; first < blocks; first += most) {
+        const dim3 grid(blocks - first < most ? blocks - first : most, row_blocks);
+        hipLaunchKernelGGL((glr_sum<In, LAST>), grid, dim3(1024), 0, s, part, rows, d, out, dlam, lam, rate, first);
+        FHC_TRY(launched(op));
+    }
+    return 0;
+}
+
 template <bool BWD>
 int run(const char* op, const Plan& p, GlrArgs& a, uint32_t dtype, void* ws, hipStream_t s) {
     if ((uint64_t)p.colblocks * p.nchunk >= 1ull << 31 || (uint64_t)a.b * p.groups >= 1ull << 31) return fail(-1, "%s: too many chunks", op);
@@ -925,12 +942,9 @@ extern "C" int fhc_glr_backward(const fhc_glr_desc* g, const fhc_seq* x, const f
         if (g->d == 0) return 0;
         if (!dlam) return fail(-1, "%s: null dlam", op);
         const hipStream_t s = (hipStream_t)stream;
-                const uint32_t dblocks = (uint32_t)ceil_div(g->d, 16);
         if (g->b == 0) {  // an empty sum
             if (!g->lam) return fail(-1, "%s: null lam", op);
-            hipLaunchKernelGGL((glr_sum<float, true>), dim3(dblocks), dim3(1024), 0, s, (const float*)nullptr,
-                               (uint64_t)0, g->d, (double*)nullptr, dlam, g->lam, g->rate);
-            return launched(op);
+            return sum<float, true>(op, nullptr, 0, g->d, 1, nullptr, dlam, g->lam, g->rate, s);
         }
         FHC_TRY(check_seq(op, "x", x, g));
         FHC_TRY(check_seq(op, "r", r, g));
@@ -949,18 +963,10 @@ extern "C" int fhc_glr_backward(const fhc_glr_desc* g, const fhc_seq* x, const f
         char* w = static_cast<char*>(ws) + (p.agg_bytes + 255) / 256 * 256;
         a.part = reinterpret_cast<float*>(w);
         FHC_TRY(run<true>(op, p, a, g->dtype, ws, s));
-        const uint64_t rows = (uint64_t)(p.chain ? p.nchunk : 1) * g->b;
-        if (rows <= 512) {
-            hipLaunchKernelGGL((glr_sum<float, true>), dim3(dblocks), dim3(1024), 0, s, a.part, rows, g->d,
-                               (double*)nullptr, dlam, g->lam, g->rate);
-            return launched(op);
-        }
+        if (!p.sum_bytes)
+            return sum<float, true>(op, a.part, p.part_rows, g->d, 1, nullptr, dlam, g->lam, g->rate, s);
         double* sums = reinterpret_cast<double*>(w + p.part_bytes);
-        hipLaunchKernelGGL((glr_sum<float, false>), dim3(dblocks, kSumRows), dim3(1024), 0, s, a.part, rows, g->d, sums,
-                           (float*)nullptr, (const float*)nullptr, 0.0f);
-        FHC_TRY(launched(op));
-        hipLaunchKernelGGL((glr_sum<double, true>), dim3(dblocks), dim3(1024), 0, s, sums, (uint64_t)kSumRows, g->d,
-                           (double*)nullptr, dlam, g->lam, g->rate);
-        return launched(op);
+        FHC_TRY((sum<float, false>(op, a.part, p.part_rows, g->d, kSumRows, sums, nullptr, nullptr, 0.0f, s)));
+        return sum<double, true>(op, sums, kSumRows, g->d, 1, nullptr, dlam, g->lam, g->rate, s);
     });
 }

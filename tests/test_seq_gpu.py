@@ -838,3 +838,21 @@ def test_norm_block_of_zeros_under_a_subnormal_eps(c, eps):
     v.update(o=None, w_post=None, gate=None)
     v["x"][5], v["x"][11] = 0, 0
     norm_check(v, 0.5, eps, 4)
+
+
+def test_glr_backward_over_more_channels_than_a_launch_of_sums_takes():
+    """dlam of sequences that are one and the same is that of one times their number (the sum is in f64)."""
+    say("glr wide sums")
+    import torch
+    m, q = mod(), Rand(29)
+    for b, d in ((520, (1 << 20) + 48), (1, (1 << 26) + 24)):
+        say(b, d)
+        x, r, i, dy = (q.normal(1, 1, d, dtype=torch.float16) for _ in range(4))
+        lam = q.normal(d) - 4
+        one = [v.expand(b, 1, d) for v in (x, r, i, dy)]
+        y, _, states = m.glr(*one[:3], lam, train=True)
+        dlam = m.glr_backward(*one[:3], lam, states, one[3])[3]
+        del y, states
+        for part in (slice(0, 500), slice(d // 2, d // 2 + 500), slice(d - 500, d)):
+            ref, err = seqref.glr(*(v[:, :, part] for v in (x, r, i)), lam[part], 8.0, dy=dy[:, :, part])
+            seqref.close(dlam[part], b * ref[5], b * err[5], "dlam")
