@@ -3,7 +3,9 @@ linear recurrence (``glr``), the norms around a block with its gate and the scal
 gated feed-forward block (``ffn``), each with its backward pass.
 
 Inputs are torch tensors on the current GPU in f16, bf16 or (not ``ffn``) f32, all of one call in the same type; states
-and the gradients of the recurrence's and norms' weights are f32. Each function returns new tensors. ``stream`` (a torch
+and the gradients of the recurrence's and norms' weights are f32. Each function returns new tensors, which autograd does
+not know: a call with tensors that require gradients is refused while autograd records (``torch.no_grad()``, and the
+``*_backward`` functions, are the way). ``stream`` (a torch
 stream) is where the call runs, the current stream if None; what it allocates belongs to that stream. The module only
 passes device pointers: when the library is missing, loading it raises, and nothing is computed on the host.
 """
@@ -101,6 +103,7 @@ class _Fast:
         self.new = functools.partial(torch.empty_like, memory_format=torch.contiguous_format)
         self.f32, self.i32, self.u8 = torch.float32, torch.int32, torch.uint8
         self.types = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}
+        self.recording = torch.is_grad_enabled
         self.device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
         self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda _: torch.cuda.current_stream().cuda_stream)
@@ -151,6 +154,15 @@ def _pack(name, pack, *fields):
 
 def _refuse(name):
     raise FhcError(f"{name}: {fhconv.last_error()}")
+
+
+def _unrecorded(k, name, *tensors):
+    """The results would lose their gradients without a word."""
+    if k.recording():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise FhcError(f"{name}: a tensor requires gradients, which this call does not record: call it under "
+                               f"torch.no_grad() or with detached tensors, and take them from the *_backward function")
 
 
 def _first(k, name, x):
@@ -228,6 +240,7 @@ def glr(x, r, i, lam, rate=8.0, h0=None, lengths=None, train=False, stream=None)
         with _on(stream):
             return glr(x, r, i, lam, rate, h0, lengths, train)
     k, op = _fast(), "glr"
+    _unrecorded(k, op, x, r, i, lam, h0)
     g, sizes, at, sx, sr, si = _glr_desc(k, op, x, r, i, lam, rate, lengths)
     b, _, d = x.shape
     start = _dense(op, "h0", h0, (b, d), k.f32, at)
@@ -249,6 +262,7 @@ def glr_backward(x, r, i, lam, states, dy, rate=8.0, dht=None, lengths=None, str
         with _on(stream):
             return glr_backward(x, r, i, lam, states, dy, rate, dht, lengths)
     k, op = _fast(), "glr_backward"
+    _unrecorded(k, op, x, r, i, lam, dy, dht)
     g, sizes, at, sx, sr, si = _glr_desc(k, op, x, r, i, lam, rate, lengths)
     b, _, d = x.shape
     end = _dense(op, "dht", dht, (b, d), k.f32, at)
@@ -301,6 +315,7 @@ def norm_block(x, o, w_post, gate, w_pre, alpha=1.0, eps=1e-6, rows_per_group=1,
         with _on(stream):
             return norm_block(x, o, w_post, gate, w_pre, alpha, eps, rows_per_group)
     k, op = _fast(), "norm_block"
+    _unrecorded(k, op, x, o, w_post, gate, w_pre)
     n, at, _, rx, ro = _norm_desc(k, op, x, o, w_post, gate, w_pre, alpha, eps, rows_per_group)
     y, u = k.new(x), k.new(x)
     c = x.shape[1]
@@ -316,6 +331,7 @@ def norm_block_backward(x, o, w_post, gate, w_pre, dy, du, alpha=1.0, eps=1e-6, 
         with _on(stream):
             return norm_block_backward(x, o, w_post, gate, w_pre, dy, du, alpha, eps, rows_per_group)
     k, op = _fast(), "norm_block_backward"
+    _unrecorded(k, op, x, o, w_post, gate, w_pre, dy, du)
     n, at, dtype, rx, ro = _norm_desc(k, op, x, o, w_post, gate, w_pre, alpha, eps, rows_per_group)
     rdy, rdu = _like_rows(op, "dy", dy, x, at), _like_rows(op, "du", du, x, at)
     rows, c = x.shape
@@ -356,6 +372,7 @@ def ffn(x, wg, wu, wd, act="silu", train=False, stream=None):
         with _on(stream):
             return ffn(x, wg, wu, wd, act, train)
     k, op = _fast(), "ffn"
+    _unrecorded(k, op, x, wg, wu, wd)
     d, at, sizes, rx, pg, pu, pd = _ffn_desc(k, op, x, wg, wu, wd, act)
     y = k.new(x)
     saved = _bytes(k, sizes[0], at) if train else None
@@ -373,6 +390,7 @@ def ffn_backward(x, wg, wu, wd, saved, dy, act="silu", stream=None):
         with _on(stream):
             return ffn_backward(x, wg, wu, wd, saved, dy, act)
     k, op = _fast(), "ffn_backward"
+    _unrecorded(k, op, x, wg, wu, wd, dy)
     d, at, sizes, rx, pg, pu, pd = _ffn_desc(k, op, x, wg, wu, wd, act)
     kept = _dense(op, "saved", saved, (sizes[0],), k.u8, at) if sizes[0] else None
     rdy = _like_rows(op, "dy", dy, x, at)

@@ -198,3 +198,25 @@ def test_ffn_backward_without_rows_reads_no_descriptor():
     assert ffn_call(True, rows=0, x=None, dy=None, dx=None, dwg=None, dwu=None, dwd=None) == 0
     assert ffn_call(True, rows=0, x=(None, 0), dy=(None, 0), dx=(None, 0), dwg=None, dwu=None, dwd=None) == 0
     assert ffn_call(False, rows=0, x=None, y=None) == 0
+
+
+def test_tensors_that_require_gradients_are_refused_while_autograd_records():
+    import torch
+    m = mod()
+    x, rows, w = torch.zeros(2, 3, 4), torch.zeros(5, 4), torch.zeros(6, 4)
+    d, lam, c = w.t().contiguous(), torch.zeros(4), torch.ones(4)
+    states = torch.zeros(1, dtype=torch.uint8)
+    calls = [(m.glr, [x, x, x, lam]), (m.glr_backward, [x, x, x, lam, states, x]),
+             (m.norm_block, [rows, rows, c, None, c]), (m.norm_block_backward, [rows, rows, c, None, c, rows, rows]),
+             (m.ffn, [rows, w, w, d]), (m.ffn_backward, [rows, w, w, d, states, rows])]
+    for call, args in calls:
+        for k, a in enumerate(args):
+            if a is None or a is states:
+                continue
+            grad = args[:k] + [a.clone().requires_grad_()] + args[k + 1:]
+            with pytest.raises(m.FhcError, match="requires gradients"):
+                call(*grad)
+            with torch.no_grad(), pytest.raises(m.FhcError, match="current GPU"):  # the next check
+                call(*grad)
+    with pytest.raises(m.FhcError, match="requires gradients"):
+        m.glr(x, x, x, lam, h0=torch.zeros(2, 4, requires_grad=True))
