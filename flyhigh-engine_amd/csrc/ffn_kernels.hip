@@ -377,8 +377,9 @@ size_t part_of(int64_t m, int64_t n, int64_t k, int segments, int pairs) {
 size_t workspace(const fhc_ffn_desc* d, bool backward) {
     const size_t rows = Operands::pack_bytes(d->rows, d->c), up = Operands::pack_bytes(d->f, d->c),
                  down = Operands::pack_bytes(d->c, d->f);
-    if (!backward) {  // h, where nothing is kept, and the second product's partial sums
+    if (!backward) {  // h, where nothing is kept, and the second product's partial sums; in one kernel neither is made
         const size_t copies = d->rows > kSkinnyRows ? rows + 2 * up + down : 0;
+        if (fused(d)) return copies;
         return hidden_bytes(d) + part_of(d->rows, d->c, d->f, 1, 1) + copies;
     }
     size_t part = 0;
@@ -406,9 +407,8 @@ int forward(const char* op, const fhc_ffn_desc* d, const fhc_rows* x, const void
                      static_cast<uint16_t*>(y->p), y->ld, (int)d->c, nullptr, nullptr, d->act};
         return skinny<T, false>(op, b, st);
     }
-    char* part = w + hidden_bytes(d);
-    Operands o{{}, 0, part + part_of(d->rows, d->c, d->f, 1, 1)};
     if (fused(d)) {
+        Operands o{{}, 0, w};
         FusedArgs a{};
         a.ldx = x->ld, a.ldg = d->c, a.ldd = d->f, a.rows = (int)d->rows, a.c = (int)d->c, a.f = (int)d->f, a.act = d->act;
         a.x = o.take(x->p, a.ldx, d->rows, d->c, true);
@@ -418,6 +418,8 @@ int forward(const char* op, const fhc_ffn_desc* d, const fhc_rows* x, const void
         a.out = static_cast<uint16_t*>(y->p), a.ldo = y->ld;
         return run_fused<T, false>(op, a, st);
     }
+    char* part = w + hidden_bytes(d);
+    Operands o{{}, 0, part + part_of(d->rows, d->c, d->f, 1, 1)};
     GemmArgs g{}, p{};
     g.lda = x->ld, g.ldb = d->c, p.ldb = d->f;
     g.a0 = o.take(x->p, g.lda, d->rows, d->c, true);

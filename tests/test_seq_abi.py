@@ -220,3 +220,12 @@ def test_tensors_that_require_gradients_are_refused_while_autograd_records():
                 call(*grad)
     with pytest.raises(m.FhcError, match="requires gradients"):
         m.glr(x, x, x, lam, h0=torch.zeros(2, 4, requires_grad=True))
+
+
+@pytest.mark.parametrize("rows,c,f", [(51840, 128, 512), (6000, 33, 4096), (40000, 250, 1 << 20)])
+def test_ffn_in_one_kernel_takes_no_room_for_the_hidden_layer(rows, c, f):
+    import ctypes
+    m = mod()
+    up = lambda n: (n + 7) // 8 * 8  # noqa: E731
+    copies = 2 * (rows * up(c) + 2 * f * up(c) + c * up(f)) + 4 * 256  # of the rows and the three weights
+    assert m._lib().fhc_ffn_workspace_bytes(ctypes.byref(m.FfnDesc(0, 0, rows, c, f)), 0) <= copies

@@ -856,3 +856,41 @@ def test_glr_backward_over_more_channels_than_a_launch_of_sums_takes():
         for part in (slice(0, 500), slice(d // 2, d // 2 + 500), slice(d - 500, d)):
             ref, err = seqref.glr(*(v[:, :, part] for v in (x, r, i)), lam[part], 8.0, dy=dy[:, :, part])
             seqref.close(dlam[part], b * ref[5], b * err[5], "dlam")
+
+
+@pytest.mark.parametrize("shape", [(20, 37, 51), (300, 37, 51), (700, 132, 1030), (6003, 37, 51), (11501, 101, 70),
+                                   (19501, 131, 33)], ids=str)
+def test_ffn_stays_in_its_workspace(shape):
+    """Widths and addresses that make a call copy every operand: what lies behind the workspace, the kept states and the
+    outputs stays as it was."""
+    rows, c, f = shape
+    say("ffn workspace", shape)
+    import ctypes
+    import torch
+    m = mod()
+    L, d = m._lib(), m.FfnDesc(1, 1, rows, c, f)
+    v = ffn_inputs(Rand(33), rows, c, f, torch.bfloat16)
+    at = {}
+    for k in ("x", "wg", "wu", "wd", "dy"):  # at odd elements
+        b = torch.empty(v[k].numel() + 1, dtype=torch.bfloat16, device="cuda")
+        b[1:] = v[k].flatten()
+        at[k] = b[1:].view(v[k].shape)
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def room(n):
+        return torch.full((n + 8192,), 0x5A, dtype=torch.uint8, device="cuda")
+
+    sizes = (L.fhc_ffn_saved_bytes(ctypes.byref(d)), L.fhc_ffn_workspace_bytes(ctypes.byref(d), 0),
+             L.fhc_ffn_workspace_bytes(ctypes.byref(d), 1), rows * c * 2, rows * c * 2, f * c * 2, f * c * 2, f * c * 2)
+    bufs = [room(n) for n in sizes]
+    saved, ws, wsb, y, dx, dwg, dwu, dwd = (b.data_ptr() for b in bufs)
+    w = [at[k].data_ptr() for k in ("wg", "wu", "wd")]
+    x, dy, yr, dxr = (m._ROWS(p, c) for p in (at["x"].data_ptr(), at["dy"].data_ptr(), y, dx))
+    assert L.fhc_ffn_forward(ctypes.byref(d), x, *w, yr, saved, ws, sizes[1], stream) == 0
+    assert L.fhc_ffn_backward(ctypes.byref(d), x, *w, saved, dy, dxr, dwg, dwu, dwd, wsb, sizes[2], stream) == 0
+    torch.cuda.synchronize()
+    for b, n in zip(bufs, sizes):
+        assert (b[n:] == 0x5A).all()
+    want, err = seqref.ffn(*(at[k] for k in ("x", "wg", "wu", "wd")), "gelu", at["dy"])
+    for name, b, n, r, e in zip(FFN_OUT, bufs[3:], sizes[3:], want, err):
+        seqref.close(b[:n].view(torch.bfloat16).view(r.shape), r, e, name)
