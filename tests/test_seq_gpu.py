@@ -894,3 +894,74 @@ def test_ffn_stays_in_its_workspace(shape):
     want, err = seqref.ffn(*(at[k] for k in ("x", "wg", "wu", "wd")), "gelu", at["dy"])
     for name, b, n, r, e in zip(FFN_OUT, bufs[3:], sizes[3:], want, err):
         seqref.close(b[:n].view(torch.bfloat16).view(r.shape), r, e, name)
+
+
+# ---- paths that only larger calls take --------------------------------------------------------------------------
+
+# one run of chained chunks is 8192 steps forward and 4096 backward: into the second run, the third and the fifth
+@pytest.mark.parametrize("shape", [(1, 8400, 34), (2, 8193, 3), (2, 16500, 3)], ids=str)
+def test_glr_of_several_runs(shape):
+    say("glr runs", shape)
+    for dtype, ragged in (("f16", False), ("f32", True)):
+        glr_check(glr_inputs(Rand(sum(shape)), *shape, types()[dtype], ragged=ragged))
+
+
+# a workgroup that takes several short groups one after the other: one row a group, two, three; wide rows and narrow ones
+@pytest.mark.parametrize("shape", [(600, 8192, 1), (2500, 2048, 2), (3100, 2040, 3), (13000, 40, 1), (26000, 24, 2)],
+                         ids=str)
+def test_norm_block_of_many_short_groups(shape):
+    say("norm short groups", shape)
+    for dtype in ("bf16", "f32"):
+        norm_check(norm_inputs(Rand(sum(shape)), *shape, types()[dtype]), math.sqrt(0.5), 1e-6, shape[2])
+
+
+def ffn_tile(m, n, pairs=1, glu=False):
+    """The tile that a product of many slabs takes: 0 narrow, 1 medium, 2 large (the rule of ffn_kernels.hip)."""
+    def rounds(bm, bn):
+        return -(-(-(-m // bm) * -(-n // (bn // (2 if glu else 1))) * pairs) // 256)
+
+    time = [rounds(128, 64) * 75, rounds(128, 128) * 100, rounds(256, 256) * 270]
+    return time.index(min(time))
+
+
+@pytest.mark.parametrize("shape", [(3301, 3275, 3283), (3298, 3276, 3282)], ids=str)
+def test_ffn_large_tiles_with_remainders(shape):
+    """Every product of a step in the largest tile: rows and columns of either operand, cut in a tile and in a slab."""
+    rows, c, f = shape
+    say("ffn large tiles", shape)
+    tiles = (ffn_tile(rows, f, glu=True), ffn_tile(rows, c), ffn_tile(rows, f), ffn_tile(rows, c), ffn_tile(f, c, 2),
+             ffn_tile(c, f))
+    assert all(t == 2 for t in tiles), tiles
+    for k, dtype in enumerate(("f16", "bf16")):
+        ffn_check(ffn_inputs(Rand(sum(shape)), *shape, types()[dtype]), "gelu" if k else "silu")
+
+
+# the one-kernel form at each of its register sizes, short of them and full, with tails of rows and features
+@pytest.mark.parametrize("shape", [(6001, 7, 33), (6130, 64, 31), (11600, 65, 129), (11777, 128, 100), (19600, 129, 31),
+                                   (20001, 256, 100)], ids=str)
+def test_ffn_in_one_kernel_at_its_edges(shape):
+    say("ffn one kernel", shape)
+    for k, dtype in enumerate(("f16", "bf16")):
+        ffn_check(ffn_inputs(Rand(sum(shape)), *shape, types()[dtype]), "silu" if k else "gelu")
+
+
+@pytest.mark.parametrize("shape", [(6003, 40, 64), (11523, 72, 136), (19523, 200, 70)], ids=str)
+def test_ffn_in_one_kernel_values_that_are_not_finite_stay_in_their_rows(shape):
+    """Forward and dx: a row of x that holds a NaN or an infinity, and one of dy, reach their own rows only."""
+    rows, c, f = shape
+    say("ffn one kernel not finite", shape)
+    import torch
+    m = mod()
+    v = ffn_inputs(Rand(23), rows, c, f, torch.bfloat16)
+    w = [v[k] for k in ("wg", "wu", "wd")]
+    y, saved = m.ffn(v["x"], *w, train=True)
+    dx = m.ffn_backward(v["x"], *w, saved, v["dy"])[0]
+    v["x"][100, 3], v["x"][5000, c - 1], v["dy"][4321, 0] = math.nan, math.inf, math.nan
+    y2, saved2 = m.ffn(v["x"], *w, train=True)
+    dx2 = m.ffn_backward(v["x"], *w, saved2, v["dy"])[0]
+    at = torch.arange(rows, device="cuda")
+    whole = (at != 100) & (at != 5000)
+    assert torch.equal(y2[whole], y[whole]) and not torch.isfinite(y2[100]).any()
+    whole &= at != 4321
+    assert torch.equal(dx2[whole], dx[whole]) and not torch.isfinite(dx2[100]).any()
+    assert not torch.isfinite(dx2[4321]).any() and torch.equal(y2[4321], y[4321])
