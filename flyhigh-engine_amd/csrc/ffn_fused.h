@@ -13,8 +13,8 @@
 //   wg, wu: chunk ^ 2 (row & 7) (c <= 64, whose rows are half as long: ^ 2 (row >> 1 & 3)); wd: chunk ^ (row >> 2 & 3).
 //
 // Bound by the chain of a slice (fragments from LDS, products, activation, products) at two waves a SIMD, which its
-// registers allow. MI355X, 51840 x 128, f 512, f16: forward 39 us (20 GFLOP, 520 TFLOP/s), backward 86 (34 GFLOP, 400
-// TFLOP/s; 96 bytes a lane spill at c > 64, f16, 144 at c > 128).
+// registers allow. MI355X, 51840 x 128, f 512, f16: forward 38 us (20 GFLOP, 540 TFLOP/s), backward 84 (34 GFLOP, 405
+// TFLOP/s). Backward spills, bytes a lane: c > 64 104 (f16) and 72 (bf16), c > 128 144 and 136.
 #pragma once
 #include "ffn_gemm.h"
 
@@ -36,7 +36,8 @@ __device__ __forceinline__ uint2 read_tr(const uint4* lds, int at) {
     asm volatile("" : "+v"(at));  // volatile: made anew for each slice rather than kept, registers are short
 #if defined(__HIP_DEVICE_COMPILE__)
     typedef __attribute__((address_space(3))) s4_t* lds_s4;
-    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(reinterpret_cast<const char*>(lds) + at)));
+    const char* p = reinterpret_cast<const char*>(lds) + at;
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p)));
 #else
     return uint2{};
 #endif
@@ -205,7 +206,8 @@ __global__ __launch_bounds__(64 * NW, 2) void ffn_fused(FusedArgs g) {
     // Slice s has landed, and every wave is done with slice s - 1, whose buffers slice s + 2 takes (see ffn_gemm). Behind
     // the fetch of s a wave has started the stores of step s - 2, the fetch of s + 1 and the stores of s - 1.
     constexpr int STORES = BWD ? 6 * MB : 0;
-    auto one = [&](int s, const uint4* bg, const uint4* bu, const uint4* bd, uint4* ng, uint4* nu, uint4* nd) __attribute__((always_inline)) {
+    auto one = [&](int s, const uint4* bg, const uint4* bu, const uint4* bd, uint4* ng, uint4* nu,
+                   uint4* nd) __attribute__((always_inline)) {
         wait_vm<NI + 2 * STORES>();
         __builtin_amdgcn_s_barrier();
         fence();

@@ -12,13 +12,15 @@
 //   multiplies. Measured on the way, TFLOP/s: three buffers and one barrier a slab for all eight waves 990; turns 984
 //   with 64-bit lane addresses, 1230 once a row's address is scalar; 128 x 256 tiles, two workgroups a CU, 924 (their LDS
 //   traffic). At that rate the matrix units are busy 64% of the cycles and the card's power holds the clock at 1.8 GHz.
-//   8192 rows, 2048 channels, 8192 features, bf16: weights' gradients 1270-1350 over two runs, dx 1250-1320, y 1140-1150,
-//   GLU 890 and dL/dh 620-630, whose f32 states pass through the epilogue; a large library product reaches 1307.
+//   8192 rows, 2048 channels, 8192 features, bf16: weights' gradients 1270-1350 over three runs, dx 1250-1320, y
+//   1140-1155, GLU 890-910 and dL/dh 620-640, whose f32 states pass through the epilogue; a large library product
+//   reaches 1307.
 // - Rows: an LDS row holds 32 k (64 bytes), its 16-byte chunk c at position c ^ (row >> 2 & 2): a fragment read (16
 //   bytes a lane) goes by lanes 0-3, 12-15, 20-23, 24-27 and the like, 16 at once, which so fall on all 64 banks (other
-//   permutations of the chunks, by row >> 2 or by 8 neighbours, measured a conflict for every read). Columns: an LDS row holds the tile's m (n) of one k, its
-//   32-byte blocks permuted by f(k) = k & 3 | (k >> 3 & 1) << 2 (64 wide: k >> 1 & 1 | (k >> 3 & 1) << 1); fragments come from the transposing LDS read (16 lanes
-//   read 4 k x 16 m and receive 4 k of one m each), whose 32 lanes at once then spread over all banks too.
+//   permutations of the chunks, by row >> 2 or by 8 neighbours, measured a conflict for every read). Columns: an LDS row
+//   holds the tile's m (n) of one k, its 32-byte blocks permuted by f(k) = k & 3 | (k >> 3 & 1) << 2 (64 wide:
+//   k >> 1 & 1 | (k >> 3 & 1) << 1); fragments come from the transposing LDS read (16 lanes read 4 k x 16 m and receive
+//   4 k of one m each), whose 32 lanes at once then spread over all banks too.
 // - The MFMA takes B's fragment as its first operand: a lane's 4 results are 4 adjacent n of one m.
 // - Workgroups go round-robin to the 8 XCDs, each with its own L2: the tile index is permuted so that an XCD works on
 //   neighbouring tiles, in groups of 8 tile rows.

@@ -179,10 +179,25 @@ constexpr uint32_t kSkinnyRows = 32;  // up to here the weights' bytes are all t
 
 // One kernel a direction (ffn_fused.h) where the channels fit its registers and the rows give it work for the chip: a
 // workgroup has 128 rows and walks all features, so the time hardly changes until the rows fill the CUs, where the
-// products of ffn_gemm.h spread few rows over features too. Measured, one kernel against products, f16, at 4096 and
-// 20000 rows: forward of c 128, f 512, 23 and 23 us against 17 and 41, its training step 93 and 103 against 64 and 159; of
-// c 128, f 8192, a training step 924 at 4096 rows against 400 and 91 ns more a row: about where those lines cross. One
-// rule for both passes and with or without states kept, so that serving gives a training forward's bits.
+// products of ffn_gemm.h spread few rows over features too. Measured, f16, us of one kernel, of products:
+//                     rows  forward   training step
+//   c  64, f  512     3000   16,  15    75,  58
+//                     6000   16,  18    76,  67
+//                    12000   16,  25    76,  85
+//   c 128, f  512     6000   22,  20    93,  75
+//                    11500   22,  30    97,  96
+//                    20000   23,  25   105, 121
+//   c 256, f 1024    10000   65,  35   242, 149
+//                    19500   67,  62   273, 286
+//                    32768   72,  81   339, 448
+//                    40000  131, 103   550, 532
+//                   131072  275, 312  1481, 1523
+// Above 128 channels a CU holds one workgroup, so 32768 rows are a round and a few rows more cost another one: from 26000
+// rows up, steps of c 160 to 256 and f 512 to 2048 took 0.72 to 1.04 of the products' time, bar 40000 rows with f 2048,
+// 1.12 to 1.19; forward 0.86 to 1.23, and 1.2 to 1.68 at 40000. There the step without a hidden layer in memory is what
+// the rule is for. f moves the crossing: c 32, f 128 is ahead from below 3000 rows (9, 12 and 37, 42); a forward of
+// c 128, f 2048 from 20000 (75, 77), its step from 11500 (276, 291). One rule for both passes and with or without states
+// kept, so that serving gives a training forward's bits; it follows the step.
 bool fused(const fhc_ffn_desc* d) {
     return d->c > 0 && d->f > 0 && d->c <= 256 && d->rows >= (d->c <= 64 ? 6000u : d->c <= 128 ? 11500u : 19500u);
 }
@@ -198,7 +213,8 @@ int check_desc(const char* op, const fhc_ffn_desc* d) {
 int check_rows(const char* op, const char* name, const fhc_rows* r, uint32_t c) {
     if (!r) return fail(-1, "%s: null %s", op, name);
     if (!r->p) return fail(-1, "%s: null pointer of %s", op, name);
-    if (r->ld < (int64_t)c) return fail(-1, "%s: rows of %s are %lld apart, below %u channels", op, name, (long long)r->ld, c);
+    if (r->ld < (int64_t)c)
+        return fail(-1, "%s: rows of %s are %lld apart, below %u channels", op, name, (long long)r->ld, c);
     if (!aligned(r->p, 2)) return fail(-1, "%s: %s is not aligned to its elements", op, name);
     return 0;
 }
@@ -220,7 +236,11 @@ struct Shape {  // a product's tiles and splits
 };
 // The tile whose workgroups, a round of 256 at a time, take the least: a medium tile's slab counts 100, a narrow one's 75
 // and a large one's 270 (of 50 and 400 by area: the wider the tile, the less LDS traffic a product). Where K may be split
-// and there are at most 128 medium tiles, it is split to one workgroup a CU, at least 8 slabs each.
+// and there are at most 128 medium tiles, it is split to one workgroup a CU, at least 8 slabs each. Training steps, us,
+// bf16, with narrow, medium, large tiles for every product that is not split, and by the rule:
+//   8192 x 2048, f 8192   4401  3074  2234  large throughout
+//   4096 x 1024, f 4096    546   470   629   458
+//   1024 x 1024, f 4096    150   143   202   141
 Shape shape_of(int64_t m, int64_t n, int64_t k, int segments, int pairs, bool glu, bool may_split) {
     Shape s{};
     const int unit = glu ? 2 : 1;

@@ -726,7 +726,15 @@ struct Plan {
 
 // One wave per column group walks kL steps at a time (one, for a single token) where that alone fills the chip or
 // there is little to split; else up to 8 waves share a chunk, and chunks are chained where the columns give fewer than
-// two workgroups a CU. v: the channels a lane takes; near: a wave's columns may run over sequences, since the offsets
+// two workgroups a CU. Measured, bf16, rows of 512 channels, us forward and a training step, at both sides of the lines:
+//   columns  steps   one wave   eight waves         columns  steps   eight waves in a stream   chained
+//   2^17        64    24   63     17   50           2^14       128    10   32                   13   35
+//              256    98  263     79  206                     1024    57  209                   37  129
+//   2^18        64    31   95     27  100           2^15       128    12   37                   15   41
+//              256   127  351    151  399                     1024    73  239                   68  240
+//   2^19        64    55  180     53  193                     4096   267  929                  255  897
+//              256   225  670    282  737           2^16      1024   138  363                  128  451
+// (2^18 columns of long sequences would be ahead with one wave, chains of few steps in a stream.) v: the channels a lane takes; near: a wave's columns may run over sequences, since the offsets
 // between them fit a lane's 32 bits; else each sequence starts a wave of its own.
 Plan plan_of(const fhc_glr_desc* g, bool backward, uint32_t v, bool near) {
     Plan p{};
@@ -773,8 +781,10 @@ int check_seq(const char* op, const char* name, const fhc_seq* s, const fhc_glr_
 int check_out(const char* op, const char* name, const fhc_seq* s, const fhc_glr_desc* g) {
     FHC_TRY(check_seq(op, name, s, g));
     // an output's elements are distinct addresses where its strides leave room for a row of channels
-    if (g->t > 1 && (uint64_t)std::llabs(s->ts) < g->d) return fail(-1, "%s: %s: steps %lld apart overlap", op, name, (long long)s->ts);
-    if (g->b > 1 && (uint64_t)std::llabs(s->bs) < g->d) return fail(-1, "%s: %s: sequences %lld apart overlap", op, name, (long long)s->bs);
+    if (g->t > 1 && (uint64_t)std::llabs(s->ts) < g->d)
+        return fail(-1, "%s: %s: steps %lld apart overlap", op, name, (long long)s->ts);
+    if (g->b > 1 && (uint64_t)std::llabs(s->bs) < g->d)
+        return fail(-1, "%s: %s: sequences %lld apart overlap", op, name, (long long)s->bs);
     return 0;
 }
 
@@ -858,7 +868,8 @@ int sum(const char* op, const In* part, uint64_t rows, uint32_t d, uint32_t row_
 
 template <bool BWD>
 int run(const char* op, const Plan& p, GlrArgs& a, uint32_t dtype, void* ws, hipStream_t s) {
-    if ((uint64_t)p.colblocks * p.nchunk >= 1ull << 31 || (uint64_t)a.b * p.groups >= 1ull << 31) return fail(-1, "%s: too many chunks", op);
+    if ((uint64_t)p.colblocks * p.nchunk >= 1ull << 31 || (uint64_t)a.b * p.groups >= 1ull << 31)
+        return fail(-1, "%s: too many chunks", op);
     FHC_TRY(check_grid(op, (uint64_t)p.colblocks * (p.chain ? p.nchunk : 1), p.w == 8 ? 512 : 256));
     FHC_TRY(check_grid(op, ceil_div(p.words, 256), 256));
     a.groups = p.groups, a.nchunk = p.nchunk, a.colblocks = p.colblocks, a.nstates = p.nstates;
@@ -957,7 +968,8 @@ extern "C" int fhc_glr_backward(const fhc_glr_desc* g, const fhc_seq* x, const f
         const Plan p = plan_for(g, true, {x, r, i, dy, dx, dr, di});
         FHC_TRY(check_workspace(op, workspace_of(p, true), ws, ws_bytes));
         GlrArgs a{};
-        a.x = col(x, g->dtype), a.r = col(r, g->dtype), a.i = col(i, g->dtype), a.dy = col(dy, g->dtype), a.dx = col(dx, g->dtype), a.dr = col(dr, g->dtype), a.di = col(di, g->dtype);
+        a.x = col(x, g->dtype), a.r = col(r, g->dtype), a.i = col(i, g->dtype), a.dy = col(dy, g->dtype);
+        a.dx = col(dx, g->dtype), a.dr = col(dr, g->dtype), a.di = col(di, g->dtype);
         a.lam = g->lam, a.lengths = g->lengths, a.states = const_cast<float*>(states), a.dht = dht, a.dh0 = dh0;
         a.b = g->b, a.t = g->t, a.d = g->d, a.rate = g->rate;
         char* w = static_cast<char*>(ws) + (p.agg_bytes + 255) / 256 * 256;

@@ -7,8 +7,10 @@
 // waves as it needs (up to 16) for wide ones.
 //
 // MI355X, where a large copy moves 5.0 TB/s: forward of 16384 x 4096 bf16 95 us (537 MB, 5.7 TB/s), of
-// 15009 x 1931 f16, whose rows lie at any 2-byte address, 51 (4.6). Backward of the former 174 us (805 MB, 4.6 TB/s; the first form, which did not have the next row's loads under way, 289), its closing
-// sums 10 us more.
+// 15009 x 1931 f16, whose rows lie at any 2-byte address, 51 (4.6). Backward of the former 174 us (805 MB, 4.6 TB/s; the
+// first form, which did not have the next row's loads under way, 289), its closing sums 10 us more. Two shapes are far
+// from that: above 8192 channels, 16 a thread, a backward pass spills 330 to 940 bytes a lane (4000 x 8192 bf16 105 us,
+// 4000 x 8200 325); and norm_sum walks groups 64 at a time (262144 x 128 bf16, backward, in 64 groups 95 us, in 4096 158).
 #include "seq_common.h"
 
 namespace fhc {
@@ -504,7 +506,8 @@ int check_desc(const char* op, const fhc_norm_desc* n) {
 int check_rows(const char* op, const char* name, const fhc_rows* r, const fhc_norm_desc* n, bool needed) {
     if (!r) return needed ? fail(-1, "%s: null %s", op, name) : 0;
     if (!r->p) return fail(-1, "%s: null pointer of %s", op, name);
-    if (r->ld < (int64_t)n->c) return fail(-1, "%s: rows of %s are %lld apart, below %u channels", op, name, (long long)r->ld, n->c);
+    if (r->ld < (int64_t)n->c)
+        return fail(-1, "%s: rows of %s are %lld apart, below %u channels", op, name, (long long)r->ld, n->c);
     if (!aligned(r->p, elem_bytes(n->dtype))) return fail(-1, "%s: %s is not aligned to its elements", op, name);
     return 0;
 }

@@ -39,8 +39,9 @@ class RecurrentBlock:
 
     def forward(self, x, u, state=None, gate1=None, gate2=None, lengths=None, train=False):
         """x, u [sequences, steps, c]: the residual stream and this block's normed input; state [sequences, c] f32 or
-        None (zeros); gate1, gate2 [sequences, c] or None. Returns (y, the next block's input, the state after the last
-        step), with train also what ``backward`` takes."""
+        None (zeros); gate1, gate2 [sequences, c] or None; lengths as in ``fhseq.glr``: past them the recurrence's output
+        is 0, and the rest of the block works on x and u there as on any row, so they have to be finite. Returns (y, the
+        next block's input, the state after the last step), with train also what ``backward`` takes."""
         p, (b, t, c) = self.p, x.shape
         xr, ur = x.reshape(-1, c), u.reshape(-1, c)
         v, r, i = ((ur @ p[k].t()).view(b, t, c) for k in PROJECTIONS)
