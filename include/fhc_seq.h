@@ -25,7 +25,8 @@ extern "C" {
 #define FHC_F32 2u
 
 /* Element (b, t, ch) of a sequence tensor at p[b * bs + t * ts + ch], strides in elements. A dense [b][t][d] tensor
- * has bs = t * d, ts = d; frames of feature maps, [t][pixels][d], have bs = d, ts = pixels * d. */
+ * has bs = t * d, ts = d; frames of feature maps, [t][pixels][d], have bs = d, ts = pixels * d. An input's elements may
+ * coincide (bs = 0: one sequence for all; windows that overlap), an output's may not. */
 typedef struct fhc_seq {
     void* p;
     int64_t bs, ts;
