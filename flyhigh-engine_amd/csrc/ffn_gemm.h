@@ -1,5 +1,6 @@
-// The matrix products of the gated feed-forward block (include/fhc_seq.h): one tiled kernel over 16-bit operands with
-// f32 accumulation, in the layouts and with the epilogues that the block's forward and backward passes need.
+// The matrix products of the gated feed-forward block and of the product with bias, activation and residual
+// (include/fhc_seq.h): one tiled kernel over 16-bit operands with f32 accumulation, in the layouts and with the epilogues
+// that their forward and backward passes need.
 //
 // out[m][n] = sum over k of A(m, k) B(n, k). An operand is stored either with k adjacent ("rows": A's row m at
 // a + m * ld) or with m (n) adjacent ("columns": A's column k at a + k * ld), so no product needs a transposed copy.
@@ -50,6 +51,7 @@ enum Epi {
     kPart,   // f32 partial sums of a split K
     kGlu,    // N counts gate and up rows: h = act(gate) * up, and both in f32 where they are kept
     kGrad,   // dh -> dL/dgate, dL/dup
+    kLinear,  // act(v + bias) + residual; v + bias in f32 too where it is kept (pre_g)
 };
 
 struct GemmArgs {
@@ -69,6 +71,8 @@ struct GemmArgs {
     float* part;           // [pair][split][m][ldpart]
     int64_t ldpart;
     uint32_t act;
+    const uint16_t *bias, *res;  // kLinear, either may be null
+    int64_t ldr;
 };
 
 // act(v) = v sigmoid(k(v)), k(v) = v (silu) or 2 sqrt(2 / pi) (v + 0.044715 v^3) (gelu, tanh form)
@@ -92,6 +96,28 @@ __device__ __forceinline__ void act_grad(uint32_t act, float v, float& value, fl
     const float q = __builtin_fminf(e * p, 1.0f);  // 1 - p; inf * 0 where e overflows
     value = v * p;
     slope = p * __builtin_fmaf(w * dk, q, 1.0f);
+}
+
+// What kLinear adds to a sum, for up to 4 adjacent columns: pre's rows are whole quads.
+struct Tail {
+    const uint16_t *bias, *res;
+    int64_t ldr;
+    float* pre;
+    int64_t ldpre;
+    uint32_t act;
+};
+template <class T>
+__device__ __forceinline__ void tail4(const Tail& e, int64_t row, int col, int valid, f4 v, uint16_t (&q)[4]) {
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+        if (e.bias && r < valid) v[r] += widen(T{}, e.bias[col + r]);
+    if (e.pre) *reinterpret_cast<f4*>(e.pre + row * e.ldpre + col) = v;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        float y = e.act == FHC_ACT_IDENTITY ? v[r] : act_of(e.act, v[r]);
+        if (e.res && r < valid) y += widen(T{}, e.res[row * e.ldr + col + r]);
+        q[r] = narrow(T{}, y);
+    }
 }
 
 // up to 8 elements at p, `valid` of them inside
@@ -185,6 +211,15 @@ __device__ __forceinline__ void put8(R rsrc, uint2 v, uint32_t at) {
 #endif
 }
 template <class R>
+__device__ __forceinline__ uint2 get8(R rsrc, uint32_t at) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const auto v = __builtin_amdgcn_raw_buffer_load_b64(rsrc, at, 0, 0);
+    return uint2{v[0], v[1]};
+#else
+    return uint2{};
+#endif
+}
+template <class R>
 __device__ __forceinline__ void put16(R rsrc, f4 v, uint32_t at) {
 #if defined(__HIP_DEVICE_COMPILE__)
     __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, v), rsrc, at, 0, 0);
@@ -195,6 +230,8 @@ template <int N>
 __device__ __forceinline__ void wait_vm() {
     __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);
 }
+
+namespace {  // a kernel of this unit: another one's is registered apart
 
 // WM x WN waves of 16 MB x 16 NB; GLU interleaves B's tile by waves: 8 NB gate rows, then the same features' up rows
 template <class T, bool AC, bool BC, Epi E, int MB, int NB, int WM, int WN>
@@ -433,6 +470,63 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ffn_gemm(GemmArgs g) {
                 }
             }
         }
+    } else if constexpr (E == kLinear) {
+        const Tail tail{g.bias, g.res, g.ldr, g.pre_g, g.ldpre, g.act};
+        if (g.quads) {
+            const auto ty = at_tile(g.o0, g.ldo), tr = at_tile(g.res ? g.res : g.o0, g.res ? g.ldr : g.ldo);
+            const auto tp = at_tile(g.pre_g, g.ldpre);
+            f4 bias[NB];
+#pragma unroll
+            for (int j = 0; j < NB; j++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    bias[j][r] = g.bias ? widen(T{}, g.bias[min(n0 + nr + j * 16 + r, g.n - 1)]) : 0.0f;
+            // the residual's next 16 rows are on their way while 16 rows are worked on (y may lie over it: an element is
+            // read before it is written, by the same lane)
+            uint2 rr[2][NB];
+            auto load = [&](int i) {
+#pragma unroll
+                for (int j = 0; j < NB; j++) rr[i & 1][j] = get8(tr, place(i, j, g.ldr, g.n, 2));
+            };
+            if (g.res) load(0);
+#pragma unroll
+            for (int i = 0; i < MB; i++) {
+                if (g.res && i + 1 < MB) load(i + 1);
+#pragma unroll
+                for (int j = 0; j < NB; j++) {
+                    f4 v = acc[i][j] + bias[j];
+                    if (g.pre_g) put16(tp, v, place(i, j, g.ldpre, (int)g.ldpre, 4));
+                    if (g.act != FHC_ACT_IDENTITY) {
+#pragma unroll
+                        for (int r = 0; r < 4; r++) v[r] = act_of(g.act, v[r]);
+                    }
+                    if (g.res) {
+                        const uint2 e = rr[i & 1][j];
+                        const uint16_t h[4] = {(uint16_t)e.x, (uint16_t)(e.x >> 16), (uint16_t)e.y, (uint16_t)(e.y >> 16)};
+#pragma unroll
+                        for (int r = 0; r < 4; r++) v[r] += widen(T{}, h[r]);
+                    }
+                    uint16_t q[4];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) q[r] = narrow(T{}, v[r]);
+                    put8(ty, pack(q), place(i, j, g.ldo, g.n, 2));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < MB; i++) {
+                const int m = m0 + mr + i * 16;
+                if (m >= g.m) continue;
+#pragma unroll
+                for (int j = 0; j < NB; j++) {
+                    const int n = n0 + nr + j * 16;
+                    if (n >= g.n) continue;
+                    uint16_t q[4];
+                    tail4<T>(tail, m, n, g.n - n, acc[i][j], q);
+                    store4(g.o0 + m * g.ldo + n, g.n - n, q);
+                }
+            }
+        }
     } else if constexpr (E == kPart) {
         const auto t = at_tile(g.part + (int64_t)(pair * g.splits + split) * g.m * g.ldpart, g.ldpart);
 #pragma unroll
@@ -469,5 +563,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ffn_gemm(GemmArgs g) {
     }
 }
 
+}  // namespace
 }  // namespace seq
 }  // namespace fhc

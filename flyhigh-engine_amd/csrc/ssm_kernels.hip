@@ -1,0 +1,879 @@
+// The selective state space scan (include/fhc_seq.h), forward and backward.
+//
+// A workgroup has 64 channels of one sequence and group, a lane one channel; its W waves share out the states, 4 or 8 of
+// them a wave, in registers. Time goes in tiles of 16 steps: the waves first prepare 16 / W steps each (D = softplus,
+// D x), which then lie in LDS for all of them; every wave runs its states through the 16 steps and leaves its part of
+// sum C h a step in LDS; the waves add the parts of their steps, apply skip and gate, and store. B and C are the same for
+// all lanes, and the f32 matrix unit's 4 x 4 x 1 blocks take them from four lanes of any block: one instruction is
+// B_t[0..3] D x + (a h)[0..3] for the four states of all 64 lanes, exact as fused multiply-adds are, and sum C h is four
+// more. The vector unit is left with a = exp2(D rate) and a h.
+//
+// Where the columns are too few for the chip, time is cut into segments: a first launch folds each to the state that it
+// leaves from zeros, and its sum of D (its decay is exp(a sum D), so one number a channel composes all of them); the
+// second launch starts each segment from the fold of those before it.
+//
+// Backward, with q = dy silu(z) and c the gradient that reaches a step's state from behind:
+//     g_t = C_t q_t + c,   c <- a_t g_t,   s1 = sum B g,   s2 = sum a[k] a_t h_(t-1) g
+//     dx = D s1 + skip q,   ddt = (s2 + x s1) sigmoid(dt + bias),   dz = dy p silu'(z)
+//     da[k] = sum of D a_t h_(t-1) g,   dB = sum over channels of D x g,   dC = sum over channels of q h
+// The forward pass keeps every tile's first state; a tile's 16 states and decays are computed again into registers and
+// walked backwards. The sums over a wave's 64 channels for dB and dC halve the values and the lanes at once, so that 8
+// values of 8 steps end one a lane; a closing launch adds the channel blocks, in their order.
+#include "seq_args.h"
+
+namespace fhc {
+namespace seq {
+namespace {
+
+constexpr int kTile = 16;
+typedef float f4 __attribute__((ext_vector_type(4)));
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+
+template <class R>
+struct SsmArgs {
+    Seq<R> x, dt, bm, cm, z, y, dy, dx, ddt, dz;
+    const float *a, *bias, *skip;
+    const int32_t* lengths;
+    const float* h0;
+    float* ht;
+    f4* states;    // [b][tile][quad][d]
+    const float* dht;
+    float* dh0;
+    f4* ends;     // segments: [segment + 1][b][quad][d], forward's slot 0 is h0
+    float* lasts;   // and their sums of D, [segment][b][d]
+    float* part;    // [segment][walk][d * n + 2 d]: da, dskip, ddt_bias
+    float* bc;      // [group and block][b][t][2][quad * 4]
+    uint32_t b, t, d, n, groups;
+    uint32_t width, blocks, quads;    // channels of a group, its blocks of 64, quads of states
+    uint32_t tiles, segs, seg_tiles;  // tiles of 16 steps; segments and theirs
+    uint32_t walks;                   // backward: workgroups that the sequences are dealt to
+};
+
+// softplus(v) = max(v, 0) + log1p(e), e = exp(-|v|): a polynomial of degree 9 in e for log1p(e) / e on [0, 1], the least
+// squares of its relative error, which is 5e-9 (and 1.1e-7 in f32): small steps keep their digits.
+__device__ __forceinline__ float softplus(float v, float& e) {
+    e = __builtin_amdgcn_exp2f(__builtin_fabsf(v) * -kLog2e);
+    float p = -0.0031640392262488604f;
+    p = __builtin_fmaf(p, e, 0.019487930461764336f);
+    p = __builtin_fmaf(p, e, -0.05627012997865677f);
+    p = __builtin_fmaf(p, e, 0.10533029586076736f);
+    p = __builtin_fmaf(p, e, -0.15263333916664124f);
+    p = __builtin_fmaf(p, e, 0.1966104507446289f);
+    p = __builtin_fmaf(p, e, -0.2495117485523224f);
+    p = __builtin_fmaf(p, e, 0.33329665660858154f);
+    p = __builtin_fmaf(p, e, -0.49999889731407166f);
+    p = __builtin_fmaf(p, e, 1.0f);
+    return __builtin_fmaf(p, e, v > 0.0f ? v : 0.0f);
+}
+// a state's rate for exp2, finite: times a step of 0 it is 0
+__device__ __forceinline__ float rate_of(float a) {
+    const float k = a * kLog2e;
+    return k < -3.4e38f ? -3.4e38f : k > 3.4e38f ? 3.4e38f : k;
+}
+
+// a's values in lanes 4 BLOCK + i times b, added to c[i]
+template <int BLOCK>
+__device__ __forceinline__ f4 outer(float a, float b, f4 c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_amdgcn_mfma_f32_4x4x1f32(a, b, c, 4, BLOCK, 0);
+#else
+    return c;
+#endif
+}
+// the sum of four lanes' values of v, the same in lanes 4 (BLOCK + k) + i for all i, times h[k]
+template <int BLOCK>
+__device__ __forceinline__ f4 inner(float v, f4 h, f4 c) {
+    c = outer<BLOCK>(v, h[0], c);
+    c = outer<BLOCK + 1>(v, h[1], c);
+    c = outer<BLOCK + 2>(v, h[2], c);
+    return outer<BLOCK + 3>(v, h[3], c);
+}
+__device__ __forceinline__ void fence() { asm volatile("" ::: "memory"); }
+
+// An address that all lanes share and a lane's own 32-bit offset from there: no vector arithmetic for an address.
+template <class R>
+__device__ __forceinline__ __attribute__((address_space(1))) R* place(R* p, uint32_t bytes) {
+    const uint64_t at = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)at);
+    const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
+    asm("" : "+v"(bytes));  // opaque: its extension to 64 bits stays here, where a load takes it for nothing
+    return (__attribute__((address_space(1))) R*)((__attribute__((address_space(1))) char*)((uint64_t)hi << 32 | lo) + bytes);
+}
+template <class F, int... I>
+__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+// f(0) .. f(N - 1) with constants for arguments
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f) {
+    each_of(f, std::make_integer_sequence<int, N>{});
+}
+
+// Where a workgroup is.
+struct Spot {
+    uint32_t seg, walk, group, block, ch;
+    bool live;
+    template <class R>
+    __device__ __forceinline__ Spot(const SsmArgs<R>& g, uint32_t lane) {
+        uint32_t q = blockIdx.x;
+        block = q % g.blocks, q /= g.blocks;
+        group = q % g.groups, q /= g.groups;
+        walk = q % g.walks, seg = q / g.walks;
+        const uint32_t at = block * 64 + lane;
+        live = at < g.width;
+        ch = group * g.width + (live ? at : g.width - 1);  // a lane without a channel repeats the last one's work
+    }
+};
+
+// A tile's B or C of one quad as a wave holds them. For outer products: lane l has step l / 4, state l % 4. For inner
+// ones: register j has steps 4 j .. 4 j + 3, lane l step l / 16, state l / 4 % 4.
+template <class R>
+__device__ __forceinline__ R load_outer(const Seq<R>& m, uint32_t b, uint32_t col, uint32_t states, uint32_t t0, uint32_t n,
+                                        uint32_t lane) {
+    const uint32_t t = t0 + (lane >> 2), k = lane & 3;
+    R v = R(0);
+    if (k < states && t < n) v = m.at(b, t)[col + k];
+    return v;
+}
+template <class R>
+__device__ __forceinline__ void load_inner(const Seq<R>& m, uint32_t b, uint32_t col, uint32_t states, uint32_t t0,
+                                           uint32_t n, uint32_t lane, R (&o)[4]) {
+    const uint32_t k = lane >> 2 & 3;
+    const R* p = m.at(b, t0 + (lane >> 4)) + (col + k);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        o[j] = R(0);
+        if (k < states && t0 + 4 * j + (lane >> 4) < n) o[j] = *p;
+        p += 4 * m.ts;
+    }
+}
+
+// the states of quad q of a [b][d][n] tensor
+__device__ __forceinline__ f4 load_states(const float* p, uint64_t at, uint32_t n, uint32_t q) {
+    f4 h;
+#pragma unroll
+    for (int k = 0; k < 4; k++) h[k] = p && 4 * q + k < n ? p[at * n + 4 * q + k] : 0.0f;
+    return h;
+}
+__device__ __forceinline__ void store_states(float* p, uint64_t at, uint32_t n, uint32_t q, f4 h) {
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+        if (4 * q + k < n) p[at * n + 4 * q + k] = h[k];
+}
+__device__ __forceinline__ f4 rates_of(const float* a, uint32_t ch, uint32_t n, uint32_t q) {
+    f4 h = load_states(a, ch, n, q);
+#pragma unroll
+    for (int k = 0; k < 4; k++) h[k] = rate_of(h[k]);
+    return h;
+}
+__device__ __forceinline__ f4 decay(float step, f4 rate) {
+    f4 a;
+#pragma unroll
+    for (int k = 0; k < 4; k++) a[k] = __builtin_amdgcn_exp2f(step * rate[k]);
+    return a;
+}
+__device__ __forceinline__ f4 fma4(f4 a, f4 b, f4 c) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) c[k] = __builtin_fmaf(a[k], b[k], c[k]);
+    return c;
+}
+
+// W waves, NQ quads of states each. FOLD: the segments' ends from zeros.
+template <class T, int W, int NQ, bool FOLD>
+__global__ __launch_bounds__(64 * W, 2) void ssm_fwd(SsmArgs<typename T::Raw> g) {
+    using R = typename T::Raw;
+    constexpr int K = kTile / W;  // steps that a wave prepares: j * W + wave
+    __shared__ float2 steps[kTile][64];
+    __shared__ float parts[FOLD ? 1 : W][kTile][64];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Spot at(g, lane);
+    const uint32_t b = at.walk, ch = at.ch, own = ch * (uint32_t)sizeof(R);
+    const uint64_t flat = (uint64_t)b * g.d + ch, slots = (uint64_t)g.b * g.quads * g.d;
+    const uint32_t n = g.lengths ? (uint32_t)min(max(g.lengths[b], 0), (int32_t)g.t) : g.t;
+    const uint32_t first = at.seg * g.seg_tiles, last = min(first + g.seg_tiles, g.tiles);
+    const uint32_t busy = min(last, (n + kTile - 1) / kTile);
+    const float bias = g.bias ? g.bias[ch] : 0.0f, skip = g.skip ? g.skip[ch] : 0.0f;
+    f4 rate[NQ], h[NQ];
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NQ; i++) {
+        const uint32_t q = wave + W * i;
+        const uint64_t slot = ((uint64_t)b * g.quads + q) * g.d + ch;
+        rate[i] = rates_of(g.a, ch, g.n, q);
+        h[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (FOLD || g.segs == 1) {
+            h[i] = load_states(g.h0, flat, g.n, q);
+        } else if (q < g.quads) {
+            h[i] = g.ends[slot];
+            for (uint32_t s = 0; s < at.seg; s++)
+                h[i] = fma4(decay(g.lasts[(uint64_t)s * g.b * g.d + flat], rate[i]), h[i], g.ends[(s + 1) * slots + slot]);
+        }
+        if constexpr (FOLD) {  // the second launch reads the first state here: the last one may lie over h0
+            if (at.seg == 0 && q < g.quads && at.live) g.ends[slot] = h[i];
+            h[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+    R x[K], dt[K], z[K], bo[NQ], ci[NQ][4];
+    auto load = [&](uint32_t tile) {
+#pragma unroll
+        for (int j = 0; j < K; j++) {
+            const uint32_t t = tile * kTile + j * W + wave;
+            x[j] = dt[j] = z[j] = R(0);
+            if (t < n) {
+                x[j] = *place(g.x.at(b, t), own), dt[j] = *place(g.dt.at(b, t), own);
+                if (!FOLD && g.z.p) z[j] = *place(g.z.at(b, t), own);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+            const uint32_t q = wave + W * i, states = g.n > 4 * q ? g.n - 4 * q : 0, col = at.group * g.n + 4 * q;
+            bo[i] = load_outer(g.bm, b, col, states, tile * kTile, n, lane);
+            if (!FOLD) load_inner(g.cm, b, col, states, tile * kTile, n, lane, ci[i]);
+        }
+    };
+    if (first < busy) load(first);
+    for (uint32_t tile = first; tile < busy; tile++) {
+        float xs[K], zs[K], bv[NQ], cv[NQ][4];
+#pragma unroll
+        for (int j = 0; j < K; j++) {
+            const uint32_t s = j * W + wave;
+            float e;
+            const float step = tile * kTile + s < n ? softplus(widen(T{}, dt[j]) + bias, e) : 0.0f;
+            xs[j] = widen(T{}, x[j]), zs[j] = widen(T{}, z[j]);
+            steps[s][lane] = float2{step, step * xs[j]};
+        }
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+            bv[i] = widen(T{}, bo[i]);
+#pragma unroll
+            for (int j = 0; j < 4 && !FOLD; j++) cv[i][j] = widen(T{}, ci[i][j]);
+        }
+        __syncthreads();
+        if (tile + 1 < busy) load(tile + 1);
+        if (!FOLD && g.states && at.live) {
+#pragma unroll
+            for (int i = 0; i < NQ; i++)
+                if (wave + W * i < g.quads)
+                    g.states[(((uint64_t)b * g.tiles + tile) * g.quads + wave + W * i) * g.d + ch] = h[i];
+        }
+        each<kTile>([&](auto c) {
+            constexpr int s = c;
+            const float2 st = steps[s][lane];
+            if constexpr (FOLD) sum += st.x;
+            f4 p = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < NQ; i++) {
+                h[i] = outer<s>(bv[i], st.y, decay(st.x, rate[i]) * h[i]);
+                if constexpr (!FOLD) p = inner<(s & 3) * 4>(cv[i][s >> 2], h[i], p);
+            }
+            if constexpr (!FOLD) parts[wave][s][lane] = p[0];
+        });
+        __syncthreads();
+        if constexpr (!FOLD) {
+#pragma unroll
+            for (int j = 0; j < K; j++) {
+                const uint32_t s = j * W + wave, t = tile * kTile + s;
+                float p = skip * xs[j];
+#pragma unroll
+                for (int w = 0; w < W; w++) p += parts[w][s][lane];
+                if (g.z.p) p *= zs[j] * sigmoid1(zs[j]);
+                if (t < g.t && at.live) *place(g.y.at(b, t), own) = t < n ? narrow(T{}, p) : R(0);
+            }
+        }
+    }
+    if constexpr (FOLD) {
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+            const uint32_t q = wave + W * i;
+            if (q < g.quads && at.live) g.ends[(at.seg + 1) * slots + ((uint64_t)b * g.quads + q) * g.d + ch] = h[i];
+        }
+        if (wave == 0 && at.live) g.lasts[(uint64_t)at.seg * g.b * g.d + flat] = sum;
+    } else {
+        for (uint32_t t = max(busy, first) * kTile + wave; t < min(last * kTile, g.t); t += W)
+            if (at.live) *place(g.y.at(b, t), own) = R(0);
+        if (g.ht && at.live && last == g.tiles) {
+#pragma unroll
+            for (int i = 0; i < NQ; i++) store_states(g.ht, flat, g.n, wave + W * i, h[i]);
+        }
+    }
+}
+
+// Few steps: a thread has one quad of one channel's states, LP threads side by side a channel, so a wave reads and writes
+// the states as they lie; the steps follow one another.
+template <class T, int LP>
+__global__ __launch_bounds__(256) void ssm_step(SsmArgs<typename T::Raw> g) {
+    using R = typename T::Raw;
+    const uint64_t all = (uint64_t)g.b * g.d * LP;
+    for (uint64_t k = (uint64_t)blockIdx.x * 256 + threadIdx.x; k < (all + 255) / 256 * 256; k += (uint64_t)gridDim.x * 256) {
+        const bool live = k < all;
+        const uint32_t q = k % LP, flat = live ? (uint32_t)(k / LP) : 0, b = flat / g.d, ch = flat - b * g.d;
+        const uint32_t col = ch / g.width * g.n + 4 * q, n = g.lengths ? (uint32_t)min(max(g.lengths[b], 0), (int32_t)g.t) : g.t;
+        const bool has = live && 4 * q < g.n;
+        const f4 rate = rates_of(has ? g.a : nullptr, ch, g.n, q);
+        f4 h = load_states(has ? g.h0 : nullptr, flat, g.n, q);
+        const float bias = g.bias ? g.bias[ch] : 0.0f, skip = g.skip ? g.skip[ch] : 0.0f;
+        for (uint32_t t = 0; t < g.t; t++) {
+            if (g.states && has && t % kTile == 0)
+                g.states[(((uint64_t)b * g.tiles + t / kTile) * g.quads + q) * g.d + ch] = h;
+            float p = 0.0f, x = 0.0f;
+            if (t < n) {
+                float e;
+                x = widen(T{}, g.x.at(b, t)[ch]);
+                const float step = softplus(widen(T{}, g.dt.at(b, t)[ch]) + bias, e), u = step * x;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float bv = 0.0f, cv = 0.0f;
+                    if (has && 4 * q + i < g.n) {
+                        bv = widen(T{}, g.bm.at(b, t)[col + i]);
+                        cv = widen(T{}, g.cm.at(b, t)[col + i]);
+                    }
+                    h[i] = __builtin_fmaf(bv, u, __builtin_amdgcn_exp2f(step * rate[i]) * h[i]);
+                    p = __builtin_fmaf(cv, h[i], p);
+                }
+            }
+#pragma unroll
+            for (int m = 1; m < LP; m *= 2) p += __shfl_xor(p, m);
+            if (live && q == 0) {
+                p = __builtin_fmaf(skip, x, p);
+                if (g.z.p && t < n) {
+                    const float z = widen(T{}, g.z.at(b, t)[ch]);
+                    p *= z * sigmoid1(z);
+                }
+                g.y.at(b, t)[ch] = t < n ? narrow(T{}, p) : R(0);
+            }
+        }
+        if (has && g.ht) store_states(g.ht, flat, g.n, q, h);
+    }
+}
+
+// The sum of two values over pairs of lanes, one kept in either lane: of a where the lane's bit is 0, of b where it is 1.
+__device__ __forceinline__ float merge32(float a, float b) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
+    const uint32_t p = r[0], q = r[1];  // (a cast of a vector's element itself takes the first one's bits for every index)
+    return __builtin_bit_cast(float, p) + __builtin_bit_cast(float, q);
+#else
+    return a + b;
+#endif
+}
+__device__ __forceinline__ float merge16(float a, float b) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
+    const uint32_t p = r[0], q = r[1];  // (a cast of a vector's element itself takes the first one's bits for every index)
+    return __builtin_bit_cast(float, p) + __builtin_bit_cast(float, q);
+#else
+    return a + b;
+#endif
+}
+// CTRL pairs lanes that differ in the bit (row_ror:8, row_half_mirror, quad_perm)
+template <int CTRL>
+__device__ __forceinline__ float merge_row(float a, float b, bool bit) {
+    const float keep = bit ? b : a, send = bit ? a : b;
+#if defined(__HIP_DEVICE_COMPILE__)
+    const int i = __builtin_bit_cast(int, send);
+    return keep + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, CTRL, 0xF, 0xF, true));
+#else
+    return keep + send;
+#endif
+}
+constexpr int kRor8 = 0x128, kHalfMirror = 0x141, kSwap2 = 0x4E, kSwap1 = 0xB1;
+
+// FOLD: the gradients that reach the states before a segment, from zeros behind it
+template <class T, int W, int NQ, bool FOLD>
+__global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void ssm_bwd(SsmArgs<typename T::Raw> g) {
+    using R = typename T::Raw;
+    constexpr int K = kTile / W;
+    __shared__ float2 steps[kTile][64];                  // D, D x
+    __shared__ float ups[kTile][64];                     // q
+    __shared__ float parts[FOLD ? 1 : 3][W][kTile][64];  // sum C h, s1, s2 of a wave's states
+    __shared__ float vectors[FOLD ? 1 : kTile][2][W * NQ * 4];  // dB, dC over the workgroup's channels
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Spot at(g, lane);
+    const uint32_t ch = at.ch, own = ch * (uint32_t)sizeof(R);
+    const uint32_t first = at.seg * g.seg_tiles, last = min(first + g.seg_tiles, g.tiles);
+    const uint64_t slots = (uint64_t)g.b * g.quads * g.d;
+    const float bias = g.bias ? g.bias[ch] : 0.0f, skip = g.skip ? g.skip[ch] : 0.0f;
+    f4 rate[NQ], da[NQ];
+    float dskip = 0.0f, dbias = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NQ; i++) {
+        rate[i] = rates_of(g.a, ch, g.n, wave + W * i);
+        da[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    for (uint32_t b = at.walk; b < g.b; b += g.walks) {
+        const uint64_t flat = (uint64_t)b * g.d + ch;
+        const uint32_t n = g.lengths ? (uint32_t)min(max(g.lengths[b], 0), (int32_t)g.t) : g.t;
+        const uint32_t busy = min(last, (n + kTile - 1) / kTile);
+        f4 c[NQ];
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+            const uint32_t q = wave + W * i;
+            const uint64_t slot = ((uint64_t)b * g.quads + q) * g.d + ch;
+            c[i] = load_states(FOLD || !at.live ? nullptr : g.dht, flat, g.n, q);
+            if (!FOLD && q < g.quads && at.live) {
+                for (uint32_t s = g.segs - 1; s > at.seg; s--)
+                    c[i] = fma4(decay(g.lasts[(uint64_t)s * g.b * g.d + flat], rate[i]), c[i], g.ends[s * slots + slot]);
+            }
+        }
+        R x[K], dt[K], z[K], dy[K], bo[NQ], co[NQ], bi[NQ][4], ci[NQ][4];
+        f4 start[NQ];
+        auto load = [&](uint32_t tile) {
+#pragma unroll
+            for (int j = 0; j < K; j++) {
+                const uint32_t t = tile * kTile + j * W + wave;
+                x[j] = dt[j] = z[j] = dy[j] = R(0);
+                if (t < n) {
+                    if (!FOLD) x[j] = *place(g.x.at(b, t), own);
+                    dt[j] = *place(g.dt.at(b, t), own), dy[j] = *place(g.dy.at(b, t), own);
+                    if (g.z.p) z[j] = *place(g.z.at(b, t), own);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NQ; i++) {
+                const uint32_t q = wave + W * i, states = g.n > 4 * q ? g.n - 4 * q : 0, col = at.group * g.n + 4 * q;
+                co[i] = load_outer(g.cm, b, col, states, tile * kTile, n, lane);
+                if constexpr (!FOLD) {
+                    bo[i] = load_outer(g.bm, b, col, states, tile * kTile, n, lane);
+                    load_inner(g.bm, b, col, states, tile * kTile, n, lane, bi[i]);
+                    load_inner(g.cm, b, col, states, tile * kTile, n, lane, ci[i]);
+                    start[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+                    if (q < g.quads && at.live) start[i] = g.states[(((uint64_t)b * g.tiles + tile) * g.quads + q) * g.d + ch];
+                }
+            }
+        };
+        if (first < busy) load(busy - 1);
+        for (uint32_t left = busy; left > first; left--) {
+            const uint32_t tile = left - 1;
+            float xs[K], slope[K], zg[K], bv[NQ], cv[NQ], bw[NQ][4], cw[NQ][4];  // the step's slope; dy silu'(z)
+#pragma unroll
+            for (int j = 0; j < K; j++) {
+                const uint32_t s = j * W + wave;
+                const bool on = tile * kTile + s < n && at.live;  // a lane without a channel adds nothing to dB and dC
+                const float v = widen(T{}, dt[j]) + bias, up = widen(T{}, dy[j]);
+                float e, gate = 1.0f, dgate = 0.0f;
+                const float d = softplus(v, e), step = on ? d : 0.0f;
+                if (g.z.p) silu_grad(widen(T{}, z[j]), gate, dgate);
+                if constexpr (!FOLD) {
+                    const float r = __builtin_amdgcn_rcpf(1.0f + e);
+                    xs[j] = widen(T{}, x[j]), slope[j] = v >= 0.0f ? r : e * r, zg[j] = up * dgate;
+                }
+                steps[s][lane] = float2{step, FOLD ? 0.0f : step * xs[j]};
+                ups[s][lane] = on ? up * gate : 0.0f;
+            }
+            f4 h0[NQ];
+#pragma unroll
+            for (int i = 0; i < NQ; i++) {
+                cv[i] = widen(T{}, co[i]);
+                if constexpr (!FOLD) {
+                    bv[i] = widen(T{}, bo[i]), h0[i] = start[i];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) bw[i][j] = widen(T{}, bi[i][j]), cw[i][j] = widen(T{}, ci[i][j]);
+                }
+            }
+            __syncthreads();
+            if (tile > first) load(tile - 1);
+            if constexpr (FOLD) {
+                each<kTile>([&](auto sc) {
+                    constexpr int s = kTile - 1 - sc;
+                    const float step = steps[s][lane].x, q = ups[s][lane];
+                    sum += step;
+#pragma unroll
+                    for (int i = 0; i < NQ; i++) c[i] = decay(step, rate[i]) * outer<s>(cv[i], q, c[i]);
+                });
+            } else {
+#pragma unroll
+                for (int i = 0; i < NQ; i++) {
+                    f4 h[kTile], a[kTile];
+                    each<4>([&](auto mc) {  // four steps' LDS reads at once, no more: registers
+                        constexpr int m = mc;
+                        float2 st[4];
+#pragma unroll
+                        for (int r = 0; r < 4; r++) st[r] = steps[4 * m + r][lane];
+                        fence();
+                        each<4>([&](auto rc) {
+                            constexpr int s = 4 * m + rc;
+                            a[s] = decay(st[rc].x, rate[i]);
+                            h[s] = outer<s>(bv[i], st[rc].y, a[s] * (s ? h[s ? s - 1 : 0] : h0[i]));
+                        });
+                    });
+                    float m4 = 0.0f, m2 = 0.0f, m1 = 0.0f;  // sums of odd steps that wait for their even neighbours
+                    each<4>([&](auto mc) {
+                        constexpr int m = 3 - mc;
+                        float2 st[4];
+                        float q[4];
+#pragma unroll
+                        for (int r = 0; r < 4; r++) st[r] = steps[4 * m + r][lane], q[r] = ups[4 * m + r][lane];
+                        fence();
+                        each<4>([&](auto rc) {
+                            constexpr int r = 3 - rc, s = 4 * m + r;
+                            const f4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+                            const f4 grad = outer<s>(cv[i], q[r], c[i]);
+                            float p = inner<r * 4>(cw[i][m], h[s], none)[0], s1 = inner<r * 4>(bw[i][m], grad, none)[0];
+                            const f4 db = grad * st[r].y, dc = h[s] * q[r];
+                            c[i] = grad * a[s];
+                            const f4 past = c[i] * (s ? h[s ? s - 1 : 0] : h0[i]);
+                            float s2 = 0.0f;
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                da[i][k] = __builtin_fmaf(past[k], st[r].x, da[i][k]);
+                                s2 = __builtin_fmaf(past[k], rate[i][k], s2);
+                            }
+                            if (i > 0) {
+                                p += parts[0][wave][s][lane], s1 += parts[1][wave][s][lane];
+                                s2 += parts[2][wave][s][lane];
+                            }
+                            parts[0][wave][s][lane] = p, parts[1][wave][s][lane] = s1, parts[2][wave][s][lane] = s2;
+                            // lanes 32 up take dC; bits 4 and 3 of the lane are the state's, then bit 2 the step's lowest,
+                            // bit 1 the next and bit 0 the third
+                            const float r0 = merge16(merge32(db[0], dc[0]), merge32(db[2], dc[2]));
+                            const float r1 = merge16(merge32(db[1], dc[1]), merge32(db[3], dc[3]));
+                            float v = merge_row<kRor8>(r0, r1, lane & 8);
+                            if constexpr ((s & 1) == 1) {
+                                m4 = v;
+                            } else {
+                                v = merge_row<kHalfMirror>(v, m4, lane & 4);
+                                if constexpr ((s & 2) == 2) {
+                                    m2 = v;
+                                } else {
+                                    v = merge_row<kSwap2>(v, m2, lane & 2);
+                                    if constexpr ((s & 4) == 4) {
+                                        m1 = v;
+                                    } else {
+                                        v = merge_row<kSwap1>(v, m1, lane & 1);
+                                        const uint32_t step = s + ((lane >> 2 & 1) | (lane & 2) | (lane & 1) << 2);
+                                        const uint32_t k = (lane >> 3 & 1) | (lane >> 3 & 2);
+                                        vectors[step][lane >> 5][(wave + W * i) * 4 + k] = v;
+                                    }
+                                }
+                            }
+                        });
+                    });
+                }
+            }
+            __syncthreads();
+            if constexpr (!FOLD) {
+#pragma unroll
+                for (int j = 0; j < K; j++) {
+                    const uint32_t s = j * W + wave, t = tile * kTile + s;
+                    float p = 0.0f, s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < W; w++) p += parts[0][w][s][lane], s1 += parts[1][w][s][lane], s2 += parts[2][w][s][lane];
+                    const float step = steps[s][lane].x, q = ups[s][lane];
+                    const float dd = __builtin_fmaf(xs[j], s1, s2 * kLn2) * slope[j];
+                    if (t < n) dskip = __builtin_fmaf(q, xs[j], dskip), dbias += dd;
+                    if (t < g.t && at.live) {
+                        *place(g.dx.at(b, t), own) = t < n ? narrow(T{}, __builtin_fmaf(step, s1, skip * q)) : R(0);
+                        *place(g.ddt.at(b, t), own) = t < n ? narrow(T{}, dd) : R(0);
+                        if (g.z.p)
+                            *place(g.dz.at(b, t), own) = t < n ? narrow(T{}, zg[j] * __builtin_fmaf(skip, xs[j], p)) : R(0);
+                    }
+                }
+                // the tile's dB and dC of this block, as they lie
+                const uint32_t row = 8 * g.quads, steps_here = min((uint32_t)kTile, g.t - tile * kTile);
+                float* to = g.bc + (((uint64_t)(at.group * g.blocks + at.block) * g.b + b) * g.t + tile * kTile) * row;
+                for (uint32_t k = threadIdx.x; k < steps_here * row; k += 64 * W) {
+                    const uint32_t s = k / row, v = k - s * row, half = v >= 4 * g.quads;
+                    to[k] = vectors[s][half][v - half * 4 * g.quads];
+                }
+                __syncthreads();
+            }
+        }
+        if constexpr (FOLD) {
+#pragma unroll
+            for (int i = 0; i < NQ; i++) {
+                const uint32_t q = wave + W * i;
+                if (q < g.quads && at.live) g.ends[at.seg * slots + ((uint64_t)b * g.quads + q) * g.d + ch] = c[i];
+            }
+            if (wave == 0 && at.live) g.lasts[(uint64_t)at.seg * g.b * g.d + flat] = sum;
+        } else {
+            for (uint32_t t = max(busy, first) * kTile + wave; t < min(last * kTile, g.t); t += W) {
+                if (!at.live) continue;
+                *place(g.dx.at(b, t), own) = *place(g.ddt.at(b, t), own) = R(0);
+                if (g.z.p) *place(g.dz.at(b, t), own) = R(0);
+            }
+            if (g.dh0 && at.live && at.seg == 0) {
+#pragma unroll
+                for (int i = 0; i < NQ; i++) store_states(g.dh0, flat, g.n, wave + W * i, c[i]);
+            }
+        }
+    }
+    if constexpr (!FOLD) {
+        float* part = g.part + ((uint64_t)at.seg * g.walks + at.walk) * g.d * (g.n + 2);
+        if (at.live) {
+#pragma unroll
+            for (int i = 0; i < NQ; i++) store_states(part, ch, g.n, wave + W * i, da[i]);
+        }
+        __syncthreads();
+        parts[0][wave][0][lane] = dskip, parts[1][wave][0][lane] = dbias;
+        __syncthreads();
+        if (wave == 0 && at.live) {
+            float s = 0.0f, u = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; w++) s += parts[0][w][0][lane], u += parts[1][w][0][lane];
+            part[(uint64_t)g.d * g.n + ch] = s, part[(uint64_t)g.d * (g.n + 1) + ch] = u;
+        }
+    }
+}
+
+// dB and dC from the channel blocks' sums, those past a length 0
+template <class R>
+struct VectorArgs {
+    const float* bc;
+    Seq<R> dbm, dcm;
+    const int32_t* lengths;
+    uint32_t b, t, n, groups, blocks, quads;
+};
+template <class T>
+__global__ __launch_bounds__(256) void ssm_vectors(VectorArgs<typename T::Raw> g) {
+    const uint64_t rows = (uint64_t)g.b * g.t, all = rows * g.groups * 2 * g.n;
+    for (uint64_t k = (uint64_t)blockIdx.x * 256 + threadIdx.x; k < all; k += (uint64_t)gridDim.x * 256) {
+        const uint32_t v = k % g.n;
+        uint64_t q = k / g.n;
+        const uint32_t half = q & 1;
+        q >>= 1;
+        const uint64_t row = q % rows;
+        const uint32_t group = (uint32_t)(q / rows), b = (uint32_t)(row / g.t), t = (uint32_t)(row - (uint64_t)b * g.t);
+        const uint32_t n = g.lengths ? (uint32_t)min(max(g.lengths[b], 0), (int32_t)g.t) : g.t;
+        float sum = 0.0f;
+        if (t < n) {
+            const float* p = g.bc + ((uint64_t)group * g.blocks * rows + row) * 8 * g.quads + half * 4 * g.quads + v;
+#pragma unroll 4
+            for (uint32_t i = 0; i < g.blocks; i++) sum += p[i * rows * 8 * g.quads];
+        }
+        (half ? g.dcm : g.dbm).at(b, t)[group * g.n + v] = narrow(T{}, sum);
+    }
+}
+
+// ---- host side ----------------------------------------------------------------------------------------------------
+
+template <class T>
+int close_vectors(const char* op, const fhc_ssm_desc* g, const float* bc, const fhc_seq* dbm, const fhc_seq* dcm,
+                  uint32_t blocks, hipStream_t st) {
+    using R = typename T::Raw;
+    const uint64_t all = (uint64_t)g->b * g->t * g->groups * 2 * g->n;
+    if (!all) return 0;
+    const VectorArgs<R> v{bc, seq_of<R>(dbm), seq_of<R>(dcm), g->lengths, g->b, g->t, g->n, g->groups, blocks,
+                          (g->n + 3) / 4};
+    const uint64_t wgs = ceil_div(all, 256);
+    hipLaunchKernelGGL((ssm_vectors<T>), dim3((uint32_t)(wgs < 1u << 16 ? wgs : 1u << 16)), dim3(256), 0, st, v);
+    return launched(op);
+}
+
+constexpr uint32_t kFewSteps = 4;  // up to here the states' bytes are what counts
+
+struct Plan {
+    uint32_t width, blocks, quads, waves, tiles, segs, seg_tiles, walks;
+    uint64_t wgs;
+    size_t ends_bytes, lasts_bytes, part_bytes, bc_bytes;
+};
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+Plan plan_of(const fhc_ssm_desc* g, bool backward) {
+    Plan p{};
+    p.width = g->d / g->groups, p.blocks = (uint32_t)ceil_div(p.width, 64), p.quads = (g->n + 3) / 4;
+    p.waves = p.quads <= 1 ? 1 : p.quads <= 2 ? 2 : p.quads <= 4 ? 4 : 8;
+    p.tiles = (uint32_t)ceil_div(g->t, kTile);
+    const uint64_t cols = (uint64_t)g->groups * p.blocks;
+    const uint64_t one = g->b * cols;
+    p.segs = 1;
+    if (one < 256 && p.tiles >= 8) {
+        const uint64_t want = 1024 / one;
+        p.segs = (uint32_t)(want < p.tiles / 4 ? want : p.tiles / 4);
+        if (p.segs > 64) p.segs = 64;
+        if (p.segs < 1) p.segs = 1;
+    }
+    p.seg_tiles = p.tiles ? (uint32_t)ceil_div(p.tiles, p.segs) : 1;
+    p.segs = p.tiles ? (uint32_t)ceil_div(p.tiles, p.seg_tiles) : 1;
+    p.walks = g->b;
+    if (backward && one > 2048) {
+        const uint64_t w = ceil_div(2048, cols);
+        p.walks = (uint32_t)(w < g->b ? w : g->b);
+    }
+    p.wgs = p.walks * cols * p.segs;
+    const uint64_t flat = (uint64_t)g->b * g->d;
+    if (p.segs > 1) {
+        p.ends_bytes = up256((size_t)(p.segs + 1) * flat * p.quads * 16);
+        p.lasts_bytes = up256((size_t)p.segs * flat * 4);
+    }
+    if (backward) {
+        p.part_bytes = up256((size_t)p.segs * p.walks * g->d * (g->n + 2) * 4);
+        p.bc_bytes = up256((size_t)cols * g->b * g->t * 8 * p.quads * 4);
+    }
+    return p;
+}
+size_t workspace_of(const Plan& p) { return p.ends_bytes + p.lasts_bytes + p.part_bytes + p.bc_bytes; }
+
+int check_desc(const char* op, const fhc_ssm_desc* g) {
+    if (!g) return fail(-1, "%s: null descriptor", op);
+    FHC_TRY(check_shape(op, g->dtype, g->b, g->t, g->d));
+    if (g->n < 1 || g->n > 64) return fail(-1, "%s: %u states a channel, 1 to 64 are possible", op, g->n);
+    if (g->groups < 1 || g->d % g->groups) return fail(-1, "%s: %u groups of %u channels", op, g->groups, g->d);
+    FHC_TRY(check_array(op, "a", g->a, 4, g->b && g->d));
+    FHC_TRY(check_array(op, "dt_bias", g->dt_bias, 4, false));
+    FHC_TRY(check_array(op, "skip", g->skip, 4, false));
+    return check_array(op, "lengths", g->lengths, 4, false);
+}
+
+template <class T>
+SsmArgs<typename T::Raw> args_of(const fhc_ssm_desc* g, const Plan& p, const fhc_seq* x, const fhc_seq* dt,
+                                 const fhc_seq* bm, const fhc_seq* cm, const fhc_seq* z, void* ws) {
+    using R = typename T::Raw;
+    SsmArgs<R> a{};
+    a.x = seq_of<R>(x), a.dt = seq_of<R>(dt), a.bm = seq_of<R>(bm), a.cm = seq_of<R>(cm), a.z = seq_of<R>(z);
+    a.a = g->a, a.bias = g->dt_bias, a.skip = g->skip, a.lengths = g->lengths;
+    a.b = g->b, a.t = g->t, a.d = g->d, a.n = g->n, a.groups = g->groups;
+    a.width = p.width, a.blocks = p.blocks, a.quads = p.quads, a.tiles = p.tiles, a.segs = p.segs;
+    a.seg_tiles = p.seg_tiles, a.walks = p.walks;
+    char* w = static_cast<char*>(ws);
+    a.ends = reinterpret_cast<f4*>(w), w += p.ends_bytes;
+    a.lasts = reinterpret_cast<float*>(w), w += p.lasts_bytes;
+    a.part = reinterpret_cast<float*>(w), w += p.part_bytes;
+    a.bc = reinterpret_cast<float*>(w);
+    return a;
+}
+
+template <class T, bool BWD, bool FOLD>
+int launch(const char* op, const Plan& p, const SsmArgs<typename T::Raw>& a, hipStream_t st) {
+    const dim3 grid((uint32_t)p.wgs);
+#define SSM(W, NQ)                                                                                            \
+    do {                                                                                                      \
+        if constexpr (BWD) hipLaunchKernelGGL((ssm_bwd<T, W, NQ, FOLD>), grid, dim3(64 * W), 0, st, a);       \
+        else hipLaunchKernelGGL((ssm_fwd<T, W, NQ, FOLD>), grid, dim3(64 * W), 0, st, a);                     \
+    } while (0)
+    if (p.waves == 1) SSM(1, 1);
+    else if (p.waves == 2) SSM(2, 1);
+    else if (p.waves == 4) SSM(4, 1);
+    else if (p.quads <= 8) SSM(8, 1);
+    else SSM(8, 2);
+#undef SSM
+    return launched(op);
+}
+
+template <class T>
+int launch_step(const char* op, const Plan& p, const SsmArgs<typename T::Raw>& a, hipStream_t st) {
+    uint32_t lp = 1;
+    while (lp < p.quads) lp *= 2;
+    const uint64_t blocks = ceil_div((uint64_t)a.b * a.d * lp, 256);
+    const dim3 grid((uint32_t)(blocks < 1u << 22 ? blocks : 1u << 22));
+    if (lp == 1) hipLaunchKernelGGL((ssm_step<T, 1>), grid, dim3(256), 0, st, a);
+    else if (lp == 2) hipLaunchKernelGGL((ssm_step<T, 2>), grid, dim3(256), 0, st, a);
+    else if (lp == 4) hipLaunchKernelGGL((ssm_step<T, 4>), grid, dim3(256), 0, st, a);
+    else if (lp == 8) hipLaunchKernelGGL((ssm_step<T, 8>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((ssm_step<T, 16>), grid, dim3(256), 0, st, a);
+    return launched(op);
+}
+
+int check_inputs(const char* op, const fhc_ssm_desc* g, const Plan& p, const fhc_seq* x, const fhc_seq* dt,
+                 const fhc_seq* bm, const fhc_seq* cm, const fhc_seq* z) {
+    FHC_TRY(check_in(op, "x", x, g->dtype, g->t));
+    FHC_TRY(check_in(op, "dt", dt, g->dtype, g->t));
+    FHC_TRY(check_in(op, "bm", bm, g->dtype, g->t));
+    FHC_TRY(check_in(op, "cm", cm, g->dtype, g->t));
+    if (z) FHC_TRY(check_in(op, "z", z, g->dtype, g->t));
+    return check_grid(op, p.wgs, 64 * p.waves);
+}
+
+}  // namespace
+}  // namespace seq
+}  // namespace fhc
+
+using namespace fhc;
+using namespace fhc::seq;
+
+extern "C" size_t fhc_ssm_states_bytes(const fhc_ssm_desc* g) {
+    return guard((size_t)0, [&]() -> size_t {
+        clear_error();
+        if (check_desc("ssm_states_bytes", g) < 0) return 0;
+        return (size_t)g->b * ceil_div(g->t, kTile) * ((g->n + 3) / 4) * g->d * 16;
+    });
+}
+
+extern "C" size_t fhc_ssm_workspace_bytes(const fhc_ssm_desc* g, int backward) {
+    return guard((size_t)0, [&]() -> size_t {
+        clear_error();
+        if (check_desc("ssm_workspace_bytes", g) < 0 || (uint64_t)g->b * g->d == 0) return 0;
+        return workspace_of(plan_of(g, backward != 0));
+    });
+}
+
+extern "C" int fhc_ssm_forward(const fhc_ssm_desc* g, const fhc_seq* x, const fhc_seq* dt, const fhc_seq* bm,
+                               const fhc_seq* cm, const fhc_seq* z, const float* h0, const fhc_seq* y, float* ht,
+                               float* states, void* ws, size_t ws_bytes, void* stream) {
+    return guard(-3, [&]() -> int {
+        clear_error();
+        const char* op = "ssm_forward";
+        FHC_TRY(check_desc(op, g));
+        if ((uint64_t)g->b * g->d == 0) return 0;
+        const Plan p = plan_of(g, false);
+        FHC_TRY(check_inputs(op, g, p, x, dt, bm, cm, z));
+        FHC_TRY(check_out(op, "y", y, g->dtype, g->b, g->t, g->d));
+        FHC_TRY(check_array(op, "h0", h0, 4, false));
+        FHC_TRY(check_array(op, "ht", ht, 4, false));
+        if (!aligned(states, 256)) return fail(-1, "%s: states is not 256-byte aligned", op);
+        FHC_TRY(check_workspace(op, workspace_of(p), ws, ws_bytes));
+        const hipStream_t st = (hipStream_t)stream;
+        int rc = 0;
+        with_type(g->dtype, [&](auto t) {
+            using T = decltype(t);
+            auto a = args_of<T>(g, p, x, dt, bm, cm, z, ws);
+            a.h0 = h0, a.y = seq_of<typename T::Raw>(y), a.ht = ht, a.states = reinterpret_cast<f4*>(states);
+            if (g->t <= kFewSteps) {
+                rc = launch_step<T>(op, p, a, st);
+                return;
+            }
+            if (p.segs > 1) rc = launch<T, false, true>(op, p, a, st);
+            if (rc == 0) rc = launch<T, false, false>(op, p, a, st);
+        });
+        return rc;
+    });
+}
+
+extern "C" int fhc_ssm_backward(const fhc_ssm_desc* g, const fhc_seq* x, const fhc_seq* dt, const fhc_seq* bm,
+                                const fhc_seq* cm, const fhc_seq* z, const float* states, const fhc_seq* dy,
+                                const float* dht, const fhc_seq* dx, const fhc_seq* ddt, const fhc_seq* dbm,
+                                const fhc_seq* dcm, const fhc_seq* dz, float* da, float* ddt_bias, float* dskip,
+                                float* dh0, void* ws, size_t ws_bytes, void* stream) {
+    return guard(-3, [&]() -> int {
+        clear_error();
+        const char* op = "ssm_backward";
+        FHC_TRY(check_desc(op, g));
+        const hipStream_t st = (hipStream_t)stream;
+        FHC_TRY(check_array(op, "da", da, 4, false));
+        FHC_TRY(check_array(op, "ddt_bias", ddt_bias, 4, false));
+        FHC_TRY(check_array(op, "dskip", dskip, 4, false));
+        FHC_TRY(check_array(op, "dh0", dh0, 4, false));
+        FHC_TRY(check_array(op, "dht", dht, 4, false));
+        const Sums sums{{da, dskip, ddt_bias}, {(uint64_t)g->d * g->n, g->d, g->d}};
+        if (g->b == 0) return close_sums(op, nullptr, 0, sums, st);  // empty ones
+        FHC_TRY(check_out(op, "dbm", dbm, g->dtype, g->b, g->t, g->groups * g->n));
+        FHC_TRY(check_out(op, "dcm", dcm, g->dtype, g->b, g->t, g->groups * g->n));
+        int rc = 0;
+        if (g->d == 0) {  // no channels that B and C act on
+            with_type(g->dtype, [&](auto t) { rc = close_vectors<decltype(t)>(op, g, nullptr, dbm, dcm, 0, st); });
+            return rc;
+        }
+        const Plan p = plan_of(g, true);
+        FHC_TRY(check_inputs(op, g, p, x, dt, bm, cm, z));
+        FHC_TRY(check_in(op, "dy", dy, g->dtype, g->t));
+        FHC_TRY(check_out(op, "dx", dx, g->dtype, g->b, g->t, g->d));
+        FHC_TRY(check_out(op, "ddt", ddt, g->dtype, g->b, g->t, g->d));
+        if (z) FHC_TRY(check_out(op, "dz", dz, g->dtype, g->b, g->t, g->d));
+        else if (dz) return fail(-1, "%s: dz without z", op);
+        if (g->t && !states) return fail(-1, "%s: null states", op);
+        if (!aligned(states, 256)) return fail(-1, "%s: states is not 256-byte aligned", op);
+        FHC_TRY(check_workspace(op, workspace_of(p), ws, ws_bytes));
+        with_type(g->dtype, [&](auto t) {
+            using T = decltype(t);
+            using R = typename T::Raw;
+            auto a = args_of<T>(g, p, x, dt, bm, cm, z, ws);
+            a.states = reinterpret_cast<f4*>(const_cast<float*>(states)), a.dy = seq_of<R>(dy), a.dht = dht;
+            a.dx = seq_of<R>(dx), a.ddt = seq_of<R>(ddt), a.dz = seq_of<R>(dz), a.dh0 = dh0;
+            if (p.segs > 1) rc = launch<T, true, true>(op, p, a, st);
+            if (rc == 0) rc = launch<T, true, false>(op, p, a, st);
+            if (rc == 0) rc = close_vectors<T>(op, g, a.bc, dbm, dcm, p.blocks, st);
+        });
+        if (rc < 0) return rc;
+        const float* part = reinterpret_cast<const float*>(static_cast<char*>(ws) + p.ends_bytes + p.lasts_bytes);
+        return close_sums(op, part, p.segs * p.walks, sums, st);
+    });
+}

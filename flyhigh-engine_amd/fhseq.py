@@ -1,9 +1,10 @@
 """Python host driver of the operators on rows of channels (ctypes over include/fhc_seq.h in libfhconv.so): a gated
-linear recurrence (``glr``), the norms around a block with its gate and the scaled residual (``norm_block``) and a
-gated feed-forward block (``ffn``), each with its backward pass.
+linear recurrence (``glr``), the norms around a block with its gate and the scaled residual (``norm_block``), a gated
+feed-forward block (``ffn``), a short causal convolution (``short_conv``), a selective state space scan (``ssm``) and a
+matrix product with bias, activation and residual (``linear``), each with its backward pass.
 
-Inputs are torch tensors on the current GPU in f16, bf16 or (not ``ffn``) f32, all of one call in the same type; states
-and the gradients of the recurrence's and norms' weights are f32. Each function returns new tensors, which autograd does
+Inputs are torch tensors on the current GPU in f16, bf16 or (not ``ffn`` and ``linear``) f32, all of one call in the same
+type; the recurrences' states and the gradients of the weights of the recurrences, the norms and the convolution are f32. Each function returns new tensors, which autograd does
 not know: a call with tensors that require gradients is refused while autograd records (``torch.no_grad()``, and the
 ``*_backward`` functions, are the way). ``stream`` (a torch
 stream) is where the call runs, the current stream if None; what it allocates belongs to that stream. The module only
@@ -44,6 +45,20 @@ class FfnDesc(ctypes.Structure):
     _fields_ = [("dtype", _U), ("act", _U), ("rows", _U), ("c", _U), ("f", _U)]
 
 
+class ShortConvDesc(ctypes.Structure):
+    _fields_ = [("dtype", _U), ("act", _U), ("b", _U), ("t", _U), ("d", _U), ("k", _U), ("w", _P), ("bias", _P),
+                ("lengths", _P)]
+
+
+class SsmDesc(ctypes.Structure):
+    _fields_ = [("dtype", _U), ("b", _U), ("t", _U), ("d", _U), ("n", _U), ("groups", _U), ("a", _P), ("dt_bias", _P),
+                ("skip", _P), ("lengths", _P)]
+
+
+class LinearDesc(ctypes.Structure):
+    _fields_ = [("dtype", _U), ("act", _U), ("rows", _U), ("c", _U), ("f", _U)]
+
+
 class _Desc:
     """A structure's argument: the structure, a reference to it, or its packed bytes."""
 
@@ -74,6 +89,17 @@ def _lib():
             "fhc_ffn_workspace_bytes": ([D, ctypes.c_int], _SZ),
             "fhc_ffn_forward": ([D, R, _P, _P, _P, R, _P, _P, _SZ, _P], ctypes.c_int),
             "fhc_ffn_backward": ([D, R, _P, _P, _P, _P, R, R, _P, _P, _P, _P, _SZ, _P], ctypes.c_int),
+            "fhc_short_conv_forward": ([D, S, _P, S, _P, _P], ctypes.c_int),
+            "fhc_short_conv_workspace_bytes": ([D], _SZ),
+            "fhc_short_conv_backward": ([D, S, _P, S, _P, S, _P, _P, _P, _P, _SZ, _P], ctypes.c_int),
+            "fhc_ssm_states_bytes": ([D], _SZ),
+            "fhc_ssm_workspace_bytes": ([D, ctypes.c_int], _SZ),
+            "fhc_ssm_forward": ([D, S, S, S, S, S, _P, S, _P, _P, _P, _SZ, _P], ctypes.c_int),
+            "fhc_ssm_backward": ([D] + [S] * 5 + [_P, S, _P] + [S] * 5 + [_P] * 5 + [_SZ, _P], ctypes.c_int),
+            "fhc_linear_saved_bytes": ([D], _SZ),
+            "fhc_linear_workspace_bytes": ([D, ctypes.c_int], _SZ),
+            "fhc_linear_forward": ([D, R, _P, _P, R, R, _P, _P, _SZ, _P], ctypes.c_int),
+            "fhc_linear_backward": ([D, R, _P, _P, R, R, _P, _P, _P, _SZ, _P], ctypes.c_int),
         }
         for name, (args, res) in sig.items():
             f = getattr(L, name)
@@ -87,6 +113,7 @@ def _lib():
 # stream's handle is read without a Stream object.
 _GLR, _SEQ = struct.Struct("@IIIIfPP").pack, struct.Struct("@Pqq").pack
 _NORM, _ROWS, _FFN = struct.Struct("@IIIIffPPP").pack, struct.Struct("@Pq").pack, struct.Struct("@IIIII").pack
+_CONV, _SSM, _LINEAR = struct.Struct("@IIIIIIPPP").pack, struct.Struct("@IIIIIIPPPP").pack, _FFN
 
 
 class _Fast:
@@ -96,7 +123,8 @@ class _Fast:
         import torch
         L = _lib()
         for name in ("fhc_glr_forward", "fhc_glr_backward", "fhc_norm_block", "fhc_norm_block_backward",
-                     "fhc_ffn_forward", "fhc_ffn_backward"):
+                     "fhc_ffn_forward", "fhc_ffn_backward", "fhc_short_conv_forward", "fhc_short_conv_backward",
+                     "fhc_ssm_forward", "fhc_ssm_backward", "fhc_linear_forward", "fhc_linear_backward"):
             types = [_SZ if t is _SZ else _P for t in getattr(L, name).argtypes]
             setattr(self, name[4:], ctypes.CFUNCTYPE(ctypes.c_int, *types)((name, L)))
         self.torch, self.empty_like, self.empty = torch, torch.empty_like, torch.empty
@@ -137,6 +165,25 @@ def _ffn_sizes(dtype, act, rows, c, f):
     """Bytes of what a training forward keeps, and of the workspace forward and backward."""
     L, d = _lib(), FfnDesc(dtype, act, rows, c, f)
     return L.fhc_ffn_saved_bytes(d), L.fhc_ffn_workspace_bytes(d, 0), L.fhc_ffn_workspace_bytes(d, 1)
+
+
+@functools.lru_cache(4096)
+def _conv_size(dtype, b, t, d, taps):
+    return _lib().fhc_short_conv_workspace_bytes(ShortConvDesc(dtype, 0, b, t, d, taps, 256, None, None))
+
+
+@functools.lru_cache(4096)
+def _ssm_sizes(dtype, b, t, d, n, groups):
+    """Bytes of the states, and of the workspace forward and backward."""
+    L, g = _lib(), SsmDesc(dtype, b, t, d, n, groups, 256, None, None, None)
+    return L.fhc_ssm_states_bytes(g), L.fhc_ssm_workspace_bytes(g, 0), L.fhc_ssm_workspace_bytes(g, 1)
+
+
+@functools.lru_cache(4096)
+def _linear_sizes(dtype, act, rows, c, f):
+    """Bytes of what a training forward keeps, and of the workspace forward and backward."""
+    L, d = _lib(), LinearDesc(dtype, act, rows, c, f)
+    return L.fhc_linear_saved_bytes(d), L.fhc_linear_workspace_bytes(d, 0), L.fhc_linear_workspace_bytes(d, 1)
 
 
 def _on(stream):
@@ -401,3 +448,190 @@ def ffn_backward(x, wg, wu, wd, saved, dy, act="silu", stream=None):
                       dwd.data_ptr(), _ptr(ws), n, k.raw_stream(at)) < 0:
         _refuse(op)
     return dx, dwg, dwu, dwd
+
+
+CONV_ACTS = {"silu": 0, "none": 2}
+
+
+def _conv_desc(k, name, x, w, bias, act, state, lengths):
+    if x.dim() != 3 or w.dim() != 2:
+        raise FhcError(f"{name}: x is [sequences, steps, channels] and w [channels, taps], got {tuple(x.shape)}, "
+                       f"{tuple(w.shape)}")
+    if act not in CONV_ACTS:
+        raise FhcError(f"{name}: act {act!r} is none of {', '.join(CONV_ACTS)}")
+    dtype, at = _first(k, name, x)
+    b, t, d = x.shape
+    ty, taps = x.dtype, w.shape[1]
+    g = _pack(name, _CONV, dtype, CONV_ACTS[act], b, t, d, taps, _dense(name, "w", w, (d, taps), ty, at) or 0,
+              _dense(name, "bias", bias, (d,), ty, at) or 0, _dense(name, "lengths", lengths, (b,), k.i32, at) or 0)
+    return g, at, dtype, taps, _seq(name, "x", x), _dense(name, "state", state, (b, taps - 1, d), ty, at)
+
+
+def short_conv(x, w, bias=None, act="silu", state=None, lengths=None, stream=None):
+    """The causal convolution of x [sequences, steps, channels] along its steps with w [channels, taps] (2 to 4 taps, the
+    last one meets a step's own input): y_t = act(bias + sum_j w[j] x_(t - taps + 1 + j)), act "silu" or "none", behind
+    ``state`` [sequences, taps - 1, channels] (or zeros), the inputs before the first, the oldest first. Returns (y, the
+    state that the next call takes). lengths: int32 [sequences]; y past a sequence's length is 0."""
+    if stream is not None:
+        with _on(stream):
+            return short_conv(x, w, bias, act, state, lengths)
+    k, op = _fast(), "short_conv"
+    _unrecorded(k, op, x, w, bias, state)
+    g, at, _, taps, sx, before = _conv_desc(k, op, x, w, bias, act, state, lengths)
+    y = _new_seq(k, x)
+    end = k.empty((x.shape[0], max(taps - 1, 0), x.shape[2]), dtype=x.dtype, device=at)
+    if k.short_conv_forward(g, sx, before, _seq(op, "y", y), end.data_ptr(), k.raw_stream(at)) < 0:
+        _refuse(op)
+    return y, end
+
+
+def short_conv_backward(x, w, bias, dy, act="silu", state=None, dstate=None, lengths=None, stream=None):
+    """(dx, dw, dbias, the gradient of ``state``) of a loss with dy and dstate (that of the state that was returned, or
+    zeros); dw and dbias are f32."""
+    if stream is not None:
+        with _on(stream):
+            return short_conv_backward(x, w, bias, dy, act, state, dstate, lengths)
+    k, op = _fast(), "short_conv_backward"
+    _unrecorded(k, op, x, w, bias, dy, state, dstate)
+    g, at, dtype, taps, sx, before = _conv_desc(k, op, x, w, bias, act, state, lengths)
+    b, t, d = x.shape
+    sdy = _like_seq(op, "dy", dy, x, at)
+    dend = _dense(op, "dstate", dstate, (b, taps - 1, d), x.dtype, at)
+    dx = _new_seq(k, x)
+    dw, dbias = k.empty((d, taps), dtype=k.f32, device=at), k.empty((d,), dtype=k.f32, device=at)
+    dbefore = k.empty((b, max(taps - 1, 0), d), dtype=x.dtype, device=at)
+    n = _conv_size(dtype, b, t, d, taps)
+    ws = _bytes(k, n, at)
+    if k.short_conv_backward(g, sx, before, sdy, dend, _seq(op, "dx", dx), dw.data_ptr(), dbias.data_ptr(),
+                             dbefore.data_ptr(), _ptr(ws), n, k.raw_stream(at)) < 0:
+        _refuse(op)
+    return dx, dw, dbias, dbefore
+
+
+def _ssm_desc(k, name, x, dt, a, bm, cm, skip, z, dt_bias, lengths):
+    if x.dim() != 3 or a.dim() != 2 or bm.dim() != 3:
+        raise FhcError(f"{name}: x is [sequences, steps, channels], a [channels, states] and bm [sequences, steps, groups "
+                       f"* states], got {tuple(x.shape)}, {tuple(a.shape)}, {tuple(bm.shape)}")
+    dtype, at = _first(k, name, x)
+    b, t, d = x.shape
+    n, wide = a.shape[1], bm.shape[2]
+    groups = wide // n if n and wide % n == 0 else 0
+    if groups < 1:
+        raise FhcError(f"{name}: bm has {wide} values a step, not a multiple of the {n} states of a")
+    g = _pack(name, _SSM, dtype, b, t, d, n, groups, _dense(name, "a", a, (d, n), k.f32, at) or 0,
+              _dense(name, "dt_bias", dt_bias, (d,), k.f32, at) or 0, _dense(name, "skip", skip, (d,), k.f32, at) or 0,
+              _dense(name, "lengths", lengths, (b,), k.i32, at) or 0)
+    for what, m in (("bm", bm), ("cm", cm)):
+        if m.dtype is not x.dtype or m.shape != (b, t, wide) or m.get_device() != at:
+            _match(name, what, m, (b, t, wide), x.dtype, at)
+    seqs = (_seq(name, "x", x), _like_seq(name, "dt", dt, x, at), _seq(name, "bm", bm), _seq(name, "cm", cm),
+            None if z is None else _like_seq(name, "z", z, x, at))
+    return g, at, _ssm_sizes(dtype, b, t, d, n, groups), n, seqs
+
+
+def ssm(x, dt, a, bm, cm, skip=None, z=None, dt_bias=None, h0=None, lengths=None, train=False, stream=None):
+    """The selective state space scan over x, dt, z [sequences, steps, channels] and bm, cm [sequences, steps, groups *
+    states] with a [channels, states], skip and dt_bias [channels] in f32: D = softplus(dt + dt_bias),
+    h = exp(D a) h + D x B from h0 ([sequences, channels, states] f32, or zeros), y = (sum C h + skip x) silu(z).
+    Returns (y, the last states), with train also the states that ``ssm_backward`` takes. lengths: int32 [sequences]; y
+    past a sequence's length is 0 and its states stay."""
+    if stream is not None:
+        with _on(stream):
+            return ssm(x, dt, a, bm, cm, skip, z, dt_bias, h0, lengths, train)
+    k, op = _fast(), "ssm"
+    _unrecorded(k, op, x, dt, a, bm, cm, skip, z, dt_bias, h0)
+    g, at, sizes, n, seqs = _ssm_desc(k, op, x, dt, a, bm, cm, skip, z, dt_bias, lengths)
+    b, _, d = x.shape
+    start = _dense(op, "h0", h0, (b, d, n), k.f32, at)
+    y = _new_seq(k, x)
+    ht = k.empty((b, d, n), dtype=k.f32, device=at)
+    states = k.empty((sizes[0],), dtype=k.u8, device=at) if train else None
+    ws = _bytes(k, sizes[1], at)
+    if k.ssm_forward(g, *seqs, start, _seq(op, "y", y), ht.data_ptr(), _ptr(states), _ptr(ws), sizes[1],
+                     k.raw_stream(at)) < 0:
+        _refuse(op)
+    return (y, ht, states) if train else (y, ht)
+
+
+def ssm_backward(x, dt, a, bm, cm, states, dy, skip=None, z=None, dt_bias=None, dht=None, lengths=None, stream=None):
+    """(dx, ddt, da, dbm, dcm, dskip, dz, ddt_bias, dh0) of a loss with dy and dht ([sequences, channels, states] f32, or
+    zeros); ``states`` from the training ``ssm`` call of the same inputs. da, dskip, ddt_bias and dh0 are f32; dskip and
+    ddt_bias also where there was no weight, dz is None without z."""
+    if stream is not None:
+        with _on(stream):
+            return ssm_backward(x, dt, a, bm, cm, states, dy, skip, z, dt_bias, dht, lengths)
+    k, op = _fast(), "ssm_backward"
+    _unrecorded(k, op, x, dt, a, bm, cm, dy, skip, z, dt_bias, dht)
+    g, at, sizes, n, seqs = _ssm_desc(k, op, x, dt, a, bm, cm, skip, z, dt_bias, lengths)
+    b, _, d = x.shape
+    end = _dense(op, "dht", dht, (b, d, n), k.f32, at)
+    kept = _dense(op, "states", states, (sizes[0],), k.u8, at)
+    sdy = _like_seq(op, "dy", dy, x, at)
+    dx, ddt, dbm, dcm = _new_seq(k, x), _new_seq(k, dt), _new_seq(k, bm), _new_seq(k, cm)
+    dz = None if z is None else _new_seq(k, z)
+    da, dskip, ddt_bias, dh0 = (k.empty(s, dtype=k.f32, device=at) for s in ((d, n), (d,), (d,), (b, d, n)))
+    ws = _bytes(k, sizes[2], at)
+    if k.ssm_backward(g, *seqs, kept, sdy, end, _seq(op, "dx", dx), _seq(op, "ddt", ddt), _seq(op, "dbm", dbm),
+                      _seq(op, "dcm", dcm), None if dz is None else _seq(op, "dz", dz), da.data_ptr(),
+                      ddt_bias.data_ptr(), dskip.data_ptr(), dh0.data_ptr(), _ptr(ws), sizes[2], k.raw_stream(at)) < 0:
+        _refuse(op)
+    return dx, ddt, da, dbm, dcm, dskip, dz, ddt_bias, dh0
+
+
+LINEAR_ACTS = {"silu": 0, "gelu": 1, "none": 2}
+
+
+def _linear_desc(k, name, x, w, act):
+    if x.dim() != 2 or w.dim() != 2:
+        raise FhcError(f"{name}: x is [rows, channels] and w [features, channels], got {tuple(x.shape)}, "
+                       f"{tuple(w.shape)}")
+    if act not in LINEAR_ACTS:
+        raise FhcError(f"{name}: act {act!r} is none of {', '.join(LINEAR_ACTS)}")
+    dtype, at = _first(k, name, x)
+    rows, c = x.shape
+    f, act = w.shape[0], LINEAR_ACTS[act]
+    return (_pack(name, _LINEAR, dtype, act, rows, c, f), at, _linear_sizes(dtype, act, rows, c, f),
+            _rows(name, "x", x), _dense(name, "w", w, (f, c), x.dtype, at))
+
+
+def linear(x, w, bias=None, residual=None, act="none", train=False, stream=None):
+    """act(x w^T + bias) + residual of rows x [rows, c] with w [f, c], bias [f] and residual [rows, f], act "none", "silu"
+    or "gelu" (tanh form), in f16 or bf16. With train: (y, what ``linear_backward`` takes)."""
+    if stream is not None:
+        with _on(stream):
+            return linear(x, w, bias, residual, act, train)
+    k, op = _fast(), "linear"
+    _unrecorded(k, op, x, w, bias, residual)
+    d, at, sizes, rx, pw = _linear_desc(k, op, x, w, act)
+    rows, f = x.shape[0], w.shape[0]
+    pb = _dense(op, "bias", bias, (f,), x.dtype, at)
+    y = k.empty((rows, f), dtype=x.dtype, device=at)
+    res = _like_rows(op, "residual", residual, y, at)
+    saved = _bytes(k, sizes[0], at) if train else None
+    n = sizes[1]
+    ws = _bytes(k, n, at)
+    if k.linear_forward(d, rx, pw, pb, res, _ROWS(y.data_ptr(), f), _ptr(saved), _ptr(ws), n, k.raw_stream(at)) < 0:
+        _refuse(op)
+    return (y, saved) if train else y
+
+
+def linear_backward(x, w, saved, dy, act="none", bias=True, stream=None):
+    """(dx, dw, dbias) for dy, dx and dw in the inputs' type and dbias in f32 (None where bias is false); ``saved`` from the
+    training ``linear`` call of the same inputs (None where it kept nothing). The residual's gradient is dy."""
+    if stream is not None:
+        with _on(stream):
+            return linear_backward(x, w, saved, dy, act, bias)
+    k, op = _fast(), "linear_backward"
+    _unrecorded(k, op, x, w, dy)
+    d, at, sizes, rx, pw = _linear_desc(k, op, x, w, act)
+    rows, f = x.shape[0], w.shape[0]
+    kept = _dense(op, "saved", saved, (sizes[0],), k.u8, at) if sizes[0] else None
+    _match(op, "dy", dy, (rows, f), x.dtype, at)
+    dx, dw = k.new(x), k.new(w)
+    dbias = k.empty((f,), dtype=k.f32, device=at) if bias else None
+    n = sizes[2]
+    ws = _bytes(k, n, at)
+    if k.linear_backward(d, rx, pw, kept, _rows(op, "dy", dy), _ROWS(dx.data_ptr(), x.shape[1]), dw.data_ptr(),
+                         _ptr(dbias), _ptr(ws), n, k.raw_stream(at)) < 0:
+        _refuse(op)
+    return dx, dw, dbias

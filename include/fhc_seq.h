@@ -1,6 +1,7 @@
 /* fhc_seq: operators of a recurrent block on rows of channels, on MI355X (gfx950), as a C ABI: a gated linear
- * recurrence along a sequence, the norms around a block with its gate and the scaled residual, and a gated
- * feed-forward block, each with its backward pass. The rows are tokens of sequences, or the pixels of NHWC feature
+ * recurrence along a sequence, the norms around a block with its gate and the scaled residual, a gated feed-forward
+ * block, a short causal convolution along a sequence, a selective state space scan, and a matrix product with bias,
+ * activation and residual, each with its backward pass. The rows are tokens of sequences, or the pixels of NHWC feature
  * maps over the frames of a stream (a frame's map is then one time step, a pixel one sequence). The reference has no
  * counterpart: its network keeps nothing from one frame pair to the next.
  *
@@ -126,6 +127,102 @@ int fhc_ffn_forward(const fhc_ffn_desc* d, const fhc_rows* x, const void* wg, co
 int fhc_ffn_backward(const fhc_ffn_desc* d, const fhc_rows* x, const void* wg, const void* wu, const void* wd,
                      const void* saved, const fhc_rows* dy, const fhc_rows* dx, void* dwg, void* dwu, void* dwd,
                      void* ws, size_t ws_bytes, void* stream);
+
+/* ---- The short causal convolution along a sequence, per channel, over k taps (2 to 4). With e the k - 1 rows of
+ * `state` and then the sequence's own n rows:
+ *     y_t = act(v_t),   v_t = bias[ch] + sum over j < k of w[ch][j] * e[t + j]       (tap k - 1 meets x_t itself)
+ * and e's last k - 1 rows are the state of a call that goes on from here. With `lengths` positions at and past a
+ * sequence's length are not read, and y and the gradients there are 0. */
+#define FHC_ACT_IDENTITY 2u
+
+typedef struct fhc_short_conv_desc {
+    uint32_t dtype;         /* FHC_F16, FHC_BF16 or FHC_F32: of x, w, bias, the states, y, dx                        */
+    uint32_t act;           /* FHC_ACT_SILU or FHC_ACT_IDENTITY                                                      */
+    uint32_t b, t, d, k;    /* sequences, steps, channels (any may be 0, b * d below 2^31); 2 <= k <= 4              */
+    const void* w;          /* device, dense [d][k]                                                                  */
+    const void* bias;       /* device, [d], or NULL                                                                  */
+    const int32_t* lengths; /* device, [b], or NULL: every sequence has t steps                                      */
+} fhc_short_conv_desc;
+
+/* state: [b][k - 1][d], the oldest row first, or NULL for zeros. state_out: the same layout, or NULL; it may be state
+ * itself (a server's state, updated in place). */
+int fhc_short_conv_forward(const fhc_short_conv_desc* g, const fhc_seq* x, const void* state, const fhc_seq* y,
+                           void* state_out, void* stream);
+
+/* 0 for a bad descriptor */
+size_t fhc_short_conv_workspace_bytes(const fhc_short_conv_desc* g);
+
+/* The gradients of a loss with dy = dL/dy and dstate_out = dL/dstate_out ([b][k - 1][d] in dtype, or NULL for zeros): dx
+ * in dtype, dw [d][k] and dbias [d] in f32, dstate [b][k - 1][d] in dtype (each may be NULL: not wanted). */
+int fhc_short_conv_backward(const fhc_short_conv_desc* g, const fhc_seq* x, const void* state, const fhc_seq* dy,
+                            const void* dstate_out, const fhc_seq* dx, float* dw, float* dbias, void* dstate, void* ws,
+                            size_t ws_bytes, void* stream);
+
+/* ---- The selective state space scan. Every channel of a sequence has n states; B and C are vectors of n for each
+ * position and group of channels (channel ch is in group ch / (d / groups)):
+ *     D_t    = softplus(dt_t + dt_bias[ch])
+ *     h_t[k] = exp(D_t a[ch][k]) h_(t-1)[k] + D_t x_t B_t[k]
+ *     y_t    = (sum over k of C_t[k] h_t[k] + skip[ch] x_t) silu(z_t)
+ * a, dt_bias and skip are f32 weights; z may be left out (no gate). With `lengths` positions at and past a sequence's
+ * length are not read, y and the gradients there are 0, and the state stays as it is. */
+typedef struct fhc_ssm_desc {
+    uint32_t dtype;          /* FHC_F16, FHC_BF16 or FHC_F32: of x, dt, z, B, C, y and their gradients               */
+    uint32_t b, t, d;        /* sequences, steps, channels; any may be 0. b * d below 2^31                            */
+    uint32_t n, groups;      /* states a channel, 1 to 64; groups, a divisor of d                                     */
+    const float* a;          /* device, dense [d][n]                                                                  */
+    const float* dt_bias;    /* device, [d], or NULL: zeros                                                           */
+    const float* skip;       /* device, [d], or NULL: zeros                                                           */
+    const int32_t* lengths;  /* device, [b], or NULL                                                                  */
+} fhc_ssm_desc;
+
+/* Bytes of the states that a training forward keeps for the backward pass, and of the workspace of either call
+ * (0 for many shapes: a NULL workspace is then fine). 0 for a bad descriptor. */
+size_t fhc_ssm_states_bytes(const fhc_ssm_desc* g);
+size_t fhc_ssm_workspace_bytes(const fhc_ssm_desc* g, int backward);
+
+/* bm and cm: B and C, sequence tensors of groups * n channels. z NULL: no gate. h0: [b][d][n] f32, or NULL for zeros.
+ * ht: the state after the last step, [b][d][n] f32, or NULL; it may be h0 itself. states: NULL, or the 256-byte aligned
+ * buffer that the backward pass of the same descriptor takes. A call with t = 1 is the single-token step. */
+int fhc_ssm_forward(const fhc_ssm_desc* g, const fhc_seq* x, const fhc_seq* dt, const fhc_seq* bm, const fhc_seq* cm,
+                    const fhc_seq* z, const float* h0, const fhc_seq* y, float* ht, float* states, void* ws,
+                    size_t ws_bytes, void* stream);
+
+/* The gradients of a loss with dy = dL/dy and dht = dL/dht ([b][d][n] f32, or NULL for zeros): dx, ddt, dbm, dcm and dz
+ * (NULL without z) in dtype; da [d][n], ddt_bias [d], dskip [d] and dh0 [b][d][n] in f32 (those may be NULL: not wanted).
+ * The inputs are those of the forward call, `states` what it wrote. */
+int fhc_ssm_backward(const fhc_ssm_desc* g, const fhc_seq* x, const fhc_seq* dt, const fhc_seq* bm, const fhc_seq* cm,
+                     const fhc_seq* z, const float* states, const fhc_seq* dy, const float* dht, const fhc_seq* dx,
+                     const fhc_seq* ddt, const fhc_seq* dbm, const fhc_seq* dcm, const fhc_seq* dz, float* da,
+                     float* ddt_bias, float* dskip, float* dh0, void* ws, size_t ws_bytes, void* stream);
+
+/* ---- The matrix product with its epilogue, on rows of c channels, f wide:
+ *     y = act(v) + residual,   v = x w^T + bias
+ * w is dense [f][c], bias [f], in dtype (f16 or bf16); act FHC_ACT_SILU, FHC_ACT_GELU or FHC_ACT_IDENTITY. v and the sum
+ * are f32, y is rounded once. A training forward with silu or gelu keeps v in f32; the backward pass rounds dL/dv to
+ * dtype once, since it is the next products' operand (dbias sums it before that rounding). The residual's gradient is
+ * dy itself. */
+typedef struct fhc_linear_desc {
+    uint32_t dtype; /* FHC_F16 or FHC_BF16 */
+    uint32_t act;
+    uint32_t rows, c, f; /* c, f <= 2^20 */
+} fhc_linear_desc;
+
+/* Bytes of what a training forward keeps for the backward pass (0: nothing, NULL is then fine), and of the workspace of
+ * either call. */
+size_t fhc_linear_saved_bytes(const fhc_linear_desc* d);
+size_t fhc_linear_workspace_bytes(const fhc_linear_desc* d, int backward);
+
+/* bias and residual may be NULL. y may be the residual, element for element. saved: NULL, or a 256-byte aligned buffer
+ * that the backward pass of the same descriptor takes. */
+int fhc_linear_forward(const fhc_linear_desc* d, const fhc_rows* x, const void* w, const void* bias,
+                       const fhc_rows* residual, const fhc_rows* y, void* saved, void* ws, size_t ws_bytes,
+                       void* stream);
+
+/* dx and dw (dense) in dtype, dbias [f] f32, for dy; those that are not wanted may be NULL. Without rows x, dy and dx are
+ * not read, and dw and dbias are 0. */
+int fhc_linear_backward(const fhc_linear_desc* d, const fhc_rows* x, const void* w, const void* saved,
+                        const fhc_rows* dy, const fhc_rows* dx, void* dw, float* dbias, void* ws, size_t ws_bytes,
+                        void* stream);
 
 #ifdef __cplusplus
 }
