@@ -1,7 +1,7 @@
 // The short causal convolution along a sequence (include/fhc_seq.h), forward and backward.
 //
-// A thread has V adjacent channels of one sequence (16 bytes) and walks R steps with the last k - 1 inputs in registers,
-// so every input is read once, bar the k - 1 rows in front of a chunk of R steps (which the caches hold: a workgroup has
+// A thread has V adjacent channels of one sequence and walks a chunk of steps with the last k - 1 inputs in registers,
+// so every input is read once, bar the k - 1 rows in front of a chunk (which the caches hold: a workgroup has
 // neighbouring chunks of the same channels). Lanes run over channels; a map of few channels gives a wave's other lanes
 // further chunks or sequences. The first chunk of a sequence also moves the state on: it alone reads the old one, so the
 // new one may lie over it.
@@ -119,7 +119,7 @@ __device__ __forceinline__ void rows_before(const ConvArgs<typename T::Raw>& g, 
     }
 }
 
-// What bounds it (MI355X): see the figures at the launch.
+// What bounds it (MI355X): HBM. 4 x 4096 x 4096 bf16, 4 taps, 58 us, 4.7 TB/s of the 5.2 that a large copy reaches.
 template <class T, int K, int V>
 __global__ __launch_bounds__(kThreads) void short_conv_fwd(ConvArgs<typename T::Raw> g) {
     using R = typename T::Raw;
@@ -208,63 +208,109 @@ __global__ __launch_bounds__(kThreads) void short_conv_bwd(ConvArgs<typename T::
         for (int k = 0; k < K; k++)
 #pragma unroll
             for (int v = 0; v < V; v++) dv[k][v] = 0.0f;
-        const uint32_t t1 = min(p.t0 + g.steps, g.t), most = t1 + K - 1;
+        const uint32_t t1 = min(p.t0 + g.steps, g.t), most = t1 + K - 1, there = min(most, p.n);
         const R *px = g.x.at(p.b, p.t0) + p.ch, *py = g.dy.at(p.b, p.t0) + p.ch;
-        for (uint32_t t = p.t0; t < most; t += U) {
-            R in[U][V], up[U][V];
+        R* pd = g.dx.at(p.b, p.t0) + p.ch;
+        // M steps' rows from step i on; those past the length or the chunk as zeros
+        auto load = [&](auto m, uint32_t i, R(*in)[V], R(*up)[V]) {
+            constexpr int M = m;
+            if (i + M <= there && p.valid >= V) {
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                if (t + u < min(most, p.n)) {
-                    load_v<R, V>(px + u * g.x.ts, p.valid, in[u]);
-                    load_v<R, V>(py + u * g.dy.ts, p.valid, up[u]);
-                } else {
+                for (int u = 0; u < M; u++) {
+                    load_raw<R, V, false>(px + u * g.x.ts, in[u]);
+                    load_raw<R, V, false>(py + u * g.dy.ts, up[u]);
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < M; u++) {
 #pragma unroll
                     for (int v = 0; v < V; v++) in[u][v] = up[u][v] = R(0);
+                    if (i + u < there) {
+                        load_v<R, V>(px + u * g.x.ts, p.valid, in[u]);
+                        load_v<R, V>(py + u * g.dy.ts, p.valid, up[u]);
+                    }
                 }
             }
+            px += M * g.x.ts, py += M * g.dy.ts;
+        };
+        // Step i: dv_i, the weights' gradients (INNER: certainly a step of this chunk inside the length), and de_i.
+        auto step = [&](auto inner, uint32_t i, const R(&in)[V], const R(&up)[V], float(&de)[V]) {
+            constexpr bool INNER = inner;
+            const bool own = INNER || (i < t1 && i < p.n);  // steps behind are the next chunk's, and so their terms
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const uint32_t i = t + u;
-                if (i >= most) break;
-                const bool own = i < t1;  // the steps behind are the next chunk's, whose weights' gradients are its own
+            for (int v = 0; v < V; v++) {
+                win[K - 1][v] = widen(T{}, in[v]);
+                float s = taps.bias[v], slope = 1.0f, value;
+#pragma unroll
+                for (int k = 0; k < K; k++) s = __builtin_fmaf(taps.w[k][v], win[k][v], s);
+                if (g.silu) silu_grad(s, value, slope);
+                const float q = INNER || i < p.n ? widen(T{}, up[v]) * slope : 0.0f;
+                dv[K - 1][v] = q;
+                if (own) {
+                    db[v] += q;
+#pragma unroll
+                    for (int k = 0; k < K; k++) dw[k][v] = __builtin_fmaf(q, win[k][v], dw[k][v]);
+                }
+                de[v] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < K; k++) de[v] = __builtin_fmaf(taps.w[k][v], dv[K - 1 - k][v], de[v]);
+#pragma unroll
+                for (int k = 0; k < K - 1; k++) win[k][v] = win[k + 1][v], dv[k][v] = dv[k + 1][v];
+            }
+            if (!INNER && i >= p.n && i < p.n + K - 1 && g.dend) {  // e_i is also a row of the state that is left
+                R end[V];
+                load_v<R, V>(g.dend + ((uint64_t)p.b * (K - 1) + (i - p.n)) * g.d + p.ch, p.valid, end);
+#pragma unroll
+                for (int v = 0; v < V; v++) de[v] += widen(T{}, end[v]);
+            }
+        };
+        {  // the first k - 1 steps complete rows in front of the chunk: the state's, or the chunk's before
+            R in[K - 1][V], up[K - 1][V], out[V];
+            load(std::integral_constant<int, K - 1>{}, p.t0, in, up);
+#pragma unroll
+            for (int u = 0; u < K - 1; u++) {
                 float de[V];
+                step(std::false_type{}, p.t0 + u, in[u], up[u], de);
 #pragma unroll
-                for (int v = 0; v < V; v++) {
-                    win[K - 1][v] = widen(T{}, in[u][v]);
-                    float s = taps.bias[v], slope = 1.0f, value;
+                for (int v = 0; v < V; v++) out[v] = narrow(T{}, de[v]);
+                if (p.t0 == 0 && g.dstate)
+                    store_v<R, V>(g.dstate + ((uint64_t)p.b * (K - 1) + u) * g.d + p.ch, p.valid, out);
+            }
+        }
+        R in[U][V], up[U][V];
+        const std::integral_constant<int, U> block{};
+        load(block, p.t0 + K - 1, in, up);
+        for (uint32_t i = p.t0 + K - 1; i < most; i += U) {
+            R now[U][V], dnow[U][V];
 #pragma unroll
-                    for (int k = 0; k < K; k++) s = __builtin_fmaf(taps.w[k][v], win[k][v], s);
-                    if (g.silu) silu_grad(s, value, slope);
-                    const float q = i < p.n ? widen(T{}, up[u][v]) * slope : 0.0f;
-                    dv[K - 1][v] = q;
-                    const float mineq = own ? q : 0.0f;
-                    db[v] += mineq;
+            for (int u = 0; u < U; u++)
 #pragma unroll
-                    for (int k = 0; k < K; k++)
-                        if (own && i < p.n) dw[k][v] = __builtin_fmaf(mineq, win[k][v], dw[k][v]);
-                    de[v] = 0.0f;
+                for (int v = 0; v < V; v++) now[u][v] = in[u][v], dnow[u][v] = up[u][v];
+            if (i + U < most) load(block, i + U, in, up);
+            const bool inner = i + U <= min(t1, p.n) && p.valid >= V && g.dx.p;
+            if (inner) {
 #pragma unroll
-                    for (int k = 0; k < K; k++) de[v] = __builtin_fmaf(taps.w[k][v], dv[K - 1 - k][v], de[v]);
+                for (int u = 0; u < U; u++) {
+                    float de[V];
+                    R out[V];
+                    step(std::true_type{}, i + u, now[u], dnow[u], de);
 #pragma unroll
-                    for (int k = 0; k < K - 1; k++) win[k][v] = win[k + 1][v], dv[k][v] = dv[k + 1][v];
+                    for (int v = 0; v < V; v++) out[v] = narrow(T{}, de[v]);
+                    store_raw<R, V, false>(pd + u * g.dx.ts, out);
                 }
-                R out[V];
-                if (i >= p.n && i < p.n + K - 1 && g.dend) {  // e_i is also a row of the state that is left
-                    load_v<R, V>(g.dend + ((uint64_t)p.b * (K - 1) + (i - p.n)) * g.d + p.ch, p.valid, out);
+            } else {
 #pragma unroll
-                    for (int v = 0; v < V; v++) de[v] += widen(T{}, out[v]);
-                }
-                const bool inside = i < K - 1 || i - (K - 1) < p.n;
+                for (int u = 0; u < U; u++) {
+                    if (i + u >= most) break;
+                    float de[V];
+                    R out[V];
+                    step(std::false_type{}, i + u, now[u], dnow[u], de);
 #pragma unroll
-                for (int v = 0; v < V; v++) out[v] = inside ? narrow(T{}, de[v]) : R(0);
-                if (i < K - 1) {
-                    if (p.t0 == 0 && g.dstate)
-                        store_v<R, V>(g.dstate + ((uint64_t)p.b * (K - 1) + i) * g.d + p.ch, p.valid, out);
-                } else if (i - (K - 1) >= p.t0 && g.dx.p) {
-                    store_v<R, V>(g.dx.at(p.b, i - (K - 1)) + p.ch, p.valid, out);
+                    for (int v = 0; v < V; v++) out[v] = i + u - (K - 1) < p.n ? narrow(T{}, de[v]) : R(0);
+                    if (g.dx.p) store_v<R, V>(pd + u * g.dx.ts, p.valid, out);
                 }
             }
-            px += U * g.x.ts, py += U * g.dy.ts;
+            pd += U * g.dx.ts;
         }
     }
     float* part = g.part + (uint64_t)walk * g.d * (K + 1);
@@ -287,17 +333,25 @@ __global__ __launch_bounds__(kThreads) void short_conv_bwd(ConvArgs<typename T::
 
 // ---- host side ----------------------------------------------------------------------------------------------------
 
+// Channels of a thread: 16 bytes forward (8-byte loads take 72 us where these take 58, 4 x 4096 x 4096 bf16); backward two
+// channels, since their windows and sums decide how many waves a SIMD has (4 with two, 2 with eight: 108 us and 320).
+constexpr int kBackV = 2;
+constexpr uint32_t kForwardV(uint32_t dtype) { return dtype == FHC_F32 ? 4 : 8; }
 struct Plan {
     uint32_t v, groups, lanes, colblocks, chunks, steps, items, blocks, walks;
 };
-Plan plan_of(const fhc_short_conv_desc* g) {
+Plan plan_of(const fhc_short_conv_desc* g, bool backward) {
     Plan p{};
-    p.v = g->dtype == FHC_F32 ? 4 : 8;
+    p.v = backward ? kBackV : kForwardV(g->dtype);
     p.groups = (uint32_t)ceil_div(g->d, p.v);
     while (p.lanes < 6 && (1u << p.lanes) < p.groups) p.lanes++;
     p.colblocks = (uint32_t)ceil_div(p.groups, 1u << p.lanes);
+    // The longest chunks that leave enough threads; shorter ones read more rows twice. us with chunks of 8, 16, 32 steps,
+    // 4 taps, forward: 1 x 4096 x 1024 bf16 12, 15, 25; 2 x 4096 x 2048 20, 24, 27 (2^18 threads with 8); 4 x 4096 x 4096
+    // 67, 62, 58 (2^18 with 32). Backward: 19, 19, 20 (2^16 with 32); 44, 37, 29.
     p.steps = 32;
-    while (p.steps > 8 && (uint64_t)g->b * ceil_div(g->t, p.steps) * p.groups < 1u << 18) p.steps /= 2;
+    const uint64_t enough = backward ? 1u << 16 : 1u << 18;
+    while (p.steps > 8 && (uint64_t)g->b * ceil_div(g->t, p.steps) * p.groups < enough) p.steps /= 2;
     p.chunks = g->t ? (uint32_t)ceil_div(g->t, p.steps) : 1;
     const uint64_t items = (uint64_t)g->b * p.chunks;
     p.items = items >= 1ull << 32 ? 0 : (uint32_t)items;
@@ -308,7 +362,7 @@ Plan plan_of(const fhc_short_conv_desc* g) {
     return p;
 }
 size_t workspace_of(const fhc_short_conv_desc* g) {
-    return (size_t)plan_of(g).walks * g->d * (g->k + 1) * 4;
+    return (size_t)plan_of(g, true).walks * g->d * (g->k + 1) * 4;
 }
 
 int check_desc(const char* op, const fhc_short_conv_desc* g) {
@@ -336,7 +390,7 @@ ConvArgs<typename T::Raw> args_of(const fhc_short_conv_desc* g, const Plan& p, c
 
 template <class T, bool BWD>
 void launch(uint32_t k, uint32_t blocks, const ConvArgs<typename T::Raw>& a, hipStream_t st) {
-    constexpr int V = sizeof(typename T::Raw) == 4 ? 4 : 8;
+    constexpr int V = BWD ? kBackV : kForwardV(T::id);
 #define CONV(K)                                                                                              \
     do {                                                                                                     \
         if constexpr (BWD) hipLaunchKernelGGL((short_conv_bwd<T, K, V>), dim3(blocks), dim3(kThreads), 0, st, a); \
@@ -366,7 +420,7 @@ extern "C" int fhc_short_conv_forward(const fhc_short_conv_desc* g, const fhc_se
         FHC_TRY(check_out(op, "y", y, g->dtype, g->b, g->t, g->d));
         FHC_TRY(check_array(op, "state", state, elem_bytes(g->dtype), false));
         FHC_TRY(check_array(op, "state_out", state_out, elem_bytes(g->dtype), false));
-        const Plan p = plan_of(g);
+        const Plan p = plan_of(g, false);
         const uint64_t grid = (uint64_t)p.blocks * p.colblocks;
         if (!p.items || !p.blocks) return fail(-1, "%s: too many workgroups", op);
         FHC_TRY(check_grid(op, grid, kThreads));
@@ -409,7 +463,7 @@ extern "C" int fhc_short_conv_backward(const fhc_short_conv_desc* g, const fhc_s
         FHC_TRY(check_array(op, "state", state, e, false));
         FHC_TRY(check_array(op, "dstate_out", dstate_out, e, false));
         FHC_TRY(check_array(op, "dstate", dstate, e, false));
-        const Plan p = plan_of(g);
+        const Plan p = plan_of(g, true);
         if (!p.items || !p.blocks) return fail(-1, "%s: too many workgroups", op);
         FHC_TRY(check_workspace(op, workspace_of(g), ws, ws_bytes));
         with_type(g->dtype, [&](auto t) {

@@ -4,9 +4,8 @@
 // them a wave, in registers. Time goes in tiles of 16 steps: the waves first prepare 16 / W steps each (D = softplus,
 // D x), which then lie in LDS for all of them; every wave runs its states through the 16 steps and leaves its part of
 // sum C h a step in LDS; the waves add the parts of their steps, apply skip and gate, and store. B and C are the same for
-// all lanes, and the f32 matrix unit's 4 x 4 x 1 blocks take them from four lanes of any block: one instruction is
-// B_t[0..3] D x + (a h)[0..3] for the four states of all 64 lanes, exact as fused multiply-adds are, and sum C h is four
-// more. The vector unit is left with a = exp2(D rate) and a h.
+// all lanes: a register holds them for 4 steps x 4 states in every row of 16 lanes, and a fused multiply-add takes a lane
+// of its row for an operand (DPP).
 //
 // Where the columns are too few for the chip, time is cut into segments: a first launch folds each to the state that it
 // leaves from zeros, and its sum of D (its decay is exp(a sum D), so one number a channel composes all of them); the
@@ -71,34 +70,106 @@ __device__ __forceinline__ float rate_of(float a) {
     return k < -3.4e38f ? -3.4e38f : k > 3.4e38f ? 3.4e38f : k;
 }
 
-// a's values in lanes 4 BLOCK + i times b, added to c[i]
-template <int BLOCK>
-__device__ __forceinline__ f4 outer(float a, float b, f4 c) {
+// NS states of a lane.
+template <int NS>
+struct States {
+    float v[NS];
+};
+
+// h[k] += B_k u, then the sum of C_k h[k], B_k and C_k from lane FROM + k of the own row of 16 lanes. In assembly: the
+// compiler spends a move on each such operand. The instructions in front may have written b or c (a DPP operand's two wait
+// states).
+template <int FROM>
+__device__ __forceinline__ float step_states(States<4>& h, float b, float u, float c) {
+    float p = 0.0f;
 #if defined(__HIP_DEVICE_COMPILE__)
-    return __builtin_amdgcn_mfma_f32_4x4x1f32(a, b, c, 4, BLOCK, 0);
-#else
-    return c;
+    asm("s_nop 1\n"
+        "v_fmac_f32_dpp %1, %5, %6 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %2, %5, %6 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %3, %5, %6 row_newbcast:%10 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %4, %5, %6 row_newbcast:%11 row_mask:0xf bank_mask:0xf\n"
+        "v_mul_f32_dpp %0, %7, %1 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %0, %7, %2 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %0, %7, %3 row_newbcast:%10 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %0, %7, %4 row_newbcast:%11 row_mask:0xf bank_mask:0xf"
+        : "=&v"(p), "+v"(h.v[0]), "+v"(h.v[1]), "+v"(h.v[2]), "+v"(h.v[3])
+        : "v"(b), "v"(u), "v"(c), "n"(FROM), "n"(FROM + 1), "n"(FROM + 2), "n"(FROM + 3));
+#endif
+    return p;
+}
+template <int FROM>
+__device__ __forceinline__ float step_states(States<2>& h, float b, float u, float c) {
+    float p = 0.0f;
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm("s_nop 1\n"
+        "v_fmac_f32_dpp %1, %3, %4 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %2, %3, %4 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n"
+        "v_mul_f32_dpp %0, %5, %1 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %0, %5, %2 row_newbcast:%7 row_mask:0xf bank_mask:0xf"
+        : "=&v"(p), "+v"(h.v[0]), "+v"(h.v[1])
+        : "v"(b), "v"(u), "v"(c), "n"(FROM), "n"(FROM + 1));
+#endif
+    return p;
+}
+// h[k] += B_k u
+template <int FROM>
+__device__ __forceinline__ void add_outer(f4& h, float b, float u) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    float h0 = h[0], h1 = h[1], h2 = h[2], h3 = h[3];
+    asm("s_nop 1\n"
+        "v_fmac_f32_dpp %0, %4, %5 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %1, %4, %5 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %2, %4, %5 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %3, %4, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf"
+        : "+v"(h0), "+v"(h1), "+v"(h2), "+v"(h3)
+        : "v"(b), "v"(u), "n"(FROM), "n"(FROM + 1), "n"(FROM + 2), "n"(FROM + 3));
+    h = f4{h0, h1, h2, h3};
 #endif
 }
-// the sum of four lanes' values of v, the same in lanes 4 (BLOCK + k) + i for all i, times h[k]
-template <int BLOCK>
-__device__ __forceinline__ f4 inner(float v, f4 h, f4 c) {
-    c = outer<BLOCK>(v, h[0], c);
-    c = outer<BLOCK + 1>(v, h[1], c);
-    c = outer<BLOCK + 2>(v, h[2], c);
-    return outer<BLOCK + 3>(v, h[3], c);
+// g[k] += C_k q, then s1 = the sum of B_k g[k] and p = the sum of C_k h[k]
+template <int FROM>
+__device__ __forceinline__ void step_back(f4& g, f4 h, float b, float c, float q, float& p, float& s1) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    float g0 = g[0], g1 = g[1], g2 = g[2], g3 = g[3];
+    asm("s_nop 1\n"
+        "v_fmac_f32_dpp %2, %11, %12 row_newbcast:%13 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %3, %11, %12 row_newbcast:%14 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %4, %11, %12 row_newbcast:%15 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %5, %11, %12 row_newbcast:%16 row_mask:0xf bank_mask:0xf\n"
+        "v_mul_f32_dpp %0, %11, %6 row_newbcast:%13 row_mask:0xf bank_mask:0xf\n"
+        "v_mul_f32_dpp %1, %10, %2 row_newbcast:%13 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %0, %11, %7 row_newbcast:%14 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %1, %10, %3 row_newbcast:%14 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %0, %11, %8 row_newbcast:%15 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %1, %10, %4 row_newbcast:%15 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %0, %11, %9 row_newbcast:%16 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %1, %10, %5 row_newbcast:%16 row_mask:0xf bank_mask:0xf"
+        : "=&v"(p), "=&v"(s1), "+v"(g0), "+v"(g1), "+v"(g2), "+v"(g3)
+        : "v"(h[0]), "v"(h[1]), "v"(h[2]), "v"(h[3]), "v"(b), "v"(c), "v"(q), "n"(FROM), "n"(FROM + 1), "n"(FROM + 2),
+          "n"(FROM + 3));
+    g = f4{g0, g1, g2, g3};
+#endif
 }
 __device__ __forceinline__ void fence() { asm volatile("" ::: "memory"); }
 
-// An address that all lanes share and a lane's own 32-bit offset from there: no vector arithmetic for an address.
+// A sequence's rows from one step on: addresses that all lanes share, and a lane's own 32-bit offset from there (no vector
+// arithmetic for an address).
 template <class R>
-__device__ __forceinline__ __attribute__((address_space(1))) R* place(R* p, uint32_t bytes) {
-    const uint64_t at = reinterpret_cast<uint64_t>(p);
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)at);
-    const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
-    asm("" : "+v"(bytes));  // opaque: its extension to 64 bits stays here, where a load takes it for nothing
-    return (__attribute__((address_space(1))) R*)((__attribute__((address_space(1))) char*)((uint64_t)hi << 32 | lo) + bytes);
-}
+struct Rows {
+    char* p;
+    int64_t ts;  // bytes
+    __device__ __forceinline__ Rows(const Seq<R>& s, uint32_t b, uint32_t t) : p(reinterpret_cast<char*>(s.p)), ts(s.ts * (int64_t)sizeof(R)) {
+        const uint64_t at = reinterpret_cast<uint64_t>(p) + (uint64_t)((int64_t)b * s.bs * (int64_t)sizeof(R) + (int64_t)t * ts);
+        const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)at);
+        const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
+        p = reinterpret_cast<char*>((uint64_t)hi << 32 | lo);
+    }
+    __device__ __forceinline__ void move(int steps) { p += steps * ts; }
+    __device__ __forceinline__ __attribute__((address_space(1))) R* at(uint32_t bytes) const {
+        asm("" : "+v"(bytes));  // opaque: its extension to 64 bits stays here, where a load takes it for nothing
+        return (__attribute__((address_space(1))) R*)((__attribute__((address_space(1))) char*)p + bytes);
+    }
+};
 template <class F, int... I>
 __device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
     (f(std::integral_constant<int, I>{}), ...);
@@ -125,28 +196,38 @@ struct Spot {
     }
 };
 
-// A tile's B or C of one quad as a wave holds them. For outer products: lane l has step l / 4, state l % 4. For inner
-// ones: register j has steps 4 j .. 4 j + 3, lane l step l / 16, state l / 4 % 4.
-template <class R>
-__device__ __forceinline__ R load_outer(const Seq<R>& m, uint32_t b, uint32_t col, uint32_t states, uint32_t t0, uint32_t n,
-                                        uint32_t lane) {
-    const uint32_t t = t0 + (lane >> 2), k = lane & 3;
-    R v = R(0);
-    if (k < states && t < n) v = m.at(b, t)[col + k];
-    return v;
-}
-template <class R>
-__device__ __forceinline__ void load_inner(const Seq<R>& m, uint32_t b, uint32_t col, uint32_t states, uint32_t t0,
-                                           uint32_t n, uint32_t lane, R (&o)[4]) {
-    const uint32_t k = lane >> 2 & 3;
-    const R* p = m.at(b, t0 + (lane >> 4)) + (col + k);
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        o[j] = R(0);
-        if (k < states && t0 + 4 * j + (lane >> 4) < n) o[j] = *p;
-        p += 4 * m.ts;
+// A tile's B or C of NS states as a wave holds them: register j has 16 / NS steps, lane l of a row step l / NS of them and
+// state l % NS. p: the lane's own element of register 0, null where it has no such state.
+template <class R, int NS>
+struct Vectors {
+    static constexpr int kSteps = 16 / NS;
+    const R* p;
+    int64_t ts;
+    uint32_t step;
+    __device__ __forceinline__ Vectors(const Seq<R>& m, uint32_t b, uint32_t t, uint32_t group, uint32_t n, uint32_t q,
+                                       uint32_t lane)
+        : p(nullptr), ts(m.ts), step((lane & 15) / NS) {
+        const uint32_t k = NS * q + lane % NS;
+        if (k < n) p = m.at(b, t + step) + (group * n + k);
     }
-}
+    // the tile that p is at, `left` steps of it there
+    __device__ __forceinline__ void load(uint32_t left, R (&o)[NS]) const {
+#pragma unroll
+        for (int j = 0; j < NS; j++) o[j] = R(0);
+        if (!p) return;
+        if (left >= kTile) {
+#pragma unroll
+            for (int j = 0; j < NS; j++) o[j] = p[kSteps * j * ts];
+        } else {
+#pragma unroll
+            for (int j = 0; j < NS; j++)
+                if (kSteps * j + step < left) o[j] = p[kSteps * j * ts];
+        }
+    }
+    __device__ __forceinline__ void move(int steps) {
+        if (p) p += steps * ts;
+    }
+};
 
 // the states of quad q of a [b][d][n] tensor
 __device__ __forceinline__ f4 load_states(const float* p, uint64_t at, uint32_t n, uint32_t q) {
@@ -178,13 +259,119 @@ __device__ __forceinline__ f4 fma4(f4 a, f4 b, f4 c) {
     return c;
 }
 
-// W waves, NQ quads of states each. FOLD: the segments' ends from zeros.
-template <class T, int W, int NQ, bool FOLD>
+// What a wave reads of the steps that it prepares: j * W + wave of a tile.
+template <class R, int W>
+struct Inputs {
+    static constexpr int K = kTile / W;
+    R x[K], dt[K], z[K];
+};
+template <class R, int W>
+struct Reader {
+    Rows<R> x, dt, z;
+    bool gate;
+    __device__ __forceinline__ Reader(const SsmArgs<R>& g, uint32_t b, uint32_t t, bool gated)
+        : x(g.x, b, t), dt(g.dt, b, t), z(g.z, b, t), gate(gated && g.z.p) {}
+    // the next tile, `left` steps of it there; a step that is not there is read as zeros
+    __device__ __forceinline__ void load(uint32_t own, uint32_t wave, uint32_t left, Inputs<R, W>& o) {
+        Rows<R> px = x, pt = dt, pz = z;
+        const bool full = left >= kTile;
+#pragma unroll
+        for (int j = 0; j < kTile / W; j++) {
+            o.x[j] = o.dt[j] = o.z[j] = R(0);
+            if (full || j * W + wave < left) {
+                o.x[j] = *px.at(own), o.dt[j] = *pt.at(own);
+                if (gate) o.z[j] = *pz.at(own);
+            }
+            px.move(W), pt.move(W), pz.move(W);
+        }
+        x.move(kTile), dt.move(kTile), z.move(kTile);
+    }
+};
+
+// The ends of segments from zeros: W waves, NQ quads of states each.
+template <class T, int W, int NQ>
+__global__ __launch_bounds__(64 * W, 2) void ssm_fold(SsmArgs<typename T::Raw> g) {
+    using R = typename T::Raw;
+    constexpr int K = kTile / W;
+    __shared__ float2 steps[2][kTile][64];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Spot at(g, lane);
+    const uint32_t b = at.walk, ch = at.ch, own = ch * (uint32_t)sizeof(R);
+    const uint64_t flat = (uint64_t)b * g.d + ch, slots = (uint64_t)g.b * g.quads * g.d;
+    const uint32_t n = g.lengths ? (uint32_t)min(max(g.lengths[b], 0), (int32_t)g.t) : g.t;
+    const uint32_t first = at.seg * g.seg_tiles, last = min(first + g.seg_tiles, g.tiles);
+    const uint32_t busy = min(last, (n + kTile - 1) / kTile);
+    const float bias = g.bias ? g.bias[ch] : 0.0f;
+    f4 rate[NQ], h[NQ];
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NQ; i++) {
+        const uint32_t q = wave + W * i;
+        rate[i] = rates_of(g.a, ch, g.n, q);
+        h[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        // the second launch reads the first state here: the last one may lie over h0
+        if (at.seg == 0 && q < g.quads && at.live) g.ends[((uint64_t)b * g.quads + q) * g.d + ch] = load_states(g.h0, flat, g.n, q);
+    }
+    Reader<R, W> reader(g, b, first * kTile + wave, false);
+    Vectors<R, 4> vec0(g.bm, b, first * kTile, at.group, g.n, wave, lane), vec1(g.bm, b, first * kTile, at.group, g.n, wave + W * (NQ - 1), lane);
+    Inputs<R, W> in;
+    R bm[NQ][4];
+    float bv[NQ][4];
+    auto load = [&](uint32_t left) {
+        reader.load(own, wave, left, in);
+        vec0.load(left, bm[0]), vec0.move(kTile);
+        if constexpr (NQ > 1) vec1.load(left, bm[1]), vec1.move(kTile);
+    };
+    auto prepare = [&](uint32_t left, int buf) {
+#pragma unroll
+        for (int j = 0; j < K; j++) {
+            float e;
+            const float d = softplus(widen(T{}, in.dt[j]) + bias, e), step = j * W + wave < left ? d : 0.0f;
+            steps[buf][j * W + wave][lane] = float2{step, step * widen(T{}, in.x[j])};
+        }
+    };
+    uint32_t left = first < busy ? n - first * kTile : 0;  // steps of the sequence from the tile on
+    if (left) {
+        load(left);
+        prepare(left, 0);
+    }
+    for (uint32_t tile = first; tile < busy; tile++, left -= kTile) {
+        const int buf = (tile - first) & 1;
+#pragma unroll
+        for (int i = 0; i < NQ; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) bv[i][j] = widen(T{}, bm[i][j]);
+        const bool more = tile + 1 < busy;
+        if (more) load(left - kTile);
+        __syncthreads();
+        each<kTile>([&](auto c) {
+            constexpr int s = c;
+            const float2 st = steps[buf][s][lane];
+            sum += st.x;
+#pragma unroll
+            for (int i = 0; i < NQ; i++) {
+                h[i] *= decay(st.x, rate[i]);
+                add_outer<(s & 3) * 4>(h[i], bv[i][s >> 2], st.y);
+            }
+        });
+        if (more) prepare(left - kTile, buf ^ 1);
+    }
+#pragma unroll
+    for (int i = 0; i < NQ; i++) {
+        const uint32_t q = wave + W * i;
+        if (q < g.quads && at.live) g.ends[(at.seg + 1) * slots + ((uint64_t)b * g.quads + q) * g.d + ch] = h[i];
+    }
+    if (wave == 0 && at.live) g.lasts[(uint64_t)at.seg * g.b * g.d + flat] = sum;
+}
+
+// W waves, NQ times NS states each. One barrier a tile: while a tile runs, the next one's steps are prepared and the one
+// before is finished, into and from the other halves of the buffers.
+template <class T, int W, int NQ, int NS>
 __global__ __launch_bounds__(64 * W, 2) void ssm_fwd(SsmArgs<typename T::Raw> g) {
     using R = typename T::Raw;
-    constexpr int K = kTile / W;  // steps that a wave prepares: j * W + wave
-    __shared__ float2 steps[kTile][64];
-    __shared__ float parts[FOLD ? 1 : W][kTile][64];
+    constexpr int K = kTile / W, SPR = 16 / NS;  // steps that a wave prepares, j * W + wave; steps a register of vectors
+    __shared__ float2 steps[2][kTile][64];
+    __shared__ float parts[2][W][kTile][64];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Spot at(g, lane);
     const uint32_t b = at.walk, ch = at.ch, own = ch * (uint32_t)sizeof(R);
@@ -193,108 +380,131 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_fwd(SsmArgs<typename T::Raw> g)
     const uint32_t first = at.seg * g.seg_tiles, last = min(first + g.seg_tiles, g.tiles);
     const uint32_t busy = min(last, (n + kTile - 1) / kTile);
     const float bias = g.bias ? g.bias[ch] : 0.0f, skip = g.skip ? g.skip[ch] : 0.0f;
-    f4 rate[NQ], h[NQ];
-    float sum = 0.0f;
+    // state k of the wave's part i: number NS * (wave + W * i) + k
+    auto number = [&](int i, int k) { return NS * (wave + W * i) + k; };
+    // its place in a buffer of quads [quad][d] of 4
+    auto in_quads = [&](int i, int k) {
+        const uint32_t s = number(i, k);
+        return ((uint64_t)(s >> 2) * g.d + ch) * 4 + (s & 3);
+    };
+    States<NS> rate[NQ], h[NQ];
 #pragma unroll
     for (int i = 0; i < NQ; i++) {
-        const uint32_t q = wave + W * i;
-        const uint64_t slot = ((uint64_t)b * g.quads + q) * g.d + ch;
-        rate[i] = rates_of(g.a, ch, g.n, q);
-        h[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (FOLD || g.segs == 1) {
-            h[i] = load_states(g.h0, flat, g.n, q);
-        } else if (q < g.quads) {
-            h[i] = g.ends[slot];
-            for (uint32_t s = 0; s < at.seg; s++)
-                h[i] = fma4(decay(g.lasts[(uint64_t)s * g.b * g.d + flat], rate[i]), h[i], g.ends[(s + 1) * slots + slot]);
-        }
-        if constexpr (FOLD) {  // the second launch reads the first state here: the last one may lie over h0
-            if (at.seg == 0 && q < g.quads && at.live) g.ends[slot] = h[i];
-            h[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
-    }
-    R x[K], dt[K], z[K], bo[NQ], ci[NQ][4];
-    auto load = [&](uint32_t tile) {
 #pragma unroll
-        for (int j = 0; j < K; j++) {
-            const uint32_t t = tile * kTile + j * W + wave;
-            x[j] = dt[j] = z[j] = R(0);
-            if (t < n) {
-                x[j] = *place(g.x.at(b, t), own), dt[j] = *place(g.dt.at(b, t), own);
-                if (!FOLD && g.z.p) z[j] = *place(g.z.at(b, t), own);
+        for (int k = 0; k < NS; k++) {
+            const uint32_t s = number(i, k);
+            rate[i].v[k] = s < g.n ? rate_of(g.a[(uint64_t)ch * g.n + s]) : 0.0f;
+            h[i].v[k] = s < g.n && g.segs == 1 && g.h0 ? g.h0[flat * g.n + s] : 0.0f;
+        }
+        if (g.segs > 1 && number(i, 0) < g.n) {
+            const float* p = reinterpret_cast<const float*>(g.ends + (uint64_t)b * g.quads * g.d);
+#pragma unroll
+            for (int k = 0; k < NS; k++) h[i].v[k] = p[in_quads(i, k)];
+            for (uint32_t s = 0; s < at.seg; s++) {
+                p += slots * 4;
+                const float total = g.lasts[(uint64_t)s * g.b * g.d + flat];
+#pragma unroll
+                for (int k = 0; k < NS; k++)
+                    h[i].v[k] = __builtin_fmaf(__builtin_amdgcn_exp2f(rate[i].v[k] * total), h[i].v[k], p[in_quads(i, k)]);
             }
         }
+    }
+    Reader<R, W> reader(g, b, first * kTile + wave, true);
+    Vectors<R, NS> vb0(g.bm, b, first * kTile, at.group, g.n, wave, lane), vc0(g.cm, b, first * kTile, at.group, g.n, wave, lane);
+    Vectors<R, NS> vb1(g.bm, b, first * kTile, at.group, g.n, wave + W * (NQ - 1), lane);
+    Vectors<R, NS> vc1(g.cm, b, first * kTile, at.group, g.n, wave + W * (NQ - 1), lane);
+    Rows<R> ry(g.y, b, first * kTile + wave);
+    Inputs<R, W> in;
+    R bm[NQ][NS], cm[NQ][NS], x[2][K], z[2][K];  // x and z of the tile that runs, and of the one before
+    float bv[NQ][NS], cv[NQ][NS];
+    auto load = [&](uint32_t left) {
+        reader.load(own, wave, left, in);
+        vb0.load(left, bm[0]), vb0.move(kTile), vc0.load(left, cm[0]), vc0.move(kTile);
+        if constexpr (NQ > 1) vb1.load(left, bm[NQ - 1]), vb1.move(kTile), vc1.load(left, cm[NQ - 1]), vc1.move(kTile);
+    };
+    auto prepare = [&](uint32_t left, int buf) {
 #pragma unroll
-        for (int i = 0; i < NQ; i++) {
-            const uint32_t q = wave + W * i, states = g.n > 4 * q ? g.n - 4 * q : 0, col = at.group * g.n + 4 * q;
-            bo[i] = load_outer(g.bm, b, col, states, tile * kTile, n, lane);
-            if (!FOLD) load_inner(g.cm, b, col, states, tile * kTile, n, lane, ci[i]);
+        for (int j = 0; j < K; j++) {
+            float e;
+            const float d = softplus(widen(T{}, in.dt[j]) + bias, e), step = j * W + wave < left ? d : 0.0f;
+            steps[buf][j * W + wave][lane] = float2{step, step * widen(T{}, in.x[j])};
         }
     };
-    if (first < busy) load(first);
-    for (uint32_t tile = first; tile < busy; tile++) {
-        float xs[K], zs[K], bv[NQ], cv[NQ][4];
+    // left: of the tile's steps those inside the length; there: those inside the tensor
+    auto finish = [&](uint32_t left, uint32_t there, int buf) {
+        Rows<R> py = ry;
 #pragma unroll
         for (int j = 0; j < K; j++) {
             const uint32_t s = j * W + wave;
-            float e;
-            const float step = tile * kTile + s < n ? softplus(widen(T{}, dt[j]) + bias, e) : 0.0f;
-            xs[j] = widen(T{}, x[j]), zs[j] = widen(T{}, z[j]);
-            steps[s][lane] = float2{step, step * xs[j]};
-        }
+            float p = skip * widen(T{}, x[1][j]);
 #pragma unroll
-        for (int i = 0; i < NQ; i++) {
-            bv[i] = widen(T{}, bo[i]);
-#pragma unroll
-            for (int j = 0; j < 4 && !FOLD; j++) cv[i][j] = widen(T{}, ci[i][j]);
+            for (int w = 0; w < W; w++) p += parts[buf][w][s][lane];
+            if (g.z.p) {
+                const float v = widen(T{}, z[1][j]);
+                p *= v * sigmoid1(v);
+            }
+            if (s < there && at.live) *py.at(own) = s < left ? narrow(T{}, p) : R(0);
+            py.move(W);
         }
-        __syncthreads();
-        if (tile + 1 < busy) load(tile + 1);
-        if (!FOLD && g.states && at.live) {
+        ry.move(kTile);
+    };
+    uint32_t left = first < busy ? n - first * kTile : 0;  // steps of the sequence from the tile on
+    if (left) {
+        load(left);
+        prepare(left, 0);
+    }
+    for (uint32_t tile = first; tile < busy; tile++, left -= kTile) {
+        const int buf = (tile - first) & 1;
 #pragma unroll
-            for (int i = 0; i < NQ; i++)
-                if (wave + W * i < g.quads)
-                    g.states[(((uint64_t)b * g.tiles + tile) * g.quads + wave + W * i) * g.d + ch] = h[i];
-        }
-        each<kTile>([&](auto c) {
-            constexpr int s = c;
-            const float2 st = steps[s][lane];
-            if constexpr (FOLD) sum += st.x;
-            f4 p = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < K; j++) x[1][j] = x[0][j], x[0][j] = in.x[j], z[1][j] = z[0][j], z[0][j] = in.z[j];
+#pragma unroll
+        for (int i = 0; i < NQ; i++)
+#pragma unroll
+            for (int j = 0; j < NS; j++) bv[i][j] = widen(T{}, bm[i][j]), cv[i][j] = widen(T{}, cm[i][j]);
+        const bool more = tile + 1 < busy;
+        if (more) load(left - kTile);
+        if (g.states && at.live) {
+            float* to = reinterpret_cast<float*>(g.states + ((uint64_t)b * g.tiles + tile) * g.quads * g.d);
 #pragma unroll
             for (int i = 0; i < NQ; i++) {
-                h[i] = outer<s>(bv[i], st.y, decay(st.x, rate[i]) * h[i]);
-                if constexpr (!FOLD) p = inner<(s & 3) * 4>(cv[i][s >> 2], h[i], p);
+                if (number(i, 0) >= 4 * g.quads) continue;
+                if constexpr (NS == 4) *reinterpret_cast<f4*>(to + in_quads(i, 0)) = f4{h[i].v[0], h[i].v[1], h[i].v[2], h[i].v[3]};
+                else *reinterpret_cast<float2*>(to + in_quads(i, 0)) = float2{h[i].v[0], h[i].v[1]};
             }
-            if constexpr (!FOLD) parts[wave][s][lane] = p[0];
-        });
+        }
         __syncthreads();
-        if constexpr (!FOLD) {
+        if (tile > first) finish(left + kTile, g.t - (tile - 1) * kTile, buf ^ 1);
+        each<kTile>([&](auto c) {
+            constexpr int s = c;
+            const float2 st = steps[buf][s][lane];
+            float p = 0.0f;
 #pragma unroll
-            for (int j = 0; j < K; j++) {
-                const uint32_t s = j * W + wave, t = tile * kTile + s;
-                float p = skip * xs[j];
+            for (int i = 0; i < NQ; i++) {
 #pragma unroll
-                for (int w = 0; w < W; w++) p += parts[w][s][lane];
-                if (g.z.p) p *= zs[j] * sigmoid1(zs[j]);
-                if (t < g.t && at.live) *place(g.y.at(b, t), own) = t < n ? narrow(T{}, p) : R(0);
+                for (int k = 0; k < NS; k++) h[i].v[k] *= __builtin_amdgcn_exp2f(st.x * rate[i].v[k]);
+                const float q = step_states<s % SPR * NS>(h[i], bv[i][s / SPR], st.y, cv[i][s / SPR]);
+                p = i ? p + q : q;
             }
-        }
+            parts[buf][wave][s][lane] = p;
+        });
+        if (more) prepare(left - kTile, buf ^ 1);
     }
-    if constexpr (FOLD) {
+    __syncthreads();
+    if (first < busy) {
 #pragma unroll
-        for (int i = 0; i < NQ; i++) {
-            const uint32_t q = wave + W * i;
-            if (q < g.quads && at.live) g.ends[(at.seg + 1) * slots + ((uint64_t)b * g.quads + q) * g.d + ch] = h[i];
-        }
-        if (wave == 0 && at.live) g.lasts[(uint64_t)at.seg * g.b * g.d + flat] = sum;
-    } else {
-        for (uint32_t t = max(busy, first) * kTile + wave; t < min(last * kTile, g.t); t += W)
-            if (at.live) *place(g.y.at(b, t), own) = R(0);
-        if (g.ht && at.live && last == g.tiles) {
+        for (int j = 0; j < K; j++) x[1][j] = x[0][j], z[1][j] = z[0][j];
+        finish(n - (busy - 1) * kTile, g.t - (busy - 1) * kTile, (busy - 1 - first) & 1);
+    }
+    for (uint32_t t = max(busy, first) * kTile + wave; t < min(last * kTile, g.t); t += W) {
+        if (at.live) *ry.at(own) = R(0);
+        ry.move(W);
+    }
+    if (g.ht && at.live && last == g.tiles) {
 #pragma unroll
-            for (int i = 0; i < NQ; i++) store_states(g.ht, flat, g.n, wave + W * i, h[i]);
-        }
+        for (int i = 0; i < NQ; i++)
+#pragma unroll
+            for (int k = 0; k < NS; k++)
+                if (number(i, k) < g.n) g.ht[flat * g.n + number(i, k)] = h[i].v[k];
     }
 }
 
@@ -416,40 +626,54 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void ssm_bwd(SsmArgs<typena
                     c[i] = fma4(decay(g.lasts[(uint64_t)s * g.b * g.d + flat], rate[i]), c[i], g.ends[s * slots + slot]);
             }
         }
-        R x[K], dt[K], z[K], dy[K], bo[NQ], co[NQ], bi[NQ][4], ci[NQ][4];
+        R x[K], dt[K], z[K], dy[K], bm[NQ][4], cm[NQ][4];
         f4 start[NQ];
+        const uint32_t from = busy > first ? (busy - 1) * kTile : 0;  // tiles go from the last to the first
+        Rows<R> rx(g.x, b, from + wave), rdt(g.dt, b, from + wave), rz(g.z, b, from + wave), rdy(g.dy, b, from + wave);
+        struct Pair {
+            Vectors<R, 4> b, c;
+        };
+        auto vectors_of = [&](int i) {
+            return Pair{Vectors<R, 4>(g.bm, b, from, at.group, g.n, wave + W * i, lane),
+                        Vectors<R, 4>(g.cm, b, from, at.group, g.n, wave + W * i, lane)};
+        };
+        Pair vec[2] = {vectors_of(0), vectors_of(NQ - 1)};
         auto load = [&](uint32_t tile) {
+            const uint32_t left = n - tile * kTile;
+            Rows<R> px = rx, pt = rdt, pz = rz, py = rdy;
 #pragma unroll
             for (int j = 0; j < K; j++) {
-                const uint32_t t = tile * kTile + j * W + wave;
                 x[j] = dt[j] = z[j] = dy[j] = R(0);
-                if (t < n) {
-                    if (!FOLD) x[j] = *place(g.x.at(b, t), own);
-                    dt[j] = *place(g.dt.at(b, t), own), dy[j] = *place(g.dy.at(b, t), own);
-                    if (g.z.p) z[j] = *place(g.z.at(b, t), own);
+                if (j * W + wave < left) {
+                    if (!FOLD) x[j] = *px.at(own);
+                    dt[j] = *pt.at(own), dy[j] = *py.at(own);
+                    if (g.z.p) z[j] = *pz.at(own);
                 }
+                px.move(W), pt.move(W), pz.move(W), py.move(W);
             }
+            rx.move(-kTile), rdt.move(-kTile), rz.move(-kTile), rdy.move(-kTile);
 #pragma unroll
             for (int i = 0; i < NQ; i++) {
-                const uint32_t q = wave + W * i, states = g.n > 4 * q ? g.n - 4 * q : 0, col = at.group * g.n + 4 * q;
-                co[i] = load_outer(g.cm, b, col, states, tile * kTile, n, lane);
+                const uint32_t q = wave + W * i;
+                vec[i].c.load(left, cm[i]);
+                vec[i].c.move(-kTile);
                 if constexpr (!FOLD) {
-                    bo[i] = load_outer(g.bm, b, col, states, tile * kTile, n, lane);
-                    load_inner(g.bm, b, col, states, tile * kTile, n, lane, bi[i]);
-                    load_inner(g.cm, b, col, states, tile * kTile, n, lane, ci[i]);
+                    vec[i].b.load(left, bm[i]);
+                    vec[i].b.move(-kTile);
                     start[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
                     if (q < g.quads && at.live) start[i] = g.states[(((uint64_t)b * g.tiles + tile) * g.quads + q) * g.d + ch];
                 }
             }
         };
+        Rows<R> rdx(g.dx, b, from + wave), rddt(g.ddt, b, from + wave), rdz(g.dz, b, from + wave);
         if (first < busy) load(busy - 1);
-        for (uint32_t left = busy; left > first; left--) {
-            const uint32_t tile = left - 1;
-            float xs[K], slope[K], zg[K], bv[NQ], cv[NQ], bw[NQ][4], cw[NQ][4];  // the step's slope; dy silu'(z)
+        for (uint32_t end = busy; end > first; end--) {
+            const uint32_t tile = end - 1, left = n - tile * kTile;
+            float xs[K], slope[K], zg[K], bv[NQ][4], cv[NQ][4];  // the step's slope; dy silu'(z)
 #pragma unroll
             for (int j = 0; j < K; j++) {
                 const uint32_t s = j * W + wave;
-                const bool on = tile * kTile + s < n && at.live;  // a lane without a channel adds nothing to dB and dC
+                const bool on = s < left && at.live;  // a lane without a channel adds nothing to dB and dC
                 const float v = widen(T{}, dt[j]) + bias, up = widen(T{}, dy[j]);
                 float e, gate = 1.0f, dgate = 0.0f;
                 const float d = softplus(v, e), step = on ? d : 0.0f;
@@ -458,17 +682,17 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void ssm_bwd(SsmArgs<typena
                     const float r = __builtin_amdgcn_rcpf(1.0f + e);
                     xs[j] = widen(T{}, x[j]), slope[j] = v >= 0.0f ? r : e * r, zg[j] = up * dgate;
                 }
-                steps[s][lane] = float2{step, FOLD ? 0.0f : step * xs[j]};
+                steps[s][lane] = float2{step, FOLD || !on ? 0.0f : step * xs[j]};
                 ups[s][lane] = on ? up * gate : 0.0f;
             }
             f4 h0[NQ];
 #pragma unroll
             for (int i = 0; i < NQ; i++) {
-                cv[i] = widen(T{}, co[i]);
-                if constexpr (!FOLD) {
-                    bv[i] = widen(T{}, bo[i]), h0[i] = start[i];
+                if constexpr (!FOLD) h0[i] = start[i];
 #pragma unroll
-                    for (int j = 0; j < 4; j++) bw[i][j] = widen(T{}, bi[i][j]), cw[i][j] = widen(T{}, ci[i][j]);
+                for (int j = 0; j < 4; j++) {
+                    cv[i][j] = widen(T{}, cm[i][j]);
+                    if constexpr (!FOLD) bv[i][j] = widen(T{}, bm[i][j]);
                 }
             }
             __syncthreads();
@@ -479,7 +703,10 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void ssm_bwd(SsmArgs<typena
                     const float step = steps[s][lane].x, q = ups[s][lane];
                     sum += step;
 #pragma unroll
-                    for (int i = 0; i < NQ; i++) c[i] = decay(step, rate[i]) * outer<s>(cv[i], q, c[i]);
+                    for (int i = 0; i < NQ; i++) {
+                        add_outer<(s & 3) * 4>(c[i], cv[i][s >> 2], q);
+                        c[i] *= decay(step, rate[i]);
+                    }
                 });
             } else {
 #pragma unroll
@@ -494,7 +721,8 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void ssm_bwd(SsmArgs<typena
                         each<4>([&](auto rc) {
                             constexpr int s = 4 * m + rc;
                             a[s] = decay(st[rc].x, rate[i]);
-                            h[s] = outer<s>(bv[i], st[rc].y, a[s] * (s ? h[s ? s - 1 : 0] : h0[i]));
+                            h[s] = a[s] * (s ? h[s ? s - 1 : 0] : h0[i]);
+                            add_outer<rc * 4>(h[s], bv[i][m], st[rc].y);
                         });
                     });
                     float m4 = 0.0f, m2 = 0.0f, m1 = 0.0f;  // sums of odd steps that wait for their even neighbours
@@ -507,13 +735,11 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void ssm_bwd(SsmArgs<typena
                         fence();
                         each<4>([&](auto rc) {
                             constexpr int r = 3 - rc, s = 4 * m + r;
-                            const f4 none = {0.0f, 0.0f, 0.0f, 0.0f};
-                            const f4 grad = outer<s>(cv[i], q[r], c[i]);
-                            float p = inner<r * 4>(cw[i][m], h[s], none)[0], s1 = inner<r * 4>(bw[i][m], grad, none)[0];
-                            const f4 db = grad * st[r].y, dc = h[s] * q[r];
-                            c[i] = grad * a[s];
+                            float p, s1, s2 = 0.0f;
+                            step_back<r * 4>(c[i], h[s], bv[i][m], cv[i][m], q[r], p, s1);
+                            const f4 db = c[i] * st[r].y, dc = h[s] * q[r];
+                            c[i] *= a[s];
                             const f4 past = c[i] * (s ? h[s ? s - 1 : 0] : h0[i]);
-                            float s2 = 0.0f;
 #pragma unroll
                             for (int k = 0; k < 4; k++) {
                                 da[i][k] = __builtin_fmaf(past[k], st[r].x, da[i][k]);
@@ -553,24 +779,27 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void ssm_bwd(SsmArgs<typena
             }
             __syncthreads();
             if constexpr (!FOLD) {
+                const uint32_t there = g.t - tile * kTile;
+                Rows<R> px = rdx, pt = rddt, pz = rdz;
 #pragma unroll
                 for (int j = 0; j < K; j++) {
-                    const uint32_t s = j * W + wave, t = tile * kTile + s;
+                    const uint32_t s = j * W + wave;
                     float p = 0.0f, s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
                     for (int w = 0; w < W; w++) p += parts[0][w][s][lane], s1 += parts[1][w][s][lane], s2 += parts[2][w][s][lane];
                     const float step = steps[s][lane].x, q = ups[s][lane];
                     const float dd = __builtin_fmaf(xs[j], s1, s2 * kLn2) * slope[j];
-                    if (t < n) dskip = __builtin_fmaf(q, xs[j], dskip), dbias += dd;
-                    if (t < g.t && at.live) {
-                        *place(g.dx.at(b, t), own) = t < n ? narrow(T{}, __builtin_fmaf(step, s1, skip * q)) : R(0);
-                        *place(g.ddt.at(b, t), own) = t < n ? narrow(T{}, dd) : R(0);
-                        if (g.z.p)
-                            *place(g.dz.at(b, t), own) = t < n ? narrow(T{}, zg[j] * __builtin_fmaf(skip, xs[j], p)) : R(0);
+                    if (s < left) dskip = __builtin_fmaf(q, xs[j], dskip), dbias += dd;
+                    if (s < there && at.live) {
+                        *px.at(own) = s < left ? narrow(T{}, __builtin_fmaf(step, s1, skip * q)) : R(0);
+                        *pt.at(own) = s < left ? narrow(T{}, dd) : R(0);
+                        if (g.z.p) *pz.at(own) = s < left ? narrow(T{}, zg[j] * __builtin_fmaf(skip, xs[j], p)) : R(0);
                     }
+                    px.move(W), pt.move(W), pz.move(W);
                 }
+                rdx.move(-kTile), rddt.move(-kTile), rdz.move(-kTile);
                 // the tile's dB and dC of this block, as they lie
-                const uint32_t row = 8 * g.quads, steps_here = min((uint32_t)kTile, g.t - tile * kTile);
+                const uint32_t row = 8 * g.quads, steps_here = min((uint32_t)kTile, there);
                 float* to = g.bc + (((uint64_t)(at.group * g.blocks + at.block) * g.b + b) * g.t + tile * kTile) * row;
                 for (uint32_t k = threadIdx.x; k < steps_here * row; k += 64 * W) {
                     const uint32_t s = k / row, v = k - s * row, half = v >= 4 * g.quads;
@@ -587,10 +816,14 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void ssm_bwd(SsmArgs<typena
             }
             if (wave == 0 && at.live) g.lasts[(uint64_t)at.seg * g.b * g.d + flat] = sum;
         } else {
-            for (uint32_t t = max(busy, first) * kTile + wave; t < min(last * kTile, g.t); t += W) {
-                if (!at.live) continue;
-                *place(g.dx.at(b, t), own) = *place(g.ddt.at(b, t), own) = R(0);
-                if (g.z.p) *place(g.dz.at(b, t), own) = R(0);
+            const uint32_t past = max(busy, first) * kTile + wave;
+            Rows<R> px(g.dx, b, past), pt(g.ddt, b, past), pz(g.dz, b, past);
+            for (uint32_t t = past; t < min(last * kTile, g.t); t += W) {
+                if (at.live) {
+                    *px.at(own) = *pt.at(own) = R(0);
+                    if (g.z.p) *pz.at(own) = R(0);
+                }
+                px.move(W), pt.move(W), pz.move(W);
             }
             if (g.dh0 && at.live && at.seg == 0) {
 #pragma unroll
@@ -664,6 +897,7 @@ constexpr uint32_t kFewSteps = 4;  // up to here the states' bytes are what coun
 
 struct Plan {
     uint32_t width, blocks, quads, waves, tiles, segs, seg_tiles, walks;
+    bool halves;  // forward: two states a lane
     uint64_t wgs;
     size_t ends_bytes, lasts_bytes, part_bytes, bc_bytes;
 };
@@ -671,7 +905,7 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 Plan plan_of(const fhc_ssm_desc* g, bool backward) {
     Plan p{};
     p.width = g->d / g->groups, p.blocks = (uint32_t)ceil_div(p.width, 64), p.quads = (g->n + 3) / 4;
-    p.waves = p.quads <= 1 ? 1 : p.quads <= 2 ? 2 : p.quads <= 4 ? 4 : 8;
+    p.waves = p.quads <= 1 ? 2 : p.quads <= 2 ? 4 : 8;  // at most
     p.tiles = (uint32_t)ceil_div(g->t, kTile);
     const uint64_t cols = (uint64_t)g->groups * p.blocks;
     const uint64_t one = g->b * cols;
@@ -681,6 +915,10 @@ Plan plan_of(const fhc_ssm_desc* g, bool backward) {
         p.segs = (uint32_t)(want < p.tiles / 4 ? want : p.tiles / 4);
         if (p.segs > 64) p.segs = 64;
         if (p.segs < 1) p.segs = 1;
+    }
+    if (!backward) {
+        if (const char* e = getenv("SSM_SEGS")) p.segs = atoi(e);
+        p.halves = p.quads <= 4 && getenv("SSM_HALVES") && atoi(getenv("SSM_HALVES"));
     }
     p.seg_tiles = p.tiles ? (uint32_t)ceil_div(p.tiles, p.segs) : 1;
     p.segs = p.tiles ? (uint32_t)ceil_div(p.tiles, p.seg_tiles) : 1;
@@ -732,19 +970,32 @@ SsmArgs<typename T::Raw> args_of(const fhc_ssm_desc* g, const Plan& p, const fhc
     return a;
 }
 
-template <class T, bool BWD, bool FOLD>
+enum Kernel { kFold, kForward, kFoldBack, kBackward };
+template <class T, Kernel KERNEL>
 int launch(const char* op, const Plan& p, const SsmArgs<typename T::Raw>& a, hipStream_t st) {
     const dim3 grid((uint32_t)p.wgs);
-#define SSM(W, NQ)                                                                                            \
-    do {                                                                                                      \
-        if constexpr (BWD) hipLaunchKernelGGL((ssm_bwd<T, W, NQ, FOLD>), grid, dim3(64 * W), 0, st, a);       \
-        else hipLaunchKernelGGL((ssm_fwd<T, W, NQ, FOLD>), grid, dim3(64 * W), 0, st, a);                     \
+#define SSM(W, NQ, NS)                                                                                             \
+    do {                                                                                                           \
+        if constexpr (KERNEL == kFold) hipLaunchKernelGGL((ssm_fold<T, W, NQ>), grid, dim3(64 * W), 0, st, a);     \
+        else if constexpr (KERNEL == kForward)                                                                     \
+            hipLaunchKernelGGL((ssm_fwd<T, W, NQ, NS>), grid, dim3(64 * W), 0, st, a);                             \
+        else if constexpr (KERNEL == kFoldBack)                                                                    \
+            hipLaunchKernelGGL((ssm_bwd<T, W, NQ, true>), grid, dim3(64 * W), 0, st, a);                           \
+        else hipLaunchKernelGGL((ssm_bwd<T, W, NQ, false>), grid, dim3(64 * W), 0, st, a);                         \
     } while (0)
-    if (p.waves == 1) SSM(1, 1);
-    else if (p.waves == 2) SSM(2, 1);
-    else if (p.waves == 4) SSM(4, 1);
-    else if (p.quads <= 8) SSM(8, 1);
-    else SSM(8, 2);
+    if constexpr (KERNEL == kForward) {
+        if (p.halves) {
+            if (p.quads == 1) SSM(2, 1, 2);
+            else if (p.quads == 2) SSM(4, 1, 2);
+            else SSM(8, 1, 2);
+            return launched(op);
+        }
+    }
+    if (p.quads == 1) SSM(1, 1, 4);
+    else if (p.quads == 2) SSM(2, 1, 4);
+    else if (p.quads <= 4) SSM(4, 1, 4);
+    else if (p.quads <= 8) SSM(8, 1, 4);
+    else SSM(8, 2, 4);
 #undef SSM
     return launched(op);
 }
@@ -821,8 +1072,8 @@ extern "C" int fhc_ssm_forward(const fhc_ssm_desc* g, const fhc_seq* x, const fh
                 rc = launch_step<T>(op, p, a, st);
                 return;
             }
-            if (p.segs > 1) rc = launch<T, false, true>(op, p, a, st);
-            if (rc == 0) rc = launch<T, false, false>(op, p, a, st);
+            if (p.segs > 1) rc = launch<T, kFold>(op, p, a, st);
+            if (rc == 0) rc = launch<T, kForward>(op, p, a, st);
         });
         return rc;
     });
@@ -868,8 +1119,8 @@ extern "C" int fhc_ssm_backward(const fhc_ssm_desc* g, const fhc_seq* x, const f
             auto a = args_of<T>(g, p, x, dt, bm, cm, z, ws);
             a.states = reinterpret_cast<f4*>(const_cast<float*>(states)), a.dy = seq_of<R>(dy), a.dht = dht;
             a.dx = seq_of<R>(dx), a.ddt = seq_of<R>(ddt), a.dz = seq_of<R>(dz), a.dh0 = dh0;
-            if (p.segs > 1) rc = launch<T, true, true>(op, p, a, st);
-            if (rc == 0) rc = launch<T, true, false>(op, p, a, st);
+            if (p.segs > 1) rc = launch<T, kFoldBack>(op, p, a, st);
+            if (rc == 0) rc = launch<T, kBackward>(op, p, a, st);
             if (rc == 0) rc = close_vectors<T>(op, g, a.bc, dbm, dcm, p.blocks, st);
         });
         if (rc < 0) return rc;
