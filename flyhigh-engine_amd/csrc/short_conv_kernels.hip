@@ -29,6 +29,7 @@ struct ConvArgs {
     uint32_t chunks, steps, items;  // chunks of `steps` a sequence; b * chunks
     uint32_t walks;                 // backward: workgroups that a column block's items are dealt to
     bool silu;
+    bool whole;  // the last thread of a row takes its last V channels, some of them twice: the same bytes are stored twice
 };
 
 constexpr uint32_t kThreads = 256;
@@ -85,13 +86,14 @@ struct Taps {
 template <int V>
 struct Place {
     uint32_t ch, b, t0, n;
-    int valid;
+    int valid, twice;  // channels there; those of them, from the first on, that the lane before has too
     bool live;
     template <class R>
     __device__ __forceinline__ Place(const ConvArgs<R>& g, uint32_t cb, uint32_t item) {
         const uint32_t cg = (cb << g.lanes) + (threadIdx.x & ((1u << g.lanes) - 1));
         live = cg < g.groups && item < g.items;
-        ch = live ? cg * V : 0;
+        ch = live ? cg * V : 0, twice = 0;
+        if (g.whole && live && ch + V > g.d) twice = ch + V - g.d, ch = g.d - V;
         valid = live ? min(V, (int)(g.d - ch)) : 0;
         const uint32_t k = live ? item : 0;
         b = k / g.chunks;
@@ -324,7 +326,7 @@ __global__ __launch_bounds__(kThreads) void short_conv_bwd(ConvArgs<typename T::
             for (int v = 0; v < V; v++) {
                 float s = 0.0f;
                 for (uint32_t r = 0; r < rows; r++) s += sums[v][(r << g.lanes) + threadIdx.x];
-                if (v < mine.valid) part[k < K ? (uint64_t)(mine.ch + v) * K + k : (uint64_t)g.d * K + mine.ch + v] = s;
+                if (v < mine.valid && v >= mine.twice) part[k < K ? (uint64_t)(mine.ch + v) * K + k : (uint64_t)g.d * K + mine.ch + v] = s;
             }
         }
         __syncthreads();
@@ -384,7 +386,7 @@ ConvArgs<typename T::Raw> args_of(const fhc_short_conv_desc* g, const Plan& p, c
     a.state = static_cast<const R*>(state), a.lengths = g->lengths;
     a.b = g->b, a.t = g->t, a.d = g->d, a.groups = p.groups, a.lanes = p.lanes, a.colblocks = p.colblocks;
     a.chunks = p.chunks, a.steps = p.steps, a.items = p.items, a.walks = p.walks;
-    a.silu = g->act == FHC_ACT_SILU;
+    a.silu = g->act == FHC_ACT_SILU, a.whole = g->d >= p.v;
     return a;
 }
 
@@ -429,6 +431,8 @@ extern "C" int fhc_short_conv_forward(const fhc_short_conv_desc* g, const fhc_se
             using R = typename T::Raw;
             auto a = args_of<T>(g, p, x, state);
             a.y = seq_of<R>(y), a.end = static_cast<R*>(state_out);
+            // over the old state, both threads of a channel have to read it before either writes: the same wave's do
+            if (state && state == state_out && p.groups % (1u << p.lanes) == 1) a.whole = false;
             launch<T, false>(g->k, (uint32_t)grid, a, (hipStream_t)stream);
         });
         return launched(op);

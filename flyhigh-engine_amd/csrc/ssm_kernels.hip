@@ -151,25 +151,24 @@ __device__ __forceinline__ void step_back(f4& g, f4 h, float b, float c, float q
 #endif
 }
 __device__ __forceinline__ void fence() { asm volatile("" ::: "memory"); }
+// and nothing is scheduled across, so that registers hold the work of one group of steps at a time
+__device__ __forceinline__ void group() {
+    fence();
+    __builtin_amdgcn_sched_barrier(0);
+}
+// A barrier for what lies in LDS: __syncthreads would also wait for the next tile's loads, which are under way.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+// The values are in registers from here on: what they come from has been waited for.
+template <int N>
+__device__ __forceinline__ void settle(float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) asm volatile("" : "+v"(v[i]));
+}
 
-// A sequence's rows from one step on: addresses that all lanes share, and a lane's own 32-bit offset from there (no vector
-// arithmetic for an address).
-template <class R>
-struct Rows {
-    char* p;
-    int64_t ts;  // bytes
-    __device__ __forceinline__ Rows(const Seq<R>& s, uint32_t b, uint32_t t) : p(reinterpret_cast<char*>(s.p)), ts(s.ts * (int64_t)sizeof(R)) {
-        const uint64_t at = reinterpret_cast<uint64_t>(p) + (uint64_t)((int64_t)b * s.bs * (int64_t)sizeof(R) + (int64_t)t * ts);
-        const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)at);
-        const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
-        p = reinterpret_cast<char*>((uint64_t)hi << 32 | lo);
-    }
-    __device__ __forceinline__ void move(int steps) { p += steps * ts; }
-    __device__ __forceinline__ __attribute__((address_space(1))) R* at(uint32_t bytes) const {
-        asm("" : "+v"(bytes));  // opaque: its extension to 64 bits stays here, where a load takes it for nothing
-        return (__attribute__((address_space(1))) R*)((__attribute__((address_space(1))) char*)p + bytes);
-    }
-};
 template <class F, int... I>
 __device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
     (f(std::integral_constant<int, I>{}), ...);
@@ -180,13 +179,16 @@ __device__ __forceinline__ void each(F&& f) {
     each_of(f, std::make_integer_sequence<int, N>{});
 }
 
-// Where a workgroup is.
+// Where a workgroup is. Workgroups go round-robin to the 8 XCDs: the index is permuted so that an XCD has neighbouring channel
+// blocks. (A block's rows are one 128-byte line each. With every eighth block an XCD's lines lie on 2 of its L2's 16
+// channels, and the wait for them is what a tile takes: 4 x 4096 x 4096 bf16 815 us, with neighbours XXX.)
 struct Spot {
     uint32_t seg, walk, group, block, ch;
     bool live;
     template <class R>
     __device__ __forceinline__ Spot(const SsmArgs<R>& g, uint32_t lane) {
-        uint32_t q = blockIdx.x;
+        const uint32_t share = gridDim.x / 8, more = gridDim.x % 8, xcd = blockIdx.x % 8;
+        uint32_t q = xcd * share + min(xcd, more) + blockIdx.x / 8;
         block = q % g.blocks, q /= g.blocks;
         group = q % g.groups, q /= g.groups;
         walk = q % g.walks, seg = q / g.walks;
@@ -196,38 +198,148 @@ struct Spot {
     }
 };
 
-// A tile's B or C of NS states as a wave holds them: register j has 16 / NS steps, lane l of a row step l / NS of them and
-// state l % NS. p: the lane's own element of register 0, null where it has no such state.
+__device__ __forceinline__ void swap32(float& a, float& b) {  // {a0 a1 b0 b1}, {a2 a3 b2 b3} by rows of 16 lanes
+#if defined(__HIP_DEVICE_COMPILE__)
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
+    const uint32_t p = r[0], q = r[1];  // (a cast of a vector's element itself takes the first one's bits for every index)
+    a = __builtin_bit_cast(float, p), b = __builtin_bit_cast(float, q);
+#endif
+}
+__device__ __forceinline__ void swap16(float& a, float& b) {  // {a0 b0 a2 b2}, {a1 b1 a3 b3}
+#if defined(__HIP_DEVICE_COMPILE__)
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
+    const uint32_t p = r[0], q = r[1];
+    a = __builtin_bit_cast(float, p), b = __builtin_bit_cast(float, q);
+#endif
+}
+// A tile's B or C of NS states: lane l reads step l / NS and state l % NS, one load, and rows of lanes are then spread over
+// the wave: register j has the 16 / NS steps of row j in every row.
 template <class R, int NS>
 struct Vectors {
-    static constexpr int kSteps = 16 / NS;
     const R* p;
     int64_t ts;
     uint32_t step;
+    bool has;
     __device__ __forceinline__ Vectors(const Seq<R>& m, uint32_t b, uint32_t t, uint32_t group, uint32_t n, uint32_t q,
                                        uint32_t lane)
-        : p(nullptr), ts(m.ts), step((lane & 15) / NS) {
+        : ts(m.ts), step(lane / NS % kTile) {
         const uint32_t k = NS * q + lane % NS;
-        if (k < n) p = m.at(b, t + step) + (group * n + k);
+        has = k < n;
+        p = m.at(b, t + step) + (group * n + (has ? k : 0));
     }
     // the tile that p is at, `left` steps of it there
-    __device__ __forceinline__ void load(uint32_t left, R (&o)[NS]) const {
+    __device__ __forceinline__ R load(uint32_t left) const { return has && step < left ? *p : R(0); }
+    __device__ __forceinline__ void move(int steps) { p += steps * ts; }
+};
+template <int NS>
+__device__ __forceinline__ void spread(float v, float (&o)[NS]) {
+    if constexpr (NS == 4) {
+        o[0] = o[2] = v;
+        swap32(o[0], o[2]);
+        o[1] = o[0], o[3] = o[2];
+        swap16(o[0], o[1]);
+        swap16(o[2], o[3]);
+    } else {  // lanes 32 up have the same values as those below
+        o[0] = o[1] = v;
+        swap16(o[0], o[1]);
+    }
+}
+
+// A wave's part of a tile outside the states: 16 / W steps, wave * K + row, each on 64 / K lanes of K adjacent channels
+// (one wide load a tensor).
+template <class R, int W>
+struct Part {
+    static constexpr int K = kTile / W;
+    uint32_t step, c0;  // of the tile; of the block's channels
+    int valid;          // channels there
+    __device__ __forceinline__ Part(uint32_t lane, uint32_t wave, uint32_t width, uint32_t block)
+        : step(wave * K + lane / (64 / K)), c0(lane % (64 / K) * K) {
+        const uint32_t c = block * 64 + c0;
+        valid = c < width ? min(K, (int)(width - c)) : 0;
+    }
+    __device__ __forceinline__ R* at(const Seq<R>& s, uint32_t b, uint32_t t, uint32_t ch) const {
+        return s.p ? s.at(b, t + step) + ch : nullptr;
+    }
+    // the channels as they lie, in dwords: taking a dword apart would wait for it
+    static constexpr int kWords = K * sizeof(R) / 4;
+    __device__ __forceinline__ void load(const R* p, bool there, uint32_t (&o)[kWords]) const {
+        constexpr int M = kWords < 4 ? kWords : 4;
+        typedef uint32_t Vec __attribute__((ext_vector_type(M)));
+        typedef Vec Mem __attribute__((aligned(sizeof(R))));
+        if (there && valid == K) {
 #pragma unroll
-        for (int j = 0; j < NS; j++) o[j] = R(0);
-        if (!p) return;
-        if (left >= kTile) {
+            for (int i = 0; i < kWords; i += M) {
+                const Vec q = *reinterpret_cast<const Mem*>(reinterpret_cast<const uint32_t*>(p) + i);
 #pragma unroll
-            for (int j = 0; j < NS; j++) o[j] = p[kSteps * j * ts];
+                for (int j = 0; j < M; j++) {
+                    if constexpr (M == 1) o[i] = q[0];
+                    else o[i + j] = q[j];
+                }
+            }
         } else {
 #pragma unroll
-            for (int j = 0; j < NS; j++)
-                if (kSteps * j + step < left) o[j] = p[kSteps * j * ts];
+            for (int i = 0; i < kWords; i++) o[i] = 0;
+            if (!there) return;
+#pragma unroll
+            for (int i = 0; i < K; i++) {
+                if (i >= valid) continue;
+                if constexpr (sizeof(R) == 2) o[i / 2] |= (uint32_t)p[i] << (16 * (i & 1));
+                else o[i] = __builtin_bit_cast(uint32_t, p[i]);
+            }
         }
     }
-    __device__ __forceinline__ void move(int steps) {
-        if (p) p += steps * ts;
+    __device__ __forceinline__ void store(R* p, bool there, const R (&o)[K]) const {
+        constexpr int M = sizeof(R) == 2 ? (K < 8 ? K : 8) : (K < 4 ? K : 4);
+        if (!there) return;
+        if (valid == K) {
+#pragma unroll
+            for (int i = 0; i < K; i += M) {
+                R q[M];
+#pragma unroll
+                for (int j = 0; j < M; j++) q[j] = o[i + j];
+                store_raw<R, M, false>(p + i, q);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < K; i++)
+                if (i < valid) p[i] = o[i];
+        }
+    }
+    // per-channel weights (zeros where there are none)
+    __device__ __forceinline__ void weights(const float* p, uint32_t ch, float (&o)[K]) const {
+#pragma unroll
+        for (int i = 0; i < K; i++) o[i] = p && i < valid ? p[ch + i] : 0.0f;
     }
 };
+// element i of such dwords
+template <class T, int N>
+__device__ __forceinline__ float element(const uint32_t (&w)[N], int i) {
+    if constexpr (sizeof(typename T::Raw) == 2) return widen(T{}, (uint16_t)(w[i / 2] >> (16 * (i & 1))));
+    else return __builtin_bit_cast(float, w[i]);
+}
+// K adjacent values of an LDS row
+template <int K>
+__device__ __forceinline__ void read_row(const float* p, float (&o)[K]) {
+    constexpr int M = K < 4 ? K : 4;
+#pragma unroll
+    for (int i = 0; i < K; i += M) {
+        float q[M];
+        load_raw<float, M, true>(p + i, q);
+#pragma unroll
+        for (int j = 0; j < M; j++) o[i + j] = q[j];
+    }
+}
+template <int K>
+__device__ __forceinline__ void write_row(float* p, const float (&o)[K]) {
+    constexpr int M = K < 4 ? K : 4;
+#pragma unroll
+    for (int i = 0; i < K; i += M) {
+        float q[M];
+#pragma unroll
+        for (int j = 0; j < M; j++) q[j] = o[i + j];
+        store_raw<float, M, true>(p + i, q);
+    }
+}
 
 // the states of quad q of a [b][d][n] tensor
 __device__ __forceinline__ f4 load_states(const float* p, uint64_t at, uint32_t n, uint32_t q) {
@@ -259,49 +371,23 @@ __device__ __forceinline__ f4 fma4(f4 a, f4 b, f4 c) {
     return c;
 }
 
-// What a wave reads of the steps that it prepares: j * W + wave of a tile.
-template <class R, int W>
-struct Inputs {
-    static constexpr int K = kTile / W;
-    R x[K], dt[K], z[K];
-};
-template <class R, int W>
-struct Reader {
-    Rows<R> x, dt, z;
-    bool gate;
-    __device__ __forceinline__ Reader(const SsmArgs<R>& g, uint32_t b, uint32_t t, bool gated)
-        : x(g.x, b, t), dt(g.dt, b, t), z(g.z, b, t), gate(gated && g.z.p) {}
-    // the next tile, `left` steps of it there; a step that is not there is read as zeros
-    __device__ __forceinline__ void load(uint32_t own, uint32_t wave, uint32_t left, Inputs<R, W>& o) {
-        Rows<R> px = x, pt = dt, pz = z;
-        const bool full = left >= kTile;
-#pragma unroll
-        for (int j = 0; j < kTile / W; j++) {
-            o.x[j] = o.dt[j] = o.z[j] = R(0);
-            if (full || j * W + wave < left) {
-                o.x[j] = *px.at(own), o.dt[j] = *pt.at(own);
-                if (gate) o.z[j] = *pz.at(own);
-            }
-            px.move(W), pt.move(W), pz.move(W);
-        }
-        x.move(kTile), dt.move(kTile), z.move(kTile);
-    }
-};
-
 // The ends of segments from zeros: W waves, NQ quads of states each.
 template <class T, int W, int NQ>
 __global__ __launch_bounds__(64 * W, 2) void ssm_fold(SsmArgs<typename T::Raw> g) {
     using R = typename T::Raw;
-    constexpr int K = kTile / W;
-    __shared__ float2 steps[2][kTile][64];
+    using P = Part<R, W>;
+    constexpr int K = P::K;
+    __shared__ __align__(16) float steps[2][kTile][128];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Spot at(g, lane);
-    const uint32_t b = at.walk, ch = at.ch, own = ch * (uint32_t)sizeof(R);
+    const P part(lane, wave, g.width, at.block);
+    const uint32_t b = at.walk, ch = at.ch, base = at.group * g.width + at.block * 64 + part.c0;
     const uint64_t flat = (uint64_t)b * g.d + ch, slots = (uint64_t)g.b * g.quads * g.d;
     const uint32_t n = g.lengths ? (uint32_t)min(max(g.lengths[b], 0), (int32_t)g.t) : g.t;
     const uint32_t first = at.seg * g.seg_tiles, last = min(first + g.seg_tiles, g.tiles);
     const uint32_t busy = min(last, (n + kTile - 1) / kTile);
-    const float bias = g.bias ? g.bias[ch] : 0.0f;
+    float bias[K];
+    part.weights(g.bias, base, bias);
     f4 rate[NQ], h[NQ];
     float sum = 0.0f;
 #pragma unroll
@@ -312,49 +398,52 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_fold(SsmArgs<typename T::Raw> g
         // the second launch reads the first state here: the last one may lie over h0
         if (at.seg == 0 && q < g.quads && at.live) g.ends[((uint64_t)b * g.quads + q) * g.d + ch] = load_states(g.h0, flat, g.n, q);
     }
-    Reader<R, W> reader(g, b, first * kTile + wave, false);
-    Vectors<R, 4> vec0(g.bm, b, first * kTile, at.group, g.n, wave, lane), vec1(g.bm, b, first * kTile, at.group, g.n, wave + W * (NQ - 1), lane);
-    Inputs<R, W> in;
-    R bm[NQ][4];
-    float bv[NQ][4];
-    auto load = [&](uint32_t left) {
-        reader.load(own, wave, left, in);
-        vec0.load(left, bm[0]), vec0.move(kTile);
-        if constexpr (NQ > 1) vec1.load(left, bm[1]), vec1.move(kTile);
+    const uint32_t from = first * kTile;
+    const R *px = part.at(g.x, b, from, base), *pt = part.at(g.dt, b, from, base);
+    Vectors<R, 4> vec[2] = {{g.bm, b, from, at.group, g.n, wave, lane}, {g.bm, b, from, at.group, g.n, wave + W * (NQ - 1), lane}};
+    uint32_t x[P::kWords], dt[P::kWords];
+    R bm[NQ];
+    auto load = [&](uint32_t left) __attribute__((always_inline)) {
+        part.load(px, part.step < left, x), part.load(pt, part.step < left, dt);
+        px += kTile * g.x.ts, pt += kTile * g.dt.ts;
+#pragma unroll
+        for (int i = 0; i < NQ; i++) bm[i] = vec[i].load(left), vec[i].move(kTile);
     };
-    auto prepare = [&](uint32_t left, int buf) {
+    uint32_t left = first < busy ? n - from : 0;  // steps of the sequence from the tile on
+    if (left) load(left);
+    for (uint32_t tile = first; tile < busy; tile++, left -= kTile) {
+        float* rows = steps[(tile - first) & 1][0];  // the other one may still be read
+        float o[2 * K], bv[NQ][4];
 #pragma unroll
         for (int j = 0; j < K; j++) {
             float e;
-            const float d = softplus(widen(T{}, in.dt[j]) + bias, e), step = j * W + wave < left ? d : 0.0f;
-            steps[buf][j * W + wave][lane] = float2{step, step * widen(T{}, in.x[j])};
+            const float d = softplus(element<T>(dt, j) + bias[j], e);
+            o[2 * j] = part.step < left && j < part.valid ? d : 0.0f, o[2 * j + 1] = o[2 * j] * element<T>(x, j);
         }
-    };
-    uint32_t left = first < busy ? n - first * kTile : 0;  // steps of the sequence from the tile on
-    if (left) {
-        load(left);
-        prepare(left, 0);
-    }
-    for (uint32_t tile = first; tile < busy; tile++, left -= kTile) {
-        const int buf = (tile - first) & 1;
+        write_row<2 * K>(rows + part.step * 128 + part.c0 * 2, o);
 #pragma unroll
-        for (int i = 0; i < NQ; i++)
+        for (int i = 0; i < NQ; i++) spread<4>(widen(T{}, bm[i]), bv[i]), settle(bv[i]);  // before the next tile's loads start
+        if (tile + 1 < busy) load(left - kTile);
+        lds_barrier();
+        float2 st[2][4];  // four steps' LDS reads are on their way while four steps run
+        auto read = [&](int m) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) bv[i][j] = widen(T{}, bm[i][j]);
-        const bool more = tile + 1 < busy;
-        if (more) load(left - kTile);
-        __syncthreads();
-        each<kTile>([&](auto c) {
-            constexpr int s = c;
-            const float2 st = steps[buf][s][lane];
-            sum += st.x;
-#pragma unroll
-            for (int i = 0; i < NQ; i++) {
-                h[i] *= decay(st.x, rate[i]);
-                add_outer<(s & 3) * 4>(h[i], bv[i][s >> 2], st.y);
-            }
+            for (int r = 0; r < 4; r++) st[m & 1][r] = *reinterpret_cast<const float2*>(rows + (4 * m + r) * 128 + lane * 2);
+        };
+        read(0);
+        each<4>([&](auto mc) {
+            constexpr int m = mc;
+            if constexpr (m < 3) read(m + 1);
+            fence();
+            each<4>([&](auto rc) {
+                constexpr int r = rc;
+                sum += st[m & 1][r].x;
+                each<NQ>([&](auto i) {
+                    h[i] *= decay(st[m & 1][r].x, rate[i]);
+                    add_outer<r * 4>(h[i], bv[i][m], st[m & 1][r].y);
+                });
+            });
         });
-        if (more) prepare(left - kTile, buf ^ 1);
     }
 #pragma unroll
     for (int i = 0; i < NQ; i++) {
@@ -364,26 +453,32 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_fold(SsmArgs<typename T::Raw> g
     if (wave == 0 && at.live) g.lasts[(uint64_t)at.seg * g.b * g.d + flat] = sum;
 }
 
-// W waves, NQ times NS states each. One barrier a tile: while a tile runs, the next one's steps are prepared and the one
-// before is finished, into and from the other halves of the buffers.
+// W waves, NQ times NS states each.
 template <class T, int W, int NQ, int NS>
 __global__ __launch_bounds__(64 * W, 2) void ssm_fwd(SsmArgs<typename T::Raw> g) {
     using R = typename T::Raw;
-    constexpr int K = kTile / W, SPR = 16 / NS;  // steps that a wave prepares, j * W + wave; steps a register of vectors
-    __shared__ float2 steps[2][kTile][64];
-    __shared__ float parts[2][W][kTile][64];
+    using P = Part<R, W>;
+    constexpr int K = P::K, SPR = 16 / NS;  // steps a register of vectors
+#ifndef PIPE
+#define PIPE 0
+#endif
+    constexpr bool AHEAD = PIPE;
+    __shared__ __align__(16) float steps[2][kTile][128];
+    __shared__ __align__(16) float parts[AHEAD ? 2 : 1][W][kTile][64];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Spot at(g, lane);
-    const uint32_t b = at.walk, ch = at.ch, own = ch * (uint32_t)sizeof(R);
+    const P part(lane, wave, g.width, at.block);
+    const uint32_t b = at.walk, ch = at.ch, base = at.group * g.width + at.block * 64 + part.c0;
     const uint64_t flat = (uint64_t)b * g.d + ch, slots = (uint64_t)g.b * g.quads * g.d;
     const uint32_t n = g.lengths ? (uint32_t)min(max(g.lengths[b], 0), (int32_t)g.t) : g.t;
     const uint32_t first = at.seg * g.seg_tiles, last = min(first + g.seg_tiles, g.tiles);
     const uint32_t busy = min(last, (n + kTile - 1) / kTile);
-    const float bias = g.bias ? g.bias[ch] : 0.0f, skip = g.skip ? g.skip[ch] : 0.0f;
+    float bias[K], skip[K];
+    part.weights(g.bias, base, bias), part.weights(g.skip, base, skip);
     // state k of the wave's part i: number NS * (wave + W * i) + k
-    auto number = [&](int i, int k) { return NS * (wave + W * i) + k; };
+    auto number = [&](int i, int k) __attribute__((always_inline)) { return NS * (wave + W * i) + k; };
     // its place in a buffer of quads [quad][d] of 4
-    auto in_quads = [&](int i, int k) {
+    auto in_quads = [&](int i, int k) __attribute__((always_inline)) {
         const uint32_t s = number(i, k);
         return ((uint64_t)(s >> 2) * g.d + ch) * 4 + (s & 3);
     };
@@ -409,95 +504,160 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_fwd(SsmArgs<typename T::Raw> g)
             }
         }
     }
-    Reader<R, W> reader(g, b, first * kTile + wave, true);
-    Vectors<R, NS> vb0(g.bm, b, first * kTile, at.group, g.n, wave, lane), vc0(g.cm, b, first * kTile, at.group, g.n, wave, lane);
-    Vectors<R, NS> vb1(g.bm, b, first * kTile, at.group, g.n, wave + W * (NQ - 1), lane);
-    Vectors<R, NS> vc1(g.cm, b, first * kTile, at.group, g.n, wave + W * (NQ - 1), lane);
-    Rows<R> ry(g.y, b, first * kTile + wave);
-    Inputs<R, W> in;
-    R bm[NQ][NS], cm[NQ][NS], x[2][K], z[2][K];  // x and z of the tile that runs, and of the one before
-    float bv[NQ][NS], cv[NQ][NS];
-    auto load = [&](uint32_t left) {
-        reader.load(own, wave, left, in);
-        vb0.load(left, bm[0]), vb0.move(kTile), vc0.load(left, cm[0]), vc0.move(kTile);
-        if constexpr (NQ > 1) vb1.load(left, bm[NQ - 1]), vb1.move(kTile), vc1.load(left, cm[NQ - 1]), vc1.move(kTile);
+    const uint32_t from = first * kTile;
+    const R *px = part.at(g.x, b, from, base), *pt = part.at(g.dt, b, from, base), *pz = part.at(g.z, b, from, base);
+    R* py = part.at(g.y, b, from, base);
+    Vectors<R, NS> vb[2] = {{g.bm, b, from, at.group, g.n, wave, lane}, {g.bm, b, from, at.group, g.n, wave + W * (NQ - 1), lane}};
+    Vectors<R, NS> vc[2] = {{g.cm, b, from, at.group, g.n, wave, lane}, {g.cm, b, from, at.group, g.n, wave + W * (NQ - 1), lane}};
+    // the inputs of the two tiles to come; x and z of the tile that runs, and of the one before
+    uint32_t x[2][P::kWords], dt[2][P::kWords], z[2][P::kWords], xs[2][P::kWords], zs[2][P::kWords];
+    R bm[2][NQ], cm[2][NQ];
+    auto load = [&](uint32_t left, auto slot) __attribute__((always_inline)) {
+        const bool there = part.step < left;
+        part.load(px, there, x[slot]), part.load(pt, there, dt[slot]);
+        if (g.z.p) part.load(pz, there, z[slot]), pz += kTile * g.z.ts;
+        px += kTile * g.x.ts, pt += kTile * g.dt.ts;
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+            bm[slot][i] = vb[i].load(left), cm[slot][i] = vc[i].load(left);
+            vb[i].move(kTile), vc[i].move(kTile);
+        }
     };
-    auto prepare = [&](uint32_t left, int buf) {
+    auto prepare = [&](uint32_t left, auto slot) __attribute__((always_inline)) {
+        float o[2 * K];
 #pragma unroll
         for (int j = 0; j < K; j++) {
             float e;
-            const float d = softplus(widen(T{}, in.dt[j]) + bias, e), step = j * W + wave < left ? d : 0.0f;
-            steps[buf][j * W + wave][lane] = float2{step, step * widen(T{}, in.x[j])};
+            const float d = softplus(element<T>(dt[slot], j) + bias[j], e);
+            o[2 * j] = part.step < left && j < part.valid ? d : 0.0f, o[2 * j + 1] = o[2 * j] * element<T>(x[slot], j);
+        }
+        write_row<2 * K>(steps[slot][part.step] + part.c0 * 2, o);
+    };
+    float bv[NQ][NS], cv[NQ][NS];
+    auto vectors = [&](auto slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {  // settled before their registers are loaded again
+            spread<NS>(widen(T{}, bm[slot][i]), bv[i]), spread<NS>(widen(T{}, cm[slot][i]), cv[i]);
+            settle(bv[i]), settle(cv[i]);
         }
     };
-    // left: of the tile's steps those inside the length; there: those inside the tensor
-    auto finish = [&](uint32_t left, uint32_t there, int buf) {
-        Rows<R> py = ry;
+    auto keep = [&](auto slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < P::kWords; j++) {
+            xs[1][j] = xs[0][j], zs[1][j] = zs[0][j], xs[0][j] = x[slot][j], zs[0][j] = z[slot][j];
+            asm volatile("" : "+v"(xs[0][j]), "+v"(zs[0][j]));
+        }
+    };
+    auto states = [&](uint32_t tile) __attribute__((always_inline)) {
+        if (!g.states || !at.live) return;
+        float* to = reinterpret_cast<float*>(g.states + ((uint64_t)b * g.tiles + tile) * g.quads * g.d);
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+            if (number(i, 0) >= 4 * g.quads) continue;
+            if constexpr (NS == 4) *reinterpret_cast<f4*>(to + in_quads(i, 0)) = f4{h[i].v[0], h[i].v[1], h[i].v[2], h[i].v[3]};
+            else *reinterpret_cast<float2*>(to + in_quads(i, 0)) = float2{h[i].v[0], h[i].v[1]};
+        }
+    };
+    auto run = [&](int buf, int pbuf) __attribute__((always_inline)) {
+        float2 st[2][4];  // four steps' LDS reads are on their way while four steps run
+        auto read = [&](int m) __attribute__((always_inline)) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) st[m & 1][r] = *reinterpret_cast<const float2*>(steps[buf][4 * m + r] + lane * 2);
+        };
+        read(0);
+        each<4>([&](auto mc) {
+            constexpr int m = mc;
+            if constexpr (m < 3) read(m + 1);
+            fence();
+            each<4>([&](auto rc) {
+                constexpr int r = rc, s = 4 * m + r;
+                float p = 0.0f;
+                each<NQ>([&](auto ic) {
+                    constexpr int i = ic;
+                    each<NS>([&](auto kc) { h[i].v[kc] *= __builtin_amdgcn_exp2f(st[m & 1][r].x * rate[i].v[kc]); });
+                    const float q = step_states<s % SPR * NS>(h[i], bv[i][s / SPR], st[m & 1][r].y, cv[i][s / SPR]);
+                    p = i ? p + q : q;
+                });
+                parts[pbuf][wave][s][lane] = p;
+            });
+        });
+    };
+    // left: of the tile's steps those inside the length; there: those inside the tensor; of: xs[of] is the tile's
+    auto finish = [&](uint32_t left, uint32_t there, int pbuf, auto of) __attribute__((always_inline)) {
+        float p[K];
+        R out[K];
+#pragma unroll
+        for (int j = 0; j < K; j++) p[j] = skip[j] * element<T>(xs[of], j);
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            float q[K];
+            read_row<K>(parts[pbuf][w][part.step] + part.c0, q);
+#pragma unroll
+            for (int j = 0; j < K; j++) p[j] += q[j];
+        }
 #pragma unroll
         for (int j = 0; j < K; j++) {
-            const uint32_t s = j * W + wave;
-            float p = skip * widen(T{}, x[1][j]);
-#pragma unroll
-            for (int w = 0; w < W; w++) p += parts[buf][w][s][lane];
             if (g.z.p) {
-                const float v = widen(T{}, z[1][j]);
-                p *= v * sigmoid1(v);
+                const float v = element<T>(zs[of], j);
+                p[j] *= v * sigmoid1(v);
             }
-            if (s < there && at.live) *py.at(own) = s < left ? narrow(T{}, p) : R(0);
-            py.move(W);
+            out[j] = part.step < left ? narrow(T{}, p[j]) : R(0);
         }
-        ry.move(kTile);
+        part.store(py, part.step < there, out);
+        py += kTile * g.y.ts;
     };
-    uint32_t left = first < busy ? n - first * kTile : 0;  // steps of the sequence from the tile on
+    using Zero = std::integral_constant<int, 0>;
+    using One = std::integral_constant<int, 1>;
+    uint32_t left = first < busy ? n - from : 0;  // steps of the sequence from the tile on
     if (left) {
-        load(left);
-        prepare(left, 0);
+        load(left, Zero{});
+        if (left > kTile) load(left - kTile, One{});
     }
-    for (uint32_t tile = first; tile < busy; tile++, left -= kTile) {
-        const int buf = (tile - first) & 1;
-#pragma unroll
-        for (int j = 0; j < K; j++) x[1][j] = x[0][j], x[0][j] = in.x[j], z[1][j] = z[0][j], z[0][j] = in.z[j];
-#pragma unroll
-        for (int i = 0; i < NQ; i++)
-#pragma unroll
-            for (int j = 0; j < NS; j++) bv[i][j] = widen(T{}, bm[i][j]), cv[i][j] = widen(T{}, cm[i][j]);
-        const bool more = tile + 1 < busy;
-        if (more) load(left - kTile);
-        if (g.states && at.live) {
-            float* to = reinterpret_cast<float*>(g.states + ((uint64_t)b * g.tiles + tile) * g.quads * g.d);
-#pragma unroll
-            for (int i = 0; i < NQ; i++) {
-                if (number(i, 0) >= 4 * g.quads) continue;
-                if constexpr (NS == 4) *reinterpret_cast<f4*>(to + in_quads(i, 0)) = f4{h[i].v[0], h[i].v[1], h[i].v[2], h[i].v[3]};
-                else *reinterpret_cast<float2*>(to + in_quads(i, 0)) = float2{h[i].v[0], h[i].v[1]};
-            }
+    if constexpr (AHEAD) {
+        // One barrier a tile: while a tile runs, the next one's steps are prepared and the one before is finished, into and
+        // from the other halves of the buffers.
+        if (left) prepare(left, Zero{});
+        auto body = [&](auto slot, auto other, uint32_t tile) __attribute__((always_inline)) {
+            keep(slot);
+            vectors(slot);
+            if (left > 2 * kTile) load(left - 2 * kTile, slot);
+            states(tile);
+            lds_barrier();
+            if (tile > first) finish(left + kTile, g.t - (tile - 1) * kTile, other, One{});
+            run(slot, slot);
+            if (tile + 1 < busy) prepare(left - kTile, other);
+            left -= kTile;
+        };
+        for (uint32_t tile = first; tile < busy; tile += 2) {
+            body(Zero{}, One{}, tile);
+            if (tile + 1 < busy) body(One{}, Zero{}, tile + 1);
         }
-        __syncthreads();
-        if (tile > first) finish(left + kTile, g.t - (tile - 1) * kTile, buf ^ 1);
-        each<kTile>([&](auto c) {
-            constexpr int s = c;
-            const float2 st = steps[buf][s][lane];
-            float p = 0.0f;
-#pragma unroll
-            for (int i = 0; i < NQ; i++) {
-#pragma unroll
-                for (int k = 0; k < NS; k++) h[i].v[k] *= __builtin_amdgcn_exp2f(st.x * rate[i].v[k]);
-                const float q = step_states<s % SPR * NS>(h[i], bv[i][s / SPR], st.y, cv[i][s / SPR]);
-                p = i ? p + q : q;
-            }
-            parts[buf][wave][s][lane] = p;
-        });
-        if (more) prepare(left - kTile, buf ^ 1);
+        lds_barrier();
+        if (first < busy) finish(n - (busy - 1) * kTile, g.t - (busy - 1) * kTile, (busy - 1 - first) & 1, Zero{});
+    } else {
+        auto body = [&](auto slot, uint32_t tile) __attribute__((always_inline)) {
+            prepare(left, slot);
+            keep(slot);
+            vectors(slot);
+            if (left > 2 * kTile) load(left - 2 * kTile, slot);
+            states(tile);
+            lds_barrier();
+            run(slot, 0);
+            lds_barrier();
+            finish(left, g.t - tile * kTile, 0, Zero{});
+            left -= kTile;
+        };
+        for (uint32_t tile = first; tile < busy; tile += 2) {
+            body(Zero{}, tile);
+            if (tile + 1 < busy) body(One{}, tile + 1);
+        }
     }
-    __syncthreads();
-    if (first < busy) {
+    for (uint32_t t = max(busy, first) * kTile; t < min(last * kTile, g.t); t += kTile) {
+        R out[K];
 #pragma unroll
-        for (int j = 0; j < K; j++) x[1][j] = x[0][j], z[1][j] = z[0][j];
-        finish(n - (busy - 1) * kTile, g.t - (busy - 1) * kTile, (busy - 1 - first) & 1);
-    }
-    for (uint32_t t = max(busy, first) * kTile + wave; t < min(last * kTile, g.t); t += W) {
-        if (at.live) *ry.at(own) = R(0);
-        ry.move(W);
+        for (int j = 0; j < K; j++) out[j] = R(0);
+        part.store(py, t + part.step < g.t, out);
+        py += kTile * g.y.ts;
     }
     if (g.ht && at.live && last == g.tiles) {
 #pragma unroll
@@ -558,22 +718,12 @@ __global__ __launch_bounds__(256) void ssm_step(SsmArgs<typename T::Raw> g) {
 
 // The sum of two values over pairs of lanes, one kept in either lane: of a where the lane's bit is 0, of b where it is 1.
 __device__ __forceinline__ float merge32(float a, float b) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
-    const uint32_t p = r[0], q = r[1];  // (a cast of a vector's element itself takes the first one's bits for every index)
-    return __builtin_bit_cast(float, p) + __builtin_bit_cast(float, q);
-#else
+    swap32(a, b);
     return a + b;
-#endif
 }
 __device__ __forceinline__ float merge16(float a, float b) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
-    const uint32_t p = r[0], q = r[1];  // (a cast of a vector's element itself takes the first one's bits for every index)
-    return __builtin_bit_cast(float, p) + __builtin_bit_cast(float, q);
-#else
+    swap16(a, b);
     return a + b;
-#endif
 }
 // CTRL pairs lanes that differ in the bit (row_ror:8, row_half_mirror, quad_perm)
 template <int CTRL>
@@ -590,21 +740,25 @@ constexpr int kRor8 = 0x128, kHalfMirror = 0x141, kSwap2 = 0x4E, kSwap1 = 0xB1;
 
 // FOLD: the gradients that reach the states before a segment, from zeros behind it
 template <class T, int W, int NQ, bool FOLD>
-__global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void ssm_bwd(SsmArgs<typename T::Raw> g) {
+__global__ __launch_bounds__(64 * W, 2) void ssm_bwd(SsmArgs<typename T::Raw> g) {
     using R = typename T::Raw;
-    constexpr int K = kTile / W;
-    __shared__ float2 steps[kTile][64];                  // D, D x
-    __shared__ float ups[kTile][64];                     // q
-    __shared__ float parts[FOLD ? 1 : 3][W][kTile][64];  // sum C h, s1, s2 of a wave's states
-    __shared__ float vectors[FOLD ? 1 : kTile][2][W * NQ * 4];  // dB, dC over the workgroup's channels
+    using P = Part<R, W>;
+    constexpr int K = P::K;
+    __shared__ __align__(16) float steps[kTile][128];                  // D, D x
+    __shared__ __align__(16) float ups[kTile][64];                     // q
+    __shared__ __align__(16) float parts[FOLD ? 1 : 3][FOLD ? 1 : W][kTile][64];  // sum C h, s1, s2 of a wave's states
+    __shared__ float vectors[FOLD ? 1 : kTile][2][W * NQ * 4];         // dB, dC over the workgroup's channels
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Spot at(g, lane);
-    const uint32_t ch = at.ch, own = ch * (uint32_t)sizeof(R);
+    const P part(lane, wave, g.width, at.block);
+    const uint32_t ch = at.ch, base = at.group * g.width + at.block * 64 + part.c0;
     const uint32_t first = at.seg * g.seg_tiles, last = min(first + g.seg_tiles, g.tiles);
     const uint64_t slots = (uint64_t)g.b * g.quads * g.d;
-    const float bias = g.bias ? g.bias[ch] : 0.0f, skip = g.skip ? g.skip[ch] : 0.0f;
+    float bias[K], skip[K], dskip[K], dbias[K];
+    part.weights(g.bias, base, bias), part.weights(g.skip, base, skip);
+#pragma unroll
+    for (int j = 0; j < K; j++) dskip[j] = dbias[j] = 0.0f;
     f4 rate[NQ], da[NQ];
-    float dskip = 0.0f, dbias = 0.0f;
 #pragma unroll
     for (int i = 0; i < NQ; i++) {
         rate[i] = rates_of(g.a, ch, g.n, wave + W * i);
@@ -626,102 +780,99 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void ssm_bwd(SsmArgs<typena
                     c[i] = fma4(decay(g.lasts[(uint64_t)s * g.b * g.d + flat], rate[i]), c[i], g.ends[s * slots + slot]);
             }
         }
-        R x[K], dt[K], z[K], dy[K], bm[NQ][4], cm[NQ][4];
-        f4 start[NQ];
         const uint32_t from = busy > first ? (busy - 1) * kTile : 0;  // tiles go from the last to the first
-        Rows<R> rx(g.x, b, from + wave), rdt(g.dt, b, from + wave), rz(g.z, b, from + wave), rdy(g.dy, b, from + wave);
-        struct Pair {
-            Vectors<R, 4> b, c;
-        };
-        auto vectors_of = [&](int i) {
-            return Pair{Vectors<R, 4>(g.bm, b, from, at.group, g.n, wave + W * i, lane),
-                        Vectors<R, 4>(g.cm, b, from, at.group, g.n, wave + W * i, lane)};
-        };
-        Pair vec[2] = {vectors_of(0), vectors_of(NQ - 1)};
-        auto load = [&](uint32_t tile) {
+        const R *px = part.at(g.x, b, from, base), *pt = part.at(g.dt, b, from, base), *pz = part.at(g.z, b, from, base);
+        const R* py = part.at(g.dy, b, from, base);
+        R *pdx = part.at(g.dx, b, from, base), *pdt = part.at(g.ddt, b, from, base), *pdz = part.at(g.dz, b, from, base);
+        Vectors<R, 4> vb[2] = {{g.bm, b, from, at.group, g.n, wave, lane}, {g.bm, b, from, at.group, g.n, wave + W * (NQ - 1), lane}};
+        Vectors<R, 4> vc[2] = {{g.cm, b, from, at.group, g.n, wave, lane}, {g.cm, b, from, at.group, g.n, wave + W * (NQ - 1), lane}};
+        uint32_t x[P::kWords], dt[P::kWords], z[P::kWords], dy[P::kWords];
+        R bm[NQ], cm[NQ];
+        f4 start[NQ];
+        auto load = [&](uint32_t tile) __attribute__((always_inline)) {
             const uint32_t left = n - tile * kTile;
-            Rows<R> px = rx, pt = rdt, pz = rz, py = rdy;
-#pragma unroll
-            for (int j = 0; j < K; j++) {
-                x[j] = dt[j] = z[j] = dy[j] = R(0);
-                if (j * W + wave < left) {
-                    if (!FOLD) x[j] = *px.at(own);
-                    dt[j] = *pt.at(own), dy[j] = *py.at(own);
-                    if (g.z.p) z[j] = *pz.at(own);
-                }
-                px.move(W), pt.move(W), pz.move(W), py.move(W);
-            }
-            rx.move(-kTile), rdt.move(-kTile), rz.move(-kTile), rdy.move(-kTile);
+            const bool there = part.step < left;
+            if (!FOLD) part.load(px, there, x), px -= kTile * g.x.ts;
+            part.load(pt, there, dt), part.load(py, there, dy);
+            if (g.z.p) part.load(pz, there, z), pz -= kTile * g.z.ts;
+            pt -= kTile * g.dt.ts, py -= kTile * g.dy.ts;
 #pragma unroll
             for (int i = 0; i < NQ; i++) {
                 const uint32_t q = wave + W * i;
-                vec[i].c.load(left, cm[i]);
-                vec[i].c.move(-kTile);
+                cm[i] = vc[i].load(left), vc[i].move(-kTile);
                 if constexpr (!FOLD) {
-                    vec[i].b.load(left, bm[i]);
-                    vec[i].b.move(-kTile);
+                    bm[i] = vb[i].load(left), vb[i].move(-kTile);
                     start[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
                     if (q < g.quads && at.live) start[i] = g.states[(((uint64_t)b * g.tiles + tile) * g.quads + q) * g.d + ch];
                 }
             }
         };
-        Rows<R> rdx(g.dx, b, from + wave), rddt(g.ddt, b, from + wave), rdz(g.dz, b, from + wave);
         if (first < busy) load(busy - 1);
         for (uint32_t end = busy; end > first; end--) {
             const uint32_t tile = end - 1, left = n - tile * kTile;
+            const bool on = part.step < left;
             float xs[K], slope[K], zg[K], bv[NQ][4], cv[NQ][4];  // the step's slope; dy silu'(z)
+            {
+                float o[2 * K], q[K];
 #pragma unroll
-            for (int j = 0; j < K; j++) {
-                const uint32_t s = j * W + wave;
-                const bool on = s < left && at.live;  // a lane without a channel adds nothing to dB and dC
-                const float v = widen(T{}, dt[j]) + bias, up = widen(T{}, dy[j]);
-                float e, gate = 1.0f, dgate = 0.0f;
-                const float d = softplus(v, e), step = on ? d : 0.0f;
-                if (g.z.p) silu_grad(widen(T{}, z[j]), gate, dgate);
-                if constexpr (!FOLD) {
-                    const float r = __builtin_amdgcn_rcpf(1.0f + e);
-                    xs[j] = widen(T{}, x[j]), slope[j] = v >= 0.0f ? r : e * r, zg[j] = up * dgate;
+                for (int j = 0; j < K; j++) {
+                    const float v = element<T>(dt, j) + bias[j], up = element<T>(dy, j);
+                    float e, gate = 1.0f, dgate = 0.0f;
+                    const float d = softplus(v, e);
+                    if (g.z.p) silu_grad(element<T>(z, j), gate, dgate);
+                    o[2 * j] = on && j < part.valid ? d : 0.0f, o[2 * j + 1] = 0.0f;
+                    q[j] = on ? up * gate : 0.0f;
+                    if constexpr (!FOLD) {
+                        const float r = __builtin_amdgcn_rcpf(1.0f + e);
+                        xs[j] = element<T>(x, j), slope[j] = v >= 0.0f ? r : e * r, zg[j] = up * dgate;
+                        o[2 * j + 1] = o[2 * j] * xs[j];
+                    }
                 }
-                steps[s][lane] = float2{step, FOLD || !on ? 0.0f : step * xs[j]};
-                ups[s][lane] = on ? up * gate : 0.0f;
+                write_row<2 * K>(steps[part.step] + part.c0 * 2, o);
+                write_row<K>(ups[part.step] + part.c0, q);
             }
             f4 h0[NQ];
 #pragma unroll
             for (int i = 0; i < NQ; i++) {
-                if constexpr (!FOLD) h0[i] = start[i];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    cv[i][j] = widen(T{}, cm[i][j]);
-                    if constexpr (!FOLD) bv[i][j] = widen(T{}, bm[i][j]);
-                }
+                spread<4>(widen(T{}, cm[i]), cv[i]), settle(cv[i]);
+                if constexpr (!FOLD) spread<4>(widen(T{}, bm[i]), bv[i]), settle(bv[i]), h0[i] = start[i];
             }
-            __syncthreads();
+            lds_barrier();
             if (tile > first) load(tile - 1);
+            auto step_of = [&](int s) __attribute__((always_inline)) { return *reinterpret_cast<const float2*>(steps[s] + lane * 2); };
             if constexpr (FOLD) {
-                each<kTile>([&](auto sc) {
-                    constexpr int s = kTile - 1 - sc;
-                    const float step = steps[s][lane].x, q = ups[s][lane];
-                    sum += step;
+                each<4>([&](auto mc) {
+                    constexpr int m = 3 - mc;
+                    float2 st[4];
+                    float q[4];
 #pragma unroll
-                    for (int i = 0; i < NQ; i++) {
-                        add_outer<(s & 3) * 4>(c[i], cv[i][s >> 2], q);
-                        c[i] *= decay(step, rate[i]);
-                    }
+                    for (int r = 0; r < 4; r++) st[r] = step_of(4 * m + r), q[r] = ups[4 * m + r][lane];
+                    group();
+                    each<4>([&](auto rc) {
+                        constexpr int r = 3 - rc;
+                        sum += st[r].x;
+                        each<NQ>([&](auto i) {
+                            add_outer<r * 4>(c[i], cv[i][m], q[r]);
+                            c[i] *= decay(st[r].x, rate[i]);
+                        });
+                    });
                 });
             } else {
-#pragma unroll
-                for (int i = 0; i < NQ; i++) {
-                    f4 h[kTile], a[kTile];
+                each<NQ>([&](auto ic) {
+                    constexpr int i = ic;
+                    // The states of the tile; the decays are computed again on the way back: kept, their 64 registers would not
+                    // fit beside them, and a register that lies in memory meanwhile makes its load wait for all that is
+                    // under way.
+                    f4 h[kTile];
                     each<4>([&](auto mc) {  // four steps' LDS reads at once, no more: registers
                         constexpr int m = mc;
                         float2 st[4];
 #pragma unroll
-                        for (int r = 0; r < 4; r++) st[r] = steps[4 * m + r][lane];
-                        fence();
+                        for (int r = 0; r < 4; r++) st[r] = step_of(4 * m + r);
+                        group();
                         each<4>([&](auto rc) {
                             constexpr int s = 4 * m + rc;
-                            a[s] = decay(st[rc].x, rate[i]);
-                            h[s] = a[s] * (s ? h[s ? s - 1 : 0] : h0[i]);
+                            h[s] = decay(st[rc].x, rate[i]) * (s ? h[s ? s - 1 : 0] : h0[i]);
                             add_outer<rc * 4>(h[s], bv[i][m], st[rc].y);
                         });
                     });
@@ -731,14 +882,14 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void ssm_bwd(SsmArgs<typena
                         float2 st[4];
                         float q[4];
 #pragma unroll
-                        for (int r = 0; r < 4; r++) st[r] = steps[4 * m + r][lane], q[r] = ups[4 * m + r][lane];
-                        fence();
+                        for (int r = 0; r < 4; r++) st[r] = step_of(4 * m + r), q[r] = ups[4 * m + r][lane];
+                        group();
                         each<4>([&](auto rc) {
                             constexpr int r = 3 - rc, s = 4 * m + r;
                             float p, s1, s2 = 0.0f;
                             step_back<r * 4>(c[i], h[s], bv[i][m], cv[i][m], q[r], p, s1);
                             const f4 db = c[i] * st[r].y, dc = h[s] * q[r];
-                            c[i] *= a[s];
+                            c[i] *= decay(st[r].x, rate[i]);
                             const f4 past = c[i] * (s ? h[s ? s - 1 : 0] : h0[i]);
 #pragma unroll
                             for (int k = 0; k < 4; k++) {
@@ -773,31 +924,40 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void ssm_bwd(SsmArgs<typena
                                     }
                                 }
                             }
+                            __builtin_amdgcn_sched_barrier(0);
                         });
                     });
-                }
+                });
             }
-            __syncthreads();
+            lds_barrier();
             if constexpr (!FOLD) {
                 const uint32_t there = g.t - tile * kTile;
-                Rows<R> px = rdx, pt = rddt, pz = rdz;
+                float p[K], s1[K], s2[K], q[K], st[2 * K];
+#pragma unroll
+                for (int j = 0; j < K; j++) p[j] = s1[j] = s2[j] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    float u[K];
+                    auto add = [&](int of, float(&to)[K]) {
+                        read_row<K>(parts[of][w][part.step] + part.c0, u);
+#pragma unroll
+                        for (int j = 0; j < K; j++) to[j] += u[j];
+                    };
+                    add(0, p), add(1, s1), add(2, s2);
+                }
+                read_row<2 * K>(steps[part.step] + part.c0 * 2, st), read_row<K>(ups[part.step] + part.c0, q);
+                R ox[K], ot[K], oz[K];
 #pragma unroll
                 for (int j = 0; j < K; j++) {
-                    const uint32_t s = j * W + wave;
-                    float p = 0.0f, s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-                    for (int w = 0; w < W; w++) p += parts[0][w][s][lane], s1 += parts[1][w][s][lane], s2 += parts[2][w][s][lane];
-                    const float step = steps[s][lane].x, q = ups[s][lane];
-                    const float dd = __builtin_fmaf(xs[j], s1, s2 * kLn2) * slope[j];
-                    if (s < left) dskip = __builtin_fmaf(q, xs[j], dskip), dbias += dd;
-                    if (s < there && at.live) {
-                        *px.at(own) = s < left ? narrow(T{}, __builtin_fmaf(step, s1, skip * q)) : R(0);
-                        *pt.at(own) = s < left ? narrow(T{}, dd) : R(0);
-                        if (g.z.p) *pz.at(own) = s < left ? narrow(T{}, zg[j] * __builtin_fmaf(skip, xs[j], p)) : R(0);
-                    }
-                    px.move(W), pt.move(W), pz.move(W);
+                    const float dd = __builtin_fmaf(xs[j], s1[j], s2[j] * kLn2) * slope[j];
+                    if (on && j < part.valid) dskip[j] = __builtin_fmaf(q[j], xs[j], dskip[j]), dbias[j] += dd;
+                    ox[j] = on ? narrow(T{}, __builtin_fmaf(st[2 * j], s1[j], skip[j] * q[j])) : R(0);
+                    ot[j] = on ? narrow(T{}, dd) : R(0);
+                    oz[j] = on ? narrow(T{}, zg[j] * __builtin_fmaf(skip[j], xs[j], p[j])) : R(0);
                 }
-                rdx.move(-kTile), rddt.move(-kTile), rdz.move(-kTile);
+                part.store(pdx, part.step < there, ox), part.store(pdt, part.step < there, ot);
+                if (g.z.p) part.store(pdz, part.step < there, oz), pdz -= kTile * g.dz.ts;
+                pdx -= kTile * g.dx.ts, pdt -= kTile * g.ddt.ts;
                 // the tile's dB and dC of this block, as they lie
                 const uint32_t row = 8 * g.quads, steps_here = min((uint32_t)kTile, there);
                 float* to = g.bc + (((uint64_t)(at.group * g.blocks + at.block) * g.b + b) * g.t + tile * kTile) * row;
@@ -805,7 +965,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void ssm_bwd(SsmArgs<typena
                     const uint32_t s = k / row, v = k - s * row, half = v >= 4 * g.quads;
                     to[k] = vectors[s][half][v - half * 4 * g.quads];
                 }
-                __syncthreads();
+                lds_barrier();
             }
         }
         if constexpr (FOLD) {
@@ -816,14 +976,16 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void ssm_bwd(SsmArgs<typena
             }
             if (wave == 0 && at.live) g.lasts[(uint64_t)at.seg * g.b * g.d + flat] = sum;
         } else {
-            const uint32_t past = max(busy, first) * kTile + wave;
-            Rows<R> px(g.dx, b, past), pt(g.ddt, b, past), pz(g.dz, b, past);
-            for (uint32_t t = past; t < min(last * kTile, g.t); t += W) {
-                if (at.live) {
-                    *px.at(own) = *pt.at(own) = R(0);
-                    if (g.z.p) *pz.at(own) = R(0);
-                }
-                px.move(W), pt.move(W), pz.move(W);
+            const uint32_t past = max(busy, first) * kTile;
+            R none[K];
+#pragma unroll
+            for (int j = 0; j < K; j++) none[j] = R(0);
+            R *ex = part.at(g.dx, b, past, base), *et = part.at(g.ddt, b, past, base), *ez = part.at(g.dz, b, past, base);
+            for (uint32_t t = past; t < min(last * kTile, g.t); t += kTile) {
+                const bool there = t + part.step < g.t;
+                part.store(ex, there, none), part.store(et, there, none);
+                if (g.z.p) part.store(ez, there, none), ez += kTile * g.dz.ts;
+                ex += kTile * g.dx.ts, et += kTile * g.ddt.ts;
             }
             if (g.dh0 && at.live && at.seg == 0) {
 #pragma unroll
@@ -832,19 +994,19 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void ssm_bwd(SsmArgs<typena
         }
     }
     if constexpr (!FOLD) {
-        float* part = g.part + ((uint64_t)at.seg * g.walks + at.walk) * g.d * (g.n + 2);
+        float* to = g.part + ((uint64_t)at.seg * g.walks + at.walk) * g.d * (g.n + 2);
         if (at.live) {
 #pragma unroll
-            for (int i = 0; i < NQ; i++) store_states(part, ch, g.n, wave + W * i, da[i]);
+            for (int i = 0; i < NQ; i++) store_states(to, ch, g.n, wave + W * i, da[i]);
         }
-        __syncthreads();
-        parts[0][wave][0][lane] = dskip, parts[1][wave][0][lane] = dbias;
-        __syncthreads();
+        lds_barrier();
+        write_row<K>(parts[0][0][part.step] + part.c0, dskip), write_row<K>(parts[1][0][part.step] + part.c0, dbias);
+        lds_barrier();
         if (wave == 0 && at.live) {
             float s = 0.0f, u = 0.0f;
 #pragma unroll
-            for (int w = 0; w < W; w++) s += parts[0][w][0][lane], u += parts[1][w][0][lane];
-            part[(uint64_t)g.d * g.n + ch] = s, part[(uint64_t)g.d * (g.n + 1) + ch] = u;
+            for (int r = 0; r < kTile; r++) s += parts[0][0][r][lane], u += parts[1][0][r][lane];
+            to[(uint64_t)g.d * g.n + ch] = s, to[(uint64_t)g.d * (g.n + 1) + ch] = u;
         }
     }
 }
@@ -916,10 +1078,8 @@ Plan plan_of(const fhc_ssm_desc* g, bool backward) {
         if (p.segs > 64) p.segs = 64;
         if (p.segs < 1) p.segs = 1;
     }
-    if (!backward) {
-        if (const char* e = getenv("SSM_SEGS")) p.segs = atoi(e);
-        p.halves = p.quads <= 4 && getenv("SSM_HALVES") && atoi(getenv("SSM_HALVES"));
-    }
+    if (const char* e = getenv(backward ? "SSM_BSEGS" : "SSM_SEGS")) p.segs = atoi(e);
+    p.halves = !backward && p.quads <= 4 && getenv("SSM_HALVES") && atoi(getenv("SSM_HALVES"));
     p.seg_tiles = p.tiles ? (uint32_t)ceil_div(p.tiles, p.segs) : 1;
     p.segs = p.tiles ? (uint32_t)ceil_div(p.tiles, p.seg_tiles) : 1;
     p.walks = g->b;
@@ -991,8 +1151,7 @@ int launch(const char* op, const Plan& p, const SsmArgs<typename T::Raw>& a, hip
             return launched(op);
         }
     }
-    if (p.quads == 1) SSM(1, 1, 4);
-    else if (p.quads == 2) SSM(2, 1, 4);
+    if (p.quads <= 2) SSM(2, 1, 4);
     else if (p.quads <= 4) SSM(4, 1, 4);
     else if (p.quads <= 8) SSM(8, 1, 4);
     else SSM(8, 2, 4);

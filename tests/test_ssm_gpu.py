@@ -120,10 +120,11 @@ def test_short_conv_stream_of_calls_is_the_whole():
         at += n
     assert at == 41 and torch.equal(state, whole[1])
     L, S = m._lib(), m.FhcSeq
-    for n in (0, 1, 2, 41):  # through the C ABI, the new state over the old one
-        x, y, st = v["x"][:, :n].contiguous(), torch.empty_like(v["x"][:, :n]), v["state"].clone()
-        g = m.ShortConvDesc(1, 0, 5, n, 72, 4, v["w"].data_ptr(), v["bias"].data_ptr(), None)
-        rc = L.fhc_short_conv_forward(g, S(x.data_ptr(), n * 72, 72), st.data_ptr(), S(y.data_ptr(), n * 72, 72),
+    for n, d in ((0, 72), (1, 72), (2, 72), (41, 72), (1, 5), (2, 37), (3, 515), (1, 515), (2, 1031)):
+        v = conv_inputs(q, 5, n, d, 4, torch.bfloat16)  # through the C ABI, the new state over the old one
+        x, y, st = v["x"], torch.empty_like(v["x"]), v["state"].clone()
+        g = m.ShortConvDesc(1, 0, 5, n, d, 4, v["w"].data_ptr(), v["bias"].data_ptr(), None)
+        rc = L.fhc_short_conv_forward(g, S(x.data_ptr(), n * d, d), st.data_ptr(), S(y.data_ptr(), n * d, d),
                                       st.data_ptr(), torch.cuda.current_stream().cuda_stream)
         assert rc == 0, m.fhconv.last_error()
         want = m.short_conv(x, v["w"], v["bias"], state=v["state"])
