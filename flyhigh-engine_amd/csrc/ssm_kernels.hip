@@ -16,8 +16,8 @@
 //     dx = D s1 + skip q,   ddt = (s2 + x s1) sigmoid(dt + bias),   dz = dy p silu'(z)
 //     da[k] = sum of D a_t h_(t-1) g,   dB = sum over channels of D x g,   dC = sum over channels of q h
 // The forward pass keeps every tile's first state; a tile's 16 states and decays are computed again into registers and
-// walked backwards. The sums over a wave's 64 channels for dB and dC halve the values and the lanes at once, so that 8
-// values of 8 steps end one a lane; a closing launch adds the channel blocks, in their order.
+// walked backwards. The sums over a wave's 64 channels for dB and dC go through LDS; a closing launch adds the channel
+// blocks, in their order.
 #include "seq_args.h"
 
 namespace fhc {
@@ -179,16 +179,14 @@ __device__ __forceinline__ void each(F&& f) {
     each_of(f, std::make_integer_sequence<int, N>{});
 }
 
-// Where a workgroup is. Workgroups go round-robin to the 8 XCDs: the index is permuted so that an XCD has neighbouring channel
-// blocks. (A block's rows are one 128-byte line each. With every eighth block an XCD's lines lie on 2 of its L2's 16
-// channels, and the wait for them is what a tile takes: 4 x 4096 x 4096 bf16 815 us, with neighbours XXX.)
+// Where a workgroup is. Channel blocks come first in the index and segments last, so every XCD (workgroups go round-robin to
+// the 8) has a share of every sequence and segment: lengths may leave the late ones empty.
 struct Spot {
     uint32_t seg, walk, group, block, ch;
     bool live;
     template <class R>
     __device__ __forceinline__ Spot(const SsmArgs<R>& g, uint32_t lane) {
-        const uint32_t share = gridDim.x / 8, more = gridDim.x % 8, xcd = blockIdx.x % 8;
-        uint32_t q = xcd * share + min(xcd, more) + blockIdx.x / 8;
+        uint32_t q = blockIdx.x;
         block = q % g.blocks, q /= g.blocks;
         group = q % g.groups, q /= g.groups;
         walk = q % g.walks, seg = q / g.walks;
@@ -365,12 +363,6 @@ __device__ __forceinline__ f4 decay(float step, f4 rate) {
     for (int k = 0; k < 4; k++) a[k] = __builtin_amdgcn_exp2f(step * rate[k]);
     return a;
 }
-__device__ __forceinline__ f4 fma4(f4 a, f4 b, f4 c) {
-#pragma unroll
-    for (int k = 0; k < 4; k++) c[k] = __builtin_fmaf(a[k], b[k], c[k]);
-    return c;
-}
-
 // The ends of segments from zeros: W waves, NQ quads of states each.
 template <class T, int W, int NQ>
 __global__ __launch_bounds__(64 * W, 2) void ssm_fold(SsmArgs<typename T::Raw> g) {
@@ -453,18 +445,39 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_fold(SsmArgs<typename T::Raw> g
     if (wave == 0 && at.live) g.lasts[(uint64_t)at.seg * g.b * g.d + flat] = sum;
 }
 
+// h through the folds of `count` segments, `step` slots apart from p on: eight segments' loads are under way together. A
+// segment that is not there is one that changes nothing.
+template <int NS>
+__device__ __forceinline__ void through(const float* p, int64_t step, const float* total, int64_t tstep, uint32_t count,
+                                        const float (&rate)[NS], float (&h)[NS]) {
+    for (uint32_t s = 0; s < count; s += 8) {
+        float end[8][NS], sum[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            sum[u] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < NS; k++) end[u][k] = 0.0f;
+            if (s + u < count) {
+                sum[u] = total[(s + u) * tstep];
+                load_raw<float, NS, false>(p + (s + u) * step, end[u]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 8; u++)
+#pragma unroll
+            for (int k = 0; k < NS; k++)
+                h[k] = __builtin_fmaf(__builtin_amdgcn_exp2f(rate[k] * sum[u]), h[k], end[u][k]);
+    }
+}
+
 // W waves, NQ times NS states each.
 template <class T, int W, int NQ, int NS>
 __global__ __launch_bounds__(64 * W, 2) void ssm_fwd(SsmArgs<typename T::Raw> g) {
     using R = typename T::Raw;
     using P = Part<R, W>;
     constexpr int K = P::K, SPR = 16 / NS;  // steps a register of vectors
-#ifndef PIPE
-#define PIPE 0
-#endif
-    constexpr bool AHEAD = PIPE;
     __shared__ __align__(16) float steps[2][kTile][128];
-    __shared__ __align__(16) float parts[AHEAD ? 2 : 1][W][kTile][64];
+    __shared__ __align__(16) float parts[W][kTile][64];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Spot at(g, lane);
     const P part(lane, wave, g.width, at.block);
@@ -492,16 +505,9 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_fwd(SsmArgs<typename T::Raw> g)
             h[i].v[k] = s < g.n && g.segs == 1 && g.h0 ? g.h0[flat * g.n + s] : 0.0f;
         }
         if (g.segs > 1 && number(i, 0) < g.n) {
-            const float* p = reinterpret_cast<const float*>(g.ends + (uint64_t)b * g.quads * g.d);
-#pragma unroll
-            for (int k = 0; k < NS; k++) h[i].v[k] = p[in_quads(i, k)];
-            for (uint32_t s = 0; s < at.seg; s++) {
-                p += slots * 4;
-                const float total = g.lasts[(uint64_t)s * g.b * g.d + flat];
-#pragma unroll
-                for (int k = 0; k < NS; k++)
-                    h[i].v[k] = __builtin_fmaf(__builtin_amdgcn_exp2f(rate[i].v[k] * total), h[i].v[k], p[in_quads(i, k)]);
-            }
+            const float* p = reinterpret_cast<const float*>(g.ends + (uint64_t)b * g.quads * g.d) + in_quads(i, 0);
+            load_raw<float, NS, false>(p, h[i].v);
+            through<NS>(p + slots * 4, slots * 4, g.lasts + flat, (int64_t)g.b * g.d, at.seg, rate[i].v, h[i].v);
         }
     }
     const uint32_t from = first * kTile;
@@ -509,8 +515,8 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_fwd(SsmArgs<typename T::Raw> g)
     R* py = part.at(g.y, b, from, base);
     Vectors<R, NS> vb[2] = {{g.bm, b, from, at.group, g.n, wave, lane}, {g.bm, b, from, at.group, g.n, wave + W * (NQ - 1), lane}};
     Vectors<R, NS> vc[2] = {{g.cm, b, from, at.group, g.n, wave, lane}, {g.cm, b, from, at.group, g.n, wave + W * (NQ - 1), lane}};
-    // the inputs of the two tiles to come; x and z of the tile that runs, and of the one before
-    uint32_t x[2][P::kWords], dt[2][P::kWords], z[2][P::kWords], xs[2][P::kWords], zs[2][P::kWords];
+    // the inputs of the two tiles to come (a tile takes about as long as its loads from memory); x and z of the tile that runs
+    uint32_t x[2][P::kWords], dt[2][P::kWords], z[2][P::kWords], xs[P::kWords], zs[P::kWords];
     R bm[2][NQ], cm[2][NQ];
     auto load = [&](uint32_t left, auto slot) __attribute__((always_inline)) {
         const bool there = part.step < left;
@@ -544,8 +550,8 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_fwd(SsmArgs<typename T::Raw> g)
     auto keep = [&](auto slot) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < P::kWords; j++) {
-            xs[1][j] = xs[0][j], zs[1][j] = zs[0][j], xs[0][j] = x[slot][j], zs[0][j] = z[slot][j];
-            asm volatile("" : "+v"(xs[0][j]), "+v"(zs[0][j]));
+            xs[j] = x[slot][j], zs[j] = z[slot][j];
+            asm volatile("" : "+v"(xs[j]), "+v"(zs[j]));
         }
     };
     auto states = [&](uint32_t tile) __attribute__((always_inline)) {
@@ -558,7 +564,7 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_fwd(SsmArgs<typename T::Raw> g)
             else *reinterpret_cast<float2*>(to + in_quads(i, 0)) = float2{h[i].v[0], h[i].v[1]};
         }
     };
-    auto run = [&](int buf, int pbuf) __attribute__((always_inline)) {
+    auto run = [&](int buf) __attribute__((always_inline)) {
         float2 st[2][4];  // four steps' LDS reads are on their way while four steps run
         auto read = [&](int m) __attribute__((always_inline)) {
 #pragma unroll
@@ -578,27 +584,27 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_fwd(SsmArgs<typename T::Raw> g)
                     const float q = step_states<s % SPR * NS>(h[i], bv[i][s / SPR], st[m & 1][r].y, cv[i][s / SPR]);
                     p = i ? p + q : q;
                 });
-                parts[pbuf][wave][s][lane] = p;
+                parts[wave][s][lane] = p;
             });
         });
     };
-    // left: of the tile's steps those inside the length; there: those inside the tensor; of: xs[of] is the tile's
-    auto finish = [&](uint32_t left, uint32_t there, int pbuf, auto of) __attribute__((always_inline)) {
+    // left: of the tile's steps those inside the length; there: those inside the tensor
+    auto finish = [&](uint32_t left, uint32_t there) __attribute__((always_inline)) {
         float p[K];
         R out[K];
 #pragma unroll
-        for (int j = 0; j < K; j++) p[j] = skip[j] * element<T>(xs[of], j);
+        for (int j = 0; j < K; j++) p[j] = skip[j] * element<T>(xs, j);
 #pragma unroll
         for (int w = 0; w < W; w++) {
             float q[K];
-            read_row<K>(parts[pbuf][w][part.step] + part.c0, q);
+            read_row<K>(parts[w][part.step] + part.c0, q);
 #pragma unroll
             for (int j = 0; j < K; j++) p[j] += q[j];
         }
 #pragma unroll
         for (int j = 0; j < K; j++) {
             if (g.z.p) {
-                const float v = element<T>(zs[of], j);
+                const float v = element<T>(zs, j);
                 p[j] *= v * sigmoid1(v);
             }
             out[j] = part.step < left ? narrow(T{}, p[j]) : R(0);
@@ -613,44 +619,21 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_fwd(SsmArgs<typename T::Raw> g)
         load(left, Zero{});
         if (left > kTile) load(left - kTile, One{});
     }
-    if constexpr (AHEAD) {
-        // One barrier a tile: while a tile runs, the next one's steps are prepared and the one before is finished, into and
-        // from the other halves of the buffers.
-        if (left) prepare(left, Zero{});
-        auto body = [&](auto slot, auto other, uint32_t tile) __attribute__((always_inline)) {
-            keep(slot);
-            vectors(slot);
-            if (left > 2 * kTile) load(left - 2 * kTile, slot);
-            states(tile);
-            lds_barrier();
-            if (tile > first) finish(left + kTile, g.t - (tile - 1) * kTile, other, One{});
-            run(slot, slot);
-            if (tile + 1 < busy) prepare(left - kTile, other);
-            left -= kTile;
-        };
-        for (uint32_t tile = first; tile < busy; tile += 2) {
-            body(Zero{}, One{}, tile);
-            if (tile + 1 < busy) body(One{}, Zero{}, tile + 1);
-        }
+    auto body = [&](auto slot, uint32_t tile) __attribute__((always_inline)) {
+        prepare(left, slot);
+        keep(slot);
+        vectors(slot);
+        if (left > 2 * kTile) load(left - 2 * kTile, slot);
+        states(tile);
         lds_barrier();
-        if (first < busy) finish(n - (busy - 1) * kTile, g.t - (busy - 1) * kTile, (busy - 1 - first) & 1, Zero{});
-    } else {
-        auto body = [&](auto slot, uint32_t tile) __attribute__((always_inline)) {
-            prepare(left, slot);
-            keep(slot);
-            vectors(slot);
-            if (left > 2 * kTile) load(left - 2 * kTile, slot);
-            states(tile);
-            lds_barrier();
-            run(slot, 0);
-            lds_barrier();
-            finish(left, g.t - tile * kTile, 0, Zero{});
-            left -= kTile;
-        };
-        for (uint32_t tile = first; tile < busy; tile += 2) {
-            body(Zero{}, tile);
-            if (tile + 1 < busy) body(One{}, tile + 1);
-        }
+        run(slot);
+        lds_barrier();
+        finish(left, g.t - tile * kTile);
+        left -= kTile;
+    };
+    for (uint32_t tile = first; tile < busy; tile += 2) {
+        body(Zero{}, tile);
+        if (tile + 1 < busy) body(One{}, tile + 1);
     }
     for (uint32_t t = max(busy, first) * kTile; t < min(last * kTile, g.t); t += kTile) {
         R out[K];
@@ -669,74 +652,91 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_fwd(SsmArgs<typename T::Raw> g)
 }
 
 // Few steps: a thread has one quad of one channel's states, LP threads side by side a channel, so a wave reads and writes
-// the states as they lie; the steps follow one another.
-template <class T, int LP>
+// the states as they lie, 16 bytes a lane; the steps follow one another. WHOLE: n is a multiple of 4.
+// What bounds it (MI355X): HBM, which the states are read from and written to. One step of 64 x 4096 channels of 16
+// states, bf16: XXX us for 34 MB.
+template <class T, int LP, bool WHOLE>
 __global__ __launch_bounds__(256) void ssm_step(SsmArgs<typename T::Raw> g) {
     using R = typename T::Raw;
-    const uint64_t all = (uint64_t)g.b * g.d * LP;
-    for (uint64_t k = (uint64_t)blockIdx.x * 256 + threadIdx.x; k < (all + 255) / 256 * 256; k += (uint64_t)gridDim.x * 256) {
-        const bool live = k < all;
-        const uint32_t q = k % LP, flat = live ? (uint32_t)(k / LP) : 0, b = flat / g.d, ch = flat - b * g.d;
-        const uint32_t col = ch / g.width * g.n + 4 * q, n = g.lengths ? (uint32_t)min(max(g.lengths[b], 0), (int32_t)g.t) : g.t;
-        const bool has = live && 4 * q < g.n;
-        const f4 rate = rates_of(has ? g.a : nullptr, ch, g.n, q);
-        f4 h = load_states(has ? g.h0 : nullptr, flat, g.n, q);
-        const float bias = g.bias ? g.bias[ch] : 0.0f, skip = g.skip ? g.skip[ch] : 0.0f;
+    const uint64_t k = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const bool live = k < (uint64_t)g.d * LP;
+    const uint32_t q = k % LP, ch = live ? (uint32_t)(k / LP) : 0, group = g.groups > 1 ? ch / g.width : 0;
+    const uint32_t here = live && 4 * q < g.n ? min(4u, g.n - 4 * q) : 0, col = group * g.n + 4 * q;
+    auto states = [&](const float* p, uint64_t at) __attribute__((always_inline)) {
+        float h[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (WHOLE && here) load_raw<float, 4, false>(p + at * g.n + 4 * q, h);
+#pragma unroll
+        for (int i = 0; i < 4 && !WHOLE; i++)
+            if (i < (int)here) h[i] = p[at * g.n + 4 * q + i];
+        return States<4>{{h[0], h[1], h[2], h[3]}};
+    };
+    auto vector = [&](const R* p, R (&v)[4]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = R(0);
+        if (WHOLE && here) load_raw<R, 4, false>(p + col, v);
+#pragma unroll
+        for (int i = 0; i < 4 && !WHOLE; i++)
+            if (i < (int)here) v[i] = p[col + i];
+    };
+    States<4> rate = states(g.a, ch);
+#pragma unroll
+    for (int i = 0; i < 4; i++) rate.v[i] = rate_of(rate.v[i]);
+    const float bias = g.bias ? g.bias[ch] : 0.0f, skip = g.skip ? g.skip[ch] : 0.0f;
+    for (uint32_t b = blockIdx.y; b < g.b; b += gridDim.y) {
+        const uint32_t n = g.lengths ? (uint32_t)min(max(g.lengths[b], 0), (int32_t)g.t) : g.t;
+        const uint64_t flat = (uint64_t)b * g.d + ch;
+        States<4> h{{0.0f, 0.0f, 0.0f, 0.0f}};
+        if (g.h0) h = states(g.h0, flat);
         for (uint32_t t = 0; t < g.t; t++) {
-            if (g.states && has && t % kTile == 0)
-                g.states[(((uint64_t)b * g.tiles + t / kTile) * g.quads + q) * g.d + ch] = h;
-            float p = 0.0f, x = 0.0f;
+            if (g.states && here && t % kTile == 0)
+                g.states[(((uint64_t)b * g.tiles + t / kTile) * g.quads + q) * g.d + ch] = f4{h.v[0], h.v[1], h.v[2], h.v[3]};
+            float p = 0.0f, x = 0.0f, gate = 1.0f;
             if (t < n) {
                 float e;
+                R bv[4], cv[4];
+                vector(g.bm.at(b, t), bv), vector(g.cm.at(b, t), cv);
                 x = widen(T{}, g.x.at(b, t)[ch]);
+                if (g.z.p) {
+                    const float z = widen(T{}, g.z.at(b, t)[ch]);
+                    gate = z * sigmoid1(z);
+                }
                 const float step = softplus(widen(T{}, g.dt.at(b, t)[ch]) + bias, e), u = step * x;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    float bv = 0.0f, cv = 0.0f;
-                    if (has && 4 * q + i < g.n) {
-                        bv = widen(T{}, g.bm.at(b, t)[col + i]);
-                        cv = widen(T{}, g.cm.at(b, t)[col + i]);
-                    }
-                    h[i] = __builtin_fmaf(bv, u, __builtin_amdgcn_exp2f(step * rate[i]) * h[i]);
-                    p = __builtin_fmaf(cv, h[i], p);
+                    h.v[i] = __builtin_fmaf(widen(T{}, bv[i]), u, __builtin_amdgcn_exp2f(step * rate.v[i]) * h.v[i]);
+                    p = __builtin_fmaf(widen(T{}, cv[i]), h.v[i], p);
                 }
             }
 #pragma unroll
             for (int m = 1; m < LP; m *= 2) p += __shfl_xor(p, m);
             if (live && q == 0) {
-                p = __builtin_fmaf(skip, x, p);
-                if (g.z.p && t < n) {
-                    const float z = widen(T{}, g.z.at(b, t)[ch]);
-                    p *= z * sigmoid1(z);
-                }
+                p = __builtin_fmaf(skip, x, p) * gate;
                 g.y.at(b, t)[ch] = t < n ? narrow(T{}, p) : R(0);
             }
         }
-        if (has && g.ht) store_states(g.ht, flat, g.n, q, h);
+        if (here && g.ht) {
+            if (WHOLE) store_raw<float, 4, false>(g.ht + flat * g.n + 4 * q, h.v);
+#pragma unroll
+            for (int i = 0; i < 4 && !WHOLE; i++)
+                if (i < (int)here) g.ht[flat * g.n + 4 * q + i] = h.v[i];
+        }
     }
 }
 
-// The sum of two values over pairs of lanes, one kept in either lane: of a where the lane's bit is 0, of b where it is 1.
-__device__ __forceinline__ float merge32(float a, float b) {
-    swap32(a, b);
-    return a + b;
-}
-__device__ __forceinline__ float merge16(float a, float b) {
-    swap16(a, b);
-    return a + b;
-}
-// CTRL pairs lanes that differ in the bit (row_ror:8, row_half_mirror, quad_perm)
-template <int CTRL>
-__device__ __forceinline__ float merge_row(float a, float b, bool bit) {
-    const float keep = bit ? b : a, send = bit ? a : b;
+// The sums over a wave's 64 lanes of 16 values: each lane's values lie in LDS, 68 floats a value, four lanes take a value's 64
+// floats in 16-byte reads (whose 16 lanes at once fall on all 64 banks) and add their sums. A halving exchange in
+// registers takes 87 cycles of the vector unit for 8 values, this 30.
+constexpr int kPitch = 68;
+// lane + 1, lane + 2 of a quad of lanes
+__device__ __forceinline__ float add_quad(float v) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    const int i = __builtin_bit_cast(int, send);
-    return keep + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, CTRL, 0xF, 0xF, true));
-#else
-    return keep + send;
+    int i = __builtin_bit_cast(int, v);
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, 0xB1, 0xF, 0xF, true));
+    i = __builtin_bit_cast(int, v);
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, 0x4E, 0xF, 0xF, true));
 #endif
+    return v;
 }
-constexpr int kRor8 = 0x128, kHalfMirror = 0x141, kSwap2 = 0x4E, kSwap1 = 0xB1;
 
 // FOLD: the gradients that reach the states before a segment, from zeros behind it
 template <class T, int W, int NQ, bool FOLD>
@@ -748,6 +748,7 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_bwd(SsmArgs<typename T::Raw> g)
     __shared__ __align__(16) float ups[kTile][64];                     // q
     __shared__ __align__(16) float parts[FOLD ? 1 : 3][FOLD ? 1 : W][kTile][64];  // sum C h, s1, s2 of a wave's states
     __shared__ float vectors[FOLD ? 1 : kTile][2][W * NQ * 4];         // dB, dC over the workgroup's channels
+    __shared__ __align__(16) float lanes[FOLD ? 1 : W][16][kPitch];    // dB, dC of two steps, lane by lane
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Spot at(g, lane);
     const P part(lane, wave, g.width, at.block);
@@ -775,9 +776,12 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_bwd(SsmArgs<typename T::Raw> g)
             const uint32_t q = wave + W * i;
             const uint64_t slot = ((uint64_t)b * g.quads + q) * g.d + ch;
             c[i] = load_states(FOLD || !at.live ? nullptr : g.dht, flat, g.n, q);
-            if (!FOLD && q < g.quads && at.live) {
-                for (uint32_t s = g.segs - 1; s > at.seg; s--)
-                    c[i] = fma4(decay(g.lasts[(uint64_t)s * g.b * g.d + flat], rate[i]), c[i], g.ends[s * slots + slot]);
+            if (!FOLD && g.segs > 1 && q < g.quads && at.live) {
+                float r[4] = {rate[i][0], rate[i][1], rate[i][2], rate[i][3]}, h[4] = {c[i][0], c[i][1], c[i][2], c[i][3]};
+                const uint32_t behind = g.segs - 1;  // from the last segment to the one behind this
+                through<4>(reinterpret_cast<const float*>(g.ends + behind * slots + slot), -(int64_t)slots * 4,
+                           g.lasts + (uint64_t)behind * g.b * g.d + flat, -(int64_t)g.b * g.d, behind - at.seg, r, h);
+                c[i] = f4{h[0], h[1], h[2], h[3]};
             }
         }
         const uint32_t from = busy > first ? (busy - 1) * kTile : 0;  // tiles go from the last to the first
@@ -876,7 +880,16 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_bwd(SsmArgs<typename T::Raw> g)
                             add_outer<rc * 4>(h[s], bv[i][m], st[rc].y);
                         });
                     });
-                    float m4 = 0.0f, m2 = 0.0f, m1 = 0.0f;  // sums of odd steps that wait for their even neighbours
+                    float sums[16];  // a lane's share of the sums of the two steps before
+                    // the sums of steps s and s + 1, whose products are in LDS: value 8 (step) + 4 (dC) + state, a quad each
+                    auto close = [&](int s) __attribute__((always_inline)) {
+                        float v = sums[0];
+#pragma unroll
+                        for (int k = 1; k < 16; k++) v += sums[k];
+                        v = add_quad(v);
+                        const uint32_t at = lane >> 2;
+                        if ((lane & 3) == 0) vectors[s + (at >> 3)][at >> 2 & 1][(wave + W * i) * 4 + (at & 3)] = v;
+                    };
                     each<4>([&](auto mc) {
                         constexpr int m = 3 - mc;
                         float2 st[4];
@@ -888,7 +901,9 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_bwd(SsmArgs<typename T::Raw> g)
                             constexpr int r = 3 - rc, s = 4 * m + r;
                             float p, s1, s2 = 0.0f;
                             step_back<r * 4>(c[i], h[s], bv[i][m], cv[i][m], q[r], p, s1);
-                            const f4 db = c[i] * st[r].y, dc = h[s] * q[r];
+                            float* to = lanes[wave][(s & 1) * 8] + lane;
+#pragma unroll
+                            for (int k = 0; k < 4; k++) to[k * kPitch] = c[i][k] * st[r].y, to[(4 + k) * kPitch] = h[s][k] * q[r];
                             c[i] *= decay(st[r].x, rate[i]);
                             const f4 past = c[i] * (s ? h[s ? s - 1 : 0] : h0[i]);
 #pragma unroll
@@ -901,32 +916,18 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_bwd(SsmArgs<typename T::Raw> g)
                                 s2 += parts[2][wave][s][lane];
                             }
                             parts[0][wave][s][lane] = p, parts[1][wave][s][lane] = s1, parts[2][wave][s][lane] = s2;
-                            // lanes 32 up take dC; bits 4 and 3 of the lane are the state's, then bit 2 the step's lowest,
-                            // bit 1 the next and bit 0 the third
-                            const float r0 = merge16(merge32(db[0], dc[0]), merge32(db[2], dc[2]));
-                            const float r1 = merge16(merge32(db[1], dc[1]), merge32(db[3], dc[3]));
-                            float v = merge_row<kRor8>(r0, r1, lane & 8);
-                            if constexpr ((s & 1) == 1) {
-                                m4 = v;
-                            } else {
-                                v = merge_row<kHalfMirror>(v, m4, lane & 4);
-                                if constexpr ((s & 2) == 2) {
-                                    m2 = v;
-                                } else {
-                                    v = merge_row<kSwap2>(v, m2, lane & 2);
-                                    if constexpr ((s & 4) == 4) {
-                                        m1 = v;
-                                    } else {
-                                        v = merge_row<kSwap1>(v, m1, lane & 1);
-                                        const uint32_t step = s + ((lane >> 2 & 1) | (lane & 2) | (lane & 1) << 2);
-                                        const uint32_t k = (lane >> 3 & 1) | (lane >> 3 & 2);
-                                        vectors[step][lane >> 5][(wave + W * i) * 4 + k] = v;
-                                    }
-                                }
+                            if constexpr ((s & 1) == 0) {
+                                // a wave's LDS accesses stay in order: the reads see the writes before them, and the next
+                                // steps' writes come after
+                                if constexpr (s < kTile - 2) close(s + 2);
+                                fence();
+                                read_row<16>(lanes[wave][lane >> 2] + (lane & 3) * 16, sums);
+                                fence();
                             }
                             __builtin_amdgcn_sched_barrier(0);
                         });
                     });
+                    close(0);
                 });
             }
             lds_barrier();
@@ -1055,7 +1056,9 @@ int close_vectors(const char* op, const fhc_ssm_desc* g, const float* bc, const 
     return launched(op);
 }
 
-constexpr uint32_t kFewSteps = 4;  // up to here the states' bytes are what counts
+// Up to here the states' bytes are what counts: 64 x 4096 channels of 16 states, bf16, us a call by steps, and by tiles: 1
+// step 15, 44; 4 20, 44; 8 32, 45 (64 x 1024 of 64 states: 33, 44).
+constexpr uint32_t kFewSteps = 8;
 
 struct Plan {
     uint32_t width, blocks, quads, waves, tiles, segs, seg_tiles, walks;
@@ -1071,15 +1074,30 @@ Plan plan_of(const fhc_ssm_desc* g, bool backward) {
     p.tiles = (uint32_t)ceil_div(g->t, kTile);
     const uint64_t cols = (uint64_t)g->groups * p.blocks;
     const uint64_t one = g->b * cols;
+    // Segments, where the columns alone leave CUs idle: each launch works on about as many workgroups as keep their vector
+    // units busy (the fold is half as much work again, so not more than that takes), of at least four tiles. Two states a
+    // lane instead of four where there are columns for every CU but not for every SIMD. us, bf16, n 16, by workgroups:
+    //   forward             one a column block, four states   two states   segments
+    //    16  (1024 steps)   118                               -            4: 57, 8: 34, 16: 23, 32: 24
+    //    64  (128 steps)    20                                18           2: 22, 4: 20
+    //   128  (2048 steps)   228                               198          8: 141, 16: 143
+    //   192  (2048)         232                               205          4: 211, 8: 202
+    //   256  (4096)         453                               398          2: 530
+    //   512  (2048)         339                               336
+    //   768  (1024)         244                               252
+    //   a training step     backward in segments of
+    //    64  (1024)         4: 183, 8: 152, 16: 164
+    //   144  (2051 at most, lengths of 0 to that)   4: 564, 7: 540, 14: 511, 20: 523
+    //   256  (1024)         1: 481, 2: 451, 4: 457
+    //   512  (1024)         1: 671, 2: 772
     p.segs = 1;
-    if (one < 256 && p.tiles >= 8) {
-        const uint64_t want = 1024 / one;
-        p.segs = (uint32_t)(want < p.tiles / 4 ? want : p.tiles / 4);
-        if (p.segs > 64) p.segs = 64;
+    const uint64_t most = p.tiles / 4 < 64 ? p.tiles / 4 : 64;
+    if (backward ? one < 512 : one < 192 && p.tiles >= 16) {
+        const uint64_t want = ceil_div(!backward ? 2048 : p.quads > 4 ? 512 : 1024, one);
+        p.segs = (uint32_t)(want < most ? want : most);
         if (p.segs < 1) p.segs = 1;
     }
-    if (const char* e = getenv(backward ? "SSM_BSEGS" : "SSM_SEGS")) p.segs = atoi(e);
-    p.halves = !backward && p.quads <= 4 && getenv("SSM_HALVES") && atoi(getenv("SSM_HALVES"));
+    p.halves = !backward && p.segs == 1 && one <= 512 && p.quads <= 4;
     p.seg_tiles = p.tiles ? (uint32_t)ceil_div(p.tiles, p.segs) : 1;
     p.segs = p.tiles ? (uint32_t)ceil_div(p.tiles, p.seg_tiles) : 1;
     p.walks = g->b;
@@ -1163,13 +1181,19 @@ template <class T>
 int launch_step(const char* op, const Plan& p, const SsmArgs<typename T::Raw>& a, hipStream_t st) {
     uint32_t lp = 1;
     while (lp < p.quads) lp *= 2;
-    const uint64_t blocks = ceil_div((uint64_t)a.b * a.d * lp, 256);
-    const dim3 grid((uint32_t)(blocks < 1u << 22 ? blocks : 1u << 22));
-    if (lp == 1) hipLaunchKernelGGL((ssm_step<T, 1>), grid, dim3(256), 0, st, a);
-    else if (lp == 2) hipLaunchKernelGGL((ssm_step<T, 2>), grid, dim3(256), 0, st, a);
-    else if (lp == 4) hipLaunchKernelGGL((ssm_step<T, 4>), grid, dim3(256), 0, st, a);
-    else if (lp == 8) hipLaunchKernelGGL((ssm_step<T, 8>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((ssm_step<T, 16>), grid, dim3(256), 0, st, a);
+    const dim3 grid((uint32_t)ceil_div((uint64_t)a.d * lp, 256), a.b < 65535 ? a.b : 65535);
+    FHC_TRY(check_grid(op, (uint64_t)grid.x * grid.y, 256));
+#define STEP(LP)                                                                                           \
+    do {                                                                                                   \
+        if (a.n % 4 == 0) hipLaunchKernelGGL((ssm_step<T, LP, true>), grid, dim3(256), 0, st, a);          \
+        else hipLaunchKernelGGL((ssm_step<T, LP, false>), grid, dim3(256), 0, st, a);                      \
+    } while (0)
+    if (lp == 1) STEP(1);
+    else if (lp == 2) STEP(2);
+    else if (lp == 4) STEP(4);
+    else if (lp == 8) STEP(8);
+    else STEP(16);
+#undef STEP
     return launched(op);
 }
 
