@@ -65,6 +65,7 @@ struct GemmArgs {
     int tiles_m, tiles_n;
     uint16_t *o0, *o1;
     int64_t ldo;
+    bool dwords;  // kLinear: residual and output of whole, 4-byte aligned pairs
     bool quads;  // kStore: outputs of whole, 8-byte aligned quads, whose offsets in a tile fit 32 bits
     float *pre_g, *pre_u;  // [m][ldpre]
     int64_t ldpre;
@@ -217,6 +218,20 @@ __device__ __forceinline__ uint2 get8(R rsrc, uint32_t at) {
     return uint2{v[0], v[1]};
 #else
     return uint2{};
+#endif
+}
+template <class R>
+__device__ __forceinline__ uint32_t get4(R rsrc, uint32_t at) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_amdgcn_raw_buffer_load_b32(rsrc, at, 0, 0);
+#else
+    return 0;
+#endif
+}
+template <class R>
+__device__ __forceinline__ void put4(R rsrc, uint32_t v, uint32_t at) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_raw_buffer_store_b32(v, rsrc, at, 0, 0);
 #endif
 }
 template <class R>
@@ -472,7 +487,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ffn_gemm(GemmArgs g) {
         }
     } else if constexpr (E == kLinear) {
         const Tail tail{g.bias, g.res, g.ldr, g.pre_g, g.ldpre, g.act};
-        if (g.quads) {
+        // PAIRS: a lane's 4 columns as two dwords, each inside or out as a whole
+        auto rows = [&](auto pairs) __attribute__((always_inline)) {
+            constexpr bool PAIRS = pairs;
             const auto ty = at_tile(g.o0, g.ldo), tr = at_tile(g.res ? g.res : g.o0, g.res ? g.ldr : g.ldo);
             const auto tp = at_tile(g.pre_g, g.ldpre);
             f4 bias[NB];
@@ -481,12 +498,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ffn_gemm(GemmArgs g) {
 #pragma unroll
                 for (int r = 0; r < 4; r++)
                     bias[j][r] = g.bias ? widen(T{}, g.bias[min(n0 + nr + j * 16 + r, g.n - 1)]) : 0.0f;
+            // of a quad the second dword, out of range where its columns are
+            auto second = [&](int j, uint32_t at) { return n0 + nr + j * 16 + 2 < g.n ? at + 4 : kFar; };
             // the residual's next 16 rows are on their way while 16 rows are worked on (y may lie over it: an element is
             // read before it is written, by the same lane)
             uint2 rr[2][NB];
             auto load = [&](int i) {
 #pragma unroll
-                for (int j = 0; j < NB; j++) rr[i & 1][j] = get8(tr, place(i, j, g.ldr, g.n, 2));
+                for (int j = 0; j < NB; j++) {
+                    const uint32_t at = place(i, j, g.ldr, g.n, 2);
+                    rr[i & 1][j] = PAIRS ? uint2{get4(tr, at), get4(tr, second(j, at))} : get8(tr, at);
+                }
             };
             if (g.res) load(0);
 #pragma unroll
@@ -509,9 +531,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ffn_gemm(GemmArgs g) {
                     uint16_t q[4];
 #pragma unroll
                     for (int r = 0; r < 4; r++) q[r] = narrow(T{}, v[r]);
-                    put8(ty, pack(q), place(i, j, g.ldo, g.n, 2));
+                    const uint2 o = pack(q);
+                    const uint32_t at = place(i, j, g.ldo, g.n, 2);
+                    if (PAIRS) put4(ty, o.x, at), put4(ty, o.y, second(j, at));
+                    else put8(ty, o, at);
                 }
             }
+        };
+        if (g.quads) {
+            rows(std::false_type{});
+        } else if (g.dwords) {
+            rows(std::true_type{});
         } else {
 #pragma unroll
             for (int i = 0; i < MB; i++) {

@@ -313,6 +313,8 @@ int product(const char* op, GemmArgs g, float* part, hipStream_t st) {
     if ((int64_t)s.tiles_m * s.tiles_n >= 1ll << 31) return fail(-1, "%s: too many tiles", op);
     g.quads = g.n % 4 == 0 && g.ldo % 4 == 0 && g.ldo <= 1 << 21 && aligned(g.o0, 8) && aligned(g.o1, 8) &&
               g.ldr % 4 == 0 && g.ldr <= 1 << 21 && aligned(g.res, 8);
+    g.dwords = g.n % 2 == 0 && g.ldo % 2 == 0 && g.ldo <= 1 << 21 && aligned(g.o0, 4) && g.ldr % 2 == 0 &&
+               g.ldr <= 1 << 21 && aligned(g.res, 4);
     if constexpr (E == kStore || E == kLinear) {
         constexpr bool LIN = E == kLinear;
         const Tail tail{g.bias, g.res, g.ldr, g.pre_g, g.ldpre, g.act};
@@ -337,19 +339,29 @@ int product(const char* op, GemmArgs g, float* part, hipStream_t st) {
 template <class T, bool GLU, bool LIN>
 int skinny(const char* op, const SkinnyArgs& a, hipStream_t st) {
     if (a.n == 0) return 0;
-    constexpr int NW = GLU ? 4 : 16;
     const dim3 grid((uint32_t)ceil_div(a.n, GLU ? 16 : 8));
     // a whole step's loads are 16-byte aligned (the second half of K starts at a multiple of 32)
     const bool al = a.k % 8 == 0 && a.ldx % 8 == 0 && a.ldw % 8 == 0 && aligned(a.x, 16) && aligned(a.w0, 16) &&
                     aligned(a.w1, 16);
-#define SKINNY(NB)                                                                                              \
+#define SKINNY_OF(NB, NW)                                                                                       \
     do {                                                                                                        \
-        if (al) hipLaunchKernelGGL((ffn_skinny<T, GLU, NB, NW, true, LIN>), grid, dim3(64 * NW), 0, st, a);          \
-        else hipLaunchKernelGGL((ffn_skinny<T, GLU, NB, NW, false, LIN>), grid, dim3(64 * NW), 0, st, a);            \
+        if (al) hipLaunchKernelGGL((ffn_skinny<T, GLU, NB, NW, true, LIN>), grid, dim3(64 * NW), 0, st, a);     \
+        else hipLaunchKernelGGL((ffn_skinny<T, GLU, NB, NW, false, LIN>), grid, dim3(64 * NW), 0, st, a);       \
+    } while (0)
+// Few waves a workgroup where there are many of them, which then all run at once: LIN, bf16, us with 16 and with 4 waves:
+// 4 x 2048 -> 8192 (1024 workgroups) 15, 11; 32 x 2048 -> 8192 30, 23; 4 x 4096 -> 4096 (512) 14, 12; 4 x 8192 -> 4096
+// 21, 22; 4 x 8192 -> 2048 (256) 12, 14.
+#define SKINNY(NB)                                                \
+    do {                                                          \
+        if constexpr (GLU) SKINNY_OF(NB, 4);                      \
+        else if constexpr (!LIN) SKINNY_OF(NB, 16);               \
+        else if (grid.x >= 512) SKINNY_OF(NB, 4);                   \
+        else SKINNY_OF(NB, 16);                                   \
     } while (0)
     if (a.rows <= 16) SKINNY(1);
     else SKINNY(2);
 #undef SKINNY
+#undef SKINNY_OF
     return launched(op);
 }
 

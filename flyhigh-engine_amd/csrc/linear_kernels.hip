@@ -4,6 +4,11 @@
 // Forward: one product, whose epilogue adds the bias in f32, keeps the sum where the backward pass needs it, applies the
 // activation and adds the residual. Backward: dv = dy act'(v), rounded once to the operands' type, with its sums over rows
 // for the bias, in one pass (without an activation dv is dy itself, and only the bias needs a pass); dx = dv w, dw = dv^T x.
+//
+// What bounds it (MI355X): matrix units for large calls, HBM for few rows. 8192 x 2048 -> 8192 bf16 with silu, bias and
+// residual: 320 us forward, 390 where v is kept (its f32 passes through the epilogue), a training step 930: dv 125 (4.3
+// TB/s), dx and dw 210 to 230 each (1200 to 1310 TFLOP/s; a large library product reaches 1344). 4 x 2048 -> 8192: 11 us for
+// 34 MB.
 #include "ffn_product.h"
 #include "seq_args.h"
 
