@@ -1,12 +1,20 @@
-"""A recurrent block on rows of channels over the operators of fhseq: a gated linear recurrence and a gated feed-forward
-block, each behind norms, a gate and a scaled residual. With u the block's normed input and x the residual stream:
+"""Recurrent blocks on rows of channels over the operators of fhseq, u a block's normed input and x the residual stream.
+
+RecurrentBlock: a gated linear recurrence and a gated feed-forward block, each behind norms, a gate and a scaled residual:
 
     s, state = glr(u wx^T, u wr^T, u wi^T, lam, state),   y1, u1 = norm_block(x, s wo^T, post1, gate1, pre1)
     y, u'    = norm_block(y1, ffn(u1, wg, wu, wd), post2, gate2, pre2)
 
+Its square projections are plain library products.
+
+StateSpaceBlock: a selective state space scan behind a short convolution, gated, with a residual:
+
+    v, z = u wi^T,   s, taps = short_conv(v, wc, bc, taps),   r, B, C = s wp^T
+    o, h = ssm(s, r wt^T, a, B, C, skip, z, dt_bias, h),   y = o wo^T + x
+
 The sequences are tokens, or a stream's feature maps: an NHWC map of h x w pixels is h * w sequences, and a frame is one
-step of each (``forward`` on [pixels, 1, channels] with the state that the last frame left). The square projections are
-plain library products. ``python fhblock.py`` streams frames through a block and trains one.
+step of each (``forward`` on [pixels, 1, channels] with the state that the last frame left). ``python fhblock.py`` streams
+frames through both blocks and trains one of each.
 """
 from __future__ import annotations
 
@@ -93,44 +101,115 @@ class RecurrentBlock:
         return g
 
 
+class StateSpaceBlock:
+    """Weights of one block of ``c`` channels, ``e`` wide inside, with ``n`` states a channel, B and C shared by the
+    channels of each of ``groups`` groups, steps of ``rank`` numbers and ``taps`` taps, in ``dtype`` (f16, bf16). The
+    states decay at rates of 1 to n times the step, which starts at 0.001 to 0.1."""
+
+    def __init__(self, c, e, n=16, groups=1, rank=None, taps=4, dtype=torch.bfloat16, seed=0, device="cuda"):
+        g = torch.Generator(device=device)
+        g.manual_seed(seed)
+        rank = max(c // 16, 1) if rank is None else rank
+
+        def normal(rows, cols):
+            return (torch.randn(rows, cols, generator=g, device=device) * cols ** -0.5).to(dtype)
+
+        self.c, self.e, self.n, self.groups, self.rank, self.taps = c, e, n, groups, rank, taps
+        first = 0.001 * 100.0 ** torch.rand(e, generator=g, device=device, dtype=torch.float64)
+        self.p = dict(wi=normal(2 * e, c), wc=normal(e, taps), bc=torch.zeros(e, dtype=dtype, device=device),
+                      wp=normal(rank + 2 * groups * n, e), wt=normal(e, rank), wo=normal(c, e))
+        self.p["rates"] = torch.log(torch.arange(1, n + 1, device=device).float()).repeat(e, 1)  # a = -exp(rates)
+        self.p["skip"] = torch.ones(e, device=device)
+        self.p["dt_bias"] = torch.log(torch.expm1(first)).float()
+
+    def _split(self, m):
+        return torch.split(m, (self.rank, self.groups * self.n, self.groups * self.n), 2)
+
+    def forward(self, x, u, state=None, lengths=None, train=False):
+        """x, u [sequences, steps, c]: the residual stream and this block's normed input; state (taps [sequences, taps -
+        1, e], h [sequences, e, n] f32) as an earlier call returned it, or None (zeros); lengths as in ``fhseq.ssm``: past
+        them y is x, and the state is that of a sequence's last step; u has to be finite there. Returns (y, state), with
+        train also what ``backward`` takes."""
+        p, (b, t, c), e = self.p, x.shape, self.e
+        before, h0 = (None, None) if state is None else state
+        ur = u.reshape(-1, c)
+        v, z = fhseq.linear(ur, p["wi"]).view(b, t, 2 * e).split(e, 2)  # no copies: the halves of a row
+        s, after = fhseq.short_conv(v, p["wc"], p["bc"], state=before, lengths=lengths)
+        m = fhseq.linear(s.reshape(-1, e), p["wp"]).view(b, t, p["wp"].shape[0])
+        r, bm, cm = self._split(m)
+        dt = fhseq.linear(r.flatten(0, 1), p["wt"]).view(b, t, e)
+        a = -torch.exp(p["rates"])
+        out = fhseq.ssm(s, dt, a, bm, cm, p["skip"], z, p["dt_bias"], h0, lengths, train)
+        y = fhseq.linear(out[0].reshape(-1, e), p["wo"], residual=x.reshape(-1, c)).view(b, t, c)
+        res = (y, (after, out[1]))
+        return res + ((ur, v, z, before, s, m, dt, a, out[0], out[2], lengths),) if train else res
+
+    def backward(self, kept, dy, dstate=None):
+        """The gradients of a loss with dy and dstate (of forward's state; it or either of its two may be None): a dict of
+        the weights' ("wi", .. "dt_bias") and "x", "u", "taps", "h"."""
+        ur, v, z, before, s, m, dt, a, o, states, lengths = kept
+        p, (b, t, e), c = self.p, s.shape, self.c
+        dafter, dend = (None, None) if dstate is None else dstate
+        r, bm, cm = self._split(m)
+        g = dict(x=dy)
+        do, g["wo"], _ = fhseq.linear_backward(o.reshape(-1, e), p["wo"], None, dy.reshape(-1, c), bias=False)
+        ds, ddt, da, dbm, dcm, g["skip"], dz, g["dt_bias"], g["h"] = fhseq.ssm_backward(
+            s, dt, a, bm, cm, states, do.view(b, t, e), p["skip"], z, p["dt_bias"], dend, lengths)
+        g["rates"] = da * a
+        dr, g["wt"], _ = fhseq.linear_backward(r.flatten(0, 1), p["wt"], None, ddt.reshape(-1, e), bias=False)
+        dm = torch.cat((dr.view(b, t, self.rank), dbm, dcm), 2)
+        ds1, g["wp"], _ = fhseq.linear_backward(s.reshape(-1, e), p["wp"], None, dm.flatten(0, 1), bias=False)
+        dv, g["wc"], g["bc"], g["taps"] = fhseq.short_conv_backward(v, p["wc"], p["bc"], ds + ds1.view(b, t, e), "silu",
+                                                                    before, dafter, lengths)
+        du, g["wi"], _ = fhseq.linear_backward(ur, p["wi"], None, torch.cat((dv, dz), 2).flatten(0, 1), bias=False)
+        g["u"] = du.view(b, t, c)
+        return g
+
+
 def main():
     torch.manual_seed(0)
     c, f, h, w, frames = 128, 512, 30, 54, 24
-    block = RecurrentBlock(c, f, torch.float16)
     maps = torch.randn(frames, h * w, c, device="cuda").half()
+    for block in (RecurrentBlock(c, f, torch.float16), StateSpaceBlock(c, 2 * c, dtype=torch.float16)):
 
-    def stream():
-        state = None
-        for m in maps:  # a frame: one step of every pixel
-            y, _, state = block.forward(m[:, None], m[:, None], state)
-        return y, state
+        def stream():
+            state = None
+            for m in maps:  # a frame: one step of every pixel
+                state = block.forward(m[:, None], m[:, None], state)[-1]
+            return state
 
-    stream()
-    torch.cuda.synchronize()
-    begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-    begin.record()
-    y, state = stream()
-    end.record()
-    torch.cuda.synchronize()
-    whole = block.forward(maps.transpose(0, 1), maps.transpose(0, 1))
-    print(f"{frames} maps of {h} x {w} x {c}, a frame at a time: {begin.elapsed_time(end) / frames * 1e3:.0f} us a frame; "
-          f"against the whole stream at once: state off by {(state - whole[2]).abs().max().item():.2g}")
+        stream()
+        torch.cuda.synchronize()
+        begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        begin.record()
+        state = stream()
+        end.record()
+        torch.cuda.synchronize()
+        whole = block.forward(maps.transpose(0, 1), maps.transpose(0, 1))[-1]
+        off = max((s.float() - q.float()).abs().max().item() for s, q in zip(state, whole))
+        print(f"{type(block).__name__}: {frames} maps of {h} x {w} x {c}, a frame at a time: "
+              f"{begin.elapsed_time(end) / frames * 1e3:.0f} us a frame; against the whole stream at once: state off by "
+              f"{off:.2g}")
 
     b, t = 8, 256
-    block = RecurrentBlock(c, f, torch.bfloat16, seed=1)
     x = torch.randn(b, t, c, device="cuda").bfloat16()
     goal = torch.roll(x, 1, 1)  # the value one step ago, which only the state carries
-    masters = {k: q.float() for k, q in block.p.items()}
-    for step in range(101):
-        y, u, _, kept = block.forward(x, x, train=True)
-        err = u.float() - goal.float()
-        if step % 25 == 0:
-            print(f"step {step}: mean square {err.square().mean().item():.4f}")
-        grads = block.backward(kept, None, (err * (2 / err.numel()) * 1024).bfloat16())
-        for k, q in masters.items():
-            d = grads[k].float() / 1024
-            q -= 0.02 * d / (d.square().mean().sqrt() + 1e-12) * q.square().mean().sqrt()
-            block.p[k].copy_(q)
+    for block in (RecurrentBlock(c, f, torch.bfloat16, seed=1), StateSpaceBlock(c, 2 * c, seed=1)):
+        masters = {k: q.float() for k, q in block.p.items()}
+        for step in range(101):
+            if isinstance(block, RecurrentBlock):
+                _, u, _, kept = block.forward(x, x, train=True)
+            else:
+                u, _, kept = block.forward(torch.zeros_like(x), x, train=True)
+            err = u.float() - goal.float()
+            if step % 25 == 0:
+                print(f"{type(block).__name__}, step {step}: mean square {err.square().mean().item():.4f}")
+            du = (err * (2 / err.numel()) * 1024).bfloat16()
+            grads = block.backward(kept, None, du) if isinstance(block, RecurrentBlock) else block.backward(kept, du)
+            for k, q in masters.items():
+                d = grads[k].float() / 1024
+                q -= 0.02 * d / (d.square().mean().sqrt() + 1e-12) * q.square().mean().sqrt()
+                block.p[k].copy_(q)
 
 
 if __name__ == "__main__":
