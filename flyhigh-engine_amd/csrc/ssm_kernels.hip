@@ -910,6 +910,9 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_bwd(SsmArgs<typename T::Raw> g)
                             for (int k = 0; k < 4; k++) {
                                 da[i][k] = __builtin_fmaf(past[k], st[r].x, da[i][k]);
                                 s2 = __builtin_fmaf(past[k], rate[i][k], s2);
+                                // added here: moved behind the tile's steps, as the compiler does, the sums would hold the 64
+                                // products of a quad in registers until then
+                                asm volatile("" : "+v"(da[i][k]));
                             }
                             if (i > 0) {
                                 p += parts[0][wave][s][lane], s1 += parts[1][wave][s][lane];
