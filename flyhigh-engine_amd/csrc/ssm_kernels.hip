@@ -1070,16 +1070,16 @@ struct Plan {
     size_t ends_bytes, lasts_bytes, part_bytes, bc_bytes;
 };
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
-Plan plan_of(const fhc_ssm_desc* g, bool backward) {
+Plan plan_of(const fhc_ssm_desc* g, bool backward, bool ragged) {
     Plan p{};
     p.width = g->d / g->groups, p.blocks = (uint32_t)ceil_div(p.width, 64), p.quads = (g->n + 3) / 4;
     p.waves = p.quads <= 1 ? 2 : p.quads <= 2 ? 4 : 8;  // at most
     p.tiles = (uint32_t)ceil_div(g->t, kTile);
     const uint64_t cols = (uint64_t)g->groups * p.blocks;
     const uint64_t one = g->b * cols;
-    // Segments, where the columns alone leave CUs idle: each launch works on about as many workgroups as keep their vector
-    // units busy (the fold is half as much work again, so not more than that takes), of at least four tiles. Two states a
-    // lane instead of four where there are columns for every CU but not for every SIMD. us, bf16, n 16, by workgroups:
+    // Segments, of at least four tiles, where the columns alone leave CUs idle. Forward as many as keep the vector units busy
+    // (the fold is half as much work again, so not more than that takes), and two states a lane instead of four where there
+    // are columns for every CU but not for every SIMD. us, bf16, n 16, by workgroups:
     //   forward             one a column block, four states   two states   segments
     //    16  (1024 steps)   118                               -            4: 57, 8: 34, 16: 23, 32: 24
     //    64  (128 steps)    20                                18           2: 22, 4: 20
@@ -1088,17 +1088,28 @@ Plan plan_of(const fhc_ssm_desc* g, bool backward) {
     //   256  (4096)         453                               398          2: 530
     //   512  (2048)         339                               336
     //   768  (1024)         244                               252
-    //   a training step     backward in segments of
-    //    64  (1024)         4: 183, 8: 152, 16: 164
-    //   144  (2051 at most, lengths of 0 to that)   4: 564, 7: 540, 14: 511, 20: 523
-    //   256  (1024)         1: 481, 2: 451, 4: 457
+    // Backward the number whose rounds of workgroups (as many at once as LDS holds) take the least, a round the tiles of a
+    // segment and two for its start, with segments 1.3 times that for the fold; with lengths, which leave some empty, as many
+    // as even that out. A training step in segments of
+    //    64  (1024)         4: 196, 8: 156, 12: 174, 16: 163
+    //   144  (512)          1: 244, 2: 249, 3: 189, 4: 208, 7: 182, 8: 191
+    //   256  (1024)         1: 473, 2: 450, 3: 461, 4: 440, 8: 451
     //   512  (1024)         1: 671, 2: 772
+    //   128  (1024, n 64)   1: 1094, 2: 769, 3: 959, 4: 771, 8: 790
+    //   144  (lengths of 0 to 2051)   4: 597, 8: 506, 11: 484, 14: 480, 18: 475, 22: 488
     p.segs = 1;
     const uint64_t most = p.tiles / 4 < 64 ? p.tiles / 4 : 64;
-    if (backward ? one < 512 : one < 192 && p.tiles >= 16) {
-        const uint64_t want = ceil_div(!backward ? 2048 : p.quads > 4 ? 512 : 1024, one);
-        p.segs = (uint32_t)(want < most ? want : most);
-        if (p.segs < 1) p.segs = 1;
+    auto at_most = [&](uint64_t want) { return (uint32_t)(want < most ? want : most < 1 ? 1 : most); };
+    if (!backward && one < 192 && p.tiles >= 16) p.segs = at_most(ceil_div(2048, one));
+    if (backward && one < 512 && ragged) {
+        p.segs = at_most(ceil_div(2048, one));
+    } else if (backward && one < 512) {
+        const uint64_t at_once = p.quads <= 2 ? 768 : p.quads <= 4 ? 512 : 256;
+        uint64_t best = 0;
+        for (uint32_t s = 1; s == 1 || s <= most; s++) {
+            const uint64_t time = ceil_div(one * s, at_once) * (ceil_div(p.tiles, s) + 2) * (s > 1 ? 13 : 10);
+            if (s == 1 || time < best) best = time, p.segs = s;
+        }
     }
     p.halves = !backward && p.segs == 1 && one <= 512 && p.quads <= 4;
     p.seg_tiles = p.tiles ? (uint32_t)ceil_div(p.tiles, p.segs) : 1;
@@ -1121,6 +1132,11 @@ Plan plan_of(const fhc_ssm_desc* g, bool backward) {
     return p;
 }
 size_t workspace_of(const Plan& p) { return p.ends_bytes + p.lasts_bytes + p.part_bytes + p.bc_bytes; }
+// one size for a shape, with and without lengths
+size_t workspace_of(const fhc_ssm_desc* g, bool backward) {
+    const size_t n = workspace_of(plan_of(g, backward, false)), m = workspace_of(plan_of(g, backward, true));
+    return n > m ? n : m;
+}
 
 int check_desc(const char* op, const fhc_ssm_desc* g) {
     if (!g) return fail(-1, "%s: null descriptor", op);
@@ -1229,7 +1245,7 @@ extern "C" size_t fhc_ssm_workspace_bytes(const fhc_ssm_desc* g, int backward) {
     return guard((size_t)0, [&]() -> size_t {
         clear_error();
         if (check_desc("ssm_workspace_bytes", g) < 0 || (uint64_t)g->b * g->d == 0) return 0;
-        return workspace_of(plan_of(g, backward != 0));
+        return workspace_of(g, backward != 0);
     });
 }
 
@@ -1241,13 +1257,13 @@ extern "C" int fhc_ssm_forward(const fhc_ssm_desc* g, const fhc_seq* x, const fh
         const char* op = "ssm_forward";
         FHC_TRY(check_desc(op, g));
         if ((uint64_t)g->b * g->d == 0) return 0;
-        const Plan p = plan_of(g, false);
+        const Plan p = plan_of(g, false, g->lengths != nullptr);
         FHC_TRY(check_inputs(op, g, p, x, dt, bm, cm, z));
         FHC_TRY(check_out(op, "y", y, g->dtype, g->b, g->t, g->d));
         FHC_TRY(check_array(op, "h0", h0, 4, false));
         FHC_TRY(check_array(op, "ht", ht, 4, false));
         if (!aligned(states, 256)) return fail(-1, "%s: states is not 256-byte aligned", op);
-        FHC_TRY(check_workspace(op, workspace_of(p), ws, ws_bytes));
+        FHC_TRY(check_workspace(op, workspace_of(g, false), ws, ws_bytes));
         const hipStream_t st = (hipStream_t)stream;
         int rc = 0;
         with_type(g->dtype, [&](auto t) {
@@ -1289,7 +1305,7 @@ extern "C" int fhc_ssm_backward(const fhc_ssm_desc* g, const fhc_seq* x, const f
             with_type(g->dtype, [&](auto t) { rc = close_vectors<decltype(t)>(op, g, nullptr, dbm, dcm, 0, st); });
             return rc;
         }
-        const Plan p = plan_of(g, true);
+        const Plan p = plan_of(g, true, g->lengths != nullptr);
         FHC_TRY(check_inputs(op, g, p, x, dt, bm, cm, z));
         FHC_TRY(check_in(op, "dy", dy, g->dtype, g->t));
         FHC_TRY(check_out(op, "dx", dx, g->dtype, g->b, g->t, g->d));
@@ -1298,7 +1314,7 @@ extern "C" int fhc_ssm_backward(const fhc_ssm_desc* g, const fhc_seq* x, const f
         else if (dz) return fail(-1, "%s: dz without z", op);
         if (g->t && !states) return fail(-1, "%s: null states", op);
         if (!aligned(states, 256)) return fail(-1, "%s: states is not 256-byte aligned", op);
-        FHC_TRY(check_workspace(op, workspace_of(p), ws, ws_bytes));
+        FHC_TRY(check_workspace(op, workspace_of(g, true), ws, ws_bytes));
         with_type(g->dtype, [&](auto t) {
             using T = decltype(t);
             using R = typename T::Raw;

@@ -214,3 +214,12 @@ def test_tensors_that_require_gradients_are_refused_while_autograd_records():
                 call(*(args[:k] + [t.clone().requires_grad_()] + args[k + 1:]))
     with pytest.raises(m.FhcError, match="requires gradients"):
         m.short_conv(x, w, state=st.requires_grad_())
+
+
+def test_ssm_workspace_is_the_same_with_and_without_lengths():
+    m = mod()
+    for n, t, d in ((16, 2051, 1532), (64, 512, 1024), (3, 100, 64)):
+        for back in (0, 1):
+            plain, ragged = (m._lib().fhc_ssm_workspace_bytes(m.SsmDesc(1, 6, t, d, n, 2, P, None, None, q), back)
+                             for q in (None, P))
+            assert plain == ragged
