@@ -339,17 +339,40 @@ __device__ __forceinline__ void write_row(float* p, const float (&o)[K]) {
     }
 }
 
-// the states of quad q of a [b][d][n] tensor
-__device__ __forceinline__ f4 load_states(const float* p, uint64_t at, uint32_t n, uint32_t q) {
-    f4 h;
+// states from s on of a [b][d][n] tensor, zeros past the last one: one wide load or store where all are there (a lane's are n
+// apart from its neighbour's, so each narrow one would touch a cache line a lane)
+template <int NS>
+__device__ __forceinline__ void load_states(const float* p, uint64_t at, uint32_t n, uint32_t s, float (&h)[NS]) {
 #pragma unroll
-    for (int k = 0; k < 4; k++) h[k] = p && 4 * q + k < n ? p[at * n + 4 * q + k] : 0.0f;
-    return h;
+    for (int k = 0; k < NS; k++) h[k] = 0.0f;
+    if (!p) return;
+    if (s + NS <= n) {
+        load_raw<float, NS, false>(p + at * n + s, h);
+    } else {
+#pragma unroll
+        for (int k = 0; k < NS; k++)
+            if (s + k < n) h[k] = p[at * n + s + k];
+    }
 }
-__device__ __forceinline__ void store_states(float* p, uint64_t at, uint32_t n, uint32_t q, f4 h) {
+template <int NS>
+__device__ __forceinline__ void store_states(float* p, uint64_t at, uint32_t n, uint32_t s, const float (&h)[NS]) {
+    if (s + NS <= n) {
+        store_raw<float, NS, false>(p + at * n + s, h);
+    } else {
 #pragma unroll
-    for (int k = 0; k < 4; k++)
-        if (4 * q + k < n) p[at * n + 4 * q + k] = h[k];
+        for (int k = 0; k < NS; k++)
+            if (s + k < n) p[at * n + s + k] = h[k];
+    }
+}
+// the same of quad q
+__device__ __forceinline__ f4 load_states(const float* p, uint64_t at, uint32_t n, uint32_t q) {
+    float h[4];
+    load_states<4>(p, at, n, 4 * q, h);
+    return f4{h[0], h[1], h[2], h[3]};
+}
+__device__ __forceinline__ void store_states(float* p, uint64_t at, uint32_t n, uint32_t q, f4 v) {
+    const float h[4] = {v[0], v[1], v[2], v[3]};
+    store_states<4>(p, at, n, 4 * q, h);
 }
 __device__ __forceinline__ f4 rates_of(const float* a, uint32_t ch, uint32_t n, uint32_t q) {
     f4 h = load_states(a, ch, n, q);
@@ -498,12 +521,10 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_fwd(SsmArgs<typename T::Raw> g)
     States<NS> rate[NQ], h[NQ];
 #pragma unroll
     for (int i = 0; i < NQ; i++) {
+        load_states<NS>(g.a, ch, g.n, number(i, 0), rate[i].v);
+        load_states<NS>(g.segs == 1 ? g.h0 : nullptr, flat, g.n, number(i, 0), h[i].v);
 #pragma unroll
-        for (int k = 0; k < NS; k++) {
-            const uint32_t s = number(i, k);
-            rate[i].v[k] = s < g.n ? rate_of(g.a[(uint64_t)ch * g.n + s]) : 0.0f;
-            h[i].v[k] = s < g.n && g.segs == 1 && g.h0 ? g.h0[flat * g.n + s] : 0.0f;
-        }
+        for (int k = 0; k < NS; k++) rate[i].v[k] = rate_of(rate[i].v[k]);
         if (g.segs > 1 && number(i, 0) < g.n) {
             const float* p = reinterpret_cast<const float*>(g.ends + (uint64_t)b * g.quads * g.d) + in_quads(i, 0);
             load_raw<float, NS, false>(p, h[i].v);
@@ -644,10 +665,7 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_fwd(SsmArgs<typename T::Raw> g)
     }
     if (g.ht && at.live && last == g.tiles) {
 #pragma unroll
-        for (int i = 0; i < NQ; i++)
-#pragma unroll
-            for (int k = 0; k < NS; k++)
-                if (number(i, k) < g.n) g.ht[flat * g.n + number(i, k)] = h[i].v[k];
+        for (int i = 0; i < NQ; i++) store_states<NS>(g.ht, flat, g.n, number(i, 0), h[i].v);
     }
 }
 
