@@ -8,8 +8,8 @@ namespace fhc {
 namespace seq {
 namespace {
 
-// out = the sum of the splits' partial sums (LIN: with the product's tail); LANES threads take every LANES-th split of a quad of columns each, and their
-// sums are added in order
+// out = the sum of the splits' partial sums (LIN: with the product's tail); LANES threads take every LANES-th split of a quad
+// of columns each, and their sums are added in order
 template <class T, int LANES, bool LIN>
 __global__ __launch_bounds__(256) void ffn_join(const float* part, int splits, int m, int n, int64_t ldpart,
                                                 uint16_t* o0, uint16_t* o1, int64_t ldo, Tail tail) {
@@ -355,7 +355,7 @@ int skinny(const char* op, const SkinnyArgs& a, hipStream_t st) {
     do {                                                          \
         if constexpr (GLU) SKINNY_OF(NB, 4);                      \
         else if constexpr (!LIN) SKINNY_OF(NB, 16);               \
-        else if (grid.x >= 512) SKINNY_OF(NB, 4);                   \
+        else if (grid.x >= 512) SKINNY_OF(NB, 4);                 \
         else SKINNY_OF(NB, 16);                                   \
     } while (0)
     if (a.rows <= 16) SKINNY(1);

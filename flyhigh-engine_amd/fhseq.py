@@ -4,11 +4,11 @@ feed-forward block (``ffn``), a short causal convolution (``short_conv``), a sel
 matrix product with bias, activation and residual (``linear``), each with its backward pass.
 
 Inputs are torch tensors on the current GPU in f16, bf16 or (not ``ffn`` and ``linear``) f32, all of one call in the same
-type; the recurrences' states and the gradients of the weights of the recurrences, the norms and the convolution are f32. Each function returns new tensors, which autograd does
-not know: a call with tensors that require gradients is refused while autograd records (``torch.no_grad()``, and the
-``*_backward`` functions, are the way). ``stream`` (a torch
-stream) is where the call runs, the current stream if None; what it allocates belongs to that stream. The module only
-passes device pointers: when the library is missing, loading it raises, and nothing is computed on the host.
+type; the recurrences' states and the gradients of the weights of the recurrences, the norms and the convolution are f32.
+Each function returns new tensors, which autograd does not know: a call with tensors that require gradients is refused while
+autograd records (``torch.no_grad()``, and the ``*_backward`` functions, are the way). ``stream`` (a torch stream) is where
+the call runs, the current stream if None; what it allocates belongs to that stream. The module only passes device pointers:
+when the library is missing, loading it raises, and nothing is computed on the host.
 """
 from __future__ import annotations
 
