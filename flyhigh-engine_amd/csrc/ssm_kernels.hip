@@ -680,7 +680,7 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_fwd(SsmArgs<typename T::Raw> g)
 // Few steps: a thread has one quad of one channel's states, LP threads side by side a channel, so a wave reads and writes
 // the states as they lie, 16 bytes a lane; the steps follow one another. WHOLE: n is a multiple of 4.
 // What bounds it (MI355X): HBM, which the states are read from and written to. One step of 64 x 4096 channels of 16
-// states, bf16: 9.9 us for 36 MB; each step more is 3.7 us, of the vector unit.
+// states, bf16: 9.9 us for 36 MB; each step more is 3.6 us, of its narrow loads.
 template <class T, int LP, bool WHOLE>
 __global__ __launch_bounds__(256) void ssm_step(SsmArgs<typename T::Raw> g) {
     using R = typename T::Raw;
@@ -1088,9 +1088,10 @@ int close_vectors(const char* op, const fhc_ssm_desc* g, const float* bc, const 
     return launched(op);
 }
 
-// Up to here steps, then tiles: 64 x 4096 channels of 16 states, bf16, us from cold caches: 1 step 17, 4 28, 8 44; 9 by
-// tiles 46, 16 48 (64 x 1024 of 64 states: 16, 28, 41; 45, 46).
-constexpr uint32_t kFewSteps = 8;
+// Up to here steps, then tiles. bf16, us from cold caches, by steps 1, 2, 3, 4, 6, 8: 64 x 4096 channels of 16 states 17, 21,
+// 24, 28, 35, 44, by tiles 5, 8: 32, 32; 64 x 1024 of 64 states 17, 20, 24, 27, 34, 41 and 29, 29; 64 x 2048 of 8 states 8, 9,
+// 11, 12 and 17, 17. A step's five loads, which the lanes of a channel repeat, are most of it.
+constexpr uint32_t kFewSteps = 4;
 
 struct Plan {
     uint32_t width, blocks, quads, waves, tiles, segs, seg_tiles, walks;
