@@ -300,6 +300,40 @@ def test_ssm(shape, dtype):
     ssm_check(ssm_inputs(q, *shape, types()[dtype], time_major=shape[2] % 4 == 2, ragged=shape[1] % 2 == 1))
 
 
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("shape", [(3, 4, 70, 16, 1), (3, 6, 70, 6, 1), (2, 8, 40, 64, 1), (9, 512, 256, 16, 1),
+                                   (2, 1030, 128, 64, 1), (5, 333, 192, 8, 3), (600, 40, 64, 16, 1)], ids=str)
+def test_ssm_sides_of_the_rules(shape, ragged):
+    """The last step kernels and the first tiles; segments by rounds of workgroups and, with lengths, by their number."""
+    say("ssm rules", shape, ragged)
+    ssm_check(ssm_inputs(Rand(sum(shape) + 1), *shape, types()["bf16"], ragged=ragged))
+
+
+def test_ssm_lengths_at_the_ends_of_tiles_and_segments():
+    say("ssm lengths at ends")
+    import torch
+    v = ssm_inputs(Rand(29), 8, 640, 72, 16, 1, torch.float16)
+    v["lengths"] = torch.tensor([640, 0, 16, 15, 17, 64, 320, 639], dtype=torch.int32, device="cuda")
+    ssm_check(v)
+
+
+def test_ssm_two_streams_at_once():
+    """Calls of their own workspaces that overlap give the bits of calls one after the other."""
+    say("ssm two streams")
+    import torch
+    vs = [ssm_inputs(Rand(31 + i), 2, 900, 128, 16, 1, torch.bfloat16) for i in range(2)]
+    want = [ssm_run(v, False) for v in vs]
+    streams = [torch.cuda.Stream() for _ in vs]
+    for _ in range(3):
+        got = []
+        for v, s in zip(vs, streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(ssm_run(v, False))
+        torch.cuda.synchronize()
+        assert all(_same(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
 def test_ssm_parts_left_out():
     say("ssm parts left out")
     import torch
