@@ -1,6 +1,6 @@
 // The selective state space scan (include/fhc_seq.h), forward and backward.
 //
-// A workgroup has 64 channels of one sequence and group, a lane one channel; its W waves share out the states, 4 or 8 of
+// A workgroup has 64 channels of one sequence and group, a lane one channel; its W waves share out the states, 2, 4 or 8 of
 // them a wave, in registers. Time goes in tiles of 16 steps: the waves first prepare 16 / W steps each (D = softplus,
 // D x), which then lie in LDS for all of them; every wave runs its states through the 16 steps and leaves its part of
 // sum C h a step in LDS; the waves add the parts of their steps, apply skip and gate, and store. B and C are the same for
