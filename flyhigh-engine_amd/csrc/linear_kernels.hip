@@ -2,13 +2,16 @@
 // products of ffn_gemm.h and, for few rows, of ffn_product.h.
 //
 // Forward: one product, whose epilogue adds the bias in f32, keeps the sum where the backward pass needs it, applies the
-// activation and adds the residual. Backward: dv = dy act'(v), rounded once to the operands' type, with its sums over rows
-// for the bias, in one pass (without an activation dv is dy itself, and only the bias needs a pass); dx = dv w, dw = dv^T x.
+// activation and adds the residual. Backward: dv = dy act'(v), with its sums over rows for the bias, in one pass (without an
+// activation dv is dy itself, and only the bias needs a pass); dx = dv w, dw = dv^T x. The matrix units take operands of 16
+// bits, so dv goes in as two numbers of the operands' type, its rounding and that rounding's remainder, one behind the other
+// along K: what is lost is half a step of the remainder, 2^-16 (bf16) or 2^-22 (f16) of dv. FHC_LINEAR_ROUND_DV leaves the
+// remainder out: half the work, and dx and dw carry dv's rounding beside their own (of random terms 1.4 times the error).
 //
 // What bounds it (MI355X): matrix units for large calls, HBM for few rows. 8192 x 2048 -> 8192 bf16 with silu, bias and
-// residual: 320 us forward, 390 where v is kept (its f32 passes through the epilogue), a training step 930: dv 125 (4.3
-// TB/s), dx and dw 210 to 230 each (1200 to 1310 TFLOP/s; a large library product reaches 1344). 4 x 2048 -> 8192: 11 us for
-// 34 MB.
+// residual: 320 us forward, 390 where v is kept (its f32 passes through the epilogue), a training step 1310, with a rounded dv
+// 910: dv 125 (4.3 TB/s), dx and dw 210 to 230 each (1200 to 1310 TFLOP/s; a large library product reaches 1344). 4 x 2048 ->
+// 8192: 11 us for 34 MB.
 #include "ffn_product.h"
 #include "seq_args.h"
 
@@ -16,14 +19,14 @@ namespace fhc {
 namespace seq {
 namespace {
 
-// dv = dy act'(v) in rows of up8(n), whose ends are zeros (dv null: dy is dv), and its sums over this workgroup's rows:
-// 64 threads side by side take 8 columns each, 4 rows at once.
+// dv = dy act'(v) and its rounding's remainder in rows of up8(n), whose ends are zeros (dv null: dy is dv), and its sums over
+// this workgroup's rows: 64 threads side by side take 8 columns each, 4 rows at once.
 struct SlopeArgs {
     const uint16_t* dy;
     int64_t ldy;
     const float* pre;
     int64_t ldpre;
-    uint16_t* dv;
+    uint16_t *dv, *rest;  // rest: dv's remainder, or null
     float* part;  // [workgroup rows][n], or null
     int rows, n, walks;
     uint32_t act;
@@ -38,7 +41,7 @@ __global__ __launch_bounds__(256) void linear_slope(SlopeArgs g) {
     if (valid > 0) {
         for (int64_t m = (int64_t)blockIdx.y * 4 + row; m < g.rows; m += (int64_t)g.walks * 4) {
             const u4_t q = load_some(g.dy + m * g.ldy + c, valid);
-            uint16_t out[8];
+            uint16_t out[8], rest[8];
             f4 pre[2] = {};
             if (g.pre) {
                 pre[0] = *reinterpret_cast<const f4*>(g.pre + m * g.ldpre + c);
@@ -51,8 +54,11 @@ __global__ __launch_bounds__(256) void linear_slope(SlopeArgs g) {
                 d = v < valid ? d * slope : 0.0f;
                 db[v] += d;
                 out[v] = narrow(T{}, d);
+                const float held = widen(T{}, out[v]);  // past the type's range it is inf, and has no remainder
+                rest[v] = narrow(T{}, __builtin_fabsf(held) < __builtin_inff() ? d - held : 0.0f);
             }
             if (g.dv) store_raw<uint16_t, 8, true>(g.dv + m * g.ldpre + c, out);
+            if (g.rest) store_raw<uint16_t, 8, true>(g.rest + m * g.ldpre + c, rest);
         }
     }
     if (!g.part) return;
@@ -72,17 +78,20 @@ __global__ __launch_bounds__(256) void linear_slope(SlopeArgs g) {
 
 // ---- host side ----------------------------------------------------------------------------------------------------
 
+uint32_t act(const fhc_linear_desc* d) { return d->act & ~FHC_LINEAR_ROUND_DV; }
 int check_desc(const char* op, const fhc_linear_desc* d) {
     if (!d) return fail(-1, "%s: null descriptor", op);
     if (d->dtype > FHC_BF16) return fail(-1, "%s: dtype %u is neither f16 nor bf16", op, d->dtype);
-    if (d->act > FHC_ACT_IDENTITY) return fail(-1, "%s: act %u", op, d->act);
+    if (act(d) > FHC_ACT_IDENTITY) return fail(-1, "%s: act %u", op, d->act);
     if (d->c > 1u << 20 || d->f > 1u << 20) return fail(-1, "%s: %u x %u channels, at most 2^20", op, d->c, d->f);
     if (d->rows > 0x7FFFFF00u) return fail(-1, "%s: %u rows", op, d->rows);
     return 0;
 }
 
-bool keeps(const fhc_linear_desc* d) { return d->act != FHC_ACT_IDENTITY; }
+bool keeps(const fhc_linear_desc* d) { return act(d) != FHC_ACT_IDENTITY; }
 size_t pre_bytes(const fhc_linear_desc* d) { return keeps(d) ? up256((size_t)d->rows * up8(d->f) * 4) : 0; }
+// products of the backward pass that dv takes along K
+int parts_of(const fhc_linear_desc* d) { return keeps(d) && !(d->act & FHC_LINEAR_ROUND_DV) ? 2 : 1; }
 // workgroups that a column block's rows are dealt to: two a CU over all columns
 uint32_t walks_of(const fhc_linear_desc* d) {
     const uint64_t cols = ceil_div(d->f, 512), most = ceil_div(d->rows, 4), want = cols ? ceil_div(1024, cols) : 0;
@@ -94,8 +103,9 @@ size_t sums_bytes(const fhc_linear_desc* d) { return up256((size_t)walks_of(d) *
 size_t workspace(const fhc_linear_desc* d, bool backward) {
     const size_t rows = Operands::pack_bytes(d->rows, d->c), w = Operands::pack_bytes(d->f, d->c);
     if (!backward) return d->rows > kSkinnyRows ? part_of(d->rows, d->f, d->c, 1, 1) + rows + w : 0;
-    const size_t dx = part_of(d->rows, d->c, d->f, 1, 1), dw = part_of(d->f, d->c, d->rows, 1, 1);
-    return Operands::pack_bytes(d->rows, d->f) + sums_bytes(d) + (dx > dw ? dx : dw) + rows + w;
+    const int parts = parts_of(d);
+    const size_t dx = part_of(d->rows, d->c, d->f, parts, 1), dw = part_of(d->f, d->c, d->rows, parts, 1);
+    return parts * Operands::pack_bytes(d->rows, d->f) + sums_bytes(d) + (dx > dw ? dx : dw) + rows + w;
 }
 
 const uint16_t* u16(const void* p) { return static_cast<const uint16_t*>(p); }
@@ -104,11 +114,11 @@ template <class T>
 int forward(const char* op, const fhc_linear_desc* d, const fhc_rows* x, const void* w, const void* bias,
             const fhc_rows* res, const fhc_rows* y, void* saved, void* ws, hipStream_t st) {
     float* pre = keeps(d) ? static_cast<float*>(saved) : nullptr;
-    const Tail tail{u16(bias), res ? u16(res->p) : nullptr, res ? res->ld : 0, pre, up8(d->f), d->act};
+    const Tail tail{u16(bias), res ? u16(res->p) : nullptr, res ? res->ld : 0, pre, up8(d->f), act(d)};
     uint16_t* out = static_cast<uint16_t*>(y->p);
     if (d->rows <= kSkinnyRows) {
         const SkinnyArgs a{u16(x->p), u16(w), nullptr, x->ld, (int64_t)d->c, (int)d->rows, (int)d->f, (int)d->c, out, y->ld,
-                           (int)d->f, nullptr, nullptr, d->act, tail};
+                           (int)d->f, nullptr, nullptr, tail.act, tail};
         return skinny<T, false, true>(op, a, st);
     }
     char* at = static_cast<char*>(ws);
@@ -119,7 +129,7 @@ int forward(const char* op, const fhc_linear_desc* d, const fhc_rows* x, const v
     g.b0 = o.take(w, g.ldb, d->f, d->c, true);
     FHC_TRY(o.copy(op, st));
     g.m = d->rows, g.n = d->f, g.k = d->c, g.o0 = out, g.ldo = y->ld;
-    g.pre_g = pre, g.ldpre = tail.ldpre, g.act = d->act, g.bias = tail.bias, g.res = tail.res, g.ldr = tail.ldr;
+    g.pre_g = pre, g.ldpre = tail.ldpre, g.act = tail.act, g.bias = tail.bias, g.res = tail.res, g.ldr = tail.ldr;
     return product<T, false, false, kLinear>(op, g, reinterpret_cast<float*>(at), st);
 }
 
@@ -129,16 +139,19 @@ int backward(const char* op, const fhc_linear_desc* d, const fhc_rows* x, const 
     char* at = static_cast<char*>(ws);
     uint16_t* dv = reinterpret_cast<uint16_t*>(at);  // dL/dv, or a copy of dy that can be fetched
     at += Operands::pack_bytes(d->rows, d->f);
+    const int parts = parts_of(d);
+    uint16_t* rest = parts > 1 ? reinterpret_cast<uint16_t*>(at) : nullptr;
+    at += (parts - 1) * Operands::pack_bytes(d->rows, d->f);
     float* sums = reinterpret_cast<float*>(at);
     at += sums_bytes(d);
-    const size_t part_dx = part_of(d->rows, d->c, d->f, 1, 1), part_dw = part_of(d->f, d->c, d->rows, 1, 1);
+    const size_t part_dx = part_of(d->rows, d->c, d->f, parts, 1), part_dw = part_of(d->f, d->c, d->rows, parts, 1);
     float* part = reinterpret_cast<float*>(at);
     at += part_dx > part_dw ? part_dx : part_dw;
     const uint32_t walks = walks_of(d);
     const bool slope = keeps(d) && (dx || dw || dbias);
     if (d->rows && d->f && (slope || dbias)) {
         SlopeArgs s{u16(dy->p), dy->ld, slope ? static_cast<const float*>(saved) : nullptr, up8(d->f),
-                    slope ? dv : nullptr, dbias ? sums : nullptr, (int)d->rows, (int)d->f, (int)walks, d->act};
+                    slope ? dv : nullptr, slope ? rest : nullptr, dbias ? sums : nullptr, (int)d->rows, (int)d->f, (int)walks, act(d)};
         hipLaunchKernelGGL((linear_slope<T>), dim3((uint32_t)ceil_div(d->f, 512), walks), dim3(256), 0, st, s);
         FHC_TRY(launched(op));
     }
@@ -157,13 +170,13 @@ int backward(const char* op, const fhc_linear_desc* d, const fhc_rows* x, const 
     FHC_TRY(o.copy(op, st));
     if (dx) {
         GemmArgs g{};
-        g.a0 = v, g.b0 = vw, g.lda = ldv, g.ldb = ldw, g.m = d->rows, g.n = d->c, g.k = d->f;
+        g.a0 = v, g.a1 = rest, g.b0 = g.b1 = vw, g.segments = parts, g.lda = ldv, g.ldb = ldw, g.m = d->rows, g.n = d->c, g.k = d->f;
         g.o0 = static_cast<uint16_t*>(dx->p), g.ldo = dx->ld;
         FHC_TRY((product<T, false, true, kStore>(op, g, part, st)));
     }
     if (dw) {
         GemmArgs g{};
-        g.a0 = v, g.b0 = vx, g.lda = ldv, g.ldb = ldx, g.m = d->f, g.n = d->c, g.k = d->rows;
+        g.a0 = v, g.a1 = rest, g.b0 = g.b1 = vx, g.segments = parts, g.lda = ldv, g.ldb = ldx, g.m = d->f, g.n = d->c, g.k = d->rows;
         g.o0 = static_cast<uint16_t*>(dw), g.ldo = d->c;
         FHC_TRY((product<T, true, true, kStore>(op, g, part, st)));
     }

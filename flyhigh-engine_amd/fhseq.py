@@ -578,10 +578,10 @@ def ssm_backward(x, dt, a, bm, cm, states, dy, skip=None, z=None, dt_bias=None, 
     return dx, ddt, da, dbm, dcm, dskip, dz, ddt_bias, dh0
 
 
-LINEAR_ACTS = {"silu": 0, "gelu": 1, "none": 2}
+LINEAR_ACTS, ROUND_DV = {"silu": 0, "gelu": 1, "none": 2}, 0x100
 
 
-def _linear_desc(k, name, x, w, act):
+def _linear_desc(k, name, x, w, act, flag=0):
     if x.dim() != 2 or w.dim() != 2:
         raise FhcError(f"{name}: x is [rows, channels] and w [features, channels], got {tuple(x.shape)}, "
                        f"{tuple(w.shape)}")
@@ -589,7 +589,7 @@ def _linear_desc(k, name, x, w, act):
         raise FhcError(f"{name}: act {act!r} is none of {', '.join(LINEAR_ACTS)}")
     dtype, at = _first(k, name, x)
     rows, c = x.shape
-    f, act = w.shape[0], LINEAR_ACTS[act]
+    f, act = w.shape[0], LINEAR_ACTS[act] + flag
     return (_pack(name, _LINEAR, dtype, act, rows, c, f), at, _linear_sizes(dtype, act, rows, c, f),
             _rows(name, "x", x), _dense(name, "w", w, (f, c), x.dtype, at))
 
@@ -615,15 +615,17 @@ def linear(x, w, bias=None, residual=None, act="none", train=False, stream=None)
     return (y, saved) if train else y
 
 
-def linear_backward(x, w, saved, dy, act="none", bias=True, stream=None):
+def linear_backward(x, w, saved, dy, act="none", bias=True, stream=None, round_dv=False):
     """(dx, dw, dbias) for dy, dx and dw in the inputs' type and dbias in f32 (None where bias is false); ``saved`` from the
-    training ``linear`` call of the same inputs (None where it kept nothing). The residual's gradient is dy."""
+    training ``linear`` call of the same inputs (None where it kept nothing). The residual's gradient is dy. ``round_dv``:
+    with an activation, the gradient behind it is rounded to the inputs' type before the products for dx and dw, which
+    halves their work."""
     if stream is not None:
         with _on(stream):
-            return linear_backward(x, w, saved, dy, act, bias)
+            return linear_backward(x, w, saved, dy, act, bias, None, round_dv)
     k, op = _fast(), "linear_backward"
     _unrecorded(k, op, x, w, dy)
-    d, at, sizes, rx, pw = _linear_desc(k, op, x, w, act)
+    d, at, sizes, rx, pw = _linear_desc(k, op, x, w, act, ROUND_DV if round_dv else 0)
     rows, f = x.shape[0], w.shape[0]
     kept = _dense(op, "saved", saved, (sizes[0],), k.u8, at) if sizes[0] else None
     _match(op, "dy", dy, (rows, f), x.dtype, at)

@@ -198,12 +198,14 @@ int fhc_ssm_backward(const fhc_ssm_desc* g, const fhc_seq* x, const fhc_seq* dt,
 /* ---- The matrix product with its epilogue, on rows of c channels, f wide:
  *     y = act(v) + residual,   v = x w^T + bias
  * w is dense [f][c], bias [f], in dtype (f16 or bf16); act FHC_ACT_SILU, FHC_ACT_GELU or FHC_ACT_IDENTITY. v and the sum
- * are f32, y is rounded once. A training forward with silu or gelu keeps v in f32; the backward pass rounds dL/dv to
- * dtype once, since it is the next products' operand (dbias sums it before that rounding). The residual's gradient is
- * dy itself. */
+ * are f32, y is rounded once. A training forward with silu or gelu keeps v in f32. dx and dw are products of dL/dv as two
+ * numbers of dtype, its rounding and the remainder; FHC_LINEAR_ROUND_DV, added to act, leaves the remainder out, for half
+ * the work at silu and gelu (dbias sums dL/dv before its rounding in both). The residual's gradient is dy itself. */
+#define FHC_LINEAR_ROUND_DV 0x100u
+
 typedef struct fhc_linear_desc {
     uint32_t dtype; /* FHC_F16 or FHC_BF16 */
-    uint32_t act;
+    uint32_t act;   /* and FHC_LINEAR_ROUND_DV, which the forward pass does not look at */
     uint32_t rows, c, f; /* c, f <= 2^20 */
 } fhc_linear_desc;
 

@@ -1,0 +1,84 @@
+"""Calls of the short convolution, the selective scan and the product with its epilogue that the shapes of test_ssm_gpu.py
+do not reach: weights' gradients over very many rows, states that grow, calls of very many sequences, and the kernels that
+only larger calls take. On the GPU, against plain 64-bit forms or closed ones."""
+import math
+
+import pytest
+
+import fhtest  # noqa: F401  (puts the package on sys.path)
+import seqref
+import ssmref
+from seqref import U
+from test_seq_gpu import Rand, mod, say, types
+from test_ssm_gpu import (LINEAR_NAMES, SSM_NAMES, _same, compare, conv_check, conv_inputs, linear_check, linear_inputs, linear_run,
+                          ssm_check, ssm_inputs)
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- dL/dv in the product's backward pass -------------------------------------------------------------------------
+
+def linear_split_ref(v, act):
+    """ssmref.linear's results and bounds with dL/dv held as the sum of two numbers of the inputs' type: what is left is
+    half a step of the second one (itself at most half a step of the first), or half the smallest number."""
+    x, w, dy = (v[k].double() for k in ("x", "w", "dy"))
+    import torch
+    hs, fi = seqref.half_step(v["x"].dtype), torch.finfo(v["x"].dtype)
+    ref, err = ssmref.linear(v["x"], v["w"], v["bias"], v["residual"], act, v["dy"])
+    pre = x @ w.t() + (0 if v["bias"] is None else v["bias"].double())
+    chain = lambda k: (2 * k / 32 + 34) * U  # noqa: E731  (two products along the same sum)
+    ev = (w.shape[1] / 32 + 34) * U * (x.abs() @ w.abs().t()) + 2 * U * pre.abs()
+    slope = seqref._act(pre, act)[1]
+    dv, edv = dy * slope, dy.abs() * (1.2 * ev + 64 * U * (slope.abs() + 1)) + 2 * U * (dy * slope).abs()
+    e = edv + hs * hs * (dv.abs() + edv) + fi.tiny * fi.eps / 2
+    size = dv.abs() * (1 + 2 * hs)
+    err[1] = e @ w.abs() + chain(w.shape[0]) * (size @ w.abs())
+    err[2] = e.t() @ x.abs() + chain(x.shape[0]) * (size.t() @ x.abs())
+    if v["bias"] is None:
+        ref[3] = None
+    return ref, err
+
+
+SPLIT = [(1, 7, 9), (20, 64, 520), (300, 72, 48), (333, 65, 47), (130, 1000, 1032), (1003, 130, 273), (2100, 2050, 40)]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("shape", SPLIT, ids=str)
+def test_linear_gradients_keep_the_bits_of_dv(shape, dtype, act):
+    """dx and dw are the products of dL/dv, not of its rounding to 16 bits."""
+    say("linear dv", shape, dtype, act)
+    v = linear_inputs(Rand(sum(shape) + 3), *shape, types()[dtype], bias=shape[0] % 2 == 0)
+    ref, err = linear_split_ref(v, act)
+    compare(LINEAR_NAMES, linear_run(v, act), ref, err)
+
+
+@pytest.mark.parametrize("dtype,act", [("f16", "gelu"), ("bf16", "silu"), ("bf16", "none")])
+@pytest.mark.parametrize("shape", SPLIT, ids=str)
+def test_linear_gradients_of_a_rounded_dv(shape, dtype, act):
+    """round_dv: within the rounding of dL/dv of the formula; without an activation there is nothing to round."""
+    say("linear rounded dv", shape, dtype, act)
+    m = mod()
+    v = linear_inputs(Rand(sum(shape) + 4), *shape, types()[dtype])
+    kept = m.linear(v["x"], v["w"], v["bias"], v["residual"], act, train=True)[1]
+    got = m.linear_backward(v["x"], v["w"], kept, v["dy"], act, round_dv=True)
+    ref, err = ssmref.linear(v["x"], v["w"], v["bias"], v["residual"], act, v["dy"])
+    compare(LINEAR_NAMES[1:], got, ref[1:], err[1:])
+    full = m.linear_backward(v["x"], v["w"], kept, v["dy"], act)
+    assert _same(got[2], full[2]) and (act != "none" or all(_same(a, b) for a, b in zip(got, full)))
+
+
+def test_linear_gradients_past_the_types_range():
+    """A dL/dv that f16 does not hold is an infinity in its row's dx and its column's dw, and no NaN."""
+    say("linear dv past the range")
+    import torch
+    m = mod()
+    v = linear_inputs(Rand(67), 40, 24, 16, torch.float16, bias=False)
+    v["x"].fill_(1.0), v["w"].fill_(0.1)  # v = 2.4, where silu's slope is 1.0998
+    v["dy"][3, 5] = 65504.0
+    for round_dv in (False, True):
+        kept = m.linear(v["x"], v["w"], None, None, "silu", train=True)[1]
+        dx, dw, _ = m.linear_backward(v["x"], v["w"], kept, v["dy"], "silu", round_dv=round_dv)
+        assert (dx[3] == math.inf).all() and (dw[5] == math.inf).all()
+        keep_x, keep_w = torch.arange(40) != 3, torch.arange(16) != 5
+        assert torch.isfinite(dx[keep_x]).all() and torch.isfinite(dw[keep_w]).all()
