@@ -25,6 +25,7 @@ namespace seq {
 namespace {
 
 constexpr int kTile = 16;
+constexpr uint32_t kStretch = 16;  // tiles whose terms of a weight's gradient are added in f32; the closing sum is f64
 typedef float f4 __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
@@ -40,12 +41,13 @@ struct SsmArgs {
     float* dh0;
     f4* ends;     // segments: [segment + 1][b][quad][d], forward's slot 0 is h0
     float* lasts;   // and their sums of D, [segment][b][d]
-    float* part;    // [segment][walk][d * n + 2 d]: da, dskip, ddt_bias
+    float* part;    // [segment][walk][stretch][d * n + 2 d]: da, dskip, ddt_bias
     float* bc;      // [group and block][b][t][2][quad * 4]
     uint32_t b, t, d, n, groups;
     uint32_t width, blocks, quads;    // channels of a group, its blocks of 64, quads of states
     uint32_t tiles, segs, seg_tiles;  // tiles of 16 steps; segments and theirs
     uint32_t walks;                   // backward: workgroups that the sequences are dealt to
+    uint32_t stretches;               // and the stretches of kStretch tiles that a workgroup has at most
 };
 
 // softplus(v) = max(v, 0) + log1p(e), e = exp(-|v|): a polynomial of degree 9 in e for log1p(e) / e on [0, 1], the least
@@ -794,6 +796,29 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_bwd(SsmArgs<typename T::Raw> g)
         rate[i] = rates_of(g.a, ch, g.n, wave + W * i);
         da[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    // The sums of the weights' gradients so far become a row of partial sums, and start again.
+    const uint64_t part_row = (uint64_t)g.d * (g.n + 2);
+    float* to = g.part + ((uint64_t)at.seg * g.walks + at.walk) * g.stretches * part_row;
+    uint32_t stretch = 0, added = 0;  // rows written; tiles in the sums
+    auto close_stretch = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+            if (at.live) store_states(to, ch, g.n, wave + W * i, da[i]);
+            da[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        lds_barrier();
+        write_row<K>(parts[0][0][part.step] + part.c0, dskip), write_row<K>(parts[FOLD ? 0 : 1][0][part.step] + part.c0, dbias);
+#pragma unroll
+        for (int j = 0; j < K; j++) dskip[j] = dbias[j] = 0.0f;
+        lds_barrier();
+        if (wave == 0 && at.live) {  // read before the next tile's parts are written, a barrier further on
+            float s = 0.0f, u = 0.0f;
+#pragma unroll
+            for (int r = 0; r < kTile; r++) s += parts[0][0][r][lane], u += parts[FOLD ? 0 : 1][0][r][lane];
+            to[(uint64_t)g.d * g.n + ch] = s, to[(uint64_t)g.d * (g.n + 1) + ch] = u;
+        }
+        to += part_row, stretch++, added = 0;
+    };
     for (uint32_t b = at.walk; b < g.b; b += g.walks) {
         const uint64_t flat = (uint64_t)b * g.d + ch;
         const uint32_t n = g.lengths ? (uint32_t)min(max(g.lengths[b], 0), (int32_t)g.t) : g.t;
@@ -993,12 +1018,13 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_bwd(SsmArgs<typename T::Raw> g)
                 pdx -= kTile * g.dx.ts, pdt -= kTile * g.ddt.ts;
                 // the tile's dB and dC of this block, as they lie
                 const uint32_t row = 8 * g.quads, steps_here = min((uint32_t)kTile, there);
-                float* to = g.bc + (((uint64_t)(at.group * g.blocks + at.block) * g.b + b) * g.t + tile * kTile) * row;
+                float* vec = g.bc + (((uint64_t)(at.group * g.blocks + at.block) * g.b + b) * g.t + tile * kTile) * row;
                 for (uint32_t k = threadIdx.x; k < steps_here * row; k += 64 * W) {
                     const uint32_t s = k / row, v = k - s * row, half = v >= 4 * g.quads;
-                    to[k] = vectors[s][half][v - half * 4 * g.quads];
+                    vec[k] = vectors[s][half][v - half * 4 * g.quads];
                 }
                 lds_barrier();
+                if (__builtin_expect(++added == kStretch, 0)) close_stretch();
             }
         }
         if constexpr (FOLD) {
@@ -1027,20 +1053,7 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_bwd(SsmArgs<typename T::Raw> g)
         }
     }
     if constexpr (!FOLD) {
-        float* to = g.part + ((uint64_t)at.seg * g.walks + at.walk) * g.d * (g.n + 2);
-        if (at.live) {
-#pragma unroll
-            for (int i = 0; i < NQ; i++) store_states(to, ch, g.n, wave + W * i, da[i]);
-        }
-        lds_barrier();
-        write_row<K>(parts[0][0][part.step] + part.c0, dskip), write_row<K>(parts[1][0][part.step] + part.c0, dbias);
-        lds_barrier();
-        if (wave == 0 && at.live) {
-            float s = 0.0f, u = 0.0f;
-#pragma unroll
-            for (int r = 0; r < kTile; r++) s += parts[0][0][r][lane], u += parts[1][0][r][lane];
-            to[(uint64_t)g.d * g.n + ch] = s, to[(uint64_t)g.d * (g.n + 1) + ch] = u;
-        }
+        while (stretch < g.stretches) close_stretch();  // behind the last one zeros, where lengths left tiles out
     }
 }
 
@@ -1094,7 +1107,7 @@ int close_vectors(const char* op, const fhc_ssm_desc* g, const float* bc, const 
 constexpr uint32_t kFewSteps = 4;
 
 struct Plan {
-    uint32_t width, blocks, quads, waves, tiles, segs, seg_tiles, walks;
+    uint32_t width, blocks, quads, waves, tiles, segs, seg_tiles, walks, stretches;
     bool halves;  // forward: two states a lane
     uint64_t wgs;
     size_t ends_bytes, lasts_bytes, part_bytes, bc_bytes;
@@ -1156,7 +1169,9 @@ Plan plan_of(const fhc_ssm_desc* g, bool backward, bool ragged) {
         p.lasts_bytes = up256((size_t)p.segs * flat * 4);
     }
     if (backward) {
-        p.part_bytes = up256((size_t)p.segs * p.walks * g->d * (g->n + 2) * 4);
+        const uint64_t stretches = ceil_div(ceil_div(g->b, p.walks ? p.walks : 1) * p.seg_tiles, kStretch);
+        p.stretches = (uint32_t)(stretches ? stretches : 1);
+        p.part_bytes = up256((size_t)p.segs * p.walks * p.stretches * g->d * (g->n + 2) * 4);
         p.bc_bytes = up256((size_t)cols * g->b * g->t * 8 * p.quads * 4);
     }
     return p;
@@ -1188,7 +1203,7 @@ SsmArgs<typename T::Raw> args_of(const fhc_ssm_desc* g, const Plan& p, const fhc
     a.a = g->a, a.bias = g->dt_bias, a.skip = g->skip, a.lengths = g->lengths;
     a.b = g->b, a.t = g->t, a.d = g->d, a.n = g->n, a.groups = g->groups;
     a.width = p.width, a.blocks = p.blocks, a.quads = p.quads, a.tiles = p.tiles, a.segs = p.segs;
-    a.seg_tiles = p.seg_tiles, a.walks = p.walks;
+    a.seg_tiles = p.seg_tiles, a.walks = p.walks, a.stretches = p.stretches;
     char* w = static_cast<char*>(ws);
     a.ends = reinterpret_cast<f4*>(w), w += p.ends_bytes;
     a.lasts = reinterpret_cast<float*>(w), w += p.lasts_bytes;
@@ -1357,6 +1372,6 @@ extern "C" int fhc_ssm_backward(const fhc_ssm_desc* g, const fhc_seq* x, const f
         });
         if (rc < 0) return rc;
         const float* part = reinterpret_cast<const float*>(static_cast<char*>(ws) + p.ends_bytes + p.lasts_bytes);
-        return close_sums(op, part, p.segs * p.walks, sums, st);
+        return close_sums(op, part, p.segs * p.walks * p.stretches, sums, st);
     });
 }

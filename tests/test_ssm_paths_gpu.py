@@ -82,3 +82,36 @@ def test_linear_gradients_past_the_types_range():
         assert (dx[3] == math.inf).all() and (dw[5] == math.inf).all()
         keep_x, keep_w = torch.arange(40) != 3, torch.arange(16) != 5
         assert torch.isfinite(dx[keep_x]).all() and torch.isfinite(dw[keep_w]).all()
+
+
+# ---- the scan's weights' gradients over very many rows: equal terms, so that a long chain of f32 additions shows ----
+
+def off_by(got, want):
+    return float(((got.double() - want) / want).abs().max())
+
+
+def test_ssm_weight_gradients_of_long_sequences():
+    """512 columns of 8192 steps run as one segment. With rates of 0 every term of a sum is the same number, which adding
+    one after the other in f32 rounds the same way at every step, a thousand half steps in all. A lane adds at most 256
+    terms of da (16 of dskip and ddt_bias, then 16 lanes' sums), each rounded to half a step of the sum so far."""
+    say("ssm long chains")
+    import torch
+    m, b, t = mod(), 512, 8192
+    full = lambda c, *s: torch.full(s or (b, t, 1), c, device="cuda")  # noqa: E731
+    dt = 20 + 0.4 * 2 ** -6  # softplus(dt) = dt to 1e-10
+    c = 1 + 0.4 * 2 ** -15
+    dt, c = (float(torch.tensor(k, dtype=torch.float32)) for k in (dt, c))
+    a, none = full(0.0, 1, 1), full(0.0)
+    # h = 1 and its gradient = 1 throughout: da = sum D; and dskip = sum dy x
+    args = (full(1.0), full(dt), a, none, none)
+    _, ht, states = m.ssm(*args, h0=full(1.0, b, 1, 1), train=True)
+    out = m.ssm_backward(*args, states, full(c), dht=full(1.0, b, 1, 1))
+    assert torch.equal(ht, full(1.0, b, 1, 1))
+    da, dskip = off_by(out[2], b * t * dt), off_by(out[5], b * t * c)
+    print("da off by", da / U, "dskip by", dskip / U, "half steps", flush=True)
+    # a state's gradient of 1 against B = 1: ddt = x sigmoid(dt), 1 to 2e-9
+    args = (full(c), full(dt), a, full(1.0), none)
+    _, _, states = m.ssm(*args, train=True)
+    bias = off_by(m.ssm_backward(*args, states, none, dht=full(1.0, b, 1, 1))[7], b * t * c)
+    print("ddt_bias off by", bias / U, "half steps", flush=True)
+    assert da <= (256 + 8) * U and dskip <= (32 + 4) * U and bias <= (32 + 24) * U
