@@ -9,8 +9,8 @@
 // Backward, with dv = dy act'(v) (v computed again) and e the state's rows and then the sequence's:
 //     de_i = sum over j of w[j] dv_(i - j),   dw[j] = sum over t of dv_t e_(t + j),   dbias = sum over t of dv_t
 // A thread walks its chunk and k - 1 steps more, whose dv it needs for its last inputs, and adds its weights' gradients
-// in registers; a workgroup's chunks of the same channels are added in LDS and the workgroups' sums by column_sums, all
-// in a fixed order.
+// in registers, over 256 steps at most; a workgroup's chunks of the same channels are added in LDS and the workgroups' sums
+// in f64 by column_sums, all in a fixed order.
 #include "seq_args.h"
 
 namespace fhc {
@@ -341,6 +341,7 @@ __global__ __launch_bounds__(kThreads) void short_conv_bwd(ConvArgs<typename T::
 // channels, since their windows and sums decide how many waves a SIMD has (4 with two, 2 with eight: 108 us and 320).
 constexpr int kBackV = 2;
 constexpr uint32_t kForwardV(uint32_t dtype) { return dtype == FHC_F32 ? 4 : 8; }
+constexpr uint32_t kMostItems = 8;  // of up to 32 steps each; the sums over workgroups are f64
 struct Plan {
     uint32_t v, groups, lanes, colblocks, chunks, steps, items, blocks, walks;
 };
@@ -361,7 +362,11 @@ Plan plan_of(const fhc_short_conv_desc* g, bool backward) {
     p.items = items >= 1ull << 32 ? 0 : (uint32_t)items;
     const uint64_t blocks = ceil_div(items, kThreads >> p.lanes);
     p.blocks = blocks >= 1ull << 32 ? 0 : (uint32_t)blocks;
-    const uint64_t walks = ceil_div(2048, p.colblocks);
+    // workgroups of a column block: 2048 over all, and as many (of one launch's) as leave a thread kMostItems chunks' terms
+    const uint64_t few = ceil_div(2048, p.colblocks), room = ((1ull << 32) / kThreads - 1) / p.colblocks;
+    uint64_t walks = ceil_div(blocks, kMostItems);
+    if (walks > room) walks = room;
+    if (walks < few) walks = few;
     p.walks = (uint32_t)(walks < blocks ? walks : blocks);
     return p;
 }

@@ -115,3 +115,25 @@ def test_ssm_weight_gradients_of_long_sequences():
     bias = off_by(m.ssm_backward(*args, states, none, dht=full(1.0, b, 1, 1))[7], b * t * c)
     print("ddt_bias off by", bias / U, "half steps", flush=True)
     assert da <= (256 + 8) * U and dskip <= (32 + 4) * U and bias <= (32 + 24) * U
+
+
+# ---- the convolution's weights' gradients over very many rows -----------------------------------------------------
+
+def test_short_conv_weight_gradients_of_long_sequences():
+    """2^27 equal steps: a thread adds at most 256 of them in f32, a workgroup of 32 threads a row 8 such sums."""
+    say("short_conv long chains")
+    import torch
+    m, t, d, k = mod(), 1 << 27, 64, 4
+    c = float(torch.tensor(1 + 0.4 * 2 ** -11, dtype=torch.float32))
+    x, dy, w = torch.ones(d, device="cuda"), torch.full((d,), c, device="cuda"), torch.zeros(d, k, device="cuda")
+    state = torch.ones(k - 1, d, device="cuda")
+    g = m.ShortConvDesc(2, m.CONV_ACTS["none"], 1, t, d, k, w.data_ptr(), None, None)
+    n = m._lib().fhc_short_conv_workspace_bytes(g)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    dw, db = torch.empty(d, k, device="cuda"), torch.empty(d, device="cuda")
+    rc = m._lib().fhc_short_conv_backward(g, m.FhcSeq(x.data_ptr(), 0, 0), state.data_ptr(), m.FhcSeq(dy.data_ptr(), 0, 0),
+                                          None, None, dw.data_ptr(), db.data_ptr(), None, ws.data_ptr(), n,
+                                          torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, m.fhconv.last_error()
+    print("dw off by", off_by(dw, t * c) / U, "dbias by", off_by(db, t * c) / U, "half steps", flush=True)
+    assert off_by(dw, t * c) <= (256 + 8 + 2) * U and off_by(db, t * c) <= (256 + 8 + 2) * U
