@@ -29,17 +29,19 @@ struct SlopeArgs {
     uint16_t *dv, *rest;  // rest: dv's remainder, or null
     float* part;  // [workgroup rows][n], or null
     int rows, n, walks;
+    uint32_t colblocks;  // of 512 columns; they come first in the workgroup's index
     uint32_t act;
 };
 template <class T>
 __global__ __launch_bounds__(256) void linear_slope(SlopeArgs g) {
     __shared__ float sums[3][8][64];
-    const int lane = threadIdx.x & 63, row = threadIdx.x >> 6, c = (blockIdx.x * 64 + lane) * 8, valid = g.n - c;
+    const uint32_t walk = blockIdx.x / g.colblocks, cb = blockIdx.x - walk * g.colblocks;
+    const int lane = threadIdx.x & 63, row = threadIdx.x >> 6, c = (cb * 64 + lane) * 8, valid = g.n - c;
     float db[8];
 #pragma unroll
     for (int v = 0; v < 8; v++) db[v] = 0.0f;
     if (valid > 0) {
-        for (int64_t m = (int64_t)blockIdx.y * 4 + row; m < g.rows; m += (int64_t)g.walks * 4) {
+        for (int64_t m = (int64_t)walk * 4 + row; m < g.rows; m += (int64_t)g.walks * 4) {
             const u4_t q = load_some(g.dy + m * g.ldy + c, valid);
             uint16_t out[8], rest[8];
             f4 pre[2] = {};
@@ -72,7 +74,7 @@ __global__ __launch_bounds__(256) void linear_slope(SlopeArgs g) {
     for (int v = 0; v < 8; v++) {
 #pragma unroll
         for (int r = 0; r < 3; r++) db[v] += sums[r][v][lane];
-        if (v < valid) g.part[(int64_t)blockIdx.y * g.n + c + v] = db[v];
+        if (v < valid) g.part[(int64_t)walk * g.n + c + v] = db[v];
     }
 }
 
@@ -92,9 +94,16 @@ bool keeps(const fhc_linear_desc* d) { return act(d) != FHC_ACT_IDENTITY; }
 size_t pre_bytes(const fhc_linear_desc* d) { return keeps(d) ? up256((size_t)d->rows * up8(d->f) * 4) : 0; }
 // products of the backward pass that dv takes along K
 int parts_of(const fhc_linear_desc* d) { return keeps(d) && !(d->act & FHC_LINEAR_ROUND_DV) ? 2 : 1; }
-// workgroups that a column block's rows are dealt to: two a CU over all columns
+// workgroups that a column block's rows are dealt to: four a CU over all columns, and as many (of one launch's) as leave a
+// thread kMostTerms rows, whose sum for the bias is f32; the sums over workgroups are f64
+constexpr uint32_t kMostTerms = 256;
 uint32_t walks_of(const fhc_linear_desc* d) {
-    const uint64_t cols = ceil_div(d->f, 512), most = ceil_div(d->rows, 4), want = cols ? ceil_div(1024, cols) : 0;
+    const uint64_t cols = ceil_div(d->f, 512), most = ceil_div(d->rows, 4);
+    if (!cols) return 0;
+    const uint64_t few = ceil_div(1024, cols), room = ((1ull << 32) / 256 - 1) / cols;
+    uint64_t want = ceil_div(most, kMostTerms);
+    if (want > room) want = room;
+    if (want < few) want = few;
     return (uint32_t)(want < most ? want : most);
 }
 size_t sums_bytes(const fhc_linear_desc* d) { return up256((size_t)walks_of(d) * d->f * 4); }
@@ -151,8 +160,8 @@ int backward(const char* op, const fhc_linear_desc* d, const fhc_rows* x, const 
     const bool slope = keeps(d) && (dx || dw || dbias);
     if (d->rows && d->f && (slope || dbias)) {
         SlopeArgs s{u16(dy->p), dy->ld, slope ? static_cast<const float*>(saved) : nullptr, up8(d->f),
-                    slope ? dv : nullptr, slope ? rest : nullptr, dbias ? sums : nullptr, (int)d->rows, (int)d->f, (int)walks, act(d)};
-        hipLaunchKernelGGL((linear_slope<T>), dim3((uint32_t)ceil_div(d->f, 512), walks), dim3(256), 0, st, s);
+                    slope ? dv : nullptr, slope ? rest : nullptr, dbias ? sums : nullptr, (int)d->rows, (int)d->f, (int)walks, (uint32_t)ceil_div(d->f, 512), act(d)};
+        hipLaunchKernelGGL((linear_slope<T>), dim3(walks * s.colblocks), dim3(256), 0, st, s);
         FHC_TRY(launched(op));
     }
     if (dbias) FHC_TRY(close_sums(op, sums, walks, Sums{{dbias, nullptr, nullptr}, {d->f, 0, 0}}, st));

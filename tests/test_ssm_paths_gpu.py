@@ -137,3 +137,24 @@ def test_short_conv_weight_gradients_of_long_sequences():
     assert rc == 0, m.fhconv.last_error()
     print("dw off by", off_by(dw, t * c) / U, "dbias by", off_by(db, t * c) / U, "half steps", flush=True)
     assert off_by(dw, t * c) <= (256 + 8 + 2) * U and off_by(db, t * c) <= (256 + 8 + 2) * U
+
+
+# ---- the product's bias' gradient over very many rows -------------------------------------------------------------
+
+def test_linear_bias_gradient_of_many_rows():
+    """2^24 equal rows: a thread adds at most 256 of them in f32."""
+    say("linear many rows")
+    import torch
+    m, rows, f = mod(), 1 << 24, 8
+    x = torch.zeros(rows, 1, dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(f, 1, dtype=torch.bfloat16, device="cuda")
+    bias = torch.linspace(-1.0, 2.5, f, device="cuda").bfloat16()
+    dy = torch.ones(rows, f, dtype=torch.bfloat16, device="cuda")
+    _, kept = m.linear(x, w, bias, act="silu", train=True)
+    db = m.linear_backward(x, w, kept, dy, "silu")[2]
+    v = bias.double()
+    slope = seqref._act(v, "silu")[1]
+    off = (db.double() - rows * slope).abs()
+    print("dbias off by", [round(float(k), 1) for k in off / (rows * U * slope.abs())], "half steps", flush=True)
+    # the slope itself to 64 U (as in ssmref.linear), 256 terms and 4 threads' sums
+    assert (off <= rows * (64 * U * (slope.abs() + 1) + (256 + 4) * U * slope.abs())).all()
