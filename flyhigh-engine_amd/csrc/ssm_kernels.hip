@@ -1107,7 +1107,7 @@ int close_vectors(const char* op, const fhc_ssm_desc* g, const float* bc, const 
 constexpr uint32_t kFewSteps = 4;
 
 struct Plan {
-    uint32_t width, blocks, quads, waves, tiles, segs, seg_tiles, walks, stretches;
+    uint32_t width, blocks, quads, tiles, segs, seg_tiles, walks, stretches;
     bool halves;  // forward: two states a lane
     uint64_t wgs;
     size_t ends_bytes, lasts_bytes, part_bytes, bc_bytes;
@@ -1116,7 +1116,6 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 Plan plan_of(const fhc_ssm_desc* g, bool backward, bool ragged) {
     Plan p{};
     p.width = g->d / g->groups, p.blocks = (uint32_t)ceil_div(p.width, 64), p.quads = (g->n + 3) / 4;
-    p.waves = p.quads <= 1 ? 2 : p.quads <= 2 ? 4 : 8;  // at most
     p.tiles = (uint32_t)ceil_div(g->t, kTile);
     const uint64_t cols = (uint64_t)g->groups * p.blocks;
     const uint64_t one = g->b * cols;
@@ -1188,6 +1187,8 @@ int check_desc(const char* op, const fhc_ssm_desc* g) {
     FHC_TRY(check_shape(op, g->dtype, g->b, g->t, g->d));
     if (g->n < 1 || g->n > 64) return fail(-1, "%s: %u states a channel, 1 to 64 are possible", op, g->n);
     if (g->groups < 1 || g->d % g->groups) return fail(-1, "%s: %u groups of %u channels", op, g->groups, g->d);
+    if ((uint64_t)g->groups * g->n >= 1ull << 31)
+        return fail(-1, "%s: %u groups of %u states, at most 2^31 - 1 values a step", op, g->groups, g->n);
     FHC_TRY(check_array(op, "a", g->a, 4, g->b && g->d));
     FHC_TRY(check_array(op, "dt_bias", g->dt_bias, 4, false));
     FHC_TRY(check_array(op, "skip", g->skip, 4, false));
@@ -1211,6 +1212,9 @@ SsmArgs<typename T::Raw> args_of(const fhc_ssm_desc* g, const Plan& p, const fhc
     a.bc = reinterpret_cast<float*>(w);
     return a;
 }
+
+// waves of a workgroup of the tile kernels (with two states a lane up to 8, but of few workgroups)
+uint32_t waves_of(const Plan& p) { return p.quads <= 2 ? 2 : p.quads <= 4 ? 4 : 8; }
 
 enum Kernel { kFold, kForward, kFoldBack, kBackward };
 template <class T, Kernel KERNEL>
@@ -1245,8 +1249,11 @@ template <class T>
 int launch_step(const char* op, const Plan& p, const SsmArgs<typename T::Raw>& a, hipStream_t st) {
     uint32_t lp = 1;
     while (lp < p.quads) lp *= 2;
-    const dim3 grid((uint32_t)ceil_div((uint64_t)a.d * lp, 256), a.b < 65535 ? a.b : 65535);
-    FHC_TRY(check_grid(op, (uint64_t)grid.x * grid.y, 256));
+    // as many sequences side by side as one launch has workgroups for
+    const uint64_t wide = ceil_div((uint64_t)a.d * lp, 256), room = ((1ull << 32) / 256 - 1) / wide;
+    FHC_TRY(check_grid(op, wide, 256));
+    const uint64_t rows = room < 65535 ? room : 65535;
+    const dim3 grid((uint32_t)wide, a.b < rows ? a.b : (uint32_t)rows);
 #define STEP(LP)                                                                                           \
     do {                                                                                                   \
         if (a.n % 4 == 0) hipLaunchKernelGGL((ssm_step<T, LP, true>), grid, dim3(256), 0, st, a);          \
@@ -1262,13 +1269,13 @@ int launch_step(const char* op, const Plan& p, const SsmArgs<typename T::Raw>& a
 }
 
 int check_inputs(const char* op, const fhc_ssm_desc* g, const Plan& p, const fhc_seq* x, const fhc_seq* dt,
-                 const fhc_seq* bm, const fhc_seq* cm, const fhc_seq* z) {
+                 const fhc_seq* bm, const fhc_seq* cm, const fhc_seq* z, bool few_steps) {
     FHC_TRY(check_in(op, "x", x, g->dtype, g->t));
     FHC_TRY(check_in(op, "dt", dt, g->dtype, g->t));
     FHC_TRY(check_in(op, "bm", bm, g->dtype, g->t));
     FHC_TRY(check_in(op, "cm", cm, g->dtype, g->t));
     if (z) FHC_TRY(check_in(op, "z", z, g->dtype, g->t));
-    return check_grid(op, p.wgs, 64 * p.waves);
+    return few_steps ? 0 : check_grid(op, p.wgs, 64 * waves_of(p));  // the step kernel's grid is checked where it is made
 }
 
 }  // namespace
@@ -1303,7 +1310,7 @@ extern "C" int fhc_ssm_forward(const fhc_ssm_desc* g, const fhc_seq* x, const fh
         FHC_TRY(check_desc(op, g));
         if ((uint64_t)g->b * g->d == 0) return 0;
         const Plan p = plan_of(g, false, g->lengths != nullptr);
-        FHC_TRY(check_inputs(op, g, p, x, dt, bm, cm, z));
+        FHC_TRY(check_inputs(op, g, p, x, dt, bm, cm, z, g->t <= kFewSteps));
         FHC_TRY(check_out(op, "y", y, g->dtype, g->b, g->t, g->d));
         FHC_TRY(check_array(op, "h0", h0, 4, false));
         FHC_TRY(check_array(op, "ht", ht, 4, false));
@@ -1351,7 +1358,7 @@ extern "C" int fhc_ssm_backward(const fhc_ssm_desc* g, const fhc_seq* x, const f
             return rc;
         }
         const Plan p = plan_of(g, true, g->lengths != nullptr);
-        FHC_TRY(check_inputs(op, g, p, x, dt, bm, cm, z));
+        FHC_TRY(check_inputs(op, g, p, x, dt, bm, cm, z, false));
         FHC_TRY(check_in(op, "dy", dy, g->dtype, g->t));
         FHC_TRY(check_out(op, "dx", dx, g->dtype, g->b, g->t, g->d));
         FHC_TRY(check_out(op, "ddt", ddt, g->dtype, g->b, g->t, g->d));

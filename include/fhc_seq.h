@@ -168,7 +168,7 @@ int fhc_short_conv_backward(const fhc_short_conv_desc* g, const fhc_seq* x, cons
 typedef struct fhc_ssm_desc {
     uint32_t dtype;          /* FHC_F16, FHC_BF16 or FHC_F32: of x, dt, z, B, C, y and their gradients               */
     uint32_t b, t, d;        /* sequences, steps, channels; any may be 0. b * d below 2^31                            */
-    uint32_t n, groups;      /* states a channel, 1 to 64; groups, a divisor of d                                     */
+    uint32_t n, groups;      /* states a channel, 1 to 64; groups, a divisor of d. groups * n below 2^31              */
     const float* a;          /* device, dense [d][n]                                                                  */
     const float* dt_bias;    /* device, [d], or NULL: zeros                                                           */
     const float* skip;       /* device, [d], or NULL: zeros                                                           */

@@ -158,3 +158,42 @@ def test_linear_bias_gradient_of_many_rows():
     print("dbias off by", [round(float(k), 1) for k in off / (rows * U * slope.abs())], "half steps", flush=True)
     # the slope itself to 64 U (as in ssmref.linear), 256 terms and 4 threads' sums
     assert (off <= rows * (64 * U * (slope.abs() + 1) + (256 + 4) * U * slope.abs())).all()
+
+
+# ---- calls of very many sequences ---------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("t", [1, 5])
+def test_ssm_of_very_many_sequences(t):
+    """2^23 sequences: as many as a launch of 256 threads a sequence has room for."""
+    say("ssm many sequences", t)
+    import torch
+    q, m, b, n = Rand(63), mod(), 1 << 23, 9
+    v = ssm_inputs(q, 4096, t, 1, n, 1, torch.bfloat16)
+    names = ("x", "dt", "bm", "cm", "z", "h0")
+    few = m.ssm(v["x"], v["dt"], v["a"], v["bm"], v["cm"], v["skip"], v["z"], v["dt_bias"], v["h0"])
+    wide = {k: v[k].repeat(b // 4096, 1, 1) for k in names}
+    y, ht = m.ssm(wide["x"], wide["dt"], v["a"], wide["bm"], wide["cm"], v["skip"], wide["z"], v["dt_bias"], wide["h0"])
+    assert torch.equal(y.view(-1, 4096, t, 1), few[0].expand(b // 4096, 4096, t, 1))
+    assert torch.equal(ht.view(-1, 4096, 1, n), few[1].expand(b // 4096, 4096, 1, n))
+    ref, err = ssmref.ssm(*(v[k] for k in ("x", "dt", "a", "bm", "cm", "skip", "z", "dt_bias", "h0")))
+    compare(("y", "ht"), few, ref, err)
+
+
+def test_ssm_step_of_many_sequences_and_channels():
+    """65536 sequences of 4112 channels of 64 states, more workgroups than a launch has: they walk the sequences."""
+    say("ssm step many")
+    import torch
+    q, m, b, d, n = Rand(65), mod(), 65536, 4112, 64
+    x, dt = (q.normal(256, 1, d, dtype=torch.bfloat16) for _ in range(2))
+    bm, cm = (q.normal(b, 1, n, dtype=torch.bfloat16) for _ in range(2))
+    a, y = -q.uniform(d, n, lo=0.5, hi=2.0), torch.empty(b, 1, d, dtype=torch.bfloat16, device="cuda")
+    wide = [p.repeat(b // 256, 1, 1) for p in (x, dt)] + [bm, cm]
+    g = m.SsmDesc(1, b, 1, d, n, 1, a.data_ptr(), None, None, None)  # through the C ABI: no states in or out
+    sq = [m.FhcSeq(p.data_ptr(), p.stride(0), p.stride(1)) for p in wide + [y]]
+    rc = m._lib().fhc_ssm_forward(g, *sq[:4], None, None, sq[4], None, None, None, 0,
+                                  torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, m.fhconv.last_error()
+    for at in (0, 4096, 65280, 65408):  # the last ones are a workgroup's second sequences
+        cut = slice(at, at + 128)
+        want = m.ssm(wide[0][cut], wide[1][cut], a, bm[cut], cm[cut])[0]
+        assert torch.equal(y[cut], want), at
