@@ -472,7 +472,9 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_fold(SsmArgs<typename T::Raw> g
 }
 
 // h through the folds of `count` segments, `step` slots apart from p on: eight segments' loads are under way together. A
-// segment that is not there is one that changes nothing.
+// segment that is not there is one that changes nothing. A segment's decay goes in as its square root, twice: from states to
+// states that f32 holds it may itself be out of range. The root is finite, so that a state of 0 stays 0 (any other normal one
+// that 2^255 multiplies is past the range with it).
 template <int NS>
 __device__ __forceinline__ void through(const float* p, int64_t step, const float* total, int64_t tstep, uint32_t count,
                                         const float (&rate)[NS], float (&h)[NS]) {
@@ -491,8 +493,10 @@ __device__ __forceinline__ void through(const float* p, int64_t step, const floa
 #pragma unroll
         for (int u = 0; u < 8; u++)
 #pragma unroll
-            for (int k = 0; k < NS; k++)
-                h[k] = __builtin_fmaf(__builtin_amdgcn_exp2f(rate[k] * sum[u]), h[k], end[u][k]);
+            for (int k = 0; k < NS; k++) {
+                const float half = rate[k] * sum[u] * 0.5f, root = __builtin_amdgcn_exp2f(half > 127.5f ? 127.5f : half);
+                h[k] = __builtin_fmaf(root, root * h[k], end[u][k]);
+            }
     }
 }
 

@@ -160,6 +160,60 @@ def test_linear_bias_gradient_of_many_rows():
     assert (off <= rows * (64 * U * (slope.abs() + 1) + (256 + 4) * U * slope.abs())).all()
 
 
+# ---- states that grow ---------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("shape", [(1, 2048, 64, 16, 1), (2, 1500, 70, 4, 1)], ids=str)
+def test_ssm_states_that_grow(shape):
+    """Rates above 0 over long stretches of no input: states and gradients of 0 stay 0 however much a stretch would grow
+    them, and what lies at the sequence's other end is that of a call of those steps alone."""
+    say("ssm growing", shape)
+    import torch
+    v = ssm_inputs(Rand(61), *shape, torch.float32)
+    v["a"], v["h0"], v["dht"], v["dt_bias"] = v["a"].abs(), None, None, None
+    m, t, steps = mod(), shape[1], ("x", "dt", "z", "bm", "cm", "dy")
+    kw = lambda q: {k: q[k] for k in ("skip", "z")}  # noqa: E731
+    v["dt"].fill_(1.0)
+    v["dt"][:, -3:], v["dt"][:, :3] = -3.0, -3.0
+    fwd = {**v, "x": v["x"].clone()}
+    fwd["x"][:, :-3] = 0.0
+    end = {k: q[:, -3:].contiguous() if k in steps else q for k, q in fwd.items()}
+    y, ht = m.ssm(fwd["x"], fwd["dt"], v["a"], v["bm"], v["cm"], **kw(fwd))
+    ref, err = ssmref.ssm(end["x"], end["dt"], v["a"], end["bm"], end["cm"], **kw(end))
+    compare(("y", "ht"), (y[:, -3:], ht), ref, err)
+    assert not y[:, :-3].any()
+    back = {**v, "x": torch.zeros_like(v["x"]), "dy": v["dy"].clone()}
+    back["dy"][:, 3:] = 0.0
+    start = {k: q[:, :3].contiguous() if k in steps else q for k, q in back.items()}
+    args = (back["x"], back["dt"], v["a"], v["bm"], v["cm"])
+    states = m.ssm(*args, train=True, **kw(back))[2]
+    got = m.ssm_backward(*args, states, back["dy"], **kw(back))
+    ref, err = ssmref.ssm(start["x"], start["dt"], v["a"], start["bm"], start["cm"], **kw(start), dy=start["dy"])
+    per_step = (0, 1, 3, 4, 6)  # of got: dx, ddt, dbm, dcm, dz
+    compare(SSM_NAMES[2:], [g[:, :3] if i in per_step else g for i, g in enumerate(got)], ref[2:], err[2:])
+    assert not any(got[i][:, 3:].any() for i in per_step)
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_ssm_stretches_that_grow_or_shrink_by_more_than_a_float(sign):
+    """64 steps that grow the states by e^95 or shrink them by that, which f32 does not hold, from 2^-100 or 2^100 on."""
+    say("ssm far decays", sign)
+    import torch
+    m, t, d = mod(), 1024, 64
+    x, one = torch.zeros(1, t, d, device="cuda"), torch.ones(1, t, 1, device="cuda")
+    dt = torch.full((1, t, d), -60.0, device="cuda")
+    dt[:, 64:128] = -4.0
+    step = math.log1p(math.exp(-4.0))
+    a = torch.full((d, 1), sign * 95.0 / (64 * step), device="cuda")
+    h0 = torch.full((1, d, 1), 2.0 ** (-100 * sign), device="cuda")
+    want = 2.0 ** (-100 * sign) * math.exp(float(a[0, 0].double()) * 64 * step)
+    # the exponents' errors: 95 times the steps' (16 U), their products' and sum's (64 + 4 U); 6 U a decay
+    tol = (95 * (16 + 64 + 4) + 6 * 64) * U
+    y, ht, states = m.ssm(x, dt, a, one, one, h0=h0, train=True)
+    dh0 = m.ssm_backward(x, dt, a, one, one, states, x, dht=h0)[8]
+    print("off by", off_by(ht, want) / U, off_by(dh0, want) / U, "half steps", flush=True)
+    assert off_by(ht, want) <= tol and off_by(dh0, want) <= tol
+
+
 # ---- calls of very many sequences ---------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("t", [1, 5])
