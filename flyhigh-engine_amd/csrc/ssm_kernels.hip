@@ -80,7 +80,8 @@ struct States {
 
 // h[k] += B_k u, then the sum of C_k h[k], B_k and C_k from lane FROM + k of the own row of 16 lanes. In assembly: the
 // compiler spends a move on each such operand. The instructions in front may have written b or c (a DPP operand's two wait
-// states).
+// states). What an instruction writes before the last input is read is an early clobber, here and below: an input of the
+// same value would otherwise be given the same register.
 template <int FROM>
 __device__ __forceinline__ float step_states(States<4>& h, float b, float u, float c) {
     float p = 0.0f;
@@ -94,7 +95,7 @@ __device__ __forceinline__ float step_states(States<4>& h, float b, float u, flo
         "v_fmac_f32_dpp %0, %7, %2 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n"
         "v_fmac_f32_dpp %0, %7, %3 row_newbcast:%10 row_mask:0xf bank_mask:0xf\n"
         "v_fmac_f32_dpp %0, %7, %4 row_newbcast:%11 row_mask:0xf bank_mask:0xf"
-        : "=&v"(p), "+v"(h.v[0]), "+v"(h.v[1]), "+v"(h.v[2]), "+v"(h.v[3])
+        : "=&v"(p), "+&v"(h.v[0]), "+&v"(h.v[1]), "+&v"(h.v[2]), "+&v"(h.v[3])
         : "v"(b), "v"(u), "v"(c), "n"(FROM), "n"(FROM + 1), "n"(FROM + 2), "n"(FROM + 3));
 #endif
     return p;
@@ -108,7 +109,7 @@ __device__ __forceinline__ float step_states(States<2>& h, float b, float u, flo
         "v_fmac_f32_dpp %2, %3, %4 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n"
         "v_mul_f32_dpp %0, %5, %1 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n"
         "v_fmac_f32_dpp %0, %5, %2 row_newbcast:%7 row_mask:0xf bank_mask:0xf"
-        : "=&v"(p), "+v"(h.v[0]), "+v"(h.v[1])
+        : "=&v"(p), "+&v"(h.v[0]), "+&v"(h.v[1])
         : "v"(b), "v"(u), "v"(c), "n"(FROM), "n"(FROM + 1));
 #endif
     return p;
@@ -123,7 +124,7 @@ __device__ __forceinline__ void add_outer(f4& h, float b, float u) {
         "v_fmac_f32_dpp %1, %4, %5 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n"
         "v_fmac_f32_dpp %2, %4, %5 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n"
         "v_fmac_f32_dpp %3, %4, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf"
-        : "+v"(h0), "+v"(h1), "+v"(h2), "+v"(h3)
+        : "+&v"(h0), "+&v"(h1), "+&v"(h2), "+&v"(h3)
         : "v"(b), "v"(u), "n"(FROM), "n"(FROM + 1), "n"(FROM + 2), "n"(FROM + 3));
     h = f4{h0, h1, h2, h3};
 #endif
@@ -146,7 +147,7 @@ __device__ __forceinline__ void step_back(f4& g, f4 h, float b, float c, float q
         "v_fmac_f32_dpp %1, %10, %4 row_newbcast:%15 row_mask:0xf bank_mask:0xf\n"
         "v_fmac_f32_dpp %0, %11, %9 row_newbcast:%16 row_mask:0xf bank_mask:0xf\n"
         "v_fmac_f32_dpp %1, %10, %5 row_newbcast:%16 row_mask:0xf bank_mask:0xf"
-        : "=&v"(p), "=&v"(s1), "+v"(g0), "+v"(g1), "+v"(g2), "+v"(g3)
+        : "=&v"(p), "=&v"(s1), "+&v"(g0), "+&v"(g1), "+&v"(g2), "+&v"(g3)
         : "v"(h[0]), "v"(h[1]), "v"(h[2]), "v"(h[3]), "v"(b), "v"(c), "v"(q), "n"(FROM), "n"(FROM + 1), "n"(FROM + 2),
           "n"(FROM + 3));
     g = f4{g0, g1, g2, g3};
