@@ -251,3 +251,53 @@ def test_ssm_step_of_many_sequences_and_channels():
         cut = slice(at, at + 128)
         want = m.ssm(wide[0][cut], wide[1][cut], a, bm[cut], cm[cut])[0]
         assert torch.equal(y[cut], want), at
+
+
+# ---- kernels that only larger calls take --------------------------------------------------------------------------
+
+LARGER = [  # rows, c, f: few rows with four waves a workgroup, whole and odd widths; 128 x 128 tiles of an unsplit K, and
+    (5, 72, 4100), (20, 65, 4099), (32, 200, 8192),  # their pairs of columns and single ones; 256 x 256 tiles likewise;
+    (1003, 130, 2734), (1003, 130, 2735), (1003, 136, 2736), (2500, 130, 4102), (2500, 130, 4101),
+    (40, 4200, 64), (40, 4096, 70),  # a K in 16 and more parts
+]
+
+
+@pytest.mark.parametrize("dtype,act", [("f16", "gelu"), ("bf16", "silu"), ("bf16", "none")])
+@pytest.mark.parametrize("shape", LARGER, ids=str)
+def test_linear_larger_calls(shape, dtype, act):
+    say("linear larger", shape, dtype, act)
+    linear_check(linear_inputs(Rand(sum(shape) + 5), *shape, types()[dtype]), act)
+
+
+@pytest.mark.parametrize("shape", [(4, 1100, 4097, 4), (3, 700, 4096, 2)], ids=str)
+def test_short_conv_several_items_a_thread(shape):
+    """More chunks than workgroups' rows: the backward pass walks them."""
+    say("short_conv items", shape)
+    import torch
+    conv_check(conv_inputs(Rand(sum(shape) + 5), *shape, torch.bfloat16, ragged=shape[2] % 2 == 1))
+
+
+def test_stream_argument():
+    """stream=: the work, and what it allocates, on that stream."""
+    say("stream argument")
+    import torch
+    m, q = mod(), Rand(65)
+    c = conv_inputs(q, 3, 40, 72, 4, torch.bfloat16)
+    s = ssm_inputs(q, 3, 40, 72, 16, 1, torch.bfloat16)
+    p = linear_inputs(q, 100, 72, 48, torch.bfloat16)
+    kw = {k: s[k] for k in ("skip", "z", "dt_bias")}
+
+    def run(**on):
+        y, ht, states = m.ssm(s["x"], s["dt"], s["a"], s["bm"], s["cm"], h0=s["h0"], train=True, **kw, **on)
+        out = (y, ht) + m.ssm_backward(s["x"], s["dt"], s["a"], s["bm"], s["cm"], states, s["dy"], dht=s["dht"], **kw, **on)
+        out += m.short_conv(c["x"], c["w"], c["bias"], state=c["state"], **on)
+        out += m.short_conv_backward(c["x"], c["w"], c["bias"], c["dy"], state=c["state"], dstate=c["dstate"], **on)
+        y, kept = m.linear(p["x"], p["w"], p["bias"], p["residual"], "gelu", train=True, **on)
+        return out + (y,) + m.linear_backward(p["x"], p["w"], kept, p["dy"], "gelu", **on)
+
+    want = run()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    got = run(stream=stream)
+    stream.synchronize()
+    assert all(_same(a, b) for a, b in zip(got, want))
