@@ -9,9 +9,9 @@
 // remainder out: half the work, and dx and dw carry dv's rounding beside their own (of random terms 1.4 times the error).
 //
 // What bounds it (MI355X): matrix units for large calls, HBM for few rows. 8192 x 2048 -> 8192 bf16 with silu, bias and
-// residual: 320 us forward, 390 where v is kept (its f32 passes through the epilogue), a training step 1310, with a rounded dv
-// 910: dv 125 (4.3 TB/s), dx and dw 210 to 230 each (1200 to 1310 TFLOP/s; a large library product reaches 1344). 4 x 2048 ->
-// 8192: 11 us for 34 MB.
+// residual: 320 us forward, 390 where v is kept (its f32 passes through the epilogue), a training step 1300: dv and its
+// remainder 155 for 671 MB (4.3 TB/s), dx and dw 446 and 449 (1230 TFLOP/s over both parts; a large library product reaches
+// 1344). With a rounded dv the step takes 910: dv 130, dx and dw 240 each. 4 x 2048 -> 8192: 11 us for 34 MB.
 #include "ffn_product.h"
 #include "seq_args.h"
 

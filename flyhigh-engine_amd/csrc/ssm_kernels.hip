@@ -51,7 +51,7 @@ struct SsmArgs {
 };
 
 // softplus(v) = max(v, 0) + log1p(e), e = exp(-|v|): a polynomial of degree 9 in e for log1p(e) / e on [0, 1], the least
-// squares of its relative error, which is 5e-9 (and 1.1e-7 in f32): small steps keep their digits.
+// squares of its relative error, which is 1.6e-8 at most (1.3e-7 as f32 evaluates it): small steps keep their digits.
 __device__ __forceinline__ float softplus(float v, float& e) {
     e = __builtin_amdgcn_exp2f(__builtin_fabsf(v) * -kLog2e);
     float p = -0.0031640392262488604f;
@@ -389,8 +389,8 @@ __device__ __forceinline__ f4 decay(float step, f4 rate) {
     for (int k = 0; k < 4; k++) a[k] = __builtin_amdgcn_exp2f(step * rate[k]);
     return a;
 }
-// The ends of segments from zeros: W waves, NQ quads of states each. What bounds it (MI355X): the vector units, as below; 32768
-// steps of 2048 channels of 16 states, bf16, in 64 segments, 205 us.
+// The ends of segments from zeros: W waves, NQ quads of states each. What bounds it (MI355X): the vector units, as below, 109
+// cycles a step of four states; 32768 steps of 2048 channels of 16 states, bf16, in 64 segments, 205 us, 99% of them issue.
 template <class T, int W, int NQ>
 __global__ __launch_bounds__(64 * W, 2) void ssm_fold(SsmArgs<typename T::Raw> g) {
     using R = typename T::Raw;
@@ -501,12 +501,14 @@ __device__ __forceinline__ void through(const float* p, int64_t step, const floa
     }
 }
 
-// W waves, NQ times NS states each. What bounds it (MI355X): the vector units. Four states' step takes an exponential (8 cycles
-// of a SIMD's issue), two products and two multiply-adds with DPP operands (4) each, about 85 cycles in all with its share of
-// the tile's preparation and end: 230 us at full issue for 2^30 steps of a state, where HBM would take 104 us. 4 x 4096 steps
-// of 4096 channels of 16 states, bf16 with a gate, 430 us (256 workgroups of 8 waves: two waves a SIMD, whose waits at a tile's
-// two barriers nothing fills); 32768 steps of 2048 channels in segments 300, after the fold's 205; 1620 x 24 steps of 256
-// channels, f16, 64 us for 135 MB (2.1 TB/s: two tiles a workgroup, whose first loads nothing covers).
+// W waves, NQ times NS states each. What bounds it (MI355X): the vector units. By the issue counters a step of four states of 64
+// channels takes 154 cycles of a SIMD, with its share of the tile's preparation and end: four exponentials (8 cycles each), eight
+// products and eight multiply-adds (4 each) are 96 of them. 2^30 steps of a state are 630,000 cycles on 1024 SIMDs, 290 us at the
+// 2.16 GHz that the chip then runs at; HBM would take 104. 32768 steps of 2048 channels of 16 states, bf16 with a gate, in
+// segments: 300 us, 97% of them issue, after the fold's 205. 4 x 4096 steps of 4096 channels: 390 us a call, 430 under the
+// profiler, 64% of them issue (256 workgroups of 8 waves: two waves a SIMD, whose waits at a tile's two barriers nothing fills).
+// 1620 x 24 steps of 256 channels, f16, 64 us for 135 MB (2.1 TB/s: two tiles a workgroup, whose first loads nothing covers). f32
+// takes as long: 391 us for 4 x 4096 x 4096, 476 for the long sequence.
 // Tried without gain: one barrier a tile with two buffers; outer products on the matrix units, which do not run beside the
 // vector unit's exponentials; a workgroup order by XCD.
 template <class T, int W, int NQ, int NS>
@@ -687,7 +689,7 @@ __global__ __launch_bounds__(64 * W, 2) void ssm_fwd(SsmArgs<typename T::Raw> g)
 // Few steps: a thread has one quad of one channel's states, LP threads side by side a channel, so a wave reads and writes
 // the states as they lie, 16 bytes a lane; the steps follow one another. WHOLE: n is a multiple of 4.
 // What bounds it (MI355X): HBM, which the states are read from and written to. One step of 64 x 4096 channels of 16
-// states, bf16: 9.9 us for 36 MB; each step more is 3.6 us, of its narrow loads.
+// states, bf16: 9.9 us for 36 MB (11 under the profiler); each step more is 2 to 4 us, of its narrow loads.
 template <class T, int LP, bool WHOLE>
 __global__ __launch_bounds__(256) void ssm_step(SsmArgs<typename T::Raw> g) {
     using R = typename T::Raw;
@@ -772,9 +774,11 @@ __device__ __forceinline__ float add_quad(float v) {
 }
 
 // FOLD: the gradients that reach the states before a segment, from zeros behind it.
-// What bounds it (MI355X): vector units and waits at once: two waves a SIMD, which LDS and the 64 registers of a tile's states
-// set, and 72% of issue while a CU has work. A step of a state takes about 50 cycles of a SIMD. 6 x 2051 steps at most of 1532
-// channels of 16 states, bf16: 250 us, after its fold's 58; 4 x 512 of 1024 channels of 64 states, f32: 123 and 29.
+// What bounds it (MI355X): waits beside the vector units. A step of a state and 64 channels takes 96 cycles of a SIMD's issue with
+// 64 states a channel and 119 with 16 and lengths; that is 66% and 60% of the kernel's time, 75% while a CU has work. The rest
+// are waits at barriers and for LDS, at two waves a SIMD, which LDS and the 64 registers of a tile's states set. 6 x 2051 steps at
+// most of 1532 channels of 16 states, bf16: 256 us, after its fold's 61; 4 x 512 of 1024 channels of 64 states, f32: 128 and 31.
+// With all its columns side by side, 4 x 4096 of 4096 channels of 16 states: 1230 us a call in bf16 and in f32.
 template <class T, int W, int NQ, bool FOLD>
 __global__ __launch_bounds__(64 * W, 2) void ssm_bwd(SsmArgs<typename T::Raw> g) {
     using R = typename T::Raw;
