@@ -60,27 +60,29 @@ inline int check_array(const char* op, const char* name, const void* p, uint32_t
 namespace {  // a kernel of this unit: another one's is registered apart
 
 // The sums over rows of part[row][.] in f64, its columns dealt to up to three outputs one after another (null: not
-// wanted): 16 threads take every 16th row of 64 columns, and their sums are added in their order.
+// wanted): of each of COLS columns, ROWS threads take every ROWS-th row, and their sums are added in their order.
 struct Sums {
     float* out[3];
     uint64_t cols[3];
 };
+template <int COLS>
 __global__ __launch_bounds__(1024) void column_sums(const float* part, uint32_t rows, Sums o) {
-    __shared__ double s[16][64];
-    const uint32_t x = threadIdx.x & 63, y = threadIdx.x >> 6;
-    uint64_t c = (uint64_t)blockIdx.x * 64 + x;
+    constexpr uint32_t ROWS = 1024 / COLS;
+    __shared__ double s[ROWS][COLS];
+    const uint32_t x = threadIdx.x % COLS, y = threadIdx.x / COLS;
+    uint64_t c = (uint64_t)blockIdx.x * COLS + x;
     const uint64_t pitch = o.cols[0] + o.cols[1] + o.cols[2];
     const bool live = c < pitch;
     double sum = 0.0;
     if (live) {
 #pragma unroll 4
-        for (uint32_t r = y; r < rows; r += 16) sum += part[r * pitch + c];
+        for (uint64_t r = y; r < rows; r += ROWS) sum += part[r * pitch + c];
     }
     s[y][x] = sum;
     __syncthreads();
     if (y > 0 || !live) return;
 #pragma unroll
-    for (int k = 1; k < 16; k++) sum += s[k][x];
+    for (uint32_t k = 1; k < ROWS; k++) sum += s[k][x];
 #pragma unroll
     for (int k = 0; k < 3; k++) {
         if (c < o.cols[k]) {
@@ -91,10 +93,15 @@ __global__ __launch_bounds__(1024) void column_sums(const float* part, uint32_t 
     }
 }
 inline int close_sums(const char* op, const float* part, uint32_t rows, const Sums& o, hipStream_t st) {
-    const uint64_t blocks = ceil_div(o.cols[0] + o.cols[1] + o.cols[2], 64);
-    if (!blocks || (!o.out[0] && !o.out[1] && !o.out[2])) return 0;
+    const uint64_t columns = o.cols[0] + o.cols[1] + o.cols[2];
+    if (!columns || (!o.out[0] && !o.out[1] && !o.out[2])) return 0;
+    // Few columns over many rows have a whole workgroup's threads to 8 columns, else to 64. us of a backward pass with 64 and with
+    // 8: 16384 rows of 1152 5275, 5190; 8192 of 320 1424, 1404; 4096 of 1152 1347, 1337; 1024 of 1280 350, 359.
+    const bool few = columns <= 2048 && rows >= 4096;
+    const uint64_t blocks = ceil_div(columns, few ? 8 : 64);
     FHC_TRY(check_grid(op, blocks, 1024));
-    hipLaunchKernelGGL(column_sums, dim3((uint32_t)blocks), dim3(1024), 0, st, part, rows, o);
+    if (few) hipLaunchKernelGGL(column_sums<8>, dim3((uint32_t)blocks), dim3(1024), 0, st, part, rows, o);
+    else hipLaunchKernelGGL(column_sums<64>, dim3((uint32_t)blocks), dim3(1024), 0, st, part, rows, o);
     return launched(op);
 }
 
