@@ -164,7 +164,9 @@ int fhc_short_conv_backward(const fhc_short_conv_desc* g, const fhc_seq* x, cons
  *     h_t[k] = exp(D_t a[ch][k]) h_(t-1)[k] + D_t x_t B_t[k]
  *     y_t    = (sum over k of C_t[k] h_t[k] + skip[ch] x_t) silu(z_t)
  * a, dt_bias and skip are f32 weights; z may be left out (no gate). With `lengths` positions at and past a sequence's
- * length are not read, y and the gradients there are 0, and the state stays as it is. */
+ * length are not read, y and the gradients there are 0, and the state stays as it is. a may be above 0 (states that grow) as
+ * long as a step's exp(D a) is in f32's range. From a step on whose D or D x is not finite, its channel's y and states are
+ * infinite or NaN. */
 typedef struct fhc_ssm_desc {
     uint32_t dtype;          /* FHC_F16, FHC_BF16 or FHC_F32: of x, dt, z, B, C, y and their gradients               */
     uint32_t b, t, d;        /* sequences, steps, channels; any may be 0. b * d below 2^31                            */
